@@ -403,6 +403,133 @@ pa_status pa_write_block_f32(pa_stream* stream, const pa_config* cfg, void* k_ca
                              float* k_scale, float* v_scale, float* k_absmax, float* v_absmax,
                              int32_t block, int32_t tokens, const float* k_in, const float* v_in);
 
+/* ---- attention over selected blocks, for long contexts ----
+ * A decode step that reads a bounded number of blocks however long the context is: every block has
+ * bounds of its keys, a query scores all blocks of its context from their bounds (a sixteenth of the
+ * K and V bytes), and attends to the best of them. No reference counterpart: the reference decodes over
+ * the whole context (DecodeOrchestrator.ComputeDecodeAttention, Phases/DecodeOrchestrator.cs:64-80).
+ *
+ * Query tokens: query r is one token with its own context length context_lens[r], of the sequence
+ * query_seqs[r] (a row of the block tables, num_seqs of them); several queries may be of one sequence (drafted
+ * tokens that are verified together). query_seqs null: query r belongs to sequence r, and num_queries
+ * must be num_seqs. A query whose query_seqs entry is out of range has an empty context. Contexts are
+ * read up to max_context_len and max_blocks_per_seq * 16 tokens. None of these calls allocates or
+ * synchronises; all may be captured into a graph. Calls that share a workspace must not overlap. */
+
+/* Bytes of the key bounds of the pool: [num_blocks][num_kv_heads][2][head_dim] elements of kv_dtype
+ * (index 0: minimum, 1: maximum of each channel over the block's keys; int8 caches: of the codes, to
+ * be read with the block's k_scale). */
+pa_status pa_key_bounds_bytes(const pa_config* cfg, size_t* bytes);
+/* Brings the bounds up to date after tokens were written into the cache (pa_kv_append and the calls
+ * that append): for sequence s, every block that holds one of its tokens start_pos[s] ..
+ * start_pos[s] + num_new[s] - 1 gets the bounds of the keys that it holds up to the last of them, read from
+ * the cache. max_new_per_seq: host-side upper bound of num_new (tokens beyond it are not looked at).
+ * Sequences with start_pos < 0 or num_new <= 0, table entries outside [0, num_blocks) and positions beyond
+ * max_blocks_per_seq * 16 are skipped. A NaN key makes its channel's bounds NaN. Two sequences of one call
+ * that name the same block must hold the same tokens in it. num_seqs at most 65535; k_cache and key_bounds
+ * 16-byte aligned. */
+pa_status pa_key_bounds_update(pa_stream* stream, const pa_config* cfg, const void* k_cache,
+                               const int32_t* block_tables, int32_t max_blocks_per_seq,
+                               const int32_t* start_pos, const int32_t* num_new, int32_t num_seqs,
+                               int32_t max_new_per_seq, void* key_bounds);
+
+/* Bytes of workspace of pa_select_blocks (8 per query, KV head and block; 8-byte aligned). */
+pa_status pa_select_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t max_context_len, size_t* bytes);
+/* The blocks each query attends to, for each KV head:
+ *   selected: [num_queries][num_kv_heads][budget] int32, logical block indices in ascending order, -1
+ *   behind the last. A context of at most `budget` blocks is selected whole. Otherwise the first
+ *   sink_blocks and the last recent_blocks are, and the rest of the budget goes to the blocks with the
+ *   largest scores
+ *     sum_d (sum_g max(q_gd, 0)) hi_bd + (sum_g min(q_gd, 0)) lo_bd       (g: the heads of the group)
+ *   (times k_scale for int8 caches), an upper bound of sum_g max_t q_g . k_t; equal scores go to the
+ *   lowest index, a score that is NaN comes first. Scores are summed in 64 bits. Blocks whose table entry
+ *   lies outside [0, num_blocks) score 0. The bounds of the sink and recent blocks do not matter
+ *   (they need not be up to date while they are among the recent ones).
+ *   q: [num_queries][num_q_heads][head_dim] of q_dtype; recent_blocks >= 1 (the block of the newest
+ *   token), sink_blocks + recent_blocks <= budget, max_context_len <= 2097152. */
+pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* q, const void* key_bounds,
+                           const float* k_scale, const int32_t* block_tables, int32_t num_seqs,
+                           int32_t max_blocks_per_seq, const int32_t* query_seqs, const int32_t* context_lens,
+                           int32_t num_queries, int32_t max_context_len, int32_t sink_blocks,
+                           int32_t recent_blocks, int32_t budget, int32_t* selected, void* workspace,
+                           size_t workspace_bytes);
+
+/* Bytes of workspace of pa_sparse_decode (partial results of rows that are split; 0 when none is; 4-byte
+ * aligned). */
+pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t budget, size_t* bytes);
+/* pa_paged_decode over the listed blocks only: query r's heads of KV head h attend to the tokens
+ * (those before context_lens[r]) of the logical blocks selected[r][h][0 .. budget).
+ *   out: [num_queries][num_q_heads][head_dim] fp32
+ * Lists come from pa_select_blocks or from the caller: entries that are negative or at or past the end
+ * of the context are skipped wherever they stand, in any order; a block listed twice counts twice.
+ * Blocks whose table entry lies outside [0, num_blocks) read as zero keys and values. A query without
+ * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter. Products are
+ * exact and sums in fp32 for every cache and query type. num_q_heads / num_kv_heads: 1, 2, 4, 8 or
+ * 16. Caches 16-byte aligned. */
+pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, const void* q,
+                           const void* k_cache, const void* v_cache, const float* k_scale,
+                           const float* v_scale, const int32_t* block_tables, int32_t num_seqs,
+                           int32_t max_blocks_per_seq, const int32_t* query_seqs, const int32_t* context_lens,
+                           int32_t num_queries, int32_t max_context_len, const int32_t* selected,
+                           int32_t budget, void* workspace, size_t workspace_bytes);
+
+/* ---- the books of the pool on the device ----
+ * Which blocks a sequence holds and how many hold a block, changed by kernels in stream order, so that a
+ * step that forks, frees or extends sequences needs no word from the host and may be captured into a graph
+ * (the reference keeps these books on the host: BlockShareManager.cs:34-105, KVCacheBlockManager.cs:
+ * 70-174). The caller owns the arrays:
+ *   refcounts    [num_blocks] int32: rows (and other owners, such as a prefix cache) that hold the block;
+ *                0: free
+ *   block tables [rows][max_blocks_per_seq] int32: a row holds its entries in [0, num_blocks); every other
+ *                entry must be negative (-1), those behind its last block too
+ * Results depend on the books alone, never on timing. Calls on one set of books must not overlap. */
+
+/* New rows from old ones: out row i is a copy of in row src[i] (table and length), or empty (length 0,
+ * every entry -1) when src[i] is outside [0, num_in). Every in row gives up its blocks and every out
+ * row takes hold of its own, so this forks (a row named twice), frees (a row not named) and reorders
+ * sequences or beams in one call. refcounts change in place; the out arrays must not overlap the in
+ * arrays. Blocks whose count falls to 0 are free. */
+pa_status pa_pages_fork(pa_stream* stream, const pa_config* cfg, const int32_t* tables_in, const int32_t* lens_in,
+                        int32_t num_in, const int32_t* src, int32_t* tables_out, int32_t* lens_out,
+                        int32_t num_out, int32_t max_blocks_per_seq, int32_t* refcounts);
+
+/* Bytes of workspace of pa_pages_reserve and pa_pages_compact (4-byte aligned). */
+pa_status pa_pages_workspace_size(const pa_config* cfg, int32_t num_rows, int32_t max_blocks_per_seq, size_t* bytes);
+
+/* Makes room for num_new[i] more tokens of row i at positions lens[i] .. (lens itself is the caller's to
+ * advance): every block of theirs that the row does not hold is taken from the free ones, and every one
+ * that others hold too is replaced by a free one (copy on write). Rows are worked off in order, the
+ * lowest free block first; when every holder of a shared block asks for it in this call, the last of them
+ * keeps it. copy_pairs [num_rows][2]: (old, new) where the replaced block holds tokens of the row, else
+ * (-1, -1); copy them with pa_copy_pages (or pa_copy_blocks) before the new tokens are written.
+ * status [2] (device): the blocks taken, and 0; or, when there are too few free blocks, 0 and how many are
+ * missing, with nothing else changed. max_new_per_row: host-side upper bound of num_new (blocks beyond
+ * it are not looked at). Positions beyond max_blocks_per_seq * 16 get no block; rows with num_new <= 0 or
+ * a negative length ask for none. Then advance lens, append (pa_build_slot_mapping, pa_kv_append) and bring the key bounds up to
+ * date. */
+pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tables, const int32_t* lens,
+                           const int32_t* num_new, int32_t num_rows, int32_t max_blocks_per_seq,
+                           int32_t max_new_per_row, int32_t* refcounts, int32_t* copy_pairs, int32_t* status,
+                           void* workspace, size_t workspace_bytes);
+
+/* Moves the highest live blocks into the lowest free ones while that lowers them, at most max_moves:
+ * pairs [max_moves][2] gets (from, to), (-1, -1) behind the last; refcounts move along and the tables'
+ * entries are renamed (other owners rename theirs by the pairs). status [2] (device): the moves, and the
+ * number of blocks from 0 on that contain every live one afterwards (the pool above it may be given
+ * back). Copy the data of every layer with pa_copy_pages(pairs, max_moves, status) before the blocks are
+ * read or reserved. */
+pa_status pa_pages_compact(pa_stream* stream, const pa_config* cfg, int32_t* tables, int32_t num_rows,
+                           int32_t max_blocks_per_seq, int32_t* refcounts, int32_t max_moves, int32_t* pairs,
+                           int32_t* status, void* workspace, size_t workspace_bytes);
+
+/* pa_copy_blocks for pairs whose number is on the device, with the key bounds: the first
+ * min(*num_pairs, max_pairs) pairs (num_pairs null: max_pairs) are copied, K, V, int8 statistics and, unless
+ * null, key_bounds. Pairs with an id outside [0, num_blocks) or src == dst are skipped. Within one call no
+ * block may be written twice, nor be both a source and a destination. */
+pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, void* v_cache,
+                        float* k_scale, float* v_scale, float* k_absmax, float* v_absmax, void* key_bounds,
+                        const int32_t* pairs, int32_t max_pairs, const int32_t* num_pairs);
+
 /* ---- the projections either side of attention (PagedAttentionLayer.ComputeAttention's
  *      _queryProj/_keyProj/_valueProj.Forward + UpdateKVCache and _outputProj.Forward,
  *      Layers/PagedAttentionLayer.cs:112-142; Linear.Forward y = x W^T without bias,

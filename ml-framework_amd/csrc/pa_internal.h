@@ -42,6 +42,21 @@ pa_status clear_error();
 // Stream handed to a launch (null pa_stream -> legacy default stream).
 inline hipStream_t native(const pa_stream* s) { return s ? s->stream : nullptr; }
 
+// Makes the stream's device current while a launch function runs (a null stream: the current one).
+struct StreamDevice {
+    int prev = -1;
+    explicit StreamDevice(const pa_stream* s) {
+        int cur = -1;
+        if (s && hipGetDevice(&cur) == hipSuccess && cur != s->ordinal && hipSetDevice(s->ordinal) == hipSuccess)
+            prev = cur;
+    }
+    ~StreamDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    StreamDevice(const StreamDevice&) = delete;
+    StreamDevice& operator=(const StreamDevice&) = delete;
+};
+
 // Fixed block size of every compiled kernel.
 constexpr int kBlockSize = 16;
 
@@ -69,6 +84,14 @@ inline float resolve_scale(const pa_config* cfg) {
     return cfg->scale > 0.0f ? cfg->scale : 1.0f / sqrtf(static_cast<float>(cfg->head_dim));
 }
 
+}  // namespace pa
+
+namespace pa {
+// Bytes of one cache element.
+inline int32_t kv_bytes(const pa_config* cfg) {
+    return cfg->kv_dtype == PA_DTYPE_FP32 ? 4 : cfg->kv_dtype == PA_DTYPE_BF16 ? 2 : 1;
+}
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 }  // namespace pa
 
 #define PA_HIP_CHECK(expr)                                            \

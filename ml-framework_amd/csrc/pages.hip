@@ -1,0 +1,514 @@
+// pages.hip -- the books of a paged cache kept on the device: which row of the block tables holds
+// which physical blocks, how many rows hold each (refcounts), forking and freeing of rows, blocks for new
+// tokens with copy on write, compaction of the pool, and the copies these ask for.
+//
+// The reference keeps these books on the host: refcounts in BlockShareManager (src/MLFramework/
+// Inference/PagedAttention/Sharing/BlockShareManager.cs:34-105), the free list in
+// KVCacheBlockManager (KVCacheBlockManager.cs:70-174). A row holds the entries of its whole width that
+// lie in [0, num_blocks); every other entry is empty. A block is free when its refcount is 0.
+//
+// All of it is whole numbers. Refcounts change by integer atomics, whose sums do not depend on their
+// order; places in a list come from prefix counts in row order, never from an atomic counter, so the
+// same books give the same result every time.
+#include <algorithm>
+#include <string>
+
+#include "pa_internal.h"
+
+namespace {
+
+constexpr int kForkThreads = 256;
+constexpr int kBookThreads = 1024;
+constexpr int kCopyThreads = 256;
+
+// ---- fork --------------------------------------------------------------------------------------
+// Workgroups 0 .. num_out - 1 write an out row each; the num_in behind them settle the refcounts of an in
+// row: its blocks are held by as many rows as the out rows that name it, instead of by one.
+__global__ __launch_bounds__(kForkThreads) void pages_fork_kernel(const int32_t* __restrict__ tables_in,
+                                                                 const int32_t* __restrict__ lens_in, int32_t num_in,
+                                                                 const int32_t* __restrict__ src, int32_t* __restrict__ tables_out,
+                                                                 int32_t* __restrict__ lens_out, int32_t num_out,
+                                                                 int32_t width, int32_t* __restrict__ refs, int32_t num_blocks) {
+    const int tid = threadIdx.x;
+    if (static_cast<int>(blockIdx.x) < num_out) {
+        const int i = blockIdx.x;
+        const int from = src[i];
+        const bool some = from >= 0 && from < num_in;
+        const int32_t* in = tables_in + static_cast<int64_t>(some ? from : 0) * width;
+        int32_t* out = tables_out + static_cast<int64_t>(i) * width;
+        for (int j = tid; j < width; j += kForkThreads) out[j] = some ? in[j] : -1;
+        if (tid == 0) lens_out[i] = some ? lens_in[from] : 0;
+        return;
+    }
+    const int i = blockIdx.x - num_out;
+    int uses = 0;
+    for (int j = tid; j < num_out; j += kForkThreads) uses += src[j] == i;
+    __shared__ int s_uses[kForkThreads / 64];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) uses += __shfl_xor(uses, o, 64);
+    if ((tid & 63) == 0) s_uses[tid >> 6] = uses;
+    __syncthreads();
+    uses = 0;
+#pragma unroll
+    for (int w = 0; w < kForkThreads / 64; w++) uses += s_uses[w];
+    if (uses == 1) return;
+    const int32_t* in = tables_in + static_cast<int64_t>(i) * width;
+    for (int j = tid; j < width; j += kForkThreads) {
+        const int id = in[j];
+        if (id >= 0 && id < num_blocks) atomicAdd(refs + id, uses - 1);
+    }
+}
+
+// ---- helpers of the one-workgroup kernels --------------------------------------------------------
+// Exclusive prefix of `mine` over the workgroup, and the total.
+__device__ __forceinline__ int block_prefix(int mine, int* s_wave, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += v;
+    }
+    __syncthreads();  // the previous call's sums have been read
+    if (lane == 63) s_wave[wave] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kBookThreads / 64; w++) {
+        const int v = s_wave[w];
+        before += w < wave ? v : 0;
+        total += v;
+    }
+    return before + incl - mine;
+}
+__device__ __forceinline__ int load_now(const int32_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void store_now(int32_t* p, int v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The workgroup's global writes before it are seen by its reads behind it.
+__device__ __forceinline__ void block_sync_global() {
+    __threadfence();
+    __syncthreads();
+}
+
+// ---- reserve -----------------------------------------------------------------------------------
+struct ReserveArgs {
+    int32_t* tables;
+    const int32_t* lens;
+    const int32_t* num_new;
+    int32_t* refs;
+    int32_t* pairs;   // [rows][2]
+    int32_t* status;  // [2]
+    int32_t* count;   // [num_blocks] scratch: demands of a shared block in this call
+    int32_t* last;    // [num_blocks] scratch: the last of them
+    int32_t* fresh;   // [demands] scratch: the blocks given out, in order
+    int32_t* want;    // [demands] scratch: the demand of each place
+    int32_t rows, width, num_blocks, reach;
+};
+
+// Demand e = row * reach + j: the j-th block that the row's new tokens go to. Its table entry, or
+// null when the row has no such block.
+__device__ __forceinline__ int32_t* demand_entry(const ReserveArgs& a, int64_t e, int& row, int& lb) {
+    row = static_cast<int>(e / a.reach);
+    const int j = static_cast<int>(e - static_cast<int64_t>(row) * a.reach);
+    const int len = a.lens[row], n = a.num_new[row];
+    if (len < 0 || n <= 0) return nullptr;
+    lb = len / 16 + j;
+    if (static_cast<int64_t>(lb) * 16 >= static_cast<int64_t>(len) + n || lb >= a.width) return nullptr;
+    return a.tables + static_cast<int64_t>(row) * a.width + lb;
+}
+
+// In row order, a block a demand: an empty entry takes the lowest free block; an entry that other rows
+// hold too takes one in its place (copy on write), except for the last of the rows that hold it when all
+// of them ask in this call: it keeps the block, as it would if the rows were worked off one by one.
+__global__ __launch_bounds__(kBookThreads) void pages_reserve_kernel(const ReserveArgs a) {
+    __shared__ int s_wave[kBookThreads / 64];
+    const int tid = threadIdx.x;
+    const int64_t demands = static_cast<int64_t>(a.rows) * a.reach;
+    for (int64_t i = tid; i < 2 * static_cast<int64_t>(a.rows); i += kBookThreads) a.pairs[i] = -1;
+    for (int64_t e = tid; e < demands; e += kBookThreads) {
+        int row, lb;
+        const int32_t* p = demand_entry(a, e, row, lb);
+        const int id = p ? *p : -1;
+        if (id >= 0 && id < a.num_blocks && a.refs[id] > 1) {
+            store_now(a.count + id, 0);
+            store_now(a.last + id, -1);
+        }
+    }
+    block_sync_global();
+    for (int64_t e = tid; e < demands; e += kBookThreads) {
+        int row, lb;
+        const int32_t* p = demand_entry(a, e, row, lb);
+        const int id = p ? *p : -1;
+        if (id >= 0 && id < a.num_blocks && a.refs[id] > 1) {
+            atomicAdd(a.count + id, 1);
+            atomicMax(a.last + id, static_cast<int>(e));
+        }
+    }
+    block_sync_global();
+    int need = 0;
+    for (int64_t e0 = 0; e0 < demands; e0 += kBookThreads) {
+        const int64_t e = e0 + tid;
+        bool takes = false;
+        if (e < demands) {
+            int row, lb;
+            const int32_t* p = demand_entry(a, e, row, lb);
+            if (p) {
+                const int id = *p;
+                if (id < 0 || id >= a.num_blocks) {
+                    takes = true;
+                } else if (a.refs[id] > 1) {
+                    takes = !(load_now(a.count + id) == a.refs[id] && load_now(a.last + id) == static_cast<int>(e));
+                }
+            }
+        }
+        int total;
+        const int at = need + block_prefix(takes, s_wave, total);
+        if (takes) store_now(a.want + at, static_cast<int>(e));
+        need += total;
+    }
+    // the lowest free blocks
+    int found = 0;
+    for (int64_t b0 = 0; b0 < a.num_blocks && found < need; b0 += kBookThreads) {
+        const int64_t b = b0 + tid;
+        const bool is_free = b < a.num_blocks && a.refs[b] <= 0;
+        int total;
+        const int at = found + block_prefix(is_free, s_wave, total);
+        if (is_free && at < need) store_now(a.fresh + at, static_cast<int>(b));
+        found += total;
+    }
+    if (tid == 0) {
+        a.status[0] = found >= need ? need : 0;
+        a.status[1] = found >= need ? 0 : need - found;
+    }
+    if (found < need) return;
+    block_sync_global();
+    for (int i = tid; i < need; i += kBookThreads) {
+        const int e = load_now(a.want + i), b = load_now(a.fresh + i);
+        int row, lb;
+        int32_t* p = demand_entry(a, e, row, lb);
+        const int old = *p;
+        if (old >= 0 && old < a.num_blocks) {
+            atomicSub(a.refs + old, 1);
+            if (static_cast<int64_t>(lb) * 16 < a.lens[row]) {  // it holds tokens of the row
+                a.pairs[2 * static_cast<int64_t>(row)] = old;
+                a.pairs[2 * static_cast<int64_t>(row) + 1] = b;
+            }
+        }
+        *p = b;
+        a.refs[b] = 1;
+    }
+}
+
+// ---- compaction --------------------------------------------------------------------------------
+struct CompactArgs {
+    int32_t* tables;
+    int32_t* refs;
+    int32_t* pairs;   // [max_moves][2]
+    int32_t* status;  // [2]
+    int32_t* rank;    // [num_blocks] scratch: the place of a moved block in the list
+    int32_t* from;    // [num_blocks] scratch
+    int32_t* to;      // [num_blocks] scratch
+    int32_t* counts;  // [2] scratch: moves, the lowest moved block
+    int32_t num_blocks, max_moves;
+    int64_t entries;  // table entries
+};
+
+// The i-th highest live block goes to the i-th lowest free one while that is lower, at most max_moves.
+// With L live blocks in all, those are the live blocks at or above L and the free ones below it.
+__global__ __launch_bounds__(kBookThreads) void pages_compact_kernel(const CompactArgs a) {
+    __shared__ int s_wave[kBookThreads / 64];
+    const int tid = threadIdx.x;
+    int live = 0;
+    for (int64_t b0 = 0; b0 < a.num_blocks; b0 += kBookThreads) {
+        const int64_t b = b0 + tid;
+        int total;
+        block_prefix(b < a.num_blocks && a.refs[b] > 0, s_wave, total);
+        live += total;
+    }
+    int before = 0, low = 0;  // live blocks below the slab; live blocks below `live`
+    for (int64_t b0 = 0; b0 < a.num_blocks; b0 += kBookThreads) {
+        const int64_t b = b0 + tid;
+        const bool is_live = b < a.num_blocks && a.refs[b] > 0;
+        int total;
+        const int lb = before + block_prefix(is_live, s_wave, total);  // live blocks below b
+        if (b < a.num_blocks) {
+            if (is_live && b >= live) {
+                store_now(a.from + (live - 1 - lb), static_cast<int>(b));
+                store_now(a.rank + b, live - 1 - lb);
+            } else if (!is_live && b < live) {
+                store_now(a.to + (b - lb), static_cast<int>(b));
+            }
+        }
+        int in;
+        block_prefix(is_live && b < live, s_wave, in);
+        low += in;
+        before += total;
+    }
+    const int full = live - low, n = min(full, a.max_moves);
+    block_sync_global();
+    if (tid == 0) {
+        a.status[0] = n;
+        a.status[1] = n == full ? live : load_now(a.from + n) + 1;
+        a.counts[0] = n;
+        a.counts[1] = n > 0 ? load_now(a.from + n - 1) : a.num_blocks;
+    }
+    for (int64_t i = tid; i < a.max_moves; i += kBookThreads) {
+        const int s = i < n ? load_now(a.from + i) : -1, d = i < n ? load_now(a.to + i) : -1;
+        a.pairs[2 * i] = s;
+        a.pairs[2 * i + 1] = d;
+        if (i < n) {
+            a.refs[d] = a.refs[s];
+            a.refs[s] = 0;
+        }
+    }
+}
+
+// Table entries of moved blocks take the new names.
+__global__ __launch_bounds__(256) void pages_rename_kernel(const CompactArgs a) {
+    const int n = a.counts[0], lowest = a.counts[1];
+    if (n == 0) return;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < a.entries; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int id = a.tables[i];
+        if (id < lowest || id >= a.num_blocks) continue;
+        const int k = a.rank[id];  // written for every moved block; anything for an id that was not live
+        if (k >= 0 && k < n && a.from[k] == id) a.tables[i] = a.to[k];
+    }
+}
+
+// ---- copies ------------------------------------------------------------------------------------
+struct CopyArgs {
+    char* k;
+    char* v;
+    char* bounds;    // null: none
+    float* stat[4];  // k_scale, v_scale, k_absmax, v_absmax (int8)
+    const int32_t* pairs;
+    const int32_t* num_pairs;  // null: max_pairs
+    int64_t part;              // bytes of K (of V) per block
+    int64_t bound;             // bytes of the key bounds per block
+    int32_t max_pairs, pieces, num_blocks, hkv;
+    bool int8;
+};
+constexpr int kPieceBytes = 8192;  // two 16-byte words a lane
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Piece u % pieces of pair u / pieces: K in pieces of 8 KB, V likewise, then the key bounds, then the statistics.
+__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(const CopyArgs c) {
+    const int n = c.num_pairs ? max(0, min(*c.num_pairs, c.max_pairs)) : c.max_pairs;
+    const int64_t units = static_cast<int64_t>(n) * c.pieces;
+    const int kp = static_cast<int>((c.part + kPieceBytes - 1) / kPieceBytes);
+    const int bp = static_cast<int>((c.bound + kPieceBytes - 1) / kPieceBytes);
+    const int tid = threadIdx.x;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t i = u / c.pieces;
+        int piece = static_cast<int>(u - i * c.pieces);
+        const int32_t src = c.pairs[2 * i], dst = c.pairs[2 * i + 1];
+        if (src < 0 || src >= c.num_blocks || dst < 0 || dst >= c.num_blocks || src == dst) continue;
+        char* base = c.k;
+        int64_t len = c.part;
+        if (piece >= kp) {
+            piece -= kp;
+            base = c.v;
+            if (piece >= kp) {
+                piece -= kp;
+                base = c.bounds;
+                len = c.bound;
+                if (piece >= bp) {  // the statistics
+                    for (int k = tid; k < 4 * c.hkv; k += kCopyThreads) {
+                        float* s = c.stat[k / c.hkv];
+                        const int h = k % c.hkv;
+                        s[static_cast<int64_t>(dst) * c.hkv + h] = s[static_cast<int64_t>(src) * c.hkv + h];
+                    }
+                    continue;
+                }
+            }
+        }
+        const int64_t off = static_cast<int64_t>(piece) * kPieceBytes + tid * 16;
+        const u32x4* from = reinterpret_cast<const u32x4*>(base + src * len + off);
+        u32x4* to = reinterpret_cast<u32x4*>(base + dst * len + off);
+        const bool a = off < len, b = off + kPieceBytes / 2 < len;
+        u32x4 x{}, y{};
+        if (a) x = __builtin_nontemporal_load(from);
+        if (b) y = __builtin_nontemporal_load(from + kPieceBytes / 32);
+        if (a) __builtin_nontemporal_store(x, to);
+        if (b) __builtin_nontemporal_store(y, to + kPieceBytes / 32);
+    }
+}
+
+// Scratch of reserve (four lists) and compact (three lists and two counts), ints.
+int64_t scratch_ints(const pa_config* cfg, int32_t num_rows, int32_t width) {
+    const int64_t nb = cfg->num_blocks, demands = static_cast<int64_t>(num_rows) * width;
+    return std::max(2 * nb + 2 * demands, 3 * nb + 2);
+}
+
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+    const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
+    return x < y + nb && y < x + na;
+}
+
+}  // namespace
+
+extern "C" {
+
+pa_status pa_pages_workspace_size(const pa_config* cfg, int32_t num_rows, int32_t max_blocks_per_seq, size_t* bytes) {
+    const std::string f = "pa_pages_workspace_size";
+    pa_status st = pa::check_config(cfg, f.c_str());
+    if (st != PA_SUCCESS) return st;
+    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": bytes is null");
+    if (num_rows < 0 || max_blocks_per_seq < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    *bytes = static_cast<size_t>(scratch_ints(cfg, num_rows, max_blocks_per_seq)) * 4;
+    return pa::clear_error();
+}
+
+pa_status pa_pages_fork(pa_stream* stream, const pa_config* cfg, const int32_t* tables_in, const int32_t* lens_in,
+                        int32_t num_in, const int32_t* src, int32_t* tables_out, int32_t* lens_out, int32_t num_out,
+                        int32_t max_blocks_per_seq, int32_t* refcounts) {
+    const std::string f = "pa_pages_fork";
+    pa_status st = pa::check_config(cfg, f.c_str());
+    if (st != PA_SUCCESS) return st;
+    if (num_in < 0 || num_out < 0 || max_blocks_per_seq < 0)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (static_cast<int64_t>(num_in) + num_out == 0) return pa::clear_error();
+    if (static_cast<int64_t>(num_in) + num_out > INT32_MAX)
+        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many rows for one call");
+    if (!refcounts || (num_in > 0 && (!tables_in || !lens_in)) || (num_out > 0 && (!src || !tables_out || !lens_out)))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+    const int64_t row = static_cast<int64_t>(max_blocks_per_seq) * 4;
+    if (num_in > 0 && num_out > 0 &&
+        (overlap(tables_in, num_in * row, tables_out, num_out * row) || overlap(lens_in, num_in * 4ll, lens_out, num_out * 4ll) ||
+         overlap(src, num_out * 4ll, lens_out, num_out * 4ll) || overlap(src, num_out * 4ll, tables_out, num_out * row)))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": the out rows must not overlap the inputs");
+    pa::StreamDevice dev(stream);
+    pages_fork_kernel<<<num_out + num_in, kForkThreads, 0, pa::native(stream)>>>(
+        tables_in, lens_in, num_in, src, tables_out, lens_out, num_out, max_blocks_per_seq, refcounts, cfg->num_blocks);
+    PA_HIP_CHECK(hipGetLastError());
+    return pa::clear_error();
+}
+
+pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tables, const int32_t* lens,
+                           const int32_t* num_new, int32_t num_rows, int32_t max_blocks_per_seq,
+                           int32_t max_new_per_row, int32_t* refcounts, int32_t* copy_pairs, int32_t* status,
+                           void* workspace, size_t workspace_bytes) {
+    const std::string f = "pa_pages_reserve";
+    pa_status st = pa::check_config(cfg, f.c_str());
+    if (st != PA_SUCCESS) return st;
+    if (num_rows < 0 || max_blocks_per_seq < 0 || max_new_per_row < 0)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (!status) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": status is null");
+    if (num_rows > 0 && (!tables || !lens || !num_new || !refcounts || !copy_pairs))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+    // Blocks that one row's new tokens can touch.
+    const int64_t reach = std::min<int64_t>(max_new_per_row == 0 ? 0 : (static_cast<int64_t>(max_new_per_row) + 14) / 16 + 1,
+                                            max_blocks_per_seq);
+    if (reach * num_rows > INT32_MAX) return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many rows for one call");
+    const size_t need = static_cast<size_t>(scratch_ints(cfg, num_rows, max_blocks_per_seq)) * 4;
+    if (need > workspace_bytes || (need > 0 && !workspace))
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(workspace) & 3)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 4-byte aligned");
+    ReserveArgs a{};
+    a.tables = tables;
+    a.lens = lens;
+    a.num_new = num_new;
+    a.refs = refcounts;
+    a.pairs = copy_pairs;
+    a.status = status;
+    a.count = static_cast<int32_t*>(workspace);
+    a.last = a.count + cfg->num_blocks;
+    a.fresh = a.last + cfg->num_blocks;
+    a.want = a.fresh + static_cast<int64_t>(num_rows) * max_blocks_per_seq;
+    a.rows = num_rows;
+    a.width = max_blocks_per_seq;
+    a.num_blocks = cfg->num_blocks;
+    a.reach = static_cast<int32_t>(reach);
+    pa::StreamDevice dev(stream);
+    pages_reserve_kernel<<<1, kBookThreads, 0, pa::native(stream)>>>(a);
+    PA_HIP_CHECK(hipGetLastError());
+    return pa::clear_error();
+}
+
+pa_status pa_pages_compact(pa_stream* stream, const pa_config* cfg, int32_t* tables, int32_t num_rows,
+                           int32_t max_blocks_per_seq, int32_t* refcounts, int32_t max_moves, int32_t* pairs,
+                           int32_t* status, void* workspace, size_t workspace_bytes) {
+    const std::string f = "pa_pages_compact";
+    pa_status st = pa::check_config(cfg, f.c_str());
+    if (st != PA_SUCCESS) return st;
+    if (num_rows < 0 || max_blocks_per_seq < 0 || max_moves < 0)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (!status || (cfg->num_blocks > 0 && !refcounts) || (max_moves > 0 && !pairs) ||
+        (num_rows > 0 && max_blocks_per_seq > 0 && !tables))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+    const size_t need = static_cast<size_t>(scratch_ints(cfg, num_rows, max_blocks_per_seq)) * 4;
+    if (need > workspace_bytes || !workspace)
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(workspace) & 3)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 4-byte aligned");
+    CompactArgs a{};
+    a.tables = tables;
+    a.refs = refcounts;
+    a.pairs = pairs;
+    a.status = status;
+    a.rank = static_cast<int32_t*>(workspace);
+    a.from = a.rank + cfg->num_blocks;
+    a.to = a.from + cfg->num_blocks;
+    a.counts = a.to + cfg->num_blocks;
+    a.num_blocks = cfg->num_blocks;
+    a.max_moves = max_moves;
+    a.entries = static_cast<int64_t>(num_rows) * max_blocks_per_seq;
+    pa::StreamDevice dev(stream);
+    hipStream_t s = pa::native(stream);
+    pages_compact_kernel<<<1, kBookThreads, 0, s>>>(a);
+    PA_HIP_CHECK(hipGetLastError());
+    if (a.entries > 0) {
+        pages_rename_kernel<<<static_cast<uint32_t>(std::min<int64_t>((a.entries + 255) / 256, 1024)), 256, 0, s>>>(a);
+        PA_HIP_CHECK(hipGetLastError());
+    }
+    return pa::clear_error();
+}
+
+pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, void* v_cache, float* k_scale,
+                        float* v_scale, float* k_absmax, float* v_absmax, void* key_bounds, const int32_t* pairs,
+                        int32_t max_pairs, const int32_t* num_pairs) {
+    const std::string f = "pa_copy_pages";
+    pa_status st = pa::check_config(cfg, f.c_str());
+    if (st != PA_SUCCESS) return st;
+    if (max_pairs < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": max_pairs < 0");
+    if (!k_cache || !v_cache) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null cache pointer");
+    if (!pa::aligned16(k_cache) || !pa::aligned16(v_cache) || !pa::aligned16(key_bounds))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": cache and key_bounds pointers must be 16-byte aligned");
+    const bool int8 = cfg->kv_dtype == PA_DTYPE_INT8;
+    if (int8 && (!k_scale || !v_scale || !k_absmax || !v_absmax))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": int8 cache needs scales and absmax");
+    if (max_pairs == 0) return pa::clear_error();
+    if (!pairs) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": pairs is null");
+    CopyArgs c{};
+    c.k = static_cast<char*>(k_cache);
+    c.v = static_cast<char*>(v_cache);
+    c.bounds = static_cast<char*>(key_bounds);
+    c.stat[0] = k_scale;
+    c.stat[1] = v_scale;
+    c.stat[2] = k_absmax;
+    c.stat[3] = v_absmax;
+    c.pairs = pairs;
+    c.num_pairs = num_pairs;
+    const int64_t head = static_cast<int64_t>(cfg->num_kv_heads) * cfg->head_dim * pa::kv_bytes(cfg);
+    c.part = head * pa::kBlockSize;
+    c.bound = key_bounds ? head * 2 : 0;
+    c.max_pairs = max_pairs;
+    c.pieces = static_cast<int32_t>(2 * ((c.part + kPieceBytes - 1) / kPieceBytes) +
+                                    (c.bound + kPieceBytes - 1) / kPieceBytes) + (int8 ? 1 : 0);
+    c.num_blocks = cfg->num_blocks;
+    c.hkv = cfg->num_kv_heads;
+    c.int8 = int8;
+    pa::StreamDevice dev(stream);
+    const int64_t units = static_cast<int64_t>(max_pairs) * c.pieces;
+    copy_pages_kernel<<<static_cast<uint32_t>(std::min<int64_t>(units, 2048)), kCopyThreads, 0, pa::native(stream)>>>(c);
+    PA_HIP_CHECK(hipGetLastError());
+    return pa::clear_error();
+}
+
+}  // extern "C"

@@ -1,0 +1,433 @@
+// sparse_decode.h -- attention of single query tokens over the blocks selected for each KV head.
+//
+// For query token r, KV head h, query head g of its group, over the tokens t of the listed blocks:
+//   s_t = scale * q_g . k_t,  out_g = sum_t exp(s_t - max s) v_t / sum_t exp(s_t - max s)
+//
+// The lists differ by KV head, so the unit of work is a row (query token, KV head), cut into `parts`
+// runs of its list, one workgroup each. Its waves take the listed blocks in turn (wave w: entries w, w +
+// kWaves, ..); a wave streams its blocks through rotating register buffers, one pass with the running maximum
+// and sum, and no wave waits for another until the part ends. There the waves' states meet in LDS; a
+// row of one part is finished at once, the parts of the others by a merge launch.
+//
+// K and V are read once and G = Hq / Hkv query heads share them (2 G flops a byte at bf16): traffic
+// bounds it. The matrix instructions are 16 columns wide and G is 1 to 16, so the columns that a
+// group leaves idle carry precision instead: an fp32 value is exactly the sum of three bf16 parts (8
+// bits each, cut off one after the other), and part p of head g sits in column g + G p. An fp32
+// query's three partial scores are summed across columns; P's three parts make three rows of O, which
+// are summed when the row ends. Every product is then exact and every sum in fp32, at the
+// instruction count of a single bf16 product for G <= 4 (two passes for G = 8, three for 16). fp32 caches
+// run on fp32 matrix instructions.
+#pragma once
+
+#include "decode_mfma.h"
+
+namespace pa {
+
+struct SparseArgs {
+    DecodeArgs d;  // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [rows][parts][G]
+    const int32_t* query_seqs;  // null: query r belongs to sequence r
+    const int32_t* selected;    // [num_queries][Hkv][budget]
+    int32_t num_seqs, num_queries, budget;
+    int32_t parts, per;         // parts per row, list entries per part
+};
+
+constexpr int kSparseWaves = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+// Rescaling is deferred until the maximum grows by this (log2 units): P stays below 2^11.
+constexpr float kSparseRescale = 11.0f;
+
+// x += the value a rotation by O lanes within each row of 16.
+template <int O>
+__device__ __forceinline__ float add_ror(float x) {
+    return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + O, 0xF, 0xF, false));
+}
+
+// Parts 0, 1, 2 of an fp32 value: its top 8 bits, the next 8, the rest; each exact in bf16.
+__device__ __forceinline__ float bf16_part(float x, int part) {
+    const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    const float r = x - hi;
+    const float mid = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+    return part == 0 ? hi : part == 1 ? mid : r - mid;
+}
+
+// K and V registers of one block, by cache type.
+template <int D, int KV>
+struct SparseBuf {
+    typename MfmaRaw<KV>::K k[D / 32];
+    typename MfmaRaw<KV>::V v[D / 16];
+};
+template <int D>
+struct SparseBuf<D, PA_DTYPE_FP32> {
+    f32x4_t k[D / 16];  // lane (q4, n): row n, dims 16 u + 4 q4 ..
+    f32x4_t v[D / 16];  // dim 16 t + n, tokens 4 q4 ..
+};
+
+// Loads of block bid of KV head kv; bid < 0 reads nothing and gives zeros.
+template <int D, int KV>
+__device__ __forceinline__ void sparse_load(const DecodeArgs& a, SparseBuf<D, KV>& b, int bid, int kv) {
+    if constexpr (KV != PA_DTYPE_FP32) {
+        load_block<D, KV>(a, b.k, b.v, bid, kv);
+    } else {
+        constexpr int TILE = 16 * D * 4;
+        const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
+        const int64_t tile = bid >= 0 ? (static_cast<int64_t>(bid) * a.num_kv_heads + kv) * TILE : 0;
+        const int bytes = bid >= 0 ? TILE : 0;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(static_cast<const char*>(a.k_cache) + tile), 0, bytes, kBufferFlags);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(static_cast<const char*>(a.v_cache) + tile), 0, bytes, kBufferFlags);
+#pragma unroll
+        for (int u = 0; u < D / 16; u++) b.k[u] = buffer_load<f32x4_t>(rk, n * D * 4 + 64 * u + 16 * q4);
+#pragma unroll
+        for (int t = 0; t < D / 16; t++) b.v[t] = buffer_load<f32x4_t>(rv, (16 * t + n) * 64 + 16 * q4);
+    }
+}
+
+// Register buffers of a wave: the one consumed and those in flight.
+template <int D, int KV>
+__host__ __device__ constexpr int sparse_buffers() {
+    return KV == PA_DTYPE_FP32 ? (D >= 256 ? 1 : D >= 128 ? 2 : 3) : D >= 256 ? (KV == PA_DTYPE_BF16 ? 1 : 2) : 3;
+}
+
+// PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
+template <int D, int KV, bool QF32, int PASSES>
+__global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const SparseArgs a) {
+    constexpr bool F32 = KV == PA_DTYPE_FP32;
+    constexpr int NSLAB = D / 32, NT = D / 16;
+    constexpr int QP = QF32 && !F32 ? PASSES : 1;  // passes of Q
+    constexpr int PP = F32 ? 1 : PASSES;           // passes of P
+    constexpr int NB = sparse_buffers<D, KV>();
+    constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
+    __shared__ float s_m[kSparseWaves][16], s_l[kSparseWaves][16];
+    __shared__ float s_o[kSparseWaves][16][CH];
+    const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int Hkv = a.d.num_kv_heads, G = a.d.group;
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const int r = row / Hkv, kvh = row - r * Hkv;
+    const int seq = a.query_seqs ? a.query_seqs[r] : r;
+    const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, a.d.context_lens[r]) : 0;
+    const int nblk = T <= 0 ? 0 : (T + 15) / 16;
+
+    // Q operand: column n holds head n % G (part n / G of it where Q is split).
+    bf16x8_t qb[F32 ? 1 : QP][F32 ? 1 : NSLAB];
+    float qf[F32 ? D / 4 : 1];
+    {
+        const int64_t q0 = (static_cast<int64_t>(r) * Hkv * G + kvh * G + n % G) * D;
+        if constexpr (F32) {
+#pragma unroll
+            for (int u = 0; u < D / 16; u++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int64_t i = q0 + 16 * u + 4 * q4 + j;
+                    qf[4 * u + j] = QF32 ? static_cast<const float*>(a.d.q)[i]
+                                         : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < NSLAB; s++) {
+                const int64_t i = q0 + k_dim0<D, KV>(s, q4);
+                if constexpr (!QF32) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] = static_cast<const uint16_t*>(a.d.q)[i + 2 * e] |
+                               static_cast<uint32_t>(static_cast<const uint16_t*>(a.d.q)[i + 2 * e + 1]) << 16;
+                    qb[0][s] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+                } else {
+#pragma unroll
+                    for (int p = 0; p < QP; p++) {
+                        const int part_n = PASSES == 1 ? n / G : p * (16 / G) + n / G;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float x0 = bf16_part(static_cast<const float*>(a.d.q)[i + 2 * e], part_n);
+                            const float x1 = bf16_part(static_cast<const float*>(a.d.q)[i + 2 * e + 1], part_n);
+                            w[e] = part_n < 3 ? pack_bf16_trunc(x0, x1) : 0;
+                        }
+                        qb[p][s] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+                    }
+                }
+            }
+        }
+    }
+    const float scale = a.d.scale * kLog2e;
+    float m_run = -INFINITY, l_run = 0.0f;
+    f32x4_t acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    bool any = false;
+
+    const int beg = part * a.per, end = min(beg + a.per, a.budget);
+    const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
+    for (int e0 = beg + wave; e0 < end; e0 += 64 * kSparseWaves) {
+        // lane l: the wave's l-th block of this stretch
+        const int e = e0 + kSparseWaves * lane;
+        const int lb = e < end ? list[e] : -1;
+        const bool listed = lb >= 0 && lb < nblk;
+        int id = -1;
+        if (listed) id = a.d.block_tables[static_cast<int64_t>(seq) * a.d.max_blocks_per_seq + lb];
+        if (id >= a.d.num_blocks) id = -1;
+        float ks = 0.0f, vs = 0.0f;
+        if constexpr (KV == PA_DTYPE_INT8) {
+            if (id >= 0) {
+                ks = a.d.k_scale[static_cast<int64_t>(id) * Hkv + kvh];
+                vs = a.d.v_scale[static_cast<int64_t>(id) * Hkv + kvh];
+            }
+        }
+        uint64_t todo = __ballot(listed);
+        any |= todo != 0;
+        auto next = [&]() {
+            if (!todo) return -1;
+            const int j = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            return j;
+        };
+        SparseBuf<D, KV> buf[NB];
+        int at[NB];
+        auto load = [&](SparseBuf<D, KV>& b, int& j) {
+            j = next();
+            sparse_load<D, KV>(a.d, b, j >= 0 ? __builtin_amdgcn_readlane(id, j) : -1, kvh);
+        };
+        auto compute = [&](SparseBuf<D, KV>& b, int j) {
+            f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (F32) {
+#pragma unroll
+                for (int u = 0; u < D / 16; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.k[u][i], qf[4 * u + i], s, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int sl = 0; sl < NSLAB; sl++) {
+                    const bf16x8_t kop = k_operand(b.k[sl]);
+#pragma unroll
+                    for (int p = 0; p < QP; p++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qb[p][sl], s, 0, 0, 0);
+                }
+            }
+            float f = scale;
+            if constexpr (KV == PA_DTYPE_INT8) f *= readlane_f(ks, j);
+            float sc[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = s[i];
+                if constexpr (QF32 && !F32) {  // the partial scores of a head's parts
+                    if (G <= 8) x = add_ror<8>(x);
+                    if (G <= 4) x = add_ror<4>(x);
+                    if (G <= 2) x = add_ror<2>(x);
+                    if (G <= 1) x = add_ror<1>(x);
+                }
+                sc[i] = x * f;
+            }
+            const int lbj = __builtin_amdgcn_readlane(lb, j);
+            const int t0 = KV == PA_DTYPE_BF16 ? 4 * tok_group<KV>(q4) : 4 * q4;
+            if constexpr (KV == PA_DTYPE_INT8) {
+#pragma unroll
+                for (int u = 0; u < D / 64; u++) int8_v_transpose(b.v[4 * u], b.v[4 * u + 1], b.v[4 * u + 2], b.v[4 * u + 3]);
+            } else if constexpr (KV == PA_DTYPE_BF16) {
+#pragma unroll
+                for (int u = 0; u < D / 32; u++) bf16_v_exchange(b.v[2 * u], b.v[2 * u + 1]);
+            }
+            if (static_cast<int64_t>(lbj) * 16 + 16 > T) {  // the context ends inside the block
+                const int lim = T - lbj * 16 - t0;          // of this lane's four tokens
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[i] = i < lim ? sc[i] : -INFINITY;
+                // their values too: a zero times what an unused slot may hold (Inf, NaN) is not zero
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if constexpr (KV == PA_DTYPE_FP32) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) b.v[t][i] = i < lim ? b.v[t][i] : 0.0f;
+                    } else if constexpr (KV == PA_DTYPE_BF16) {
+                        b.v[t].x = lim >= 2 ? b.v[t].x : lim == 1 ? b.v[t].x & 0xffffu : 0u;
+                        b.v[t].y = lim >= 4 ? b.v[t].y : lim == 3 ? b.v[t].y & 0xffffu : 0u;
+                    }
+                }
+            }
+            const float bm = rows_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+            const bool grow = bm > m_run + kSparseRescale || (m_run == -INFINITY && bm > -INFINITY);
+            if (__any(grow)) {
+                const float m_new = grow ? bm : m_run;
+                const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                l_run *= alpha;
+                m_run = m_new;
+                float ar[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * q4 + i, 64);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] *= ar[i];
+            }
+            const float m0 = m_run == -INFINITY ? 0.0f : m_run;  // no score above -inf yet: P is zero
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                p[i] = __builtin_amdgcn_exp2f(sc[i] - m0);
+                l_run += p[i];
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], b.v[t][i], acc[t], 0, 0, 0);
+            } else {
+                if constexpr (KV == PA_DTYPE_INT8) {
+                    const float vf = readlane_f(vs, j);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[i] *= vf;
+                }
+                s16x4_t pb[PP];
+#pragma unroll
+                for (int q = 0; q < PP; q++) {
+                    const int part_n = PASSES == 1 ? n / G : q * (16 / G) + n / G;
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = part_n < 3 ? bf16_part(p[i], part_n) : 0.0f;
+                    pb[q] = __builtin_bit_cast(s16x4_t, make_uint2(pack_bf16_trunc(x[0], x[1]), pack_bf16_trunc(x[2], x[3])));
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const s16x4_t vop = v_operand(b.v[t]);
+#pragma unroll
+                    for (int q = 0; q < PP; q++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb[q], vop, acc[t], 0, 0, 0);
+                }
+            }
+        };
+        if constexpr (NB == 1) {
+            for (;;) {
+                load(buf[0], at[0]);
+                if (at[0] < 0) break;
+                compute(buf[0], at[0]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NB - 1; i++) load(buf[i], at[i]);
+            bool more = true;
+            while (more) {
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    load(buf[(i + NB - 1) % NB], at[(i + NB - 1) % NB]);
+                    if (at[i] < 0) {
+                        more = false;
+                        break;
+                    }
+                    compute(buf[i], at[i]);
+                }
+            }
+        }
+    }
+
+    // ---- the waves' states meet ----
+    // A wave whose every score was -inf (or NaN) still has its maximum at -inf: its sum says so.
+    if (any && m_run == -INFINITY) l_run = __builtin_nanf("");
+    const float l_tot = rows_sum(l_run);
+    if (q4 == 0) {
+        s_m[wave][n] = m_run;
+        s_l[wave][n] = l_tot;
+    }
+    constexpr int TT = CH / 16;  // tiles per round
+    const int nparts = F32 ? 1 : min(3, PASSES == 1 ? 3 : 16 / G);  // rows of O that hold a head's parts
+#pragma unroll
+    for (int c = 0; c < D / CH; c++) {
+        __syncthreads();
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = acc[c * TT + tt][i];
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < G * CH; idx += 64 * kSparseWaves) {
+            const int g = idx / CH, d = idx % CH;
+            float M = s_m[0][g];
+#pragma unroll
+            for (int w = 1; w < kSparseWaves; w++) M = fmaxf(M, s_m[w][g]);
+            float L = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kSparseWaves; w++) {
+                const float mw = s_m[w][g];
+                if (mw == -INFINITY && M > -INFINITY) continue;  // nothing of this wave's counts
+                const float f = mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M);
+                float x = 0.0f;
+                for (int k = 0; k < nparts; k++) x += s_o[w][g + G * k][d];
+                L += s_l[w][g] * f;
+                o += x * f;
+            }
+            const int dim = c * CH + d;
+            if (a.parts == 1) {
+                // no token: zeros
+                a.d.out[(static_cast<int64_t>(row) * G + g) * D + dim] = L == 0.0f ? 0.0f : o / L;
+            } else {
+                const int64_t pi = (static_cast<int64_t>(row) * a.parts + part) * G + g;
+                a.d.ws_o[pi * D + dim] = o;
+                if (dim == 0) {
+                    a.d.ws_m[pi] = M;
+                    a.d.ws_l[pi] = L;
+                }
+            }
+        }
+    }
+}
+
+// The parts of a row: one wave per (row, query head), lanes over dims.
+template <int D>
+__global__ __launch_bounds__(256) void sparse_merge_kernel(const SparseArgs a) {
+    constexpr int DPL = (D + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t rows = static_cast<int64_t>(a.num_queries) * a.d.num_kv_heads * a.d.group;
+    const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (u >= rows) return;
+    const int64_t row = u / a.d.group;
+    const int g = static_cast<int>(u - row * a.d.group);
+    const int64_t p0 = row * a.parts * a.d.group + g;
+    float M = -INFINITY;
+    for (int p = 0; p < a.parts; p++) M = fmaxf(M, a.d.ws_m[p0 + static_cast<int64_t>(p) * a.d.group]);
+    float L = 0.0f, o[DPL];
+#pragma unroll
+    for (int k = 0; k < DPL; k++) o[k] = 0.0f;
+    for (int p = 0; p < a.parts; p++) {
+        const int64_t pi = p0 + static_cast<int64_t>(p) * a.d.group;
+        const float mp = a.d.ws_m[pi];
+        if (mp == -INFINITY && M > -INFINITY) continue;
+        const float f = mp == M ? 1.0f : __builtin_amdgcn_exp2f(mp - M);
+        L += a.d.ws_l[pi] * f;
+#pragma unroll
+        for (int k = 0; k < DPL; k++)
+            if (lane + 64 * k < D) o[k] += a.d.ws_o[pi * D + lane + 64 * k] * f;
+    }
+#pragma unroll
+    for (int k = 0; k < DPL; k++)
+        if (lane + 64 * k < D) a.d.out[u * D + lane + 64 * k] = L == 0.0f ? 0.0f : o[k] / L;
+}
+
+template <int D>
+void launch_sparse_decode(const SparseArgs& a, int kv_dtype, bool q_f32, hipStream_t s) {
+    const uint32_t grid = static_cast<uint32_t>(static_cast<int64_t>(a.num_queries) * a.d.num_kv_heads * a.parts);
+    const int G = a.d.group;
+    const auto go = [&](auto kernel) { kernel<<<grid, 64 * kSparseWaves, 0, s>>>(a); };
+    const auto by_q = [&](auto kv, auto passes) {
+        constexpr int KV = decltype(kv)::value, P = decltype(passes)::value;
+        if (q_f32) go(sparse_decode_kernel<D, KV, true, P>);
+        else go(sparse_decode_kernel<D, KV, false, P>);
+    };
+    const auto by_group = [&](auto kv) {
+        if (G <= 4) by_q(kv, std::integral_constant<int, 1>());
+        else if (G == 8) by_q(kv, std::integral_constant<int, 2>());
+        else by_q(kv, std::integral_constant<int, 3>());
+    };
+    if (kv_dtype == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>(), std::integral_constant<int, 1>());
+    else if (kv_dtype == PA_DTYPE_BF16) by_group(std::integral_constant<int, PA_DTYPE_BF16>());
+    else if constexpr (D >= 64) by_group(std::integral_constant<int, PA_DTYPE_INT8>());
+    if (a.parts > 1) {
+        const int64_t waves = static_cast<int64_t>(a.num_queries) * a.d.num_kv_heads * G;
+        sparse_merge_kernel<D><<<static_cast<uint32_t>((waves + 3) / 4), 256, 0, s>>>(a);
+    }
+}
+#ifndef PA_SPARSE_INSTANTIATE
+extern template void launch_sparse_decode<32>(const SparseArgs&, int, bool, hipStream_t);
+extern template void launch_sparse_decode<64>(const SparseArgs&, int, bool, hipStream_t);
+extern template void launch_sparse_decode<128>(const SparseArgs&, int, bool, hipStream_t);
+extern template void launch_sparse_decode<256>(const SparseArgs&, int, bool, hipStream_t);
+#endif
+
+}  // namespace pa

@@ -1,0 +1,115 @@
+// sparse_decode.hip -- entry points of the attention over selected blocks (sparse_decode.h).
+#include <algorithm>
+#include <string>
+
+#include "sparse_decode.h"
+
+namespace {
+
+// Parts per row: enough workgroups for the chip's CUs, but two list entries a wave at least.
+int32_t sparse_parts(const pa_config* cfg, int32_t num_queries, int32_t budget) {
+    const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(num_queries) * cfg->num_kv_heads);
+    const int64_t want = (512 + rows - 1) / rows;
+    const int64_t most = std::max<int64_t>(1, budget / (2 * pa::kSparseWaves));
+    return static_cast<int32_t>(std::min(want, most));
+}
+
+// Partial states of all rows; 0 when every row is one part.
+size_t partial_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
+    const int32_t parts = sparse_parts(cfg, num_queries, budget);
+    return parts == 1 ? 0 : static_cast<size_t>(num_queries) * cfg->num_q_heads * parts;
+}
+
+pa_status check_shape(const std::string& f, const pa_config* cfg, int32_t num_queries, int32_t budget) {
+    pa_status st = pa::check_config(cfg, f.c_str());
+    if (st != PA_SUCCESS) return st;
+    const int32_t g = cfg->num_q_heads / cfg->num_kv_heads;
+    if (g > 16 || (g & (g - 1)) != 0)
+        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": num_q_heads / num_kv_heads must be 1, 2, 4, 8 or 16");
+    if (num_queries < 0 || budget < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (static_cast<int64_t>(num_queries) * cfg->num_kv_heads * std::max(budget, 1) > INT32_MAX)
+        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many query tokens for one call");
+    return PA_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" {
+
+pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t budget, size_t* bytes) {
+    const std::string f = "pa_sparse_workspace_size";
+    pa_status st = check_shape(f, cfg, num_queries, budget);
+    if (st != PA_SUCCESS) return st;
+    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": bytes is null");
+    *bytes = partial_count(cfg, num_queries, budget) * (cfg->head_dim + 2) * sizeof(float);
+    return pa::clear_error();
+}
+
+pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, const void* q, const void* k_cache,
+                           const void* v_cache, const float* k_scale, const float* v_scale,
+                           const int32_t* block_tables, int32_t num_seqs, int32_t max_blocks_per_seq,
+                           const int32_t* query_seqs, const int32_t* context_lens, int32_t num_queries,
+                           int32_t max_context_len, const int32_t* selected, int32_t budget, void* workspace,
+                           size_t workspace_bytes) {
+    const std::string f = "pa_sparse_decode";
+    pa_status st = check_shape(f, cfg, num_queries, budget);
+    if (st != PA_SUCCESS) return st;
+    if (num_seqs < 0 || max_blocks_per_seq < 0 || max_context_len < 0)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (max_blocks_per_seq > INT32_MAX / pa::kBlockSize)
+        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": max_blocks_per_seq * 16 must fit 32 bits");
+    if (num_queries == 0) return pa::clear_error();
+    if (budget == 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": budget must be >= 1");
+    if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens || !selected)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+    if (!query_seqs && num_queries != num_seqs)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": num_queries must be num_seqs when query_seqs is null");
+    if (cfg->kv_dtype == PA_DTYPE_INT8 && (!k_scale || !v_scale))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": int8 cache needs k_scale and v_scale");
+    if (!pa::aligned16(k_cache) || !pa::aligned16(v_cache))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": cache pointers must be 16-byte aligned");
+    const size_t partials = partial_count(cfg, num_queries, budget);
+    const size_t need = partials * (cfg->head_dim + 2) * sizeof(float);
+    if (need > workspace_bytes || (need > 0 && !workspace))
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(workspace) & 3)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 4-byte aligned");
+    pa::SparseArgs a{};
+    a.d.out = out;
+    a.d.q = q;
+    a.d.k_cache = k_cache;
+    a.d.v_cache = v_cache;
+    a.d.k_scale = k_scale;
+    a.d.v_scale = v_scale;
+    a.d.block_tables = block_tables;
+    a.d.context_lens = context_lens;
+    a.d.ws_o = static_cast<float*>(workspace);
+    a.d.ws_m = a.d.ws_o + partials * cfg->head_dim;
+    a.d.ws_l = a.d.ws_m + partials;
+    a.d.num_kv_heads = cfg->num_kv_heads;
+    a.d.group = cfg->num_q_heads / cfg->num_kv_heads;
+    a.d.max_blocks_per_seq = max_blocks_per_seq;
+    a.d.num_blocks = cfg->num_blocks;
+    a.d.max_context_len = max_context_len;
+    a.d.scale = pa::resolve_scale(cfg);
+    a.query_seqs = query_seqs;
+    a.selected = selected;
+    a.num_seqs = num_seqs;
+    a.num_queries = num_queries;
+    a.budget = budget;
+    a.parts = sparse_parts(cfg, num_queries, budget);
+    a.per = (budget + a.parts - 1) / a.parts;
+    pa::StreamDevice dev(stream);
+    hipStream_t s = pa::native(stream);
+    const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
+    switch (cfg->head_dim) {
+        case 32: pa::launch_sparse_decode<32>(a, cfg->kv_dtype, q_f32, s); break;
+        case 64: pa::launch_sparse_decode<64>(a, cfg->kv_dtype, q_f32, s); break;
+        case 128: pa::launch_sparse_decode<128>(a, cfg->kv_dtype, q_f32, s); break;
+        default: pa::launch_sparse_decode<256>(a, cfg->kv_dtype, q_f32, s); break;
+    }
+    PA_HIP_CHECK(hipGetLastError());
+    return pa::clear_error();
+}
+
+}  // extern "C"

@@ -1,0 +1,5 @@
+// sparse_decode_d256.hip -- head_dim 256 instantiations of the attention over selected blocks.
+#define PA_SPARSE_INSTANTIATE
+#include "sparse_decode.h"
+
+template void pa::launch_sparse_decode<256>(const pa::SparseArgs&, int, bool, hipStream_t);

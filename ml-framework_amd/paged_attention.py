@@ -61,6 +61,9 @@ EXPORTS = (
     "pa_qkv_workspace_size", "pa_qkv_project_append", "pa_o_workspace_size", "pa_o_project",
     "pa_prefix_plan_bytes", "pa_prefix_plan_build", "pa_prefix_plan_fill", "pa_prefix_workspace_size",
     "pa_paged_decode_prefix",
+    "pa_key_bounds_bytes", "pa_key_bounds_update", "pa_select_workspace_size", "pa_select_blocks",
+    "pa_sparse_workspace_size", "pa_sparse_decode",
+    "pa_pages_fork", "pa_pages_workspace_size", "pa_pages_reserve", "pa_pages_compact", "pa_copy_pages",
 )
 
 
@@ -163,6 +166,17 @@ _SIGNATURES = {
     "pa_qkv_project_append": [_P, _CFG, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ],
     "pa_o_workspace_size": [_CFG, _I32, _I32, ctypes.POINTER(_SZ)],
     "pa_o_project": [_P, _CFG, _P, _P, _I32, _I32, _P, _P, _SZ],
+    "pa_key_bounds_bytes": [_CFG, ctypes.POINTER(_SZ)],
+    "pa_key_bounds_update": [_P, _CFG, _P, _P, _I32, _P, _P, _I32, _I32, _P],
+    "pa_select_workspace_size": [_CFG, _I32, _I32, ctypes.POINTER(_SZ)],
+    "pa_select_blocks": [_P, _CFG, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _SZ],
+    "pa_sparse_workspace_size": [_CFG, _I32, _I32, ctypes.POINTER(_SZ)],
+    "pa_sparse_decode": [_P, _CFG, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _P, _I32, _P, _SZ],
+    "pa_pages_fork": [_P, _CFG, _P, _P, _I32, _P, _P, _P, _I32, _I32, _P],
+    "pa_pages_workspace_size": [_CFG, _I32, _I32, ctypes.POINTER(_SZ)],
+    "pa_pages_reserve": [_P, _CFG, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P, _SZ],
+    "pa_pages_compact": [_P, _CFG, _P, _I32, _I32, _P, _I32, _P, _P, _P, _SZ],
+    "pa_copy_pages": [_P, _CFG, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P],
 }
 
 _lib = None
@@ -450,6 +464,83 @@ def write_block_f32(stream, cfg: PaConfig, k_cache, v_cache, k_scale, v_scale, k
                     k_in, v_in):
     call("pa_write_block_f32", stream.handle if stream else None, ctypes.byref(cfg), _ptr(k_cache), _ptr(v_cache),
          _ptr(k_scale), _ptr(v_scale), _ptr(k_absmax), _ptr(v_absmax), block, tokens, _ptr(k_in), _ptr(v_in))
+
+
+# ---- attention over selected blocks -----------------------------------------------------------
+def key_bounds_bytes(cfg: PaConfig) -> int:
+    n = ctypes.c_size_t()
+    call("pa_key_bounds_bytes", ctypes.byref(cfg), ctypes.byref(n))
+    return n.value
+
+
+def key_bounds_update(stream, cfg: PaConfig, k_cache, block_tables, max_blocks_per_seq, start_pos, num_new, num_seqs,
+                      max_new_per_seq, key_bounds):
+    call("pa_key_bounds_update", stream.handle if stream else None, ctypes.byref(cfg), _ptr(k_cache),
+         _ptr(block_tables), max_blocks_per_seq, _ptr(start_pos), _ptr(num_new), num_seqs, max_new_per_seq,
+         _ptr(key_bounds))
+
+
+def select_workspace_size(cfg: PaConfig, num_queries: int, max_context_len: int) -> int:
+    n = ctypes.c_size_t()
+    call("pa_select_workspace_size", ctypes.byref(cfg), num_queries, max_context_len, ctypes.byref(n))
+    return n.value
+
+
+def select_blocks(stream, cfg: PaConfig, q, key_bounds, k_scale, block_tables, num_seqs, max_blocks_per_seq,
+                  query_seqs, context_lens, num_queries, max_context_len, sink_blocks, recent_blocks, budget, selected,
+                  workspace=None, workspace_bytes=0):
+    call("pa_select_blocks", stream.handle if stream else None, ctypes.byref(cfg), _ptr(q), _ptr(key_bounds),
+         _ptr(k_scale), _ptr(block_tables), num_seqs, max_blocks_per_seq, _ptr(query_seqs), _ptr(context_lens),
+         num_queries, max_context_len, sink_blocks, recent_blocks, budget, _ptr(selected), _ptr(workspace),
+         workspace_bytes)
+
+
+def sparse_workspace_size(cfg: PaConfig, num_queries: int, budget: int) -> int:
+    n = ctypes.c_size_t()
+    call("pa_sparse_workspace_size", ctypes.byref(cfg), num_queries, budget, ctypes.byref(n))
+    return n.value
+
+
+def sparse_decode(stream, cfg: PaConfig, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, num_seqs,
+                  max_blocks_per_seq, query_seqs, context_lens, num_queries, max_context_len, selected, budget,
+                  workspace=None, workspace_bytes=0):
+    call("pa_sparse_decode", stream.handle if stream else None, ctypes.byref(cfg), _ptr(out), _ptr(q), _ptr(k_cache),
+         _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables), num_seqs, max_blocks_per_seq,
+         _ptr(query_seqs), _ptr(context_lens), num_queries, max_context_len, _ptr(selected), budget, _ptr(workspace),
+         workspace_bytes)
+
+
+# ---- the books of the pool on the device --------------------------------------------------------
+def pages_fork(stream, cfg: PaConfig, tables_in, lens_in, num_in, src, tables_out, lens_out, num_out,
+               max_blocks_per_seq, refcounts):
+    call("pa_pages_fork", stream.handle if stream else None, ctypes.byref(cfg), _ptr(tables_in), _ptr(lens_in), num_in,
+         _ptr(src), _ptr(tables_out), _ptr(lens_out), num_out, max_blocks_per_seq, _ptr(refcounts))
+
+
+def pages_workspace_size(cfg: PaConfig, num_rows: int, max_blocks_per_seq: int) -> int:
+    n = ctypes.c_size_t()
+    call("pa_pages_workspace_size", ctypes.byref(cfg), num_rows, max_blocks_per_seq, ctypes.byref(n))
+    return n.value
+
+
+def pages_reserve(stream, cfg: PaConfig, tables, lens, num_new, num_rows, max_blocks_per_seq, max_new_per_row,
+                  refcounts, copy_pairs, status, workspace=None, workspace_bytes=0):
+    call("pa_pages_reserve", stream.handle if stream else None, ctypes.byref(cfg), _ptr(tables), _ptr(lens),
+         _ptr(num_new), num_rows, max_blocks_per_seq, max_new_per_row, _ptr(refcounts), _ptr(copy_pairs), _ptr(status),
+         _ptr(workspace), workspace_bytes)
+
+
+def pages_compact(stream, cfg: PaConfig, tables, num_rows, max_blocks_per_seq, refcounts, max_moves, pairs, status,
+                  workspace=None, workspace_bytes=0):
+    call("pa_pages_compact", stream.handle if stream else None, ctypes.byref(cfg), _ptr(tables), num_rows,
+         max_blocks_per_seq, _ptr(refcounts), max_moves, _ptr(pairs), _ptr(status), _ptr(workspace), workspace_bytes)
+
+
+def copy_pages(stream, cfg: PaConfig, k_cache, v_cache, k_scale, v_scale, k_absmax, v_absmax, key_bounds, pairs,
+               max_pairs, num_pairs=None):
+    call("pa_copy_pages", stream.handle if stream else None, ctypes.byref(cfg), _ptr(k_cache), _ptr(v_cache),
+         _ptr(k_scale), _ptr(v_scale), _ptr(k_absmax), _ptr(v_absmax), _ptr(key_bounds), _ptr(pairs), max_pairs,
+         _ptr(num_pairs))
 
 
 # ---- projections either side of attention ----------------------------------------------------
