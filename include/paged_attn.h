@@ -433,7 +433,8 @@ pa_status pa_key_bounds_update(pa_stream* stream, const pa_config* cfg, const vo
                                const int32_t* start_pos, const int32_t* num_new, int32_t num_seqs,
                                int32_t max_new_per_seq, void* key_bounds);
 
-/* Bytes of workspace of pa_select_blocks (8 per query, KV head and block; 8-byte aligned). */
+/* Bytes of workspace of pa_select_blocks (8 per query, KV head and block, and for int8 caches 12 head_dim + 8
+ * per query and KV head; 16-byte aligned). */
 pa_status pa_select_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t max_context_len, size_t* bytes);
 /* The blocks each query attends to, for each KV head:
  *   selected: [num_queries][num_kv_heads][budget] int32, logical block indices in ascending order, -1
@@ -442,11 +443,13 @@ pa_status pa_select_workspace_size(const pa_config* cfg, int32_t num_queries, in
  *   largest scores
  *     sum_d (sum_g max(q_gd, 0)) hi_bd + (sum_g min(q_gd, 0)) lo_bd       (g: the heads of the group)
  *   (times k_scale for int8 caches), an upper bound of sum_g max_t q_g . k_t; equal scores go to the
- *   lowest index, a score that is NaN comes first. Scores are summed in 64 bits. Blocks whose table entry
+ *   lowest index, a score that is NaN comes first (int8 caches: any score of a query that is not finite
+ *   is). Scores are summed in 64 bits. Blocks whose table entry
  *   lies outside [0, num_blocks) score 0. The bounds of the sink and recent blocks do not matter
  *   (they need not be up to date while they are among the recent ones).
  *   q: [num_queries][num_q_heads][head_dim] of q_dtype; recent_blocks >= 1 (the block of the newest
- *   token), sink_blocks + recent_blocks <= budget, max_context_len <= 2097152. */
+ *   token), sink_blocks + recent_blocks <= budget, max_context_len <= 2097152; q and key_bounds 16-byte
+ *   aligned. */
 pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* q, const void* key_bounds,
                            const float* k_scale, const int32_t* block_tables, int32_t num_seqs,
                            int32_t max_blocks_per_seq, const int32_t* query_seqs, const int32_t* context_lens,
