@@ -60,27 +60,31 @@ __global__ __launch_bounds__(kForkThreads) void pages_fork_kernel(const int32_t*
 }
 
 // ---- helpers of the one-workgroup kernels --------------------------------------------------------
-// Exclusive prefix of `mine` over the workgroup, and the total.
-__device__ __forceinline__ int block_prefix(int mine, int* s_wave, int& total) {
+constexpr int kBookWaves = kBookThreads / 64;
+// The sum of `mine` (the same in every lane of a wave) over the waves before this one, and over all.
+__device__ __forceinline__ int waves_before(int mine, int* s_wave, int& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += v;
-    }
     __syncthreads();  // the previous call's sums have been read
-    if (lane == 63) s_wave[wave] = incl;
+    if (lane == 0) s_wave[wave] = mine;
     __syncthreads();
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kBookThreads / 64; w++) {
+    for (int w = 0; w < kBookWaves; w++) {
         const int v = s_wave[w];
         before += w < wave ? v : 0;
         total += v;
     }
-    return before + incl - mine;
+    return before;
+}
+// Set bits of a ballot in the lanes below this one.
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+// Exclusive prefix of a truth value over the workgroup, and the total.
+__device__ __forceinline__ int block_prefix(bool mine, int* s_wave, int& total) {
+    const uint64_t mask = __ballot(mine);
+    return waves_before(__popcll(mask), s_wave, total) + lanes_before(mask);
 }
 __device__ __forceinline__ int load_now(const int32_t* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -124,6 +128,102 @@ __device__ __forceinline__ int32_t* demand_entry(const ReserveArgs& a, int64_t e
 // In row order, a block a demand: an empty entry takes the lowest free block; an entry that other rows
 // hold too takes one in its place (copy on write), except for the last of the rows that hold it when all
 // of them ask in this call: it keeps the block, as it would if the rows were worked off one by one.
+//
+// Up to kBookThreads demands, a thread each: three dependent loads (lengths; table entry; refcount) with the
+// refcounts of the pool's first blocks on their way meanwhile, and everything else in registers and
+// LDS. What bounds it is the chain of those round trips and of the barriers.
+static_assert(2 * kBookThreads == 1 << 11, "the hash has 11 bits");
+constexpr int kScan = 8;  // 64-block words of a wave per scan of the pool: 8192 blocks a round
+__global__ __launch_bounds__(kBookThreads) void pages_reserve_small_kernel(const ReserveArgs a) {
+    __shared__ int s_wave[kBookWaves], s_fresh[kBookThreads];
+    // shared blocks that are asked for, by a hash of the id: how many ask, and the last that does
+    __shared__ int s_id[2 * kBookThreads], s_count[2 * kBookThreads], s_last[2 * kBookThreads];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // free[k]: the blocks base + 64 k + lane of this wave's part of the round that are free
+    uint64_t free[kScan];
+    int refs[kScan];
+    auto read = [&](int64_t base) {
+#pragma unroll
+        for (int k = 0; k < kScan; k++) {
+            const int64_t b = base + 64 * (kScan * wave + k) + lane;
+            refs[k] = b < a.num_blocks ? a.refs[b] : 1;
+        }
+    };
+    read(0);
+    const bool asks = tid < a.rows * a.reach;
+    int row = 0, lb = 0;
+    int32_t* entry = asks ? demand_entry(a, tid, row, lb) : nullptr;
+    int id = entry ? *entry : -1;
+    if (id >= a.num_blocks) id = -1;
+    const int held = entry && id >= 0 ? a.refs[id] : 0;
+    const bool shared = held > 1;
+    bool takes = entry && id < 0;
+    if (__syncthreads_or(shared)) {
+        for (int i = tid; i < 2 * kBookThreads; i += kBookThreads) {
+            s_id[i] = -1;
+            s_count[i] = 0;
+            s_last[i] = -1;
+        }
+        __syncthreads();
+        uint32_t slot = (static_cast<uint32_t>(id) * 2654435761u) >> 21;
+        if (shared) {
+            for (;;) {  // at most half of the places are ever taken
+                const int there = atomicCAS(&s_id[slot], -1, id);
+                if (there == -1 || there == id) break;
+                slot = (slot + 1) % (2 * kBookThreads);
+            }
+            atomicAdd(&s_count[slot], 1);
+            atomicMax(&s_last[slot], tid);
+        }
+        __syncthreads();
+        if (shared) takes = !(s_count[slot] == held && s_last[slot] == tid);
+    }
+    int need;
+    const int at = block_prefix(takes, s_wave, need);
+    int found = 0;
+    for (int64_t base = 0; found < need && base < a.num_blocks; base += 64 * kScan * kBookWaves) {
+        if (base > 0) read(base);
+        int mine = 0, total;
+#pragma unroll
+        for (int k = 0; k < kScan; k++) {
+            free[k] = __ballot(refs[k] <= 0);
+            mine += __popcll(free[k]);
+        }
+        int rank = found + waves_before(mine, s_wave, total);
+#pragma unroll
+        for (int k = 0; k < kScan; k++) {
+            const int r = rank + lanes_before(free[k]);
+            if ((free[k] >> lane & 1) && r < need) s_fresh[r] = static_cast<int>(base) + 64 * (kScan * wave + k) + lane;
+            rank += __popcll(free[k]);
+        }
+        found += total;
+    }
+    if (tid == 0) {
+        a.status[0] = found >= need ? need : 0;
+        a.status[1] = found >= need ? 0 : need - found;
+    }
+    __syncthreads();
+    int from = -1, to = -1;
+    if (takes && found >= need) {
+        const int b = s_fresh[at];
+        if (id >= 0) {
+            atomicSub(a.refs + id, 1);
+            if (static_cast<int64_t>(lb) * 16 < a.lens[row]) {  // it holds tokens of the row
+                from = id;
+                to = b;
+            }
+        }
+        *entry = b;
+        a.refs[b] = 1;
+    }
+    // only a row's first demand can be for a block that holds tokens
+    if (asks && tid % a.reach == 0) {
+        a.pairs[2 * (tid / a.reach)] = from;
+        a.pairs[2 * (tid / a.reach) + 1] = to;
+    }
+}
+
+// Any number of demands: the same through lists in the workspace.
 __global__ __launch_bounds__(kBookThreads) void pages_reserve_kernel(const ReserveArgs a) {
     __shared__ int s_wave[kBookThreads / 64];
     const int tid = threadIdx.x;
@@ -210,8 +310,6 @@ struct CompactArgs {
     int32_t* pairs;   // [max_moves][2]
     int32_t* status;  // [2]
     int32_t* rank;    // [num_blocks] scratch: the place of a moved block in the list
-    int32_t* from;    // [num_blocks] scratch
-    int32_t* to;      // [num_blocks] scratch
     int32_t* counts;  // [2] scratch: moves, the lowest moved block
     int32_t num_blocks, max_moves;
     int64_t entries;  // table entries
@@ -219,63 +317,113 @@ struct CompactArgs {
 
 // The i-th highest live block goes to the i-th lowest free one while that is lower, at most max_moves.
 // With L live blocks in all, those are the live blocks at or above L and the free ones below it.
+// A word is a ballot over 64 blocks; with the words and the live blocks before each of them in LDS a block's place
+// among the live ones is a count of bits. Pools of up to 262144 blocks are read once.
+constexpr int kWords = 4096;
 __global__ __launch_bounds__(kBookThreads) void pages_compact_kernel(const CompactArgs a) {
-    __shared__ int s_wave[kBookThreads / 64];
-    const int tid = threadIdx.x;
-    int live = 0;
-    for (int64_t b0 = 0; b0 < a.num_blocks; b0 += kBookThreads) {
-        const int64_t b = b0 + tid;
-        int total;
-        block_prefix(b < a.num_blocks && a.refs[b] > 0, s_wave, total);
-        live += total;
-    }
-    int before = 0, low = 0;  // live blocks below the slab; live blocks below `live`
-    for (int64_t b0 = 0; b0 < a.num_blocks; b0 += kBookThreads) {
-        const int64_t b = b0 + tid;
-        const bool is_live = b < a.num_blocks && a.refs[b] > 0;
-        int total;
-        const int lb = before + block_prefix(is_live, s_wave, total);  // live blocks below b
-        if (b < a.num_blocks) {
-            if (is_live && b >= live) {
-                store_now(a.from + (live - 1 - lb), static_cast<int>(b));
-                store_now(a.rank + b, live - 1 - lb);
-            } else if (!is_live && b < live) {
-                store_now(a.to + (b - lb), static_cast<int>(b));
+    __shared__ uint64_t s_word[kWords];  // live blocks
+    __shared__ int s_before[kWords];     // live blocks of the round before each word
+    __shared__ int s_wave[kBookWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int kRound = 64 * kWords;
+    const auto words_of = [&](int base) { return static_cast<int>(min(static_cast<int64_t>(kWords), (static_cast<int64_t>(a.num_blocks) - base + 63) / 64)); };
+    // the words of the blocks from `base` on; returns their live blocks
+    const auto scan = [&](int base) {
+        const int words = words_of(base);
+        constexpr int UN = 8;  // loads in flight
+        for (int k0 = wave; k0 < words; k0 += UN * kBookWaves) {
+            int refs[UN];
+#pragma unroll
+            for (int j = 0; j < UN; j++) {
+                const int64_t b = static_cast<int64_t>(base) + 64 * (k0 + j * kBookWaves) + lane;
+                refs[j] = b < a.num_blocks ? a.refs[b] : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < UN; j++) {
+                const uint64_t w = __ballot(refs[j] > 0);
+                if (lane == 0 && k0 + j * kBookWaves < words) s_word[k0 + j * kBookWaves] = w;
             }
         }
-        int in;
-        block_prefix(is_live && b < live, s_wave, in);
-        low += in;
+        __syncthreads();
+        constexpr int PT = kWords / kBookThreads;
+        int n[PT], mine = 0, total;
+#pragma unroll
+        for (int k = 0; k < PT; k++) {
+            n[k] = tid * PT + k < words ? __popcll(s_word[tid * PT + k]) : 0;
+            mine += n[k];
+        }
+        const int incl = pa::wave_prefix(mine);
+        int at = waves_before(__builtin_amdgcn_readlane(incl, 63), s_wave, total) + incl - mine;
+#pragma unroll
+        for (int k = 0; k < PT; k++) {
+            if (tid * PT + k < words) s_before[tid * PT + k] = at;
+            at += n[k];
+        }
+        __syncthreads();
+        return total;
+    };
+    int live = 0;
+    for (int64_t base = 0; base < a.num_blocks; base += kRound) live += scan(static_cast<int>(base));
+    int low = 0;  // live blocks below `live`
+    const bool once = a.num_blocks <= kRound;
+    for (int64_t base = 0, before = 0; base < live; base += kRound) {
+        const int total = once ? live : scan(static_cast<int>(base));
+        const int64_t at = live - base;
+        if (at >= 64ll * words_of(static_cast<int>(base))) {
+            low = static_cast<int>(before) + total;
+        } else {
+            low = static_cast<int>(before) + s_before[at / 64] + __popcll(s_word[at / 64] & ((1ull << (at % 64)) - 1));
+        }
         before += total;
     }
     const int full = live - low, n = min(full, a.max_moves);
-    block_sync_global();
-    if (tid == 0) {
-        a.status[0] = n;
-        a.status[1] = n == full ? live : load_now(a.from + n) + 1;
-        a.counts[0] = n;
-        a.counts[1] = n > 0 ? load_now(a.from + n - 1) : a.num_blocks;
-    }
-    for (int64_t i = tid; i < a.max_moves; i += kBookThreads) {
-        const int s = i < n ? load_now(a.from + i) : -1, d = i < n ? load_now(a.to + i) : -1;
-        a.pairs[2 * i] = s;
-        a.pairs[2 * i + 1] = d;
-        if (i < n) {
-            a.refs[d] = a.refs[s];
-            a.refs[s] = 0;
+    int before = 0;  // live blocks of earlier rounds
+    for (int64_t base = 0; base < a.num_blocks; base += kRound) {
+        const int total = once ? live : scan(static_cast<int>(base));
+        const int words = words_of(static_cast<int>(base));
+        for (int k = wave; k < words; k += kBookWaves) {
+            const uint64_t word = s_word[k];
+            const int64_t b64 = base + 64 * k + lane;
+            const int lb = before + s_before[k] + lanes_before(word);  // live blocks below b
+            if (b64 >= a.num_blocks) continue;
+            const int b = static_cast<int>(b64), i = live - 1 - lb;  // i: a live block's place from the top
+            if (!(word >> lane & 1)) {
+                if (b < live && b - lb < n) a.pairs[2 * static_cast<int64_t>(b - lb) + 1] = b;
+            } else if (i < n) {  // (at or above `live`)
+                a.pairs[2 * static_cast<int64_t>(i)] = b;
+                a.rank[b] = i;
+                if (i == n - 1) a.counts[1] = b;
+            } else if (i == n && n < full) {
+                a.status[1] = b + 1;  // the highest that stays, where the moves are cut short
+            }
         }
+        before += total;
+    }
+    if (tid == 0) {
+        a.status[0] = a.counts[0] = n;
+        if (n == full) a.status[1] = live;
     }
 }
 
-// Table entries of moved blocks take the new names.
+// Refcounts move along, table entries of moved blocks take the new names, and the list's tail is cleared.
 __global__ __launch_bounds__(256) void pages_rename_kernel(const CompactArgs a) {
-    const int n = a.counts[0], lowest = a.counts[1];
-    if (n == 0) return;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < a.entries; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int n = a.counts[0], lowest = n > 0 ? a.counts[1] : a.num_blocks;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = first; i < a.max_moves; i += step) {
+        if (i < n) {
+            const int s = a.pairs[2 * i], d = a.pairs[2 * i + 1];
+            a.refs[d] = a.refs[s];
+            a.refs[s] = 0;
+        } else {
+            a.pairs[2 * i] = -1;
+            a.pairs[2 * i + 1] = -1;
+        }
+    }
+    for (int64_t i = first; i < a.entries; i += step) {
         const int id = a.tables[i];
         if (id < lowest || id >= a.num_blocks) continue;
         const int k = a.rank[id];  // written for every moved block; anything for an id that was not live
-        if (k >= 0 && k < n && a.from[k] == id) a.tables[i] = a.to[k];
+        if (k >= 0 && k < n && a.pairs[2 * static_cast<int64_t>(k)] == id) a.tables[i] = a.pairs[2 * static_cast<int64_t>(k) + 1];
     }
 }
 
@@ -339,10 +487,10 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(const CopyArgs
     }
 }
 
-// Scratch of reserve (four lists) and compact (three lists and two counts), ints.
+// Scratch of reserve (four lists) and compact (a list and two counts), ints.
 int64_t scratch_ints(const pa_config* cfg, int32_t num_rows, int32_t width) {
     const int64_t nb = cfg->num_blocks, demands = static_cast<int64_t>(num_rows) * width;
-    return std::max(2 * nb + 2 * demands, 3 * nb + 2);
+    return std::max(2 * nb + 2 * demands, nb + 2);
 }
 
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -426,7 +574,10 @@ pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tab
     a.num_blocks = cfg->num_blocks;
     a.reach = static_cast<int32_t>(reach);
     pa::StreamDevice dev(stream);
-    pages_reserve_kernel<<<1, kBookThreads, 0, pa::native(stream)>>>(a);
+    if (reach >= 1 && reach * num_rows <= kBookThreads)
+        pages_reserve_small_kernel<<<1, kBookThreads, 0, pa::native(stream)>>>(a);
+    else
+        pages_reserve_kernel<<<1, kBookThreads, 0, pa::native(stream)>>>(a);
     PA_HIP_CHECK(hipGetLastError());
     return pa::clear_error();
 }
@@ -453,9 +604,7 @@ pa_status pa_pages_compact(pa_stream* stream, const pa_config* cfg, int32_t* tab
     a.pairs = pairs;
     a.status = status;
     a.rank = static_cast<int32_t*>(workspace);
-    a.from = a.rank + cfg->num_blocks;
-    a.to = a.from + cfg->num_blocks;
-    a.counts = a.to + cfg->num_blocks;
+    a.counts = a.rank + cfg->num_blocks;
     a.num_blocks = cfg->num_blocks;
     a.max_moves = max_moves;
     a.entries = static_cast<int64_t>(num_rows) * max_blocks_per_seq;
@@ -463,8 +612,9 @@ pa_status pa_pages_compact(pa_stream* stream, const pa_config* cfg, int32_t* tab
     hipStream_t s = pa::native(stream);
     pages_compact_kernel<<<1, kBookThreads, 0, s>>>(a);
     PA_HIP_CHECK(hipGetLastError());
-    if (a.entries > 0) {
-        pages_rename_kernel<<<static_cast<uint32_t>(std::min<int64_t>((a.entries + 255) / 256, 1024)), 256, 0, s>>>(a);
+    const int64_t work = std::max<int64_t>(a.entries, max_moves);
+    if (work > 0) {
+        pages_rename_kernel<<<static_cast<uint32_t>(std::min<int64_t>((work + 255) / 256, 1024)), 256, 0, s>>>(a);
         PA_HIP_CHECK(hipGetLastError());
     }
     return pa::clear_error();

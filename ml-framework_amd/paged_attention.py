@@ -215,18 +215,21 @@ def check(status: int, fn: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    lib = load_library()
-    check(getattr(lib, name)(*args), name)
+    status = getattr(_lib or load_library(), name)(*args)
+    if status != PA_SUCCESS:
+        check(status, name)
 
 
 def _ptr(t) -> int | None:
     """Device (or host) address of a torch tensor / numpy array / int / None."""
     if t is None:
         return None
+    try:  # half the time of asking for the attribute first, and a call takes about ten of them
+        return t.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(t, int):
         return t
-    if hasattr(t, "data_ptr"):
-        return t.data_ptr()
     if hasattr(t, "ctypes"):
         return t.ctypes.data
     raise TypeError(f"cannot take the address of {type(t)}")

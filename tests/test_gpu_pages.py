@@ -153,6 +153,51 @@ def test_reserve_large():
     same(run_reserve(config(len(refs)), tables, lens, new, refs), ref.reserve(tables, lens, new, refs))
 
 
+@pytest.mark.parametrize("rows", [200, 511, 1024])
+def test_reserve_as_many_demands_as_threads(rows):
+    """A demand for each thread, nearly all of them for shared blocks, in a pool whose free blocks lie behind its first
+    thousands."""
+    nb = 30000
+    tables, lens, refs = books(10, [20 + i % 400 for i in range(60)], nb, width=30)
+    src = [(i * 7) % 60 for i in range(rows)]
+    tables, lens, refs = ref.fork(tables, lens, src, refs)
+    refs[:nb - 1100][refs[:nb - 1100] == 0] = 1
+    new = [1 if i % 9 else 0 for i in range(rows)]
+    same(run_reserve(config(nb), tables, lens, new, refs), ref.reserve(tables, lens, new, refs))
+
+
+def test_reserve_one_block_held_by_all():
+    tables, lens, refs = books(11, [5], 1100, width=2)
+    tables, lens, refs = ref.fork(tables, lens, [0] * 1024, refs)
+    for new in ([1] * 1024, [1] * 1000 + [0] * 24):
+        same(run_reserve(config(1100), tables, lens, new, refs), ref.reserve(tables, lens, new, refs))
+
+
+@pytest.mark.parametrize("nb,live,moves", [(20000, 9000, 10 ** 5), (300001, 70000, 10 ** 6), (600000, 299000, 1000), (530000, 529000, 10 ** 6)])
+def test_compact_large_pools(nb, live, moves):
+    """Pools past one round of the counting, checked against the definition in whole arrays."""
+    rng = np.random.default_rng(nb)
+    refs = np.zeros(nb, np.int32)
+    ids = rng.permutation(nb)[:live].astype(np.int32)
+    refs[ids] = rng.integers(1, 4, live)
+    tables = ids.reshape(-1, 100)
+    moves = min(moves, nb)
+    t, r, pairs, st = run_compact(config(nb), tables, refs, moves)
+    up, down = np.nonzero(refs > 0)[0][::-1], np.nonzero(refs == 0)[0]
+    k = min(len(up), len(down), moves)
+    up, down = up[:k], down[:k]
+    up, down = up[down < up], down[down < up]
+    want = refs.copy()
+    want[down], want[up] = refs[up], 0
+    name = np.arange(nb, dtype=np.int32)
+    name[up] = down
+    np.testing.assert_array_equal(pairs[:len(up)], np.stack([up, down], 1))
+    assert (pairs[len(up):] == -1).all()
+    np.testing.assert_array_equal(r, want)
+    np.testing.assert_array_equal(t, name[tables])
+    assert st.tolist() == [len(up), np.nonzero(want > 0)[0][-1] + 1]
+
+
 @pytest.mark.parametrize("moves", [0, 1, 7, 10 ** 4])
 @pytest.mark.parametrize("rows,nb", [(1, 3), (6, 60), (40, 1024), (200, 3001)])
 def test_compact(rows, nb, moves):

@@ -194,6 +194,34 @@ def test_select_infinities_nan_and_huge_scores():
         np.testing.assert_array_equal(got, ref.select(p, qs, range(4), p.lens, 1, 2, 20))
 
 
+@pytest.mark.parametrize("kv", [FP32, BF16, INT8])
+def test_select_many_queries_in_any_order(kv):
+    """More queries than sequences, of each sequence anywhere in the list, past one look at the list."""
+    p = ref.Pool(36 + kv, [16 * 40 + 5, 16 * 25, 16 * 300 + 1, 0, 16 * 12], 8, 2, 64, kv, values=False)
+    rng = np.random.default_rng(3)
+    rows = rng.integers(-1, 6, 150).tolist()
+    lens = [int(rng.integers(0, 16 * 300 + 2)) if 0 <= s < 5 and s == 2 else int(rng.integers(0, 700)) for s in rows]
+    lens = [min(t, int(p.lens[s])) if 0 <= s < 5 else t for s, t in zip(rows, lens)]
+    qs = p.queries(150)
+    g = {"bounds": to_gpu(p.bounds), "tables": to_gpu(p.tables), "stats": [to_gpu(s) for s in p.stats] if p.stats else [None] * 4}
+    np.testing.assert_array_equal(run_select(p, g, qs, rows, lens, 1, 2, 8), ref.select(p, qs, rows, lens, 1, 2, 8))
+
+
+def test_select_int8_weights_of_any_size():
+    """Weights far apart within a query, zeros, and values that are not finite (their scores are NaN: the lowest indices)."""
+    p = ref.Pool(39, [16 * 90] * 5, 8, 2, 64, INT8, FP32, values=False)
+    qs = p.queries(5)
+    qs[0] *= np.float32(1e-30)
+    qs[1, :, ::2] *= np.float32(1e6)
+    qs[2] = 0
+    qs[3, 0, 3] = np.inf
+    qs[4, 5, 1] = np.nan
+    g = {"bounds": to_gpu(p.bounds), "tables": to_gpu(p.tables), "stats": [to_gpu(s) for s in p.stats]}
+    got = run_select(p, g, qs, None, p.lens, 1, 2, 20)
+    want = ref.select(p, np.nan_to_num(qs, nan=np.float32(np.nan), posinf=np.float32(np.nan)), range(5), p.lens, 1, 2, 20)
+    np.testing.assert_array_equal(got, want)
+
+
 def test_select_ignores_bounds_of_the_recent_blocks_and_reads_no_bad_page():
     p = ref.Pool(34, [16 * 60 - 5, 16 * 60], 8, 2, 64, BF16, values=False)
     p.bounds[p.tables[0, 58:]] = 0x7fc0  # not brought up to date: NaN
