@@ -468,7 +468,7 @@ pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, in
  * Blocks whose table entry lies outside [0, num_blocks) read as zero keys and values. A query without
  * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter. Products are
  * exact and sums in fp32 for every cache and query type. num_q_heads / num_kv_heads: 1, 2, 4, 8 or
- * 16. Caches 16-byte aligned. */
+ * 16. q and caches 16-byte aligned. */
 pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, const void* q,
                            const void* k_cache, const void* v_cache, const float* k_scale,
                            const float* v_scale, const int32_t* block_tables, int32_t num_seqs,

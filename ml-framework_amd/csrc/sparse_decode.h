@@ -3,11 +3,15 @@
 // For query token r, KV head h, query head g of its group, over the tokens t of the listed blocks:
 //   s_t = scale * q_g . k_t,  out_g = sum_t exp(s_t - max s) v_t / sum_t exp(s_t - max s)
 //
-// The lists differ by KV head, so the unit of work is a row (query token, KV head), cut into `parts`
-// runs of its list, one workgroup each. Its waves take the listed blocks in turn (wave w: entries w, w +
-// kWaves, ..); a wave streams its blocks through rotating register buffers, one pass with the running maximum
-// and sum, and no wave waits for another until the part ends. There the waves' states meet in LDS; a
-// row of one part is finished at once, the parts of the others by a merge launch.
+// The lists differ by KV head, so a row is a (query token, KV head). The rows' lists are laid end to end and
+// cut into ranges of equal length, one for each workgroup of a chip full of them, so that every CU streams the
+// same number of blocks whatever the number of rows. The part of a row in a range is a segment; a workgroup works
+// its segments off one after another. Its waves take a segment's blocks in turn (wave w: entries w, w +
+// kSparseWaves, ..); a wave streams its blocks through rotating register buffers, one pass with the running maximum
+// and sum, and no wave waits for another until the segment ends. There the waves' states meet in LDS; a
+// segment that is a whole row is finished at once, the parts of the others (at most two a range) by a merge launch.
+// Measured: 256 rows of 128 bf16 blocks (D 128, 269 MB) 48 us, 5.6 TB/s; in two workgroups a row, with
+// a merge, 55 us. 384 rows of 255 int8 blocks (404 MB) 87 us, 4.7 TB/s; in three rounds of half rows 95 us.
 //
 // K and V are read once and G = Hq / Hkv query heads share them (2 G flops a byte at bf16): traffic
 // bounds it. The matrix instructions are 16 columns wide and G is 1 to 16, so the columns that a
@@ -16,7 +20,11 @@
 // query's three partial scores are summed across columns; P's three parts make three rows of O, which
 // are summed when the row ends. Every product is then exact and every sum in fp32, at the
 // instruction count of a single bf16 product for G <= 4 (two passes for G = 8, three for 16). fp32 caches
-// run on fp32 matrix instructions.
+// run on fp32 matrix instructions. int8 keys go to the byte matrix instruction as they are, against Q as a
+// 31-bit integer in units of 2^(e - 30), 2^e > max |q|, in four signed digits, one in each group of columns; P V runs
+// in bf16 as above, its codes converted by placing them in the fraction of 2^23 (an instruction of a quarter of the
+// conversion's time). The int8 case is bound by its traffic all the same: with the P V product left out
+// altogether it takes 86 us. What it lacks against bf16 is the run length, 2 KiB instead of 4 a tile.
 #pragma once
 
 #include "decode_mfma.h"
@@ -24,11 +32,11 @@
 namespace pa {
 
 struct SparseArgs {
-    DecodeArgs d;  // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [rows][parts][G]
+    DecodeArgs d;  // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [slots][G]
     const int32_t* query_seqs;  // null: query r belongs to sequence r
     const int32_t* selected;    // [num_queries][Hkv][budget]
     int32_t num_seqs, num_queries, budget;
-    int32_t parts, per;         // parts per row, list entries per part
+    int32_t rows, range;        // rows; list entries per workgroup (rows * budget fits 32 bits)
 };
 
 constexpr int kSparseWaves = 8;
@@ -83,10 +91,25 @@ __device__ __forceinline__ void sparse_load(const DecodeArgs& a, SparseBuf<D, KV
     }
 }
 
-// Register buffers of a wave: the one consumed and those in flight.
+// int8 codes k, k + 1 of w (of k: 0 or 2) as two bf16, exactly; w with every byte's top bit flipped (code + 128).
+__device__ __forceinline__ uint32_t bf16_pair_of(uint32_t w, int k) {
+    const float base = 8388736.0f;  // 2^23 + 128
+    const float lo = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k)) - base;
+    const float hi = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k + 1)) - base;
+    return pack_bf16_trunc(lo, hi);
+}
+// The PV operand of four tokens of one dim.
+__device__ __forceinline__ s16x4_t sparse_v_operand(const uint2& r) { return v_operand(r); }
+__device__ __forceinline__ s16x4_t sparse_v_operand(uint32_t r) {
+    const uint32_t w = r ^ 0x80808080u;
+    return __builtin_bit_cast(s16x4_t, make_uint2(bf16_pair_of(w, 0), bf16_pair_of(w, 2)));
+}
+
+// Register buffers of a wave: the one consumed and those in flight. (Three cost more registers and time nothing
+// less: bf16 47.7 us of two, 47.9 of three; int8 86.6, 88.5, 91.7 of four, 96.6 of six; one: 107.)
 template <int D, int KV>
 __host__ __device__ constexpr int sparse_buffers() {
-    return KV == PA_DTYPE_FP32 ? (D >= 256 ? 1 : D >= 128 ? 2 : 3) : D >= 256 ? (KV == PA_DTYPE_BF16 ? 1 : 2) : 3;
+    return D >= 256 ? 1 : 2;
 }
 
 // PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
@@ -94,7 +117,9 @@ template <int D, int KV, bool QF32, int PASSES>
 __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const SparseArgs a) {
     constexpr bool F32 = KV == PA_DTYPE_FP32;
     constexpr int NSLAB = D / 32, NT = D / 16;
-    constexpr int QP = QF32 && !F32 ? PASSES : 1;  // passes of Q
+    constexpr bool I8 = KV == PA_DTYPE_INT8;
+    constexpr int NI8 = I8 ? D / 64 : 1;           // QK slabs of 64 dims
+    constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
     constexpr int PP = F32 ? 1 : PASSES;           // passes of P
     constexpr int NB = sparse_buffers<D, KV>();
     constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
@@ -103,15 +128,25 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
     const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.d.num_kv_heads, G = a.d.group;
-    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const uint32_t budget = a.budget, all = static_cast<uint32_t>(a.rows) * budget;
+    uint32_t at_entry = blockIdx.x * static_cast<uint32_t>(a.range);
+    const uint32_t stop = min(all, at_entry + a.range);
+    for (; at_entry < stop;) {
+    const int row = static_cast<int>(at_entry / budget);
+    const int beg = static_cast<int>(at_entry - row * budget);
+    const int end = static_cast<int>(min(budget, beg + (stop - at_entry)));
+    at_entry += end - beg;
     const int r = row / Hkv, kvh = row - r * Hkv;
     const int seq = a.query_seqs ? a.query_seqs[r] : r;
     const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, a.d.context_lens[r]) : 0;
     const int nblk = T <= 0 ? 0 : (T + 15) / 16;
 
     // Q operand: column n holds head n % G (part n / G of it where Q is split).
-    bf16x8_t qb[F32 ? 1 : QP][F32 ? 1 : NSLAB];
+    bf16x8_t qb[F32 || I8 ? 1 : QP][F32 || I8 ? 1 : NSLAB];
     float qf[F32 ? D / 4 : 1];
+    i32x4_t qd[I8 ? QP : 1][NI8];   // int8: digits of dims (D / 4) q4 + 16 t ..
+    float place[I8 ? QP : 1];       // what a unit of this column's sums is worth
+    const float scale = a.d.scale * kLog2e;
     {
         const int64_t q0 = (static_cast<int64_t>(r) * Hkv * G + kvh * G + n % G) * D;
         if constexpr (F32) {
@@ -123,27 +158,62 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
                     qf[4 * u + j] = QF32 ? static_cast<const float*>(a.d.q)[i]
                                          : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
                 }
+        } else if constexpr (I8) {
+            float x[D / 4];
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < D / 4; e++) {
+                const int64_t i = q0 + (D / 4) * q4 + e;
+                x[e] = QF32 ? static_cast<const float*>(a.d.q)[i] : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
+                const float f = fabsf(x[e]);
+                top = fmaxf(top, f < INFINITY ? f : INFINITY);  // NaN too
+            }
+            top = rows_max(top);
+            const bool bad = !(top < INFINITY);
+            // |q| < 2^ex; below 2^-96 (nothing that fp32 sums would keep) all of it counts as zero
+            const int ex = max(bad ? 0 : __builtin_amdgcn_frexp_expf(top), -95);
+            int32_t z[D / 4];
+#pragma unroll
+            for (int e = 0; e < D / 4; e++)  // |z| <= 2^30, biased so that its lower three bytes are digits + 128
+                z[e] = (bad ? 0 : static_cast<int32_t>(__builtin_rintf(__builtin_amdgcn_ldexpf(x[e], 30 - ex)))) + 0x808080;
+#pragma unroll
+            for (int p = 0; p < QP; p++) {
+                const int j = QP == 1 ? n / G : p * (16 / G) + n / G;  // this column's digit
+                const int shift = 8 * min(j, 3);
+                const uint32_t flip = j < 3 ? 0x80808080u : 0u, keep = j < 4 ? 0xffffffffu : 0u;
+                place[p] = bad ? __builtin_nanf("") : j < 4 ? __builtin_amdgcn_ldexpf(scale, ex - 30 + 8 * j) : 0.0f;
+#pragma unroll
+                for (int t = 0; t < NI8; t++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        w[k] = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            w[k] |= (static_cast<uint32_t>(z[16 * t + 4 * k + b]) >> shift & 255u) << (8 * b);
+                        w[k] = (w[k] ^ flip) & keep;
+                    }
+                    qd[p][t] = __builtin_bit_cast(i32x4_t, make_uint4(w[0], w[1], w[2], w[3]));
+                }
+            }
         } else {
 #pragma unroll
             for (int s = 0; s < NSLAB; s++) {
                 const int64_t i = q0 + k_dim0<D, KV>(s, q4);
                 if constexpr (!QF32) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        w[e] = static_cast<const uint16_t*>(a.d.q)[i + 2 * e] |
-                               static_cast<uint32_t>(static_cast<const uint16_t*>(a.d.q)[i + 2 * e + 1]) << 16;
-                    qb[0][s] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+                    qb[0][s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d.q) + i));
                 } else {
+                    const f32x4_t* src = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.d.q) + i);
+                    const f32x4_t x0 = src[0], x1 = src[1];
 #pragma unroll
                     for (int p = 0; p < QP; p++) {
                         const int part_n = PASSES == 1 ? n / G : p * (16 / G) + n / G;
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const float x0 = bf16_part(static_cast<const float*>(a.d.q)[i + 2 * e], part_n);
-                            const float x1 = bf16_part(static_cast<const float*>(a.d.q)[i + 2 * e + 1], part_n);
-                            w[e] = part_n < 3 ? pack_bf16_trunc(x0, x1) : 0;
+                            const float lo = bf16_part(e < 2 ? x0[2 * e] : x1[2 * e - 4], part_n);
+                            const float hi = bf16_part(e < 2 ? x0[2 * e + 1] : x1[2 * e - 3], part_n);
+                            w[e] = part_n < 3 ? pack_bf16_trunc(lo, hi) : 0;
                         }
                         qb[p][s] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
                     }
@@ -151,14 +221,12 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
             }
         }
     }
-    const float scale = a.d.scale * kLog2e;
     float m_run = -INFINITY, l_run = 0.0f;
     f32x4_t acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     bool any = false;
 
-    const int beg = part * a.per, end = min(beg + a.per, a.budget);
     const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
     for (int e0 = beg + wave; e0 < end; e0 += 64 * kSparseWaves) {
         // lane l: the wave's l-th block of this stretch
@@ -197,6 +265,24 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.k[u][i], qf[4 * u + i], s, 0, 0, 0);
+            } else if constexpr (I8) {
+                const float k_scale = readlane_f(ks, j);
+                i32x4_t c[QP];
+#pragma unroll
+                for (int p = 0; p < QP; p++) {
+                    c[p] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+                    for (int t = 0; t < NI8; t++)
+                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                            __builtin_bit_cast(i32x4_t, make_uint4(b.k[2 * t].x, b.k[2 * t].y, b.k[2 * t + 1].x, b.k[2 * t + 1].y)),
+                            qd[p][t], c[p], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+#pragma unroll
+                    for (int p = 0; p < QP; p++) s[i] = __builtin_fmaf(static_cast<float>(c[p][i]), place[p], s[i]);
+                    s[i] *= k_scale;
+                }
             } else {
 #pragma unroll
                 for (int sl = 0; sl < NSLAB; sl++) {
@@ -205,19 +291,17 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
                     for (int p = 0; p < QP; p++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qb[p][sl], s, 0, 0, 0);
                 }
             }
-            float f = scale;
-            if constexpr (KV == PA_DTYPE_INT8) f *= readlane_f(ks, j);
             float sc[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float x = s[i];
-                if constexpr (QF32 && !F32) {  // the partial scores of a head's parts
+                if constexpr ((QF32 && !F32) || I8) {  // the partial scores of a head's parts
                     if (G <= 8) x = add_ror<8>(x);
                     if (G <= 4) x = add_ror<4>(x);
                     if (G <= 2) x = add_ror<2>(x);
                     if (G <= 1) x = add_ror<1>(x);
                 }
-                sc[i] = x * f;
+                sc[i] = I8 ? x : x * scale;
             }
             const int lbj = __builtin_amdgcn_readlane(lb, j);
             const int t0 = KV == PA_DTYPE_BF16 ? 4 * tok_group<KV>(q4) : 4 * q4;
@@ -289,7 +373,7 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
                 }
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const s16x4_t vop = v_operand(b.v[t]);
+                    const s16x4_t vop = sparse_v_operand(b.v[t]);
 #pragma unroll
                     for (int q = 0; q < PP; q++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb[q], vop, acc[t], 0, 0, 0);
                 }
@@ -354,11 +438,11 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
                 o += x * f;
             }
             const int dim = c * CH + d;
-            if (a.parts == 1) {
+            if (end - beg == a.budget) {
                 // no token: zeros
                 a.d.out[(static_cast<int64_t>(row) * G + g) * D + dim] = L == 0.0f ? 0.0f : o / L;
             } else {
-                const int64_t pi = (static_cast<int64_t>(row) * a.parts + part) * G + g;
+                const int64_t pi = (2 * static_cast<int64_t>(blockIdx.x) + (beg == 0)) * G + g;
                 a.d.ws_o[pi * D + dim] = o;
                 if (dim == 0) {
                     a.d.ws_m[pi] = M;
@@ -367,33 +451,41 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
             }
         }
     }
+    if (at_entry < stop) __syncthreads();  // the states have been read
+    }
 }
 
-// The parts of a row: one wave per (row, query head), lanes over dims.
+// The parts of a row that was cut: one wave per (row, query head), lanes over dims. The first part lies in slot 1
+// of its range, the others in slot 0 of theirs.
 template <int D>
 __global__ __launch_bounds__(256) void sparse_merge_kernel(const SparseArgs a) {
     constexpr int DPL = (D + 63) / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t rows = static_cast<int64_t>(a.num_queries) * a.d.num_kv_heads * a.d.group;
-    const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (u >= rows) return;
-    const int64_t row = u / a.d.group;
-    const int g = static_cast<int>(u - row * a.d.group);
-    const int64_t p0 = row * a.parts * a.d.group + g;
+    const int lane = threadIdx.x & 63, G = a.d.group;
+    const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (u >= static_cast<int64_t>(a.rows) * G) return;
+    const uint32_t row = static_cast<uint32_t>(u) / G, range = a.range;
+    const int g = static_cast<int>(u - static_cast<int64_t>(row) * G);
+    const uint32_t first = row * a.budget / range, last = (row * a.budget + a.budget - 1) / range;
+    if (first == last) return;  // written whole
+    const auto part = [&](uint32_t w) { return (2 * static_cast<int64_t>(w) + (w == first)) * G + g; };
     float M = -INFINITY;
-    for (int p = 0; p < a.parts; p++) M = fmaxf(M, a.d.ws_m[p0 + static_cast<int64_t>(p) * a.d.group]);
+    for (uint32_t w0 = first; w0 <= last; w0 += 64) M = fmaxf(M, w0 + lane <= last ? a.d.ws_m[part(w0 + lane)] : -INFINITY);
+    M = wave_max(M);
     float L = 0.0f, o[DPL];
 #pragma unroll
     for (int k = 0; k < DPL; k++) o[k] = 0.0f;
-    for (int p = 0; p < a.parts; p++) {
-        const int64_t pi = p0 + static_cast<int64_t>(p) * a.d.group;
-        const float mp = a.d.ws_m[pi];
-        if (mp == -INFINITY && M > -INFINITY) continue;
-        const float f = mp == M ? 1.0f : __builtin_amdgcn_exp2f(mp - M);
-        L += a.d.ws_l[pi] * f;
+#pragma unroll 4
+    for (uint32_t w = first; w <= last; w++) {
+        const int64_t pi = part(w);
+        const float mp = a.d.ws_m[pi], lp = a.d.ws_l[pi];
+        float x[DPL];
 #pragma unroll
-        for (int k = 0; k < DPL; k++)
-            if (lane + 64 * k < D) o[k] += a.d.ws_o[pi * D + lane + 64 * k] * f;
+        for (int k = 0; k < DPL; k++) x[k] = lane + 64 * k < D ? a.d.ws_o[pi * D + lane + 64 * k] : 0.0f;
+        if (mp == -INFINITY && M > -INFINITY) continue;  // nothing of this part counts
+        const float f = mp == M ? 1.0f : __builtin_amdgcn_exp2f(mp - M);
+        L += lp * f;
+#pragma unroll
+        for (int k = 0; k < DPL; k++) o[k] += x[k] * f;
     }
 #pragma unroll
     for (int k = 0; k < DPL; k++)
@@ -402,7 +494,7 @@ __global__ __launch_bounds__(256) void sparse_merge_kernel(const SparseArgs a) {
 
 template <int D>
 void launch_sparse_decode(const SparseArgs& a, int kv_dtype, bool q_f32, hipStream_t s) {
-    const uint32_t grid = static_cast<uint32_t>(static_cast<int64_t>(a.num_queries) * a.d.num_kv_heads * a.parts);
+    const uint32_t all = static_cast<uint32_t>(a.rows) * a.budget, grid = (all + a.range - 1) / a.range;
     const int G = a.d.group;
     const auto go = [&](auto kernel) { kernel<<<grid, 64 * kSparseWaves, 0, s>>>(a); };
     const auto by_q = [&](auto kv, auto passes) {
@@ -418,8 +510,8 @@ void launch_sparse_decode(const SparseArgs& a, int kv_dtype, bool q_f32, hipStre
     if (kv_dtype == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>(), std::integral_constant<int, 1>());
     else if (kv_dtype == PA_DTYPE_BF16) by_group(std::integral_constant<int, PA_DTYPE_BF16>());
     else if constexpr (D >= 64) by_group(std::integral_constant<int, PA_DTYPE_INT8>());
-    if (a.parts > 1) {
-        const int64_t waves = static_cast<int64_t>(a.num_queries) * a.d.num_kv_heads * G;
+    if (a.range % a.budget != 0) {
+        const int64_t waves = static_cast<int64_t>(a.rows) * G;
         sparse_merge_kernel<D><<<static_cast<uint32_t>((waves + 3) / 4), 256, 0, s>>>(a);
     }
 }

@@ -6,18 +6,23 @@
 
 namespace {
 
-// Parts per row: enough workgroups for the chip's CUs, but two list entries a wave at least.
-int32_t sparse_parts(const pa_config* cfg, int32_t num_queries, int32_t budget) {
-    const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(num_queries) * cfg->num_kv_heads);
-    const int64_t want = (512 + rows - 1) / rows;
-    const int64_t most = std::max<int64_t>(1, budget / (2 * pa::kSparseWaves));
-    return static_cast<int32_t>(std::min(want, most));
+// List entries per workgroup: equal ranges for kGroups workgroups, one per CU, but kLeast entries a wave at least; whole
+// rows where that leaves few CUs idle, since no merge is needed then.
+constexpr int32_t kGroups = 256;
+constexpr int32_t kLeast = 2;
+int32_t sparse_range(int64_t rows, int32_t budget) {
+    int64_t r = (rows * budget + kGroups - 1) / kGroups;
+    r = std::max<int64_t>(r, kLeast * pa::kSparseWaves);
+    if (r > budget * 3ll / 4 && r <= budget) return budget;
+    return static_cast<int32_t>((r + pa::kSparseWaves - 1) / pa::kSparseWaves * pa::kSparseWaves);
 }
 
-// Partial states of all rows; 0 when every row is one part.
-size_t partial_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
-    const int32_t parts = sparse_parts(cfg, num_queries, budget);
-    return parts == 1 ? 0 : static_cast<size_t>(num_queries) * cfg->num_q_heads * parts;
+// Slots of partial states: two per range, none if no row is cut.
+size_t slot_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
+    const int64_t rows = static_cast<int64_t>(num_queries) * cfg->num_kv_heads;
+    if (rows == 0 || budget == 0) return 0;
+    const int32_t range = sparse_range(rows, budget);
+    return range % budget == 0 ? 0 : 2 * static_cast<size_t>((rows * budget + range - 1) / range) * (cfg->num_q_heads / cfg->num_kv_heads);
 }
 
 pa_status check_shape(const std::string& f, const pa_config* cfg, int32_t num_queries, int32_t budget) {
@@ -41,7 +46,7 @@ pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, in
     pa_status st = check_shape(f, cfg, num_queries, budget);
     if (st != PA_SUCCESS) return st;
     if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": bytes is null");
-    *bytes = partial_count(cfg, num_queries, budget) * (cfg->head_dim + 2) * sizeof(float);
+    *bytes = slot_count(cfg, num_queries, budget) * (cfg->head_dim + 2) * sizeof(float);
     return pa::clear_error();
 }
 
@@ -66,9 +71,9 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": num_queries must be num_seqs when query_seqs is null");
     if (cfg->kv_dtype == PA_DTYPE_INT8 && (!k_scale || !v_scale))
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": int8 cache needs k_scale and v_scale");
-    if (!pa::aligned16(k_cache) || !pa::aligned16(v_cache))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": cache pointers must be 16-byte aligned");
-    const size_t partials = partial_count(cfg, num_queries, budget);
+    if (!pa::aligned16(k_cache) || !pa::aligned16(v_cache) || !pa::aligned16(q))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": q and cache pointers must be 16-byte aligned");
+    const size_t partials = slot_count(cfg, num_queries, budget);
     const size_t need = partials * (cfg->head_dim + 2) * sizeof(float);
     if (need > workspace_bytes || (need > 0 && !workspace))
         return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
@@ -97,8 +102,8 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     a.num_seqs = num_seqs;
     a.num_queries = num_queries;
     a.budget = budget;
-    a.parts = sparse_parts(cfg, num_queries, budget);
-    a.per = (budget + a.parts - 1) / a.parts;
+    a.rows = num_queries * cfg->num_kv_heads;
+    a.range = sparse_range(a.rows, budget);
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
     const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;

@@ -55,6 +55,7 @@ def select(c=None, q=FAKE, b=FAKE, ks=None, tables=FAKE, seqs=4, width=300, rows
     (ARG, "null", dict(q=None)), (ARG, "null", dict(b=None)), (ARG, "null", dict(tables=None)),
     (ARG, "null", dict(lens=None)), (ARG, "null", dict(out=None)), (ARG, "query_seqs", dict(n=5)),
     (ARG, "k_scale", dict(c=cfg(kv_dtype=2))), (ARG, "aligned", dict(b=FAKE + 8)),
+    (ARG, "aligned", dict(q=FAKE + 8)), (CONFIG, "num_blocks", dict(c=cfg(num_blocks=0))),
     (SMALL, "workspace", dict(size=4 * 8 * 256 * 8 - 1)), (SMALL, "workspace", dict(ws=None)), (ARG, "aligned", dict(ws=FAKE + 4)),
 ])
 def test_select(status, text, kw):
@@ -75,6 +76,7 @@ def sparse(c=None, out=FAKE, q=FAKE, k=FAKE, v=FAKE, ks=None, vs=None, tables=FA
     (ARG, "budget", dict(budget=0)), (ARG, "null", dict(out=None)), (ARG, "null", dict(q=None)), (ARG, "null", dict(k=None)),
     (ARG, "null", dict(v=None)), (ARG, "null", dict(tables=None)), (ARG, "null", dict(lens=None)), (ARG, "null", dict(sel=None)),
     (ARG, "query_seqs", dict(n=5)), (ARG, "v_scale", dict(c=cfg(kv_dtype=2), ks=FAKE)), (ARG, "aligned", dict(v=FAKE + 8)),
+    (ARG, "aligned", dict(q=FAKE + 4)),
     (SMALL, "workspace", dict(size=0)), (SMALL, "workspace", dict(ws=None)), (ARG, "aligned", dict(ws=FAKE + 2)),
 ])
 def test_sparse_decode(status, text, kw):
