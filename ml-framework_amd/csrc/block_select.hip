@@ -63,7 +63,7 @@ __device__ __forceinline__ float elem(const uint4& w, int e) {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 // Bounds are read once: non-temporal loads (32 sequences of 8k to 32k tokens, 8 heads of 128 channels, bf16: 35.3 us
-// a selection, 39.9 with ordinary ones; the int8 kernel, whose instructions read half lines, loses by them).
+// a selection, 39.9 with ordinary ones; as the int8 kernel below has it).
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
     return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p)));
 }
@@ -346,9 +346,13 @@ __global__ __launch_bounds__(64 * kScoreWaves, score_waves(D, KV, QT)) void bloc
 // column a digit, eight columns a query, two queries a tile. The instruction sums the products over all 2 D
 // channels in 32 bits exactly; a block's score is its six column sums by their places, times the unit and
 // k_scale. The sums go through LDS to a lane per (query, block). Over 108 MB of bounds, three queries a sequence:
-// 114 us with byte dot products in the vector unit, 44 with the columns summed across lanes in fp64, 32 so.
+// 114 us with byte dot products in the vector unit, 44 with the columns summed across lanes in fp64, 32 with
+// the sums through LDS, 29 with the codes through LDS as well: whole rows a load instead of half lines, which also lets
+// the loads be non-temporal (67 us without that).
 constexpr int kDigits = 6;
-constexpr int kInt8Blocks = 128;  // blocks per wave (64: 49.7 us a selection where 128 takes 48.0, 256: 56.8)
+constexpr int kInt8Waves = 4;
+constexpr int kInt8Ahead = 2;  // tiles on their way (4: 32.3 us)
+constexpr int kInt8Blocks = 128;  // blocks per wave (29.2 us; 64: 31.6; 256 56.8 a selection where 128 took 48.0)
 
 // The digits of a (query, KV head), made once: one wave each. (Made by every wave of the scores, they took 27 of
 // its 46 us.)
@@ -396,15 +400,17 @@ __global__ __launch_bounds__(64) void int8_weights_kernel(const SelectArgs a) {
 // time, two tiles on their way while a third is scored. (The waves of a workgroup take neighbouring heads of the
 // same blocks, whose bounds lie side by side.)
 template <int D, int QT>
-__global__ __launch_bounds__(64 * kScoreWaves, D == 256 ? 2 : QT > 1 ? 3 : 4) void block_score_int8_kernel(const SelectArgs a, int32_t units,
+__global__ __launch_bounds__(64 * kInt8Waves, D == 256 ? 2 : QT > 1 ? 3 : 4) void block_score_int8_kernel(const SelectArgs a, int32_t units,
                                                                                             int32_t chunks, int32_t per) {
     constexpr int SL = 2 * D / 64;            // matrix slabs of 64 channels
     constexpr int SETS = (QT + 1) / 2;
     constexpr int TILES = kScoreBlocks / 16;
-    __shared__ i32x4 s_sum[kScoreWaves][SETS * 16][4];  // of each wave: [column][block] sums of a tile
+    constexpr int PPR = 2 * D / 16, RPI = 64 / PPR;  // 16-byte pieces of a block's bounds; blocks per load
+    __shared__ uint4 s_tile[kInt8Waves][16][PPR];    // of each wave: a tile, piece p of block b at p ^ b (no bank twice)
+    __shared__ i32x4 s_sum[kInt8Waves][SETS * 16][4];  // of each wave: [column][block] sums of a tile
     const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t u = blockIdx.x * kScoreWaves + wave;
+    const uint32_t u = blockIdx.x * kInt8Waves + wave;
     const uint32_t rc = u / static_cast<uint32_t>(a.hkv), unit = rc / static_cast<uint32_t>(chunks);
     const int h = static_cast<int>(u - rc * a.hkv);
     const int start = static_cast<int>(rc - unit * chunks) * per;
@@ -439,35 +445,47 @@ __global__ __launch_bounds__(64 * kScoreWaves, D == 256 ? 2 : QT > 1 ? 3 : 4) vo
         const int64_t row_of = static_cast<int64_t>(r_of) * a.hkv + h;
         const double unit_of = a.units[row_of];
         double* out = a.scores + row_of * a.max_blocks;
-        uint4 v[2][SL];
-        float ks[2];
-        auto load = [&](int gi, uint4 (&x)[SL], float& sc) {  // tile gi: lane (q4, n) the codes 64 s + 16 q4 .. of block n
+        uint4 v[kInt8Ahead][SL];
+        float ks[kInt8Ahead];
+        auto load = [&](int gi, uint4 (&x)[SL], float& sc) {  // tile gi: blocks side by side, a row of lanes each
             // (a block out of the pool or past the chunk: block 0, times a scale of zero)
-            const int o = __shfl(id, (16 * gi + n) & 63, 64), b = max(0, o);
-            const uint4* row = reinterpret_cast<const uint4*>(base + (static_cast<int64_t>(b) * a.hkv + h) * 2 * D) + q4;
 #pragma unroll
-            for (int s = 0; s < SL; s++) x[s] = row[4 * s];
-            const float k = a.k_scale[static_cast<int64_t>(b) * a.hkv + h];
+            for (int i = 0; i < SL; i++) {
+                const int b = max(0, __shfl(id, (16 * gi + RPI * i + lane / PPR) & 63, 64));
+                x[i] = load_once(reinterpret_cast<const uint4*>(base + (static_cast<int64_t>(b) * a.hkv + h) * 2 * D) + lane % PPR);
+            }
+            const int o = __shfl(id, (16 * gi + n) & 63, 64);
+            const float k = a.k_scale[static_cast<int64_t>(max(0, o)) * a.hkv + h];
             sc = o >= 0 ? k : 0.0f;
         };
-        load(0, v[0], ks[0]);
-        load(1, v[1], ks[1]);
+#pragma unroll
+        for (int k = 0; k < kInt8Ahead; k++) load(k, v[k], ks[k]);
         while (first < g.last) {
             // the ids of the next 64 blocks
             const int after = first + kScoreBlocks;
             int next = -1;
             if (after + lane < g.last) next = a.tables[static_cast<int64_t>(seq) * a.width + after + lane];
 #pragma unroll 1
-            for (int g0 = 0; g0 < TILES; g0 += 2) {
+            for (int g0 = 0; g0 < TILES; g0 += kInt8Ahead) {
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
+                for (int k = 0; k < kInt8Ahead; k++) {
                     const int gi = g0 + k;
+#pragma unroll
+                    for (int i = 0; i < SL; i++) {
+                        const int row = RPI * i + lane / PPR;
+                        s_tile[wave][row][(lane % PPR) ^ (row % PPR)] = v[k][i];
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    i32x4 x[SL];  // the matrix operand: lane (q4, n) codes 64 s + 16 q4 .. of block n
+#pragma unroll
+                    for (int s = 0; s < SL; s++) x[s] = __builtin_bit_cast(i32x4, s_tile[wave][n][(4 * s + q4) ^ (n % PPR)]);
 #pragma unroll
                     for (int p = 0; p < SETS; p++) {
                         i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
                         for (int s = 0; s < SL; s++)
-                            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, v[k][s]), wt[p][s], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[s], wt[p][s], acc, 0, 0, 0);
                         s_sum[wave][16 * p + n][q4] = acc;  // blocks 4 q4 .. + 3 of column n
                     }
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -482,8 +500,8 @@ __global__ __launch_bounds__(64 * kScoreWaves, D == 256 ? 2 : QT > 1 ? 3 : 4) vo
                     if (q4 < QT && b < end_of) out[b] = y * unit_of * static_cast<double>(ks[k]);
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     __builtin_amdgcn_wave_barrier();
-                    if (gi == TILES - 2) id = next < a.num_blocks ? next : -1;  // tiles 0 and 1 of the next ones follow
-                    load((gi + 2) % TILES, v[k], ks[k]);
+                    if (gi == TILES - kInt8Ahead) id = next < a.num_blocks ? next : -1;  // the next ones' tiles follow
+                    load((gi + kInt8Ahead) % TILES, v[k], ks[k]);
                 }
             }
             first = after;
@@ -704,9 +722,9 @@ bool launch_score(const SelectArgs& a, int kv, int32_t most, hipStream_t s) {
             const int32_t per = kInt8Blocks;
             const int32_t chunks = (most + per - 1) / per;
             const int64_t waves = static_cast<int64_t>(units) * chunks * a.hkv;
-            if (waves > INT32_MAX - kScoreWaves) return false;
+            if (waves > INT32_MAX - kInt8Waves) return false;
             const auto go = [&](auto kernel) {
-                kernel<<<static_cast<uint32_t>((waves + kScoreWaves - 1) / kScoreWaves), 64 * kScoreWaves, 0, s>>>(a, units, chunks, per);
+                kernel<<<static_cast<uint32_t>((waves + kInt8Waves - 1) / kInt8Waves), 64 * kInt8Waves, 0, s>>>(a, units, chunks, per);
             };
             int8_weights_kernel<D><<<a.num_queries * a.hkv, 64, 0, s>>>(a);
             if (grouped) go(block_score_int8_kernel<D, kQueryTile>);
@@ -740,14 +758,14 @@ void launch_choose(const SelectArgs& a, int32_t most, hipStream_t s) {
     block_choose_kernel<T, HELD><<<a.num_queries * a.hkv, T, words * (12 + (HELD ? 256 : 0)) + 8, s>>>(a);
 }
 
-pa_status check_sizes(const std::string& f, const pa_config* cfg, int32_t num_queries, int32_t max_context_len) {
+pa_status check_sizes(const char* f, const pa_config* cfg, int32_t num_queries, int32_t max_context_len) {
     if (num_queries < 0 || max_context_len < 0)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (max_context_len > kMaxBlocks * pa::kBlockSize)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": max_context_len must be <= " +
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": max_context_len must be <= " +
                                                        std::to_string(kMaxBlocks * pa::kBlockSize));
     if (static_cast<int64_t>(num_queries) * cfg->num_kv_heads > 1 << 24)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many query tokens for one call");
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many query tokens for one call");
     return PA_SUCCESS;
 }
 
@@ -768,10 +786,10 @@ size_t workspace_of(const pa_config* cfg, int32_t num_queries, int32_t max_conte
 extern "C" {
 
 pa_status pa_select_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t max_context_len, size_t* bytes) {
-    const std::string f = "pa_select_workspace_size";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_select_workspace_size";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
-    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": bytes is null");
+    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": bytes is null");
     st = check_sizes(f, cfg, num_queries, max_context_len);
     if (st != PA_SUCCESS) return st;
     *bytes = workspace_of(cfg, num_queries, max_context_len);
@@ -783,33 +801,33 @@ pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* 
                            int32_t max_blocks_per_seq, const int32_t* query_seqs, const int32_t* context_lens,
                            int32_t num_queries, int32_t max_context_len, int32_t sink_blocks, int32_t recent_blocks,
                            int32_t budget, int32_t* selected, void* workspace, size_t workspace_bytes) {
-    const std::string f = "pa_select_blocks";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_select_blocks";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
-    if (num_seqs < 0 || max_blocks_per_seq < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (num_seqs < 0 || max_blocks_per_seq < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     st = check_sizes(f, cfg, num_queries, max_context_len);
     if (st != PA_SUCCESS) return st;
     if (sink_blocks < 0 || recent_blocks < 1)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": sink_blocks must be >= 0 and recent_blocks >= 1");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": sink_blocks must be >= 0 and recent_blocks >= 1");
     if (budget < 1 || static_cast<int64_t>(sink_blocks) + recent_blocks > budget)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": budget must hold the sink and recent blocks");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": budget must hold the sink and recent blocks");
     if (static_cast<int64_t>(num_queries) * cfg->num_kv_heads * budget > INT32_MAX)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many query tokens for one call");
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many query tokens for one call");
     if (num_queries == 0) return pa::clear_error();
-    if (cfg->num_blocks == 0) return pa::set_error(PA_ERROR_INVALID_CONFIG, f + ": num_blocks must be > 0");
+    if (cfg->num_blocks == 0) return pa::set_error(PA_ERROR_INVALID_CONFIG, std::string(f) + ": num_blocks must be > 0");
     if (!q || !key_bounds || !block_tables || !context_lens || !selected)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
     if (!query_seqs && num_queries != num_seqs)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": num_queries must be num_seqs when query_seqs is null");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": num_queries must be num_seqs when query_seqs is null");
     if (cfg->kv_dtype == PA_DTYPE_INT8 && !k_scale)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": int8 cache needs k_scale");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": int8 cache needs k_scale");
     if (!pa::aligned16(key_bounds) || !pa::aligned16(q))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": q and key_bounds must be 16-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": q and key_bounds must be 16-byte aligned");
     const size_t need = workspace_of(cfg, num_queries, max_context_len);
     if (need > workspace_bytes || (need > 0 && !workspace))
-        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, std::string(f) + ": workspace needs " + std::to_string(need) + " bytes");
     if (!pa::aligned16(workspace))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 16-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": workspace must be 16-byte aligned");
     SelectArgs a{};
     a.q = q;
     a.bounds = key_bounds;
@@ -844,7 +862,7 @@ pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* 
             case 128: fits = launch_score<128>(a, cfg->kv_dtype, most, s); break;
             default: fits = launch_score<256>(a, cfg->kv_dtype, most, s); break;
         }
-        if (!fits) return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many blocks for one call");
+        if (!fits) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
         PA_HIP_CHECK(hipGetLastError());
     }
     // (512 threads of 1024 blocks 5.1 us, 256 5.7; 1024 of 2048 blocks 7.0 us, 512 8.0)

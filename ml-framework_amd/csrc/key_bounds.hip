@@ -132,21 +132,21 @@ pa_status pa_key_bounds_bytes(const pa_config* cfg, size_t* bytes) {
 pa_status pa_key_bounds_update(pa_stream* stream, const pa_config* cfg, const void* k_cache, const int32_t* block_tables,
                                int32_t max_blocks_per_seq, const int32_t* start_pos, const int32_t* num_new,
                                int32_t num_seqs, int32_t max_new_per_seq, void* key_bounds) {
-    const std::string f = "pa_key_bounds_update";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_key_bounds_update";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
     if (num_seqs < 0 || max_new_per_seq < 0 || max_blocks_per_seq < 0)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (num_seqs == 0 || max_new_per_seq == 0 || max_blocks_per_seq == 0) return pa::clear_error();
-    if (num_seqs > 65535) return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": num_seqs must be <= 65535");
+    if (num_seqs > 65535) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": num_seqs must be <= 65535");
     if (!k_cache || !block_tables || !start_pos || !num_new || !key_bounds)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
     if (!pa::aligned16(k_cache) || !pa::aligned16(key_bounds))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": k_cache and key_bounds must be 16-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": k_cache and key_bounds must be 16-byte aligned");
     // A sequence's new tokens touch at most this many blocks (the first may start inside one).
     const int64_t reach = std::min<int64_t>((static_cast<int64_t>(max_new_per_seq) + 14) / 16 + 1, max_blocks_per_seq);
     const int64_t waves = reach * cfg->num_kv_heads;
-    if (waves > INT32_MAX) return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many blocks for one call");
+    if (waves > INT32_MAX) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
     pa::StreamDevice dev(stream);
     const dim3 grid(static_cast<uint32_t>((waves + kWaves - 1) / kWaves), num_seqs);
     hipStream_t s = pa::native(stream);

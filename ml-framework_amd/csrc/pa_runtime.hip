@@ -45,24 +45,24 @@ pa_status clear_error() {
 }
 
 pa_status check_config(const pa_config* cfg, const char* fn) {
-    std::string f(fn);
-    if (!cfg) return set_error(PA_ERROR_INVALID_ARGUMENT, f + ": cfg is null");
+    // (strings are built for a refusal only: this runs on every call)
+    const auto refuse = [&](pa_status st, const char* text) { return set_error(st, std::string(fn) + text); };
+    if (!cfg) return refuse(PA_ERROR_INVALID_ARGUMENT, ": cfg is null");
     if (cfg->block_size != kBlockSize)
-        return set_error(PA_ERROR_UNSUPPORTED, f + ": block_size must be 16");
+        return refuse(PA_ERROR_UNSUPPORTED, ": block_size must be 16");
     if (cfg->num_q_heads <= 0 || cfg->num_kv_heads <= 0 || cfg->num_q_heads % cfg->num_kv_heads != 0)
-        return set_error(PA_ERROR_INVALID_CONFIG,
-                         f + ": num_q_heads must be a positive multiple of num_kv_heads");
+        return refuse(PA_ERROR_INVALID_CONFIG, ": num_q_heads must be a positive multiple of num_kv_heads");
     if (cfg->head_dim != 32 && cfg->head_dim != 64 && cfg->head_dim != 128 && cfg->head_dim != 256)
-        return set_error(PA_ERROR_UNSUPPORTED, f + ": head_dim must be 32, 64, 128 or 256");
+        return refuse(PA_ERROR_UNSUPPORTED, ": head_dim must be 32, 64, 128 or 256");
     if (cfg->kv_dtype != PA_DTYPE_FP32 && cfg->kv_dtype != PA_DTYPE_BF16 && cfg->kv_dtype != PA_DTYPE_INT8)
-        return set_error(PA_ERROR_UNSUPPORTED, f + ": kv_dtype must be FP32, BF16 or INT8");
+        return refuse(PA_ERROR_UNSUPPORTED, ": kv_dtype must be FP32, BF16 or INT8");
     // int8 codes meet the int8 MFMA (64 dims per instruction) and 64-lane quantiser rows.
     if (cfg->kv_dtype == PA_DTYPE_INT8 && cfg->head_dim < 64)
-        return set_error(PA_ERROR_UNSUPPORTED, f + ": int8 caches take head_dim 64, 128 or 256");
+        return refuse(PA_ERROR_UNSUPPORTED, ": int8 caches take head_dim 64, 128 or 256");
     if (cfg->q_dtype != PA_DTYPE_FP32 && cfg->q_dtype != PA_DTYPE_BF16)
-        return set_error(PA_ERROR_UNSUPPORTED, f + ": q_dtype must be FP32 or BF16");
-    if (cfg->num_blocks < 0) return set_error(PA_ERROR_INVALID_CONFIG, f + ": num_blocks < 0");
-    if (!(cfg->scale == cfg->scale)) return set_error(PA_ERROR_INVALID_CONFIG, f + ": scale is NaN");
+        return refuse(PA_ERROR_UNSUPPORTED, ": q_dtype must be FP32 or BF16");
+    if (cfg->num_blocks < 0) return refuse(PA_ERROR_INVALID_CONFIG, ": num_blocks < 0");
+    if (!(cfg->scale == cfg->scale)) return refuse(PA_ERROR_INVALID_CONFIG, ": scale is NaN");
     return PA_SUCCESS;
 }
 

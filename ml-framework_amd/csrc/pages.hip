@@ -503,11 +503,11 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 extern "C" {
 
 pa_status pa_pages_workspace_size(const pa_config* cfg, int32_t num_rows, int32_t max_blocks_per_seq, size_t* bytes) {
-    const std::string f = "pa_pages_workspace_size";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_pages_workspace_size";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
-    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": bytes is null");
-    if (num_rows < 0 || max_blocks_per_seq < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": bytes is null");
+    if (num_rows < 0 || max_blocks_per_seq < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     *bytes = static_cast<size_t>(scratch_ints(cfg, num_rows, max_blocks_per_seq)) * 4;
     return pa::clear_error();
 }
@@ -515,21 +515,21 @@ pa_status pa_pages_workspace_size(const pa_config* cfg, int32_t num_rows, int32_
 pa_status pa_pages_fork(pa_stream* stream, const pa_config* cfg, const int32_t* tables_in, const int32_t* lens_in,
                         int32_t num_in, const int32_t* src, int32_t* tables_out, int32_t* lens_out, int32_t num_out,
                         int32_t max_blocks_per_seq, int32_t* refcounts) {
-    const std::string f = "pa_pages_fork";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_pages_fork";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
     if (num_in < 0 || num_out < 0 || max_blocks_per_seq < 0)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (static_cast<int64_t>(num_in) + num_out == 0) return pa::clear_error();
     if (static_cast<int64_t>(num_in) + num_out > INT32_MAX)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many rows for one call");
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many rows for one call");
     if (!refcounts || (num_in > 0 && (!tables_in || !lens_in)) || (num_out > 0 && (!src || !tables_out || !lens_out)))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
     const int64_t row = static_cast<int64_t>(max_blocks_per_seq) * 4;
     if (num_in > 0 && num_out > 0 &&
         (overlap(tables_in, num_in * row, tables_out, num_out * row) || overlap(lens_in, num_in * 4ll, lens_out, num_out * 4ll) ||
          overlap(src, num_out * 4ll, lens_out, num_out * 4ll) || overlap(src, num_out * 4ll, tables_out, num_out * row)))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": the out rows must not overlap the inputs");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": the out rows must not overlap the inputs");
     pa::StreamDevice dev(stream);
     pages_fork_kernel<<<num_out + num_in, kForkThreads, 0, pa::native(stream)>>>(
         tables_in, lens_in, num_in, src, tables_out, lens_out, num_out, max_blocks_per_seq, refcounts, cfg->num_blocks);
@@ -541,23 +541,23 @@ pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tab
                            const int32_t* num_new, int32_t num_rows, int32_t max_blocks_per_seq,
                            int32_t max_new_per_row, int32_t* refcounts, int32_t* copy_pairs, int32_t* status,
                            void* workspace, size_t workspace_bytes) {
-    const std::string f = "pa_pages_reserve";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_pages_reserve";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
     if (num_rows < 0 || max_blocks_per_seq < 0 || max_new_per_row < 0)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
-    if (!status) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": status is null");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
+    if (!status) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": status is null");
     if (num_rows > 0 && (!tables || !lens || !num_new || !refcounts || !copy_pairs))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
     // Blocks that one row's new tokens can touch.
     const int64_t reach = std::min<int64_t>(max_new_per_row == 0 ? 0 : (static_cast<int64_t>(max_new_per_row) + 14) / 16 + 1,
                                             max_blocks_per_seq);
-    if (reach * num_rows > INT32_MAX) return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many rows for one call");
+    if (reach * num_rows > INT32_MAX) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many rows for one call");
     const size_t need = static_cast<size_t>(scratch_ints(cfg, num_rows, max_blocks_per_seq)) * 4;
     if (need > workspace_bytes || (need > 0 && !workspace))
-        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, std::string(f) + ": workspace needs " + std::to_string(need) + " bytes");
     if (reinterpret_cast<uintptr_t>(workspace) & 3)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 4-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": workspace must be 4-byte aligned");
     ReserveArgs a{};
     a.tables = tables;
     a.lens = lens;
@@ -585,19 +585,19 @@ pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tab
 pa_status pa_pages_compact(pa_stream* stream, const pa_config* cfg, int32_t* tables, int32_t num_rows,
                            int32_t max_blocks_per_seq, int32_t* refcounts, int32_t max_moves, int32_t* pairs,
                            int32_t* status, void* workspace, size_t workspace_bytes) {
-    const std::string f = "pa_pages_compact";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_pages_compact";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
     if (num_rows < 0 || max_blocks_per_seq < 0 || max_moves < 0)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (!status || (cfg->num_blocks > 0 && !refcounts) || (max_moves > 0 && !pairs) ||
         (num_rows > 0 && max_blocks_per_seq > 0 && !tables))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
     const size_t need = static_cast<size_t>(scratch_ints(cfg, num_rows, max_blocks_per_seq)) * 4;
     if (need > workspace_bytes || !workspace)
-        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, std::string(f) + ": workspace needs " + std::to_string(need) + " bytes");
     if (reinterpret_cast<uintptr_t>(workspace) & 3)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 4-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": workspace must be 4-byte aligned");
     CompactArgs a{};
     a.tables = tables;
     a.refs = refcounts;
@@ -623,18 +623,18 @@ pa_status pa_pages_compact(pa_stream* stream, const pa_config* cfg, int32_t* tab
 pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, void* v_cache, float* k_scale,
                         float* v_scale, float* k_absmax, float* v_absmax, void* key_bounds, const int32_t* pairs,
                         int32_t max_pairs, const int32_t* num_pairs) {
-    const std::string f = "pa_copy_pages";
-    pa_status st = pa::check_config(cfg, f.c_str());
+    const char* const f = "pa_copy_pages";
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
-    if (max_pairs < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": max_pairs < 0");
-    if (!k_cache || !v_cache) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null cache pointer");
+    if (max_pairs < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": max_pairs < 0");
+    if (!k_cache || !v_cache) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null cache pointer");
     if (!pa::aligned16(k_cache) || !pa::aligned16(v_cache) || !pa::aligned16(key_bounds))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": cache and key_bounds pointers must be 16-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": cache and key_bounds pointers must be 16-byte aligned");
     const bool int8 = cfg->kv_dtype == PA_DTYPE_INT8;
     if (int8 && (!k_scale || !v_scale || !k_absmax || !v_absmax))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": int8 cache needs scales and absmax");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": int8 cache needs scales and absmax");
     if (max_pairs == 0) return pa::clear_error();
-    if (!pairs) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": pairs is null");
+    if (!pairs) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": pairs is null");
     CopyArgs c{};
     c.k = static_cast<char*>(k_cache);
     c.v = static_cast<char*>(v_cache);

@@ -25,15 +25,15 @@ size_t slot_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
     return range % budget == 0 ? 0 : 2 * static_cast<size_t>((rows * budget + range - 1) / range) * (cfg->num_q_heads / cfg->num_kv_heads);
 }
 
-pa_status check_shape(const std::string& f, const pa_config* cfg, int32_t num_queries, int32_t budget) {
-    pa_status st = pa::check_config(cfg, f.c_str());
+pa_status check_shape(const char* f, const pa_config* cfg, int32_t num_queries, int32_t budget) {
+    pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
     const int32_t g = cfg->num_q_heads / cfg->num_kv_heads;
     if (g > 16 || (g & (g - 1)) != 0)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": num_q_heads / num_kv_heads must be 1, 2, 4, 8 or 16");
-    if (num_queries < 0 || budget < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": num_q_heads / num_kv_heads must be 1, 2, 4, 8 or 16");
+    if (num_queries < 0 || budget < 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (static_cast<int64_t>(num_queries) * cfg->num_kv_heads * std::max(budget, 1) > INT32_MAX)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": too many query tokens for one call");
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many query tokens for one call");
     return PA_SUCCESS;
 }
 
@@ -42,10 +42,10 @@ pa_status check_shape(const std::string& f, const pa_config* cfg, int32_t num_qu
 extern "C" {
 
 pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t budget, size_t* bytes) {
-    const std::string f = "pa_sparse_workspace_size";
+    const char* const f = "pa_sparse_workspace_size";
     pa_status st = check_shape(f, cfg, num_queries, budget);
     if (st != PA_SUCCESS) return st;
-    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": bytes is null");
+    if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": bytes is null");
     *bytes = slot_count(cfg, num_queries, budget) * (cfg->head_dim + 2) * sizeof(float);
     return pa::clear_error();
 }
@@ -56,29 +56,29 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
                            const int32_t* query_seqs, const int32_t* context_lens, int32_t num_queries,
                            int32_t max_context_len, const int32_t* selected, int32_t budget, void* workspace,
                            size_t workspace_bytes) {
-    const std::string f = "pa_sparse_decode";
+    const char* const f = "pa_sparse_decode";
     pa_status st = check_shape(f, cfg, num_queries, budget);
     if (st != PA_SUCCESS) return st;
     if (num_seqs < 0 || max_blocks_per_seq < 0 || max_context_len < 0)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": negative size");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (max_blocks_per_seq > INT32_MAX / pa::kBlockSize)
-        return pa::set_error(PA_ERROR_UNSUPPORTED, f + ": max_blocks_per_seq * 16 must fit 32 bits");
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": max_blocks_per_seq * 16 must fit 32 bits");
     if (num_queries == 0) return pa::clear_error();
-    if (budget == 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": budget must be >= 1");
+    if (budget == 0) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": budget must be >= 1");
     if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens || !selected)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": null pointer");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
     if (!query_seqs && num_queries != num_seqs)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": num_queries must be num_seqs when query_seqs is null");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": num_queries must be num_seqs when query_seqs is null");
     if (cfg->kv_dtype == PA_DTYPE_INT8 && (!k_scale || !v_scale))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": int8 cache needs k_scale and v_scale");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": int8 cache needs k_scale and v_scale");
     if (!pa::aligned16(k_cache) || !pa::aligned16(v_cache) || !pa::aligned16(q))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": q and cache pointers must be 16-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": q and cache pointers must be 16-byte aligned");
     const size_t partials = slot_count(cfg, num_queries, budget);
     const size_t need = partials * (cfg->head_dim + 2) * sizeof(float);
     if (need > workspace_bytes || (need > 0 && !workspace))
-        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, f + ": workspace needs " + std::to_string(need) + " bytes");
+        return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, std::string(f) + ": workspace needs " + std::to_string(need) + " bytes");
     if (reinterpret_cast<uintptr_t>(workspace) & 3)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, f + ": workspace must be 4-byte aligned");
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": workspace must be 4-byte aligned");
     pa::SparseArgs a{};
     a.d.out = out;
     a.d.q = q;
