@@ -466,7 +466,8 @@ pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, in
  * Lists come from pa_select_blocks or from the caller: entries that are negative or at or past the end
  * of the context are skipped wherever they stand, in any order; a block listed twice counts twice.
  * Blocks whose table entry lies outside [0, num_blocks) read as zero keys and values. A query without
- * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter. Products are
+ * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter; queries, keys and
+ * values of listed tokens that are not finite give outputs that are not. Products are
  * exact and sums in fp32 for every cache and query type. num_q_heads / num_kv_heads: 1, 2, 4, 8 or
  * 16. q and caches 16-byte aligned. */
 pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, const void* q,

@@ -717,6 +717,7 @@ bool launch_score(const SelectArgs& a, int kv, int32_t most, hipStream_t s) {
     // Units are sequences where they have several queries each on average, else queries.
     const bool grouped = a.query_seqs && a.num_queries > a.num_seqs;
     const int32_t units = grouped ? a.num_seqs : a.num_queries;
+    if (units == 0) return true;  // queries of no sequence: nothing is scored
     if (kv == PA_DTYPE_INT8) {
         if constexpr (D >= 64) {
             const int32_t per = kInt8Blocks;

@@ -341,6 +341,56 @@ def test_sparse_decode_several_queries_of_a_sequence():
     close(run_sparse(p, g, qs, rows, [10 ** 6] * 10, sel, max_len=555), want, tol)
 
 
+@pytest.mark.parametrize("kv", [BF16, INT8])
+def test_no_sequences_and_empty_contexts(kv):
+    """Queries whose sequence does not exist (none does, or theirs does not): nothing selected, zeros attended."""
+    p = ref.Pool(52, [16 * 30], 8, 2, 64, kv)
+    qs, g = p.queries(3), gpu_pool(p)
+    for seqs, rows in ((0, [0, 0, 0]), (1, [1, -1, 7])):
+        q, p.tables = p.tables, p.tables[:seqs] if seqs else p.tables[:0]
+        sel = run_select(p, g, qs, rows, [480, 480, 480], 1, 2, 9)
+        out = run_sparse(p, g, qs, rows, [480, 480, 480], np.tile(np.arange(9, dtype=np.int32), (3, 2, 1)))
+        p.tables = q
+        assert (sel == -1).all() and (out == 0).all()
+
+
+@pytest.mark.parametrize("kv,hkv,d,nb", [(BF16, 8, 128, 150000), (FP32, 8, 256, 36000), (INT8, 8, 256, 140000)])
+def test_blocks_past_four_gigabytes(kv, hkv, d, nb):
+    """The same blocks at the far end of a pool whose keys pass 4 GiB (and whose bounds, for fp32, do not): the same bits."""
+    import torch
+    lens = [16 * 20 + 3, 16 * 9]
+    p = ref.Pool(53, lens, hkv, hkv, d, kv, BF16)
+    qs, g = p.queries(2), gpu_pool(p)
+    near = [run_bounds(p, g, [0, 0], lens), run_select(p, g, qs, None, lens, 1, 2, 8)]
+    near.append(run_sparse(p, g, qs, None, lens, near[1]))
+    dt = {FP32: torch.float32, BF16: torch.int16, INT8: torch.int8}[kv]
+    far = {"k": torch.empty(nb, hkv, 16, d, dtype=dt, device="cuda:0"), "v": torch.empty(nb, hkv, d, 16, dtype=dt, device="cuda:0"),
+           "bounds": torch.empty(nb, hkv, 2, d, dtype=dt, device="cuda:0")}
+    assert far["k"].numel() * far["k"].element_size() > 1 << 32
+    shift = nb - p.nb
+    for name in ("k", "v", "bounds"):
+        far[name][shift - 100:shift - 100 + p.nb] = g[name]  # (bounds are as key_bounds_update left them)
+    far["stats"] = [torch.zeros(nb, hkv, device="cuda:0") if s is not None else None for s in g["stats"]]
+    for a, b in zip(far["stats"], g["stats"]):
+        if a is not None:
+            a[shift - 100:shift - 100 + p.nb] = b
+    # copied page by page to the very end, then everything done there
+    small, p.cfg.num_blocks = p.nb, nb
+    pairs = to_gpu(np.stack([np.arange(small) + shift - 100, np.arange(small) + shift], 1).astype(np.int32))
+    pa.copy_pages(None, p.cfg, far["k"], far["v"], *far["stats"], far["bounds"], pairs, small)
+    p.tables = np.where(p.tables >= 0, p.tables + shift, -1).astype(np.int32)
+    far["tables"] = to_gpu(p.tables)
+    far["bounds"][shift:] = 0
+    pa.key_bounds_update(None, p.cfg, far["k"], far["tables"], p.width, to_gpu(np.zeros(2, np.int32)), to_gpu(p.lens), 2, max(lens),
+                         far["bounds"])
+    torch.cuda.synchronize()
+    moved = to_np(far["bounds"][shift:], ref.NP_DTYPE[kv])
+    used = np.unique(p.tables[p.tables >= 0]) - shift
+    np.testing.assert_array_equal(moved[used], near[0][used])
+    np.testing.assert_array_equal(run_select(p, far, qs, None, lens, 1, 2, 8), near[1])
+    np.testing.assert_array_equal(run_sparse(p, far, qs, None, lens, near[1]), near[2])
+
+
 def test_all_blocks_selected_is_the_dense_decode():
     import torch
     lens = [5, 300, 1024, 77]
