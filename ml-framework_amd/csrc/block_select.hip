@@ -10,8 +10,9 @@
 // choose differently wherever two scores near the border are closer than its rounding.
 //
 // Two launches. The scores read 2 D elements per (block, KV head), which bounds them by traffic (a
-// sixteenth of the K and V bytes): one wave per 64 blocks of a KV head, 16-byte loads. The choice is
-// one workgroup per (query token, KV head): see block_choose_kernel.
+// sixteenth of the K and V bytes): a wave per 32 blocks of a KV head (int8: 128), 16-byte loads. The choice is
+// one workgroup per (query token, KV head): see block_choose_kernel. (Both in one launch, a workgroup a row, is slower at
+// every size tried: one row of 313 blocks 10.7 us where this takes 9.1, 512 rows 26.6 and 21.4.)
 #include <algorithm>
 #include <string>
 
@@ -143,7 +144,7 @@ struct QueryGroup {
 
 // f(group, sequence, id) for the queries of unit `unit`: the query itself, or (QT > 1) all those of sequence
 // `unit`, QT at a time. id: the sequence's table entry at block `at` of its context, read without waiting for the
-// context's length (any value past it). Everything else is the same in all lanes of the workgroup.
+// context's length (any value past it). Everything else is the same in all lanes of the wave.
 template <int QT, typename F>
 __device__ __forceinline__ void for_query_groups(const SelectArgs& a, int unit, int first, int per, int at, F&& f) {
     QueryGroup<QT> g;
@@ -733,7 +734,8 @@ bool launch_score(const SelectArgs& a, int kv, int32_t most, hipStream_t s) {
         }
         return true;
     }
-    // Blocks per wave: a whole number of batches, halved while the waves are too few for the chip.
+    // Blocks per wave: 32 (64 time the same where the chip is full, 16 leave too little to stream: 49 us a selection of
+    // 32 long contexts where 32 took 42), a batch at least, halved while the waves are too few for the chip.
     const int32_t lanes = std::min(64, 2 * D * (kv == PA_DTYPE_FP32 ? 4 : 2) / 16);
     const int32_t batch = 64 / lanes * score_batch(grouped ? kQueryTile : 1);
     int32_t per = std::max(batch, 32);
