@@ -10,8 +10,8 @@
 // kSparseWaves, ..); a wave streams its blocks through rotating register buffers, one pass with the running maximum
 // and sum, and no wave waits for another until the segment ends. There the waves' states meet in LDS; a
 // segment that is a whole row is finished at once, the parts of the others (at most two a range) by a merge launch.
-// Measured: 256 rows of 128 bf16 blocks (D 128, 269 MB) 48 us, 5.6 TB/s; in two workgroups a row, with
-// a merge, 55 us. 384 rows of 255 int8 blocks (404 MB) 87 us, 4.7 TB/s; in three rounds of half rows 95 us.
+// Measured: 256 rows of 128 bf16 blocks (D 128, 269 MB) 47 us, 5.7 TB/s; in two workgroups a row, with
+// a merge, 55 us. 384 rows of 255 int8 blocks (404 MB) 85 us, 4.8 TB/s; in three rounds of half rows 95 us.
 //
 // K and V are read once and G = Hq / Hkv query heads share them (2 G flops a byte at bf16): traffic
 // bounds it. The matrix instructions are 16 columns wide and G is 1 to 16, so the columns that a
@@ -26,6 +26,8 @@
 // conversion's time). The int8 case is bound by its traffic all the same: with the P V product left out
 // altogether it takes 86 us. What it lacks against bf16 is the run length, 2 KiB instead of 4 a tile.
 #pragma once
+
+#include <cfloat>
 
 #include "decode_mfma.h"
 
@@ -404,18 +406,21 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
     }
 
     // ---- the waves' states meet ----
-    // A wave whose every score was -inf (or NaN) still has its maximum at -inf: its sum says so.
-    if (any && m_run == -INFINITY) l_run = __builtin_nanf("");
+    // A wave that saw tokens but no score above -inf is told from one that saw none by the lowest finite maximum:
+    // where no score of the row is, its sum is 0 and the outcome 0 / 0. A NaN score leaves the sum NaN. (The exchange
+    // with a branch per wave and its reads one by one took 8000 of 17000 cycles at 8 rows of 64 blocks: 12.1 us for
+    // 10.8 with the merge.)
+    if (any && m_run == -INFINITY) m_run = -FLT_MAX;
     const float l_tot = rows_sum(l_run);
     if (q4 == 0) {
         s_m[wave][n] = m_run;
         s_l[wave][n] = l_tot;
     }
-    constexpr int TT = CH / 16;  // tiles per round
-    const int nparts = F32 ? 1 : min(3, PASSES == 1 ? 3 : 16 / G);  // rows of O that hold a head's parts
+    constexpr int TT = CH / 16;                                             // tiles per round
+    constexpr int NPART = F32 ? 1 : PASSES == 1 ? 3 : PASSES == 2 ? 2 : 1;  // rows of O that hold a head's parts
 #pragma unroll
     for (int c = 0; c < D / CH; c++) {
-        __syncthreads();
+        if (c > 0) __syncthreads();
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
 #pragma unroll
@@ -423,24 +428,31 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
         __syncthreads();
         for (int idx = threadIdx.x; idx < G * CH; idx += 64 * kSparseWaves) {
             const int g = idx / CH, d = idx % CH;
-            float M = s_m[0][g];
+            // every read of LDS goes out before any is used
+            float m[kSparseWaves], l[kSparseWaves], x[kSparseWaves][NPART];
 #pragma unroll
-            for (int w = 1; w < kSparseWaves; w++) M = fmaxf(M, s_m[w][g]);
+            for (int w = 0; w < kSparseWaves; w++) {
+                m[w] = s_m[w][g];
+                l[w] = s_l[w][g];
+#pragma unroll
+                for (int k = 0; k < NPART; k++) x[w][k] = s_o[w][g + G * k][d];
+            }
+            float M = m[0];
+#pragma unroll
+            for (int w = 1; w < kSparseWaves; w++) M = fmaxf(M, m[w]);
             float L = 0.0f, o = 0.0f;
 #pragma unroll
             for (int w = 0; w < kSparseWaves; w++) {
-                const float mw = s_m[w][g];
-                if (mw == -INFINITY && M > -INFINITY) continue;  // nothing of this wave's counts
-                const float f = mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M);
-                float x = 0.0f;
-                for (int k = 0; k < nparts; k++) x += s_o[w][g + G * k][d];
-                L += s_l[w][g] * f;
-                o += x * f;
+                const float f = m[w] == M ? 1.0f : __builtin_amdgcn_exp2f(m[w] - M);
+                float y = x[w][0];
+#pragma unroll
+                for (int k = 1; k < NPART; k++) y += x[w][k];
+                L += l[w] * f;
+                o += y * f;
             }
             const int dim = c * CH + d;
             if (end - beg == a.budget) {
-                // no token: zeros
-                a.d.out[(static_cast<int64_t>(row) * G + g) * D + dim] = L == 0.0f ? 0.0f : o / L;
+                a.d.out[(static_cast<int64_t>(row) * G + g) * D + dim] = M == -INFINITY ? 0.0f : o / L;  // no token: zeros
             } else {
                 const int64_t pi = (2 * static_cast<int64_t>(blockIdx.x) + (beg == 0)) * G + g;
                 a.d.ws_o[pi * D + dim] = o;
@@ -468,28 +480,45 @@ __global__ __launch_bounds__(256) void sparse_merge_kernel(const SparseArgs a) {
     const uint32_t first = row * a.budget / range, last = (row * a.budget + a.budget - 1) / range;
     if (first == last) return;  // written whole
     const auto part = [&](uint32_t w) { return (2 * static_cast<int64_t>(w) + (w == first)) * G + g; };
+    // Lanes hold the maxima and sums of 64 parts, the outputs are loaded kAhead parts at a time, the first ones
+    // beside the maxima.
+    constexpr int kAhead = 8;
+    float x[kAhead][DPL];
+    auto load = [&](uint32_t w0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t pi = part(min(w0 + j, last));
+#pragma unroll
+            for (int k = 0; k < DPL; k++) x[j][k] = a.d.ws_o[pi * D + min(lane + 64 * k, D - 1)];
+        }
+    };
+    load(first);
     float M = -INFINITY;
-    for (uint32_t w0 = first; w0 <= last; w0 += 64) M = fmaxf(M, w0 + lane <= last ? a.d.ws_m[part(w0 + lane)] : -INFINITY);
-    M = wave_max(M);
+    for (uint32_t w0 = first; w0 <= last; w0 += 64) M = fmaxf(M, a.d.ws_m[part(min(w0 + lane, last))]);
+    M = wave_max_dpp(M);
     float L = 0.0f, o[DPL];
 #pragma unroll
     for (int k = 0; k < DPL; k++) o[k] = 0.0f;
-#pragma unroll 4
-    for (uint32_t w = first; w <= last; w++) {
-        const int64_t pi = part(w);
-        const float mp = a.d.ws_m[pi], lp = a.d.ws_l[pi];
-        float x[DPL];
+    for (uint32_t w0 = first; w0 <= last; w0 += 64) {
+        const int64_t pi = part(min(w0 + lane, last));
+        const float m = a.d.ws_m[pi], l = a.d.ws_l[pi];
+        const float f = w0 + lane > last ? 0.0f : m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M);
+        L += w0 + lane > last ? 0.0f : l * f;
+        for (uint32_t w = w0; w <= min(last, w0 + 63); w += kAhead) {
+            if (w > first) load(w);
 #pragma unroll
-        for (int k = 0; k < DPL; k++) x[k] = lane + 64 * k < D ? a.d.ws_o[pi * D + lane + 64 * k] : 0.0f;
-        if (mp == -INFINITY && M > -INFINITY) continue;  // nothing of this part counts
-        const float f = mp == M ? 1.0f : __builtin_amdgcn_exp2f(mp - M);
-        L += lp * f;
+            for (int j = 0; j < kAhead; j++) {
+                if (w + j > last) break;
+                const float fj = readlane_f(f, static_cast<int>(w + j - w0));
 #pragma unroll
-        for (int k = 0; k < DPL; k++) o[k] += x[k] * f;
+                for (int k = 0; k < DPL; k++) o[k] += x[j][k] * fj;
+            }
+        }
     }
+    L = wave_sum(L);
 #pragma unroll
     for (int k = 0; k < DPL; k++)
-        if (lane + 64 * k < D) a.d.out[u * D + lane + 64 * k] = L == 0.0f ? 0.0f : o[k] / L;
+        if (lane + 64 * k < D) a.d.out[u * D + lane + 64 * k] = M == -INFINITY ? 0.0f : o[k] / L;
 }
 
 template <int D>

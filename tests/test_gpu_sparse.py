@@ -318,6 +318,23 @@ def test_sparse_decode_infinite_keys():
     assert np.isnan(got[1:]).all()
 
 
+@pytest.mark.parametrize("kv", [FP32, BF16])
+@pytest.mark.parametrize("budget", [20, 600])
+def test_sparse_decode_nan_in_a_block_of_its_own(kv, budget):
+    """A single token with a NaN key, alone in its block, and so alone with the wave or the part that has the block: its query's
+    outputs are NaN whatever the others are; beside it the rows stay as they were."""
+    lens = [16 * (budget - 1) + 1] * 3
+    p = ref.Pool(54, lens, 4, 2, 64, kv, BF16)
+    qs = p.queries(3)
+    sel = np.tile(np.arange(budget, dtype=np.int32), (3, 2, 1))
+    clean = run_sparse(p, gpu_pool(p), qs, None, lens, sel)
+    p.k[p.tables[1, budget - 1], 0, 0] = ref.of_type(np.full(1, np.nan, np.float32), kv)[0]
+    got = run_sparse(p, gpu_pool(p), qs, None, lens, sel)
+    assert np.isnan(got[1, :2]).all()
+    np.testing.assert_array_equal(got[[0, 2]], clean[[0, 2]])
+    np.testing.assert_array_equal(got[1, 2:], clean[1, 2:])
+
+
 def test_sparse_decode_large_scores_and_scale():
     lens = [400, 77, 640]
     p = ref.Pool(49, lens, 8, 2, 64, BF16, FP32)
