@@ -143,6 +143,22 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
     const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, a.d.context_lens[r]) : 0;
     const int nblk = T <= 0 ? 0 : (T + 15) / 16;
 
+    // Lane l holds the wave's l-th block of a stretch of 512 entries: its place in the sequence, its physical block. The
+    // first stretch's are on their way while Q is split. Neither load is under a condition, which would make the
+    // compiler wait at its end: past the segment the last entry is read again, and where there is no table or place in
+    // it, the list.
+    const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
+    const int32_t* table = T > 0 ? a.d.block_tables + static_cast<int64_t>(seq) * a.d.max_blocks_per_seq : list;
+    int lb, id;
+    bool listed;
+    auto fetch = [&](int e0) {
+        const int e = e0 + kSparseWaves * lane;
+        lb = list[min(e, end - 1)];
+        listed = e < end && lb >= 0 && lb < nblk;
+        id = table[listed ? lb : 0];
+    };
+    fetch(beg + wave);
+
     // Q operand: column n holds head n % G (part n / G of it where Q is split).
     bf16x8_t qb[F32 || I8 ? 1 : QP][F32 || I8 ? 1 : NSLAB];
     float qf[F32 ? D / 4 : 1];
@@ -229,15 +245,8 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
     for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     bool any = false;
 
-    const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
-    for (int e0 = beg + wave; e0 < end; e0 += 64 * kSparseWaves) {
-        // lane l: the wave's l-th block of this stretch
-        const int e = e0 + kSparseWaves * lane;
-        const int lb = e < end ? list[e] : -1;
-        const bool listed = lb >= 0 && lb < nblk;
-        int id = -1;
-        if (listed) id = a.d.block_tables[static_cast<int64_t>(seq) * a.d.max_blocks_per_seq + lb];
-        if (id >= a.d.num_blocks) id = -1;
+    for (int e0 = beg + wave; e0 < end;) {
+        if (!listed || id >= a.d.num_blocks) id = -1;
         float ks = 0.0f, vs = 0.0f;
         if constexpr (KV == PA_DTYPE_INT8) {
             if (id >= 0) {
@@ -403,6 +412,8 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
                 }
             }
         }
+        e0 += 64 * kSparseWaves;
+        if (e0 < end) fetch(e0);
     }
 
     // ---- the waves' states meet ----

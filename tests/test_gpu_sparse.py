@@ -258,7 +258,7 @@ def test_sparse_decode(kv, q, hq, hkv, d):
         close(run_sparse(p, g, qs, None, lens, sel), want, tol, f"budget {budget}")
 
 
-@pytest.mark.parametrize("n,budget", [(1, 64), (1, 600), (1, 1300), (3, 130), (40, 33), (90, 20), (50, 77), (700, 9), (129, 64)])
+@pytest.mark.parametrize("n,budget", [(1, 64), (1, 600), (1, 1300), (3, 130), (40, 33), (90, 20), (50, 77), (700, 9), (129, 64), (190, 24)])
 @pytest.mark.parametrize("kv", [BF16, INT8])
 def test_sparse_decode_splits(kv, n, budget):
     """Few rows of long lists, in parts, and many rows in one: the same attention."""
