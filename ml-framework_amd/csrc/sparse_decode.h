@@ -7,11 +7,11 @@
 // cut into ranges of equal length, one for each workgroup of a chip full of them, so that every CU streams the
 // same number of blocks whatever the number of rows. The part of a row in a range is a segment; a workgroup works
 // its segments off one after another. Its waves take a segment's blocks in turn (wave w: entries w, w +
-// kSparseWaves, ..); a wave streams its blocks through rotating register buffers, one pass with the running maximum
+// waves, ..); a wave streams its blocks through rotating register buffers, one pass with the running maximum
 // and sum, and no wave waits for another until the segment ends. There the waves' states meet in LDS; a
 // segment that is a whole row is finished at once, the parts of the others (at most two a range) by a merge launch.
 // Measured: 256 rows of 128 bf16 blocks (D 128, 269 MB) 47 us, 5.7 TB/s; in two workgroups a row, with
-// a merge, 55 us. 384 rows of 255 int8 blocks (404 MB) 85 us, 4.8 TB/s; in three rounds of half rows 95 us.
+// a merge, 55 us. 384 rows of 255 int8 blocks (404 MB) 82 us, 4.9 TB/s; in three rounds of half rows 95 us.
 //
 // K and V are read once and G = Hq / Hkv query heads share them (2 G flops a byte at bf16): traffic
 // bounds it. The matrix instructions are 16 columns wide and G is 1 to 16, so the columns that a
@@ -24,7 +24,7 @@
 // 31-bit integer in units of 2^(e - 30), 2^e > max |q|, in four signed digits, one in each group of columns; P V runs
 // in bf16 as above, its codes converted by placing them in the fraction of 2^23 (an instruction of a quarter of the
 // conversion's time). The int8 case is bound by its traffic all the same: with the P V product left out
-// altogether it takes 86 us. What it lacks against bf16 is the run length, 2 KiB instead of 4 a tile.
+// altogether it took 86 us of 87. What it lacks against bf16 is the run length, 2 KiB instead of 4 a tile.
 #pragma once
 
 #include <cfloat>
@@ -41,7 +41,15 @@ struct SparseArgs {
     int32_t rows, range;        // rows; list entries per workgroup (rows * budget fits 32 bits)
 };
 
-constexpr int kSparseWaves = 8;
+// Workgroups of a full chip: one per CU; two for blocks of few bytes, whose kernels fit 128 registers (D 64, 512 rows:
+// int8 of 128 blocks 38 us with one, 31 with two; bf16 of 64 blocks 24.9 and 23.5; fp32, at 147 registers, stays with
+// one, and int8 with D 128 spills if it is made to fit: 103 us where one took 82).
+__host__ __device__ constexpr int sparse_groups(int head_dim, int kv) {
+    return head_dim <= 64 && head_dim * (kv == PA_DTYPE_FP32 ? 4 : kv == PA_DTYPE_BF16 ? 2 : 1) <= 128 ? 512 : 256;
+}
+// Waves of a workgroup. For D 256 one per SIMD, since two would have no registers for a second buffer (512 rows: 64
+// fp32 blocks 311 us with two and one buffer, 217 with one and two buffers; 128 int8 blocks 155 and 112).
+__host__ __device__ constexpr int sparse_waves(int head_dim) { return head_dim >= 256 ? 4 : 8; }
 constexpr float kLog2e = 1.4426950408889634f;
 // Rescaling is deferred until the maximum grows by this (log2 units): P stays below 2^11.
 constexpr float kSparseRescale = 11.0f;
@@ -109,24 +117,22 @@ __device__ __forceinline__ s16x4_t sparse_v_operand(uint32_t r) {
 
 // Register buffers of a wave: the one consumed and those in flight. (Three cost more registers and time nothing
 // less: bf16 47.7 us of two, 47.9 of three; int8 86.6, 88.5, 91.7 of four, 96.6 of six; one: 107.)
-template <int D, int KV>
-__host__ __device__ constexpr int sparse_buffers() {
-    return D >= 256 ? 1 : 2;
-}
+constexpr int kSparseBuffers = 2;
 
 // PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
 template <int D, int KV, bool QF32, int PASSES>
-__global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const SparseArgs a) {
+__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / 256 * sparse_waves(D) / 4) void sparse_decode_kernel(const SparseArgs a) {
     constexpr bool F32 = KV == PA_DTYPE_FP32;
     constexpr int NSLAB = D / 32, NT = D / 16;
     constexpr bool I8 = KV == PA_DTYPE_INT8;
     constexpr int NI8 = I8 ? D / 64 : 1;           // QK slabs of 64 dims
     constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
     constexpr int PP = F32 ? 1 : PASSES;           // passes of P
-    constexpr int NB = sparse_buffers<D, KV>();
+    constexpr int W = sparse_waves(D);
+    constexpr int NB = kSparseBuffers;
     constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
-    __shared__ float s_m[kSparseWaves][16], s_l[kSparseWaves][16];
-    __shared__ float s_o[kSparseWaves][16][CH];
+    __shared__ float s_m[W][16], s_l[W][16];
+    __shared__ float s_o[W][16][CH];
     const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.d.num_kv_heads, G = a.d.group;
@@ -143,7 +149,7 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
     const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, a.d.context_lens[r]) : 0;
     const int nblk = T <= 0 ? 0 : (T + 15) / 16;
 
-    // Lane l holds the wave's l-th block of a stretch of 512 entries: its place in the sequence, its physical block. The
+    // Lane l holds the wave's l-th block of a stretch of 64 W entries: its place in the sequence, its physical block. The
     // first stretch's are on their way while Q is split. Neither load is under a condition, which would make the
     // compiler wait at its end: past the segment the last entry is read again, and where there is no table or place in
     // it, the list.
@@ -152,7 +158,7 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
     int lb, id;
     bool listed;
     auto fetch = [&](int e0) {
-        const int e = e0 + kSparseWaves * lane;
+        const int e = e0 + W * lane;
         lb = list[min(e, end - 1)];
         listed = e < end && lb >= 0 && lb < nblk;
         id = table[listed ? lb : 0];
@@ -390,29 +396,21 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
                 }
             }
         };
-        if constexpr (NB == 1) {
-            for (;;) {
-                load(buf[0], at[0]);
-                if (at[0] < 0) break;
-                compute(buf[0], at[0]);
-            }
-        } else {
 #pragma unroll
-            for (int i = 0; i < NB - 1; i++) load(buf[i], at[i]);
-            bool more = true;
-            while (more) {
+        for (int i = 0; i < NB - 1; i++) load(buf[i], at[i]);
+        bool more = true;
+        while (more) {
 #pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    load(buf[(i + NB - 1) % NB], at[(i + NB - 1) % NB]);
-                    if (at[i] < 0) {
-                        more = false;
-                        break;
-                    }
-                    compute(buf[i], at[i]);
+            for (int i = 0; i < NB; i++) {
+                load(buf[(i + NB - 1) % NB], at[(i + NB - 1) % NB]);
+                if (at[i] < 0) {
+                    more = false;
+                    break;
                 }
+                compute(buf[i], at[i]);
             }
         }
-        e0 += 64 * kSparseWaves;
+        e0 += 64 * W;
         if (e0 < end) fetch(e0);
     }
 
@@ -437,12 +435,12 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
 #pragma unroll
             for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = acc[c * TT + tt][i];
         __syncthreads();
-        for (int idx = threadIdx.x; idx < G * CH; idx += 64 * kSparseWaves) {
+        for (int idx = threadIdx.x; idx < G * CH; idx += 64 * W) {
             const int g = idx / CH, d = idx % CH;
             // every read of LDS goes out before any is used
-            float m[kSparseWaves], l[kSparseWaves], x[kSparseWaves][NPART];
+            float m[W], l[W], x[W][NPART];
 #pragma unroll
-            for (int w = 0; w < kSparseWaves; w++) {
+            for (int w = 0; w < W; w++) {
                 m[w] = s_m[w][g];
                 l[w] = s_l[w][g];
 #pragma unroll
@@ -450,10 +448,10 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_decode_kernel(const 
             }
             float M = m[0];
 #pragma unroll
-            for (int w = 1; w < kSparseWaves; w++) M = fmaxf(M, m[w]);
+            for (int w = 1; w < W; w++) M = fmaxf(M, m[w]);
             float L = 0.0f, o = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kSparseWaves; w++) {
+            for (int w = 0; w < W; w++) {
                 const float f = m[w] == M ? 1.0f : __builtin_amdgcn_exp2f(m[w] - M);
                 float y = x[w][0];
 #pragma unroll
@@ -536,7 +534,7 @@ template <int D>
 void launch_sparse_decode(const SparseArgs& a, int kv_dtype, bool q_f32, hipStream_t s) {
     const uint32_t all = static_cast<uint32_t>(a.rows) * a.budget, grid = (all + a.range - 1) / a.range;
     const int G = a.d.group;
-    const auto go = [&](auto kernel) { kernel<<<grid, 64 * kSparseWaves, 0, s>>>(a); };
+    const auto go = [&](auto kernel) { kernel<<<grid, 64 * sparse_waves(D), 0, s>>>(a); };
     const auto by_q = [&](auto kv, auto passes) {
         constexpr int KV = decltype(kv)::value, P = decltype(passes)::value;
         if (q_f32) go(sparse_decode_kernel<D, KV, true, P>);

@@ -6,28 +6,28 @@
 
 namespace {
 
-// List entries per workgroup: equal ranges for kGroups workgroups, one per CU, but kLeast entries a wave at least. Whole
+// List entries per workgroup: equal ranges for the workgroups of a full chip, but kLeast entries a wave at least. Whole
 // rows where they give no workgroup more than kWaste entries, or a third, over an equal range: a cut row costs another
 // start, another exchange of states and the merge. (bf16, D 128, equal ranges against whole rows: 136 rows of 40 blocks
 // 18.8 and 13.4 us, 384 of 40 32.3 and 27.8; at 32 entries more, 384 of 64, 40.4 and 39.4, at 34, 296 of 40, 24.8 and
 // 27.7, at 62, 8 of 64, 11.2 and 14.4.)
-constexpr int32_t kGroups = 256;
 constexpr int32_t kLeast = 2;
 constexpr int32_t kWaste = 32;
-int32_t sparse_range(int64_t rows, int32_t budget) {
-    int64_t r = (rows * budget + kGroups - 1) / kGroups;
-    const int64_t whole = (rows + kGroups - 1) / kGroups * budget;
+int32_t sparse_range(const pa_config* cfg, int64_t rows, int32_t budget) {
+    const int32_t waves = pa::sparse_waves(cfg->head_dim), groups = pa::sparse_groups(cfg->head_dim, cfg->kv_dtype);
+    int64_t r = (rows * budget + groups - 1) / groups;
+    const int64_t whole = (rows + groups - 1) / groups * budget;
     if (whole - r <= kWaste) return static_cast<int32_t>(whole);
-    r = std::max<int64_t>(r, kLeast * pa::kSparseWaves);
+    r = std::max<int64_t>(r, kLeast * waves);
     if (r > budget * 3ll / 4 && r <= budget) return budget;
-    return static_cast<int32_t>((r + pa::kSparseWaves - 1) / pa::kSparseWaves * pa::kSparseWaves);
+    return static_cast<int32_t>((r + waves - 1) / waves * waves);
 }
 
 // Slots of partial states: two per range, none if no row is cut.
 size_t slot_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
     const int64_t rows = static_cast<int64_t>(num_queries) * cfg->num_kv_heads;
     if (rows == 0 || budget == 0) return 0;
-    const int32_t range = sparse_range(rows, budget);
+    const int32_t range = sparse_range(cfg, rows, budget);
     return range % budget == 0 ? 0 : 2 * static_cast<size_t>((rows * budget + range - 1) / range) * (cfg->num_q_heads / cfg->num_kv_heads);
 }
 
@@ -109,7 +109,7 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     a.num_queries = num_queries;
     a.budget = budget;
     a.rows = num_queries * cfg->num_kv_heads;
-    a.range = sparse_range(a.rows, budget);
+    a.range = sparse_range(cfg, a.rows, budget);
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
     const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;

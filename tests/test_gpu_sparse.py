@@ -270,6 +270,19 @@ def test_sparse_decode_splits(kv, n, budget):
     close(run_sparse(p, g, qs, None, lens, sel), want, tol)
 
 
+@pytest.mark.parametrize("n,budget", [(3, 130), (20, 70), (90, 20), (260, 11)])
+@pytest.mark.parametrize("kv,hq,hkv,d", [(FP32, 8, 2, 32), (FP32, 8, 2, 64), (INT8, 16, 1, 64), (BF16, 32, 2, 128), (FP32, 8, 2, 128),
+                                         (INT8, 8, 2, 128), (FP32, 8, 2, 256), (BF16, 16, 2, 256), (INT8, 16, 1, 256)])
+def test_sparse_decode_splits_of_other_shapes(kv, hq, hkv, d, n, budget):
+    """Workgroups of four and of eight waves, one or two to a CU: cut rows, whole ones, several whole ones."""
+    lens = [16 * (budget + 2) - 3 * (i % 40) for i in range(n)]
+    p = ref.Pool(46, lens, hq, hkv, d, kv, FP32)
+    qs, g = p.queries(n), gpu_pool(p)
+    sel = random_lists(p, range(n), lens, budget, p.rng)
+    want, tol = ref.attend(p, qs, range(n), lens, sel)
+    close(run_sparse(p, g, qs, None, lens, sel), want, tol)
+
+
 @pytest.mark.parametrize("kv", [FP32, BF16, INT8])
 def test_sparse_decode_lists_of_the_callers(kv):
     """Entries in any order, holes, blocks past the context, the same block twice, nothing at all, bad pages."""
