@@ -145,25 +145,24 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / 256 * 
     const int end = static_cast<int>(min(budget, beg + (stop - at_entry)));
     at_entry += end - beg;
     const int r = row / Hkv, kvh = row - r * Hkv;
-    const int seq = a.query_seqs ? a.query_seqs[r] : r;
-    const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, a.d.context_lens[r]) : 0;
-    const int nblk = T <= 0 ? 0 : (T + 15) / 16;
-
     // Lane l holds the wave's l-th block of a stretch of 64 W entries: its place in the sequence, its physical block. The
-    // first stretch's are on their way while Q is split. Neither load is under a condition, which would make the
-    // compiler wait at its end: past the segment the last entry is read again, and where there is no table or place in
-    // it, the list.
+    // first stretch's places come together with the sequence's number and length, its blocks while Q is split. No load is
+    // under a condition, which would make the compiler wait at its end: past the segment the last entry is read again,
+    // and where there is no table or place in it, the list.
     const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
+    int lb = list[min(beg + wave + W * lane, end - 1)];
+    const int raw_len = a.d.context_lens[r], named = (a.query_seqs ? a.query_seqs : a.d.context_lens)[r];
+    const int seq = a.query_seqs ? named : r;
+    const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, raw_len) : 0;
+    const int nblk = T <= 0 ? 0 : (T + 15) / 16;
     const int32_t* table = T > 0 ? a.d.block_tables + static_cast<int64_t>(seq) * a.d.max_blocks_per_seq : list;
-    int lb, id;
+    int id;
     bool listed;
-    auto fetch = [&](int e0) {
-        const int e = e0 + W * lane;
-        lb = list[min(e, end - 1)];
-        listed = e < end && lb >= 0 && lb < nblk;
+    auto find = [&](int e0) {
+        listed = (e0 + W * lane < end) & (lb >= 0) & (lb < nblk);
         id = table[listed ? lb : 0];
     };
-    fetch(beg + wave);
+    find(beg + wave);
 
     // Q operand: column n holds head n % G (part n / G of it where Q is split).
     bf16x8_t qb[F32 || I8 ? 1 : QP][F32 || I8 ? 1 : NSLAB];
@@ -411,7 +410,10 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / 256 * 
             }
         }
         e0 += 64 * W;
-        if (e0 < end) fetch(e0);
+        if (e0 < end) {
+            lb = list[min(e0 + W * lane, end - 1)];
+            find(e0);
+        }
     }
 
     // ---- the waves' states meet ----
