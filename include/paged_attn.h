@@ -457,8 +457,9 @@ pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* 
                            int32_t recent_blocks, int32_t budget, int32_t* selected, void* workspace,
                            size_t workspace_bytes);
 
-/* Bytes of workspace of pa_sparse_decode (partial results of rows that are split; 0 when none is; 4-byte
- * aligned). */
+/* Bytes of workspace that pa_sparse_decode needs for up to num_queries query tokens and lists of up to budget
+ * entries (partial results of rows that are split; at most a few MB; 4-byte aligned). A call whose own rows are not
+ * split needs none. */
 pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, int32_t budget, size_t* bytes);
 /* pa_paged_decode over the listed blocks only: query r's heads of KV head h attend to the tokens
  * (those before context_lens[r]) of the logical blocks selected[r][h][0 .. budget).

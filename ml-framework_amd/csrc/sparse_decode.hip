@@ -31,6 +31,14 @@ size_t slot_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
     return range % budget == 0 ? 0 : 2 * static_cast<size_t>((rows * budget + range - 1) / range) * (cfg->num_q_heads / cfg->num_kv_heads);
 }
 
+// What no call of that many query tokens and entries, or of fewer, exceeds (fewer rows may be cut where more are not).
+size_t most_slots(const pa_config* cfg, int32_t num_queries, int32_t budget) {
+    const int64_t all = static_cast<int64_t>(num_queries) * cfg->num_kv_heads * budget;
+    const int64_t least = kLeast * pa::sparse_waves(cfg->head_dim);
+    const int64_t ranges = std::min<int64_t>(pa::sparse_groups(cfg->head_dim, cfg->kv_dtype), (all + least - 1) / least);
+    return 2 * static_cast<size_t>(ranges) * (cfg->num_q_heads / cfg->num_kv_heads);
+}
+
 pa_status check_shape(const char* f, const pa_config* cfg, int32_t num_queries, int32_t budget) {
     pa_status st = pa::check_config(cfg, f);
     if (st != PA_SUCCESS) return st;
@@ -52,7 +60,7 @@ pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, in
     pa_status st = check_shape(f, cfg, num_queries, budget);
     if (st != PA_SUCCESS) return st;
     if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": bytes is null");
-    *bytes = slot_count(cfg, num_queries, budget) * (cfg->head_dim + 2) * sizeof(float);
+    *bytes = most_slots(cfg, num_queries, budget) * (cfg->head_dim + 2) * sizeof(float);
     return pa::clear_error();
 }
 

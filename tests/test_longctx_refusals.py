@@ -145,8 +145,22 @@ def test_sizes_and_empty_calls():
     assert pa.select_workspace_size(cfg(), 3, 100) == 3 * 8 * 7 * 8
     assert pa.select_workspace_size(cfg(), 0, 100) == 0
     assert pa.sparse_workspace_size(cfg(), 0, 100) == 0
-    assert pa.sparse_workspace_size(cfg(), 4096, 64) == 0  # rows enough for the chip: none is split
     assert pa.sparse_workspace_size(cfg(), 1, 512) > 0
+
+
+@pytest.mark.parametrize("c", [cfg(), cfg(num_q_heads=16, num_kv_heads=1, head_dim=256), cfg(head_dim=64), cfg(head_dim=64, kv_dtype=2),
+                               cfg(head_dim=256, kv_dtype=0)])
+def test_sparse_workspace_serves_smaller_calls(c):
+    """One workspace of the largest call's size is enough for every smaller call: a call reports what it needs itself."""
+    for n, budget in ((512, 64), (40, 130), (7, 300)):
+        size = pa.sparse_workspace_size(c, n, budget)
+        assert size <= 16 << 20
+        for m in (1, 2, 3, 5, 7, 16, 17, 31, 40, 64, 65, 100, 129, 200, 257, 300, 511, 512):
+            for b in (1, 2, 9, 16, 17, 33, 63, 64, 90, 129, 130, 299, 300):
+                if m <= n and b <= budget:
+                    assert pa.sparse_workspace_size(c, m, b) <= size
+                    # (the alignment is checked behind the size)
+                    refused(ARG, "aligned", lambda: sparse(c=c, ks=FAKE, vs=FAKE, n=m, rows=FAKE, budget=b, ws=FAKE + 2, size=size))
     bounds(seqs=0, k=None, tables=None, start=None, new=None, out=None)
     bounds(most=0)
     select(n=0, q=None, b=None, tables=None, lens=None, out=None)
