@@ -44,8 +44,9 @@ struct SparseArgs {
 // Workgroups of a full chip: one per CU; two for blocks of few bytes, whose kernels fit 128 registers (D 64, 512 rows:
 // int8 of 128 blocks 38 us with one, 31 with two; bf16 of 64 blocks 24.9 and 23.5; fp32, at 147 registers, stays with
 // one, and int8 with D 128 spills if it is made to fit: 103 us where one took 82).
+constexpr int kSparseCUs = 256;
 __host__ __device__ constexpr int sparse_groups(int head_dim, int kv) {
-    return head_dim <= 64 && head_dim * (kv == PA_DTYPE_FP32 ? 4 : kv == PA_DTYPE_BF16 ? 2 : 1) <= 128 ? 512 : 256;
+    return head_dim <= 64 && head_dim * (kv == PA_DTYPE_FP32 ? 4 : kv == PA_DTYPE_BF16 ? 2 : 1) <= 128 ? 2 * kSparseCUs : kSparseCUs;
 }
 // Waves of a workgroup. For D 256 one per SIMD, since two would have no registers for a second buffer (512 rows: 64
 // fp32 blocks 311 us with two and one buffer, 217 with one and two buffers; 128 int8 blocks 155 and 112).
@@ -121,7 +122,7 @@ constexpr int kSparseBuffers = 2;
 
 // PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
 template <int D, int KV, bool QF32, int PASSES>
-__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / 256 * sparse_waves(D) / 4) void sparse_decode_kernel(const SparseArgs a) {
+__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSparseCUs * sparse_waves(D) / 4) void sparse_decode_kernel(const SparseArgs a) {
     constexpr bool F32 = KV == PA_DTYPE_FP32;
     constexpr int NSLAB = D / 32, NT = D / 16;
     constexpr bool I8 = KV == PA_DTYPE_INT8;

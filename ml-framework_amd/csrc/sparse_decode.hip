@@ -6,19 +6,21 @@
 
 namespace {
 
-// List entries per workgroup: equal ranges for the workgroups of a full chip, but kLeast entries a wave at least. Whole
-// rows where they give no workgroup more than kWaste entries, or a third, over an equal range: a cut row costs another
-// start, another exchange of states and the merge. (bf16, D 128, equal ranges against whole rows: 136 rows of 40 blocks
-// 18.8 and 13.4 us, 384 of 40 32.3 and 27.8; at 32 entries more, 384 of 64, 40.4 and 39.4, at 34, 296 of 40, 24.8 and
-// 27.7, at 62, 8 of 64, 11.2 and 14.4.)
-constexpr int32_t kLeast = 2;
+// List entries per workgroup: equal ranges for the workgroups of a full chip, of two entries a wave at least, or of one
+// where that cuts no row into more than kParts parts and every range still has a CU: 8 rows of 64 blocks (bf16, fp32,
+// D 128) 11.5 and 16.4 us with two, 10.8 and 14.1 with one; 8 rows of 400 (bf16, D 64) 12.6 in 25 parts a row, 15.8 in 50.
+// Whole rows where they give no workgroup more than kWaste entries, or a third, over an equal range: a cut row costs
+// another start, another exchange of states and the merge. (bf16, D 128, equal ranges against whole rows: 136 rows of 40
+// blocks 18.8 and 13.4 us, 384 of 40 32.3 and 27.8; at 32 entries more, 384 of 64, 40.4 and 39.4, at 34, 296 of 40, 24.8
+// and 27.7, at 62, 8 of 64, 11.2 and 14.4.)
+constexpr int32_t kParts = 8;
 constexpr int32_t kWaste = 32;
 int32_t sparse_range(const pa_config* cfg, int64_t rows, int32_t budget) {
     const int32_t waves = pa::sparse_waves(cfg->head_dim), groups = pa::sparse_groups(cfg->head_dim, cfg->kv_dtype);
     int64_t r = (rows * budget + groups - 1) / groups;
     const int64_t whole = (rows + groups - 1) / groups * budget;
     if (whole - r <= kWaste) return static_cast<int32_t>(whole);
-    r = std::max<int64_t>(r, kLeast * waves);
+    r = std::max(r, budget <= kParts * waves ? std::max<int64_t>(waves, (rows * budget + pa::kSparseCUs - 1) / pa::kSparseCUs) : 2 * waves);
     if (r > budget * 3ll / 4 && r <= budget) return budget;
     return static_cast<int32_t>((r + waves - 1) / waves * waves);
 }
@@ -34,7 +36,7 @@ size_t slot_count(const pa_config* cfg, int32_t num_queries, int32_t budget) {
 // What no call of that many query tokens and entries, or of fewer, exceeds (fewer rows may be cut where more are not).
 size_t most_slots(const pa_config* cfg, int32_t num_queries, int32_t budget) {
     const int64_t all = static_cast<int64_t>(num_queries) * cfg->num_kv_heads * budget;
-    const int64_t least = kLeast * pa::sparse_waves(cfg->head_dim);
+    const int64_t least = pa::sparse_waves(cfg->head_dim);
     const int64_t ranges = std::min<int64_t>(pa::sparse_groups(cfg->head_dim, cfg->kv_dtype), (all + least - 1) / least);
     return 2 * static_cast<size_t>(ranges) * (cfg->num_q_heads / cfg->num_kv_heads);
 }
