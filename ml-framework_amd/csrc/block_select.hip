@@ -491,12 +491,13 @@ __global__ __launch_bounds__(64 * kInt8Waves, D == 256 ? 2 : QT > 1 ? 3 : 4) voi
                     }
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     __builtin_amdgcn_wave_barrier();
-                    // a column sum is below 2^22: two digits in 32 bits, the three pairs in 64
+                    // A column sum is at most 2^23 (512 places, codes and digits down to -128) and a pair of digits 2^31 + 2^23,
+                    // more than 32 bits hold: joined in 64, exactly.
                     const int32_t* sums = reinterpret_cast<const int32_t*>(s_sum[wave][8 * (q4 < QT ? q4 : 0)]) + n;
                     double y = 0.0;
 #pragma unroll
                     for (int j = kDigits - 2; j >= 0; j -= 2)
-                        y = __builtin_fma(y, 65536.0, static_cast<double>(sums[16 * (j + 1)] * 256 + sums[16 * j]));
+                        y = __builtin_fma(y, 65536.0, __builtin_fma(static_cast<double>(sums[16 * (j + 1)]), 256.0, static_cast<double>(sums[16 * j])));
                     const int b = first + 16 * gi + n;
                     if (q4 < QT && b < end_of) out[b] = y * unit_of * static_cast<double>(ks[k]);
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

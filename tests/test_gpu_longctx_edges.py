@@ -1,0 +1,38 @@
+"""Calls at the edges of what the long-context operators and the page books accept, on the GPU against their 64-bit forms
+(longctx_ref.py)."""
+import numpy as np
+import pytest
+
+import longctx_ref as ref
+from helpers import to_gpu
+from test_gpu_sparse import run_select
+
+pytestmark = pytest.mark.gpu
+
+INT8, FP32 = 2, 0
+
+
+def select_pool(p):
+    return {"bounds": to_gpu(p.bounds), "tables": to_gpu(p.tables), "stats": [to_gpu(s) for s in p.stats] if p.stats else [None] * 4}
+
+
+@pytest.mark.parametrize("queries", [1, 3])
+def test_select_int8_codes_of_minus_128(queries):
+    """Codes of -128 in all 512 places of a block's bounds at head_dim 256, against weights whose fourth digit (of base 256) is -128 in
+    every place: the digit's sum over the places is 2^23, and a digit pair's 2^31. The weights are a = 1/2 - 2^-14 of the maxima and -b
+    = -(1 + 2^-14) of the minima, so such a block has 128 * 256 (b - a), the best score, and a block with -127 for n of its channels
+    n (b - a) less, all of them exact in 64 bits."""
+    blocks = 120
+    p = ref.Pool(71, [16 * blocks] * 2, 2, 1, 256, INT8, FP32, values=False)
+    p.stats[0][:] = 0.03125
+    p.bounds[:] = -128
+    for i in range(2 * blocks):
+        if i % 3:
+            p.bounds[p.tables.ravel()[i], 0, :, :1 + (7 * i) % 15] = -127
+    rows = [0, 1] * queries
+    qs = np.empty((len(rows), 2, 256), np.float32)
+    qs[:, 0], qs[:, 1] = 0.5 - 2.0 ** -14, -(1 + 2.0 ** -14)
+    lens = [16 * blocks] * len(rows)
+    want = ref.select(p, qs, rows, lens, 1, 2, 30)
+    got = run_select(p, select_pool(p), qs, rows if queries > 1 else None, lens, 1, 2, 30)
+    np.testing.assert_array_equal(got, want)
