@@ -365,15 +365,18 @@ __global__ __launch_bounds__(64) void int8_weights_kernel(const SelectArgs a) {
     const bool up = i0 >= D;
     double x[N];
     group_weights<N, D>(a, u * a.group * D + (up ? i0 - D : i0), up, x);
-    float top = 0.0f;
+    // The largest weight's exponent, in 64 bits: a finite query's sums over its heads may pass fp32's largest value.
+    constexpr float kNone = -4096.0f, kBad = 4096.0f;  // no weight but zeros; one that is not finite
+    double top = 0.0;
+    bool finite = true;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-        const float f = fabsf(static_cast<float>(x[e]));
-        top = fmaxf(top, f < INFINITY ? f : INFINITY);  // NaN too
+        finite &= fabs(x[e]) < static_cast<double>(INFINITY);
+        top = fmax(top, fabs(x[e]));
     }
-    top = pa::wave_max_dpp(top);
-    const bool bad = !(top < INFINITY);
-    const int ex = top > 0.0f && !bad ? __builtin_amdgcn_frexp_exp(static_cast<double>(top)) - 1 : 0;
+    const float most = pa::wave_max_dpp(!finite ? kBad : top > 0.0 ? static_cast<float>(__builtin_amdgcn_frexp_exp(top) - 1) : kNone);
+    const bool bad = most == kBad;
+    const int ex = bad || most == kNone ? 0 : static_cast<int>(most);
     if (lane == 0) a.units[u] = bad ? static_cast<double>(__builtin_nanf("")) : __builtin_amdgcn_ldexp(1.0, ex - 45);
     // |z| <= 2^46; with 128 added in every place the digits are plain bytes, 128 too large each
     uint64_t y[N];

@@ -36,3 +36,16 @@ def test_select_int8_codes_of_minus_128(queries):
     want = ref.select(p, qs, rows, lens, 1, 2, 30)
     got = run_select(p, select_pool(p), qs, rows if queries > 1 else None, lens, 1, 2, 30)
     np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("kv", [FP32, 1, INT8])
+def test_select_group_sums_past_the_largest_fp32(kv):
+    """Finite queries whose sums over the heads of a group pass the largest fp32 value: ordinary scores in 64 bits."""
+    p = ref.Pool(72 + kv, [16 * 90] * 3, 32, 2, 64, kv, FP32, values=False)
+    qs = p.queries(3)
+    qs[1] = np.clip(qs[1], -2, 2) * np.float32(1.5e38)
+    qs[2, :16] = np.float32(3.4e38) * np.sign(qs[2, :16])
+    with np.errstate(over="ignore"):
+        assert np.isinf(np.maximum(qs[1], 0).reshape(2, 16, 64).sum(1, dtype=np.float32)).any() and np.isfinite(qs).all()
+    got = run_select(p, select_pool(p), qs, None, p.lens, 1, 2, 20)
+    np.testing.assert_array_equal(got, ref.select(p, qs, range(3), p.lens, 1, 2, 20))
