@@ -577,7 +577,8 @@ pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tab
     a.num_blocks = cfg->num_blocks;
     a.reach = static_cast<int32_t>(reach);
     pa::StreamDevice dev(stream);
-    if (reach >= 1 && reach * num_rows <= kBookThreads)
+    // (no rows: refcounts may be null, and only the other kernel reads them for a demand alone)
+    if (num_rows > 0 && reach >= 1 && reach * num_rows <= kBookThreads)
         pages_reserve_small_kernel<<<1, kBookThreads, 0, pa::native(stream)>>>(a);
     else
         pages_reserve_kernel<<<1, kBookThreads, 0, pa::native(stream)>>>(a);

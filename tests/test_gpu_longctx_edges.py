@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 import longctx_ref as ref
-from helpers import to_gpu
+import paged_attention as pa
+from helpers import empty_gpu, to_gpu, to_np
 from test_gpu_sparse import run_select
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +50,20 @@ def test_select_group_sums_past_the_largest_fp32(kv):
         assert np.isinf(np.maximum(qs[1], 0).reshape(2, 16, 64).sum(1, dtype=np.float32)).any() and np.isfinite(qs).all()
     got = run_select(p, select_pool(p), qs, None, p.lens, 1, 2, 20)
     np.testing.assert_array_equal(got, ref.select(p, qs, range(3), p.lens, 1, 2, 20))
+
+
+@pytest.mark.parametrize("width,most", [(9, 1), (9, 1000), (9, 0), (0, 5)])
+@pytest.mark.parametrize("null", [True, False])
+def test_reserve_for_no_rows(null, width, most):
+    """An empty batch, whose arrays may all be null: nothing taken, nothing missing, the books not looked at."""
+    import torch
+    cfg = pa.make_config(num_q_heads=2, num_kv_heads=2, head_dim=64, kv_dtype=1, num_blocks=100)
+    refs, some, status = to_gpu(np.arange(100, dtype=np.int32) % 3), empty_gpu((8,), np.int32), empty_gpu((2,), np.int32)
+    status.fill_(77)
+    size = pa.pages_workspace_size(cfg, 0, width)
+    ws = empty_gpu((size,), np.uint8)
+    given = (None,) * 5 if null else (some, some, some, refs, some)
+    pa.pages_reserve(None, cfg, *given[:3], 0, width, most, *given[3:], status, ws, size)
+    torch.cuda.synchronize()
+    assert to_np(status).tolist() == [0, 0]
+    np.testing.assert_array_equal(to_np(refs), np.arange(100) % 3)
