@@ -330,6 +330,7 @@ __global__ __launch_bounds__(kBookThreads) void pages_compact_kernel(const Compa
     // the words of the blocks from `base` on; returns their live blocks
     const auto scan = [&](int base) {
         const int words = words_of(base);
+        __syncthreads();  // the words of the round before have been read
         constexpr int UN = 8;  // loads in flight
         for (int k0 = wave; k0 < words; k0 += UN * kBookWaves) {
             int refs[UN];

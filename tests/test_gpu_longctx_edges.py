@@ -6,6 +6,7 @@ import pytest
 import longctx_ref as ref
 import paged_attention as pa
 from helpers import empty_gpu, to_gpu, to_np
+from test_gpu_pages import run_compact
 from test_gpu_sparse import run_select
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +68,35 @@ def test_reserve_for_no_rows(null, width, most):
     torch.cuda.synchronize()
     assert to_np(status).tolist() == [0, 0]
     np.testing.assert_array_equal(to_np(refs), np.arange(100) % 3)
+
+
+@pytest.mark.parametrize("live", [262144, 262145, 262144 + 64 * 100 + 17, 2 * 262144 - 1, 2 * 262144, 2 * 262144 + 4095])
+def test_compact_where_the_rounds_words_differ(live):
+    """Pools of several rounds of 262144 blocks whose words around the live count are full in one round and empty in the other, so
+    that a word of the wrong round would give another number of moves."""
+    config = pa.make_config(num_q_heads=2, num_kv_heads=2, head_dim=64, kv_dtype=1, num_blocks=3 * 262144 + 5)
+    nb = config.num_blocks
+    held = np.ones(nb, bool)
+    at = live % 262144  # the word that is read, and the same one of every other round
+    for r in range(4):
+        lo = max(0, r * 262144 + at - 200)
+        held[lo:r * 262144 + at + 200] = r != live // 262144
+    spare = np.nonzero(held)[0]
+    held[spare[spare > live + 300][::-1][:held.sum() - live]] = False
+    extra = np.nonzero(held)[0][::7][:held.sum() - live]
+    held[extra] = False
+    assert held.sum() == live
+    refs = held.astype(np.int32) * 2
+    ids = np.nonzero(held)[0].astype(np.int32)
+    tables = np.full((1, live + 3), -1, np.int32)
+    tables[0, :live] = ids
+    t, r, pairs, st = run_compact(config, tables, refs, nb)
+    up, down = ids[ids >= live][::-1], np.nonzero(~held[:live])[0]
+    assert len(up) == len(down)
+    name = np.arange(nb, dtype=np.int32)
+    name[up] = down
+    np.testing.assert_array_equal(pairs[:len(up)], np.stack([up, down], 1))
+    assert (pairs[len(up):] == -1).all()
+    np.testing.assert_array_equal(r, (np.arange(nb) < live) * 2)
+    np.testing.assert_array_equal(t[0, :live], name[ids])
+    assert (t[0, live:] == -1).all() and st.tolist() == [len(up), live]
