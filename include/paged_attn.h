@@ -480,7 +480,8 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
 
 /* ---- the books of the pool on the device ----
  * Which blocks a sequence holds and how many hold a block, changed by kernels in stream order, so that a
- * step that forks, frees or extends sequences needs no word from the host and may be captured into a graph
+ * step that forks, frees or extends sequences may be captured into a graph; whether its reservation succeeded
+ * is for the step itself or the host to ask before anything is appended (pa_pages_reserve)
  * (the reference keeps these books on the host: BlockShareManager.cs:34-105, KVCacheBlockManager.cs:
  * 70-174). The caller owns the arrays:
  *   refcounts    [num_blocks] int32: rows (and other owners, such as a prefix cache) that hold the block;
@@ -510,8 +511,14 @@ pa_status pa_pages_workspace_size(const pa_config* cfg, int32_t num_rows, int32_
  * status [2] (device): the blocks taken, and 0; or, when there are too few free blocks, 0 and how many are
  * missing, with nothing else changed. max_new_per_row: host-side upper bound of num_new (blocks beyond
  * it are not looked at). Positions beyond max_blocks_per_seq * 16 get no block; rows with num_new <= 0 or
- * a negative length ask for none. Then advance lens, append (pa_build_slot_mapping, pa_kv_append) and bring the key bounds up to
- * date. */
+ * a negative length ask for none. Then append (pa_build_slot_mapping, pa_kv_append), bring the key bounds up to date
+ * and advance lens; but not when blocks are missing (status[1] != 0): the tables are then as they were, so a row's tokens
+ * would go into blocks that others still hold, or nowhere. Nothing behind this call looks at status by itself. Either the
+ * host reads it before the append is enqueued, or knows that there is room before the call (it takes at most
+ * num_rows times the blocks that max_new_per_row tokens can touch), or the step makes the append harmless on the device: start
+ * positions of INT32_MIN for pa_build_slot_mapping and pa_key_bounds_update where status[1] != 0 (their slots are
+ * -1, which every append by slots skips; no bounds are touched; pa_paged_decode_append goes by the context length: 0), and
+ * lens advanced by nothing. */
 pa_status pa_pages_reserve(pa_stream* stream, const pa_config* cfg, int32_t* tables, const int32_t* lens,
                            const int32_t* num_new, int32_t num_rows, int32_t max_blocks_per_seq,
                            int32_t max_new_per_row, int32_t* refcounts, int32_t* copy_pairs, int32_t* status,

@@ -100,3 +100,113 @@ def test_compact_where_the_rounds_words_differ(live):
     np.testing.assert_array_equal(r, (np.arange(nb) < live) * 2)
     np.testing.assert_array_equal(t[0, :live], name[ids])
     assert (t[0, live:] == -1).all() and st.tolist() == [len(up), live]
+
+
+@pytest.mark.parametrize("kv", [1, INT8])
+def test_step_in_a_graph_whose_reservation_fails(kv):
+    """Fork, reservation, copies and append in one graph. Where too few blocks are free the step's slots are -1 (its start positions are
+    made negative by status) and its lengths stay, so no byte of the cache, no count and no length changes behind the fork;
+    the next replay, which forks every row to itself, repeats the reservation alone, and succeeds once a block is free."""
+    import torch
+    B, hkv, d, width, nb = 4, 2, 64, 4, 12
+    rng = np.random.default_rng(80 + kv)
+    cfg = pa.make_config(num_q_heads=hkv, num_kv_heads=hkv, head_dim=d, kv_dtype=kv, q_dtype=FP32, num_blocks=nb)
+    k, v, bounds = (to_gpu(ref.of_type(rng.standard_normal(s, np.float32), kv)) for s in ((nb, hkv, 16, d), (nb, hkv, d, 16), (nb, hkv, 2, d)))
+    stats = [to_gpu(np.full((nb, hkv), x, np.float32)) for x in (0.03, 0.04, 0.03 * 127, 0.04 * 127)] if kv == INT8 else [None] * 4
+    first = np.full((B, width), -1, np.int32)
+    first[0, :2], first[1, :2], first[2, 0] = (7, 3), (1, 9), 5  # 20, 32 and 5 tokens
+    tables = [to_gpu(first), empty_gpu((B, width), np.int32)]
+    lens = [to_gpu(np.array([20, 32, 5, 0], np.int32)), empty_gpu((B,), np.int32)]
+    held = np.ones(nb, np.int32)
+    held[11] = 0  # one block is free, the others that no row holds are a prefix cache's
+    refs, src = to_gpu(held), to_gpu(np.array([0, 0, 1, 2], np.int32))
+    one, off = to_gpu(np.ones(B, np.int32)), to_gpu(np.arange(B, dtype=np.int32))
+    pairs, status, slots = empty_gpu((B, 2), np.int32), empty_gpu((2,), np.int32), empty_gpu((B,), np.int64)
+    size = pa.pages_workspace_size(cfg, B, width)
+    ws, start, granted = empty_gpu((size,), np.uint8), empty_gpu((B,), np.int32), empty_gpu((B,), np.int32)
+    none, ok = to_gpu(np.full(B, -2 ** 31, np.int32)), torch.zeros(1, dtype=torch.bool, device="cuda:0")
+    kn, vn = empty_gpu((B, hkv, d), np.float32), empty_gpu((B, hkv, d), np.float32)
+    dev = pa.Device(0)
+    ts = pa.Stream(dev)
+    tstream = torch.cuda.ExternalStream(ts.native(), device="cuda:0")
+
+    def gate(b):
+        with torch.cuda.stream(tstream):
+            torch.eq(status[1:], 0, out=ok)
+            torch.where(ok, lens[b], none, out=start)
+            torch.mul(one, ok, out=granted)
+
+    def step(a, b):
+        pa.pages_fork(ts, cfg, tables[a], lens[a], B, src, tables[b], lens[b], B, width, refs)
+        pa.pages_reserve(ts, cfg, tables[b], lens[b], one, B, width, 1, refs, pairs, status, ws, size)
+        pa.copy_pages(ts, cfg, k, v, *stats, bounds, pairs, B)
+        gate(b)
+        pa.build_slot_mapping(ts, cfg, tables[b], width, start, one, off, B, 1, slots)
+        pa.kv_append(ts, cfg, kn, vn, slots, B, k, v, *stats)
+        pa.key_bounds_update(ts, cfg, k, tables[b], width, start, one, B, 1, bounds)
+        with torch.cuda.stream(tstream):
+            lens[b].add_(granted)
+
+    torch.cuda.synchronize()
+    gate(1)
+    lens[1].add_(granted)  # (loaded before a capture)
+    torch.cuda.synchronize()
+    graphs = []
+    for a, b in ((0, 1), (1, 0)):
+        gr = pa.Graph().capture(ts)
+        step(a, b)
+        graphs.append(gr.end())
+    data = [t for t in (k, v, bounds, *stats) if t is not None]
+    short = np.array([[7, 3, -1, -1], [7, 3, -1, -1], [1, 9, -1, -1], [5, -1, -1, -1]], np.int32)  # behind the fork
+    held[[7, 3]] = 2
+    for n in range(5):
+        x = [rng.standard_normal((B, hkv, d), np.float32) for _ in range(2)]
+        kn.copy_(to_gpu(x[0]))
+        vn.copy_(to_gpu(x[1]))
+        if n == 1:
+            src.copy_(off)  # every row to itself
+        if n == 3:
+            refs[10] = 0  # the prefix cache gives a block back
+            held[10] = 0
+        before = [to_np(t).copy() for t in data]
+        torch.cuda.synchronize()
+        graphs[n % 2].launch(ts)
+        ts.synchronize()
+        now = (n + 1) % 2
+        if n < 3:  # rows 0 (a copy of the tail it shares) and 2 (a new block) ask for one each
+            assert to_np(status).tolist() == [0, 1] and (to_np(pairs) == -1).all() and (to_np(slots) == -1).all()
+            for t, was in zip(data, before):
+                np.testing.assert_array_equal(to_np(t), was)
+            np.testing.assert_array_equal(to_np(tables[now]), short)
+            np.testing.assert_array_equal(to_np(refs), held)
+            assert to_np(lens[now]).tolist() == [20, 20, 32, 5]
+        junk = torch.randn(1 << 20, device="cuda:0").sum()  # the program's own work between replays
+        torch.cuda.synchronize()
+        del junk
+        if n < 3:
+            continue
+        at = [20 + n - 3, 20 + n - 3, 32 + n - 3, 5 + n - 3]
+        if n == 3:
+            assert to_np(status).tolist() == [2, 0] and to_np(pairs).tolist() == [[3, 10]] + [[-1, -1]] * 3
+            short[0, 1], short[2, 2] = 10, 11
+            held[[3, 10, 11]] = 1
+            if kv == 1:  # the tail's four tokens went along
+                np.testing.assert_array_equal(to_np(k)[10, :, :4], before[0][3, :, :4])
+                np.testing.assert_array_equal(to_np(v)[10, :, :, :4], before[1][3, :, :, :4])
+        np.testing.assert_array_equal(to_np(tables[now]), short)
+        np.testing.assert_array_equal(to_np(refs), held)
+        assert to_np(lens[now]).tolist() == [t + 1 for t in at]
+        for i, t in enumerate(at):
+            b = short[i, t // 16]
+            for which, (cache, new) in enumerate(((k, x[0][i]), (v, x[1][i]))):
+                got = to_np(cache, ref.NP_DTYPE[kv])[b]
+                got = got[:, t % 16] if which == 0 else got[:, :, t % 16]
+                if kv == 1:  # the upper 16 bits, as pa_kv_append stores them
+                    np.testing.assert_array_equal(got, ref.bf16_of(new))
+                else:  # a code is off by half a step, its product with the scale and the division by 2^-22 of the value
+                    sc = to_np(stats[which])[b][:, None].astype(np.float64)
+                    assert (np.abs(ref.f64(got) * sc - new) <= 0.5 * sc + np.abs(new) * 2.0 ** -22).all()
+    for gr in graphs:
+        gr.destroy()
+    ts.destroy()
+    dev.close()
