@@ -414,7 +414,8 @@ pa_status pa_write_block_f32(pa_stream* stream, const pa_config* cfg, void* k_ca
  * tokens that are verified together). query_seqs null: query r belongs to sequence r, and num_queries
  * must be num_seqs. A query whose query_seqs entry is out of range has an empty context. Contexts are
  * read up to max_context_len and max_blocks_per_seq * 16 tokens. None of these calls allocates or
- * synchronises; all may be captured into a graph. Calls that share a workspace must not overlap. */
+ * synchronises; all may be captured into a graph. Calls that share a workspace must not overlap. A call that needs a
+ * launch of 2^32 threads or more is refused (PA_ERROR_UNSUPPORTED) before anything is launched. */
 
 /* Bytes of the key bounds of the pool: [num_blocks][num_kv_heads][2][head_dim] elements of kv_dtype
  * (index 0: minimum, 1: maximum of each channel over the block's keys; int8 caches: of the codes, to
@@ -494,7 +495,7 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
  * every entry -1) when src[i] is outside [0, num_in). Every in row gives up its blocks and every out
  * row takes hold of its own, so this forks (a row named twice), frees (a row not named) and reorders
  * sequences or beams in one call. refcounts change in place; the out arrays must not overlap the in
- * arrays. Blocks whose count falls to 0 are free. */
+ * arrays. Blocks whose count falls to 0 are free. num_in + num_out below 2^24. */
 pa_status pa_pages_fork(pa_stream* stream, const pa_config* cfg, const int32_t* tables_in, const int32_t* lens_in,
                         int32_t num_in, const int32_t* src, int32_t* tables_out, int32_t* lens_out,
                         int32_t num_out, int32_t max_blocks_per_seq, int32_t* refcounts);

@@ -716,7 +716,7 @@ __global__ __launch_bounds__(T) void block_choose_kernel(const SelectArgs a) {
         out[i < a.sink ? i : a.budget - a.recent + (i - a.sink)] = i < a.sink ? i : r0 + (i - a.sink);
 }
 
-// Launches the scores; false for more workgroups than a grid holds.
+// Launches the scores; nothing, and false, for more workgroups than a grid holds.
 template <int D>
 bool launch_score(const SelectArgs& a, int kv, int32_t most, hipStream_t s) {
     // Units are sequences where they have several queries each on average, else queries.
@@ -728,10 +728,9 @@ bool launch_score(const SelectArgs& a, int kv, int32_t most, hipStream_t s) {
             const int32_t per = kInt8Blocks;
             const int32_t chunks = (most + per - 1) / per;
             const int64_t waves = static_cast<int64_t>(units) * chunks * a.hkv;
-            if (waves > INT32_MAX - kInt8Waves) return false;
-            const auto go = [&](auto kernel) {
-                kernel<<<static_cast<uint32_t>((waves + kInt8Waves - 1) / kInt8Waves), 64 * kInt8Waves, 0, s>>>(a, units, chunks, per);
-            };
+            const int64_t grid = (waves + kInt8Waves - 1) / kInt8Waves;
+            if (!pa::fits_grid(grid, 64 * kInt8Waves)) return false;
+            const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(grid), 64 * kInt8Waves, 0, s>>>(a, units, chunks, per); };
             int8_weights_kernel<D><<<a.num_queries * a.hkv, 64, 0, s>>>(a);
             if (grouped) go(block_score_int8_kernel<D, kQueryTile>);
             else go(block_score_int8_kernel<D, 1>);
@@ -746,8 +745,8 @@ bool launch_score(const SelectArgs& a, int kv, int32_t most, hipStream_t s) {
     while (per > batch && static_cast<int64_t>(units) * a.hkv * ((most + per - 1) / per) < kScoreWorkers) per /= 2;
     const int32_t chunks = (most + per - 1) / per;
     const int64_t waves = static_cast<int64_t>(units) * chunks * a.hkv;
-    if (waves > INT32_MAX - kScoreWaves) return false;
     const int64_t grid = (waves + kScoreWaves - 1) / kScoreWaves;
+    if (!pa::fits_grid(grid, 64 * kScoreWaves)) return false;
     const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(grid), 64 * kScoreWaves, 0, s>>>(a, units, chunks, per); };
     if (kv == PA_DTYPE_FP32) {
         if (grouped) go(block_score_kernel<D, PA_DTYPE_FP32, kQueryTile>);
@@ -861,6 +860,10 @@ pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* 
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
     const int32_t most = std::min(a.max_blocks, max_blocks_per_seq);  // blocks of the longest context
+    // Threads a row of the choice: 512 of 1024 blocks 5.1 us, 256 5.7; 1024 of 2048 blocks 7.0 us, 512 8.0.
+    const int32_t threads = most <= 1024 ? 512 : 1024;
+    if (!pa::fits_grid(static_cast<int64_t>(num_queries) * a.hkv, threads))
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many query tokens for one call");
     if (most > budget) {
         bool fits = true;
         switch (cfg->head_dim) {
@@ -872,8 +875,7 @@ pa_status pa_select_blocks(pa_stream* stream, const pa_config* cfg, const void* 
         if (!fits) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
         PA_HIP_CHECK(hipGetLastError());
     }
-    // (512 threads of 1024 blocks 5.1 us, 256 5.7; 1024 of 2048 blocks 7.0 us, 512 8.0)
-    if (most <= 1024) launch_choose<512, true>(a, most, s);
+    if (threads == 512) launch_choose<512, true>(a, most, s);
     else if (most <= kHeld) launch_choose<1024, true>(a, most, s);
     else launch_choose<1024, false>(a, most, s);
     PA_HIP_CHECK(hipGetLastError());

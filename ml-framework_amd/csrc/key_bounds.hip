@@ -145,10 +145,10 @@ pa_status pa_key_bounds_update(pa_stream* stream, const pa_config* cfg, const vo
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": k_cache and key_bounds must be 16-byte aligned");
     // A sequence's new tokens touch at most this many blocks (the first may start inside one).
     const int64_t reach = std::min<int64_t>((static_cast<int64_t>(max_new_per_seq) + 14) / 16 + 1, max_blocks_per_seq);
-    const int64_t waves = reach * cfg->num_kv_heads;
-    if (waves > INT32_MAX) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
+    const int64_t groups = (reach * cfg->num_kv_heads + kWaves - 1) / kWaves;
+    if (!pa::fits_grid(groups, 64 * kWaves)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
     pa::StreamDevice dev(stream);
-    const dim3 grid(static_cast<uint32_t>((waves + kWaves - 1) / kWaves), num_seqs);
+    const dim3 grid(static_cast<uint32_t>(groups), num_seqs);
     hipStream_t s = pa::native(stream);
     const auto go = [&](auto launcher) {
         launcher(cfg->kv_dtype, grid, s, k_cache, block_tables, max_blocks_per_seq, start_pos, num_new,

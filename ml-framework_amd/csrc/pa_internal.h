@@ -91,6 +91,8 @@ namespace pa {
 inline int32_t kv_bytes(const pa_config* cfg) {
     return cfg->kv_dtype == PA_DTYPE_FP32 ? 4 : cfg->kv_dtype == PA_DTYPE_BF16 ? 2 : 1;
 }
+// Whether that many workgroups of `threads` threads fit a grid's dimension (fewer than 2^32 threads).
+inline bool fits_grid(int64_t groups, int64_t threads) { return groups <= static_cast<int64_t>(UINT32_MAX) / threads; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 }  // namespace pa
 

@@ -525,7 +525,7 @@ pa_status pa_pages_fork(pa_stream* stream, const pa_config* cfg, const int32_t* 
     if (num_in < 0 || num_out < 0 || max_blocks_per_seq < 0)
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": negative size");
     if (static_cast<int64_t>(num_in) + num_out == 0) return pa::clear_error();
-    if (static_cast<int64_t>(num_in) + num_out > INT32_MAX)
+    if (!pa::fits_grid(static_cast<int64_t>(num_in) + num_out, kForkThreads))
         return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many rows for one call");
     if (!refcounts || (num_in > 0 && (!tables_in || !lens_in)) || (num_out > 0 && (!src || !tables_out || !lens_out)))
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");

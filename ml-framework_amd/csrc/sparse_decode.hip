@@ -93,6 +93,9 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     const size_t need = partials * (cfg->head_dim + 2) * sizeof(float);
     if (need > workspace_bytes || (need > 0 && !workspace))
         return pa::set_error(PA_ERROR_WORKSPACE_TOO_SMALL, std::string(f) + ": workspace needs " + std::to_string(need) + " bytes");
+    // the parts of cut rows are joined by a wave per (row, query head), four to a workgroup
+    if (partials > 0 && !pa::fits_grid((static_cast<int64_t>(num_queries) * cfg->num_q_heads + 3) / 4, 256))
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many query tokens for one call");
     if (reinterpret_cast<uintptr_t>(workspace) & 3)
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": workspace must be 4-byte aligned");
     pa::SparseArgs a{};
