@@ -424,7 +424,8 @@ pa_status pa_key_bounds_bytes(const pa_config* cfg, size_t* bytes);
 /* Brings the bounds up to date after tokens were written into the cache (pa_kv_append and the calls
  * that append): for sequence s, every block that holds one of its tokens start_pos[s] ..
  * start_pos[s] + num_new[s] - 1 gets the bounds of the keys that it holds up to the last of them, read from
- * the cache. max_new_per_seq: host-side upper bound of num_new (tokens beyond it are not looked at).
+ * the cache. max_new_per_seq: host-side upper bound of num_new; it bounds the blocks that are looked at, the first
+ * (max_new_per_seq + 14) / 16 + 1 (none for 0) that the new tokens lie in, and tokens in further ones are not.
  * Sequences with start_pos < 0 or num_new <= 0, table entries outside [0, num_blocks) and positions beyond
  * max_blocks_per_seq * 16 are skipped. A NaN key makes its channel's bounds NaN. Two sequences of one call
  * that name the same block must hold the same tokens in it. num_seqs at most 65535; k_cache and key_bounds
@@ -445,8 +446,9 @@ pa_status pa_select_workspace_size(const pa_config* cfg, int32_t num_queries, in
  *     sum_d (sum_g max(q_gd, 0)) hi_bd + (sum_g min(q_gd, 0)) lo_bd       (g: the heads of the group)
  *   (times k_scale for int8 caches), an upper bound of sum_g max_t q_g . k_t; equal scores go to the
  *   lowest index, a score that is NaN comes first (int8 caches: any score of a query that is not finite
- *   is). Scores are summed in 64 bits. Blocks whose table entry
- *   lies outside [0, num_blocks) score 0. The bounds of the sink and recent blocks do not matter
+ *   is). Scores are summed in 64 bits; for int8 caches from the sums over the group's heads rounded, each by at
+ *   most 2^-46 of the largest of them, so scores closer than this makes may come in either order. Blocks whose
+ *   table entry lies outside [0, num_blocks) score 0. The bounds of the sink and recent blocks do not matter
  *   (they need not be up to date while they are among the recent ones).
  *   q: [num_queries][num_q_heads][head_dim] of q_dtype; recent_blocks >= 1 (the block of the newest
  *   token), sink_blocks + recent_blocks <= budget, max_context_len <= 2097152; q and key_bounds 16-byte
@@ -468,9 +470,12 @@ pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, in
  * Lists come from pa_select_blocks or from the caller: entries that are negative or at or past the end
  * of the context are skipped wherever they stand, in any order; a block listed twice counts twice.
  * Blocks whose table entry lies outside [0, num_blocks) read as zero keys and values. A query without
- * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter; queries, keys and
- * values of listed tokens that are not finite give outputs that are not. Products are
- * exact and sums in fp32 for every cache and query type. num_q_heads / num_kv_heads: 1, 2, 4, 8 or
+ * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter. Queries
+ * that are not finite, NaN keys, and keys that make a score +Inf give outputs that are not finite, and so do values that are
+ * not, in their channel. A score of -Inf counts nothing beside finite ones (fp32 queries of bf16 caches, whose products
+ * are formed in parts: it is NaN); a query with no other gives NaN. Sums are in fp32; products are exact, for int8 caches
+ * with queries that were rounded by at most 2^-30 of the largest value of their head (or 2^-126, where that is more) and
+ * probabilities whose product with v_scale was rounded to fp32. num_q_heads / num_kv_heads: 1, 2, 4, 8 or
  * 16. q and caches 16-byte aligned. */
 pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, const void* q,
                            const void* k_cache, const void* v_cache, const float* k_scale,
@@ -510,10 +515,10 @@ pa_status pa_pages_workspace_size(const pa_config* cfg, int32_t num_rows, int32_
  * keeps it. copy_pairs [num_rows][2]: (old, new) where the replaced block holds tokens of the row, else
  * (-1, -1); copy them with pa_copy_pages (or pa_copy_blocks) before the new tokens are written.
  * status [2] (device): the blocks taken, and 0; or, when there are too few free blocks, 0 and how many are
- * missing, with nothing else changed. max_new_per_row: host-side upper bound of num_new (blocks beyond
- * it are not looked at). Positions beyond max_blocks_per_seq * 16 get no block; rows with num_new <= 0 or
- * a negative length ask for none. Then append (pa_build_slot_mapping, pa_kv_append), bring the key bounds up to date
- * and advance lens; but not when blocks are missing (status[1] != 0): the tables are then as they were, so a row's tokens
+ * missing, with nothing else changed. max_new_per_row: host-side upper bound of num_new; of
+ * the blocks that a row's new tokens lie in the first (max_new_per_row + 14) / 16 + 1 are looked at (none for 0).
+ * Positions beyond max_blocks_per_seq * 16 get no block; rows with num_new <= 0 or a negative length ask for none.
+ * Then append (pa_build_slot_mapping, pa_kv_append), bring the key bounds up to date and advance lens; but not when blocks are missing (status[1] != 0): the tables are then as they were, so a row's tokens
  * would go into blocks that others still hold, or nowhere. Nothing behind this call looks at status by itself. Either the
  * host reads it before the append is enqueued, or knows that there is room before the call (it takes at most
  * num_rows times the blocks that max_new_per_row tokens can touch), or the step makes the append harmless on the device: start

@@ -21,7 +21,9 @@
 // are summed when the row ends. Every product is then exact and every sum in fp32, at the
 // instruction count of a single bf16 product for G <= 4 (two passes for G = 8, three for 16). fp32 caches
 // run on fp32 matrix instructions. int8 keys go to the byte matrix instruction as they are, against Q as a
-// 31-bit integer in units of 2^(e - 30), 2^e > max |q|, in four signed digits, one in each group of columns; P V runs
+// 31-bit integer in units of 2^(e - 30), 2^e > max |q|, in four signed digits, one in each group of columns: these products are
+// exact too, but of a Q rounded by up to 2^-30 of its largest value, which is what fp32 sums would keep beside that one,
+// and less where its codes are zero (a fifth digit would take a second pass at G = 4); P V runs
 // in bf16 as above, its codes converted by placing them in the fraction of 2^23 (an instruction of a quarter of the
 // conversion's time). The int8 case is bound by its traffic all the same: with the P V product left out
 // altogether it took 86 us of 87. What it lacks against bf16 is the run length, 2 KiB instead of 4 a tile.

@@ -7,7 +7,7 @@ import longctx_ref as ref
 import paged_attention as pa
 from helpers import empty_gpu, to_gpu, to_np
 from test_gpu_pages import run_compact
-from test_gpu_sparse import run_select
+from test_gpu_sparse import close, gpu_pool, random_lists, run_select, run_sparse
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +210,23 @@ def test_step_in_a_graph_whose_reservation_fails(kv):
         gr.destroy()
     ts.destroy()
     dev.close()
+
+
+@pytest.mark.parametrize("far", [4, 16, 20, 24])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (32, 8, 128), (8, 1, 128), (16, 1, 256)])
+def test_sparse_decode_int8_queries_far_apart(hq, hkv, d, far):
+    """One channel of a query 2^far times the others, and its codes zero: the others decide.
+
+    Tolerance: that of the exact products, and the queries' rounding: 2^-30 of the largest value in every channel, all of one
+    sign at worst, makes e = 2^-30 max|q| sum_d |k_d| scale of a score and twice that of a probability."""
+    lens = [100, 16 * 30 + 7, 16 * 12]
+    p = ref.Pool(90 + far, lens, hq, hkv, d, INT8, FP32)
+    p.k[:, :, :, 5] = 0
+    qs = p.queries(3)
+    qs[:, :, 5] = 2.0 ** far
+    sel = random_lists(p, range(3), lens, 24, p.rng)
+    want, tol = ref.attend(p, qs, range(3), lens, sel)
+    k = np.abs(ref.f64(p.k)).sum(3).max() * p.stats[0].max()
+    v = np.abs(ref.f64(p.v)).max() * p.stats[1].max()
+    tol = tol + 2 * 2.0 ** -30 * np.abs(qs).max(2, keepdims=True) * k / np.sqrt(d) * v
+    close(run_sparse(p, gpu_pool(p), qs, None, lens, sel), want, tol)
