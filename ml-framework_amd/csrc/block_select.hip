@@ -186,7 +186,7 @@ __device__ __forceinline__ void for_query_groups(const SelectArgs& a, int unit, 
 __device__ __forceinline__ double weight_of(float q, bool up) {
     return static_cast<double>(up ? __builtin_elementwise_maximum(q, 0.0f) : __builtin_elementwise_minimum(q, 0.0f));
 }
-// The weights of N channels from `i` on (elements of q) over the query heads of the group, D apart; four heads'
+// The weights of N channels (an even number) from `i` on (elements of q) over the query heads of the group, D apart; four heads'
 // loads are issued together.
 template <int N, int D>
 __device__ __forceinline__ void group_weights(const SelectArgs& a, int64_t i, bool up, double (&w)[N]) {
@@ -198,15 +198,11 @@ __device__ __forceinline__ void group_weights(const SelectArgs& a, int64_t i, bo
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint16_t* q = static_cast<const uint16_t*>(a.q) + i + min(j0 + k, a.group - 1) * D;
-                if constexpr (N == 1) {
-                    f[k][0] = pa::bf16_to_f32(*q);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < N; e += 2) {
-                        const uint32_t x = reinterpret_cast<const uint32_t*>(q)[e / 2];
-                        f[k][e] = pa::bf16_lo(x);
-                        f[k][e + 1] = pa::bf16_hi(x);
-                    }
+                for (int e = 0; e < N; e += 2) {
+                    const uint32_t x = reinterpret_cast<const uint32_t*>(q)[e / 2];
+                    f[k][e] = pa::bf16_lo(x);
+                    f[k][e + 1] = pa::bf16_hi(x);
                 }
             }
         } else {

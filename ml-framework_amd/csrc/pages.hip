@@ -439,7 +439,6 @@ struct CopyArgs {
     int64_t part;              // bytes of K (of V) per block
     int64_t bound;             // bytes of the key bounds per block
     int32_t max_pairs, pieces, num_blocks, hkv;
-    bool int8;
 };
 constexpr int kPieceWords = 2;  // 16-byte words a lane
 constexpr int kPieceBytes = kCopyThreads * 16 * kPieceWords;
@@ -658,7 +657,6 @@ pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, 
                                     (c.bound + kPieceBytes - 1) / kPieceBytes) + (int8 ? 1 : 0);
     c.num_blocks = cfg->num_blocks;
     c.hkv = cfg->num_kv_heads;
-    c.int8 = int8;
     pa::StreamDevice dev(stream);
     const int64_t units = static_cast<int64_t>(max_pairs) * c.pieces;
     copy_pages_kernel<<<static_cast<uint32_t>(std::min<int64_t>(units, kCopyGroups)), kCopyThreads, 0, pa::native(stream)>>>(c);

@@ -39,7 +39,7 @@ struct SparseArgs {
     DecodeArgs d;  // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [slots][G]
     const int32_t* query_seqs;  // null: query r belongs to sequence r
     const int32_t* selected;    // [num_queries][Hkv][budget]
-    int32_t num_seqs, num_queries, budget;
+    int32_t num_seqs, budget;
     int32_t rows, range;        // rows; list entries per workgroup (rows * budget fits 32 bits)
 };
 

@@ -119,7 +119,6 @@ pa_status pa_sparse_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     a.query_seqs = query_seqs;
     a.selected = selected;
     a.num_seqs = num_seqs;
-    a.num_queries = num_queries;
     a.budget = budget;
     a.rows = num_queries * cfg->num_kv_heads;
     a.range = sparse_range(cfg, a.rows, budget);
