@@ -129,9 +129,10 @@ __device__ __forceinline__ int32_t* demand_entry(const ReserveArgs& a, int64_t e
 // hold too takes one in its place (copy on write), except for the last of the rows that hold it when all
 // of them ask in this call: it keeps the block, as it would if the rows were worked off one by one.
 //
-// Up to kBookThreads demands, a thread each: three dependent loads (lengths; table entry; refcount) with the
-// refcounts of the pool's first blocks on their way meanwhile, and everything else in registers and
-// LDS. What bounds it is the chain of those round trips and of the barriers.
+// Up to kBookThreads demands, a thread each: three dependent loads (lengths; table entry; refcount) behind the
+// refcounts of the pool's first blocks, and everything else in registers and LDS. What bounds it is the chain of those
+// round trips and of the barriers. (The scan's eight loads are compiled to a branch and a wait each, since they
+// are under a condition, so they are round trips of this chain too.)
 static_assert(2 * kBookThreads == 1 << 11, "the hash has 11 bits");
 constexpr int kScan = 8;  // 64-block words of a wave per scan of the pool: 8192 blocks a round
 __global__ __launch_bounds__(kBookThreads) void pages_reserve_small_kernel(const ReserveArgs a) {
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(kBookThreads) void pages_compact_kernel(const Compa
     const auto scan = [&](int base) {
         const int words = words_of(base);
         __syncthreads();  // the words of the round before have been read
-        constexpr int UN = 8;  // loads in flight
+        constexpr int UN = 8;  // words a step; each load, being under a condition, is waited for before the next
         for (int k0 = wave; k0 < words; k0 += UN * kBookWaves) {
             int refs[UN];
 #pragma unroll

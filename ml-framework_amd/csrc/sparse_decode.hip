@@ -12,7 +12,8 @@ namespace {
 // Whole rows where they give no workgroup more than kWaste entries, or a third, over an equal range: a cut row costs
 // another start, another exchange of states and the merge. (bf16, D 128, equal ranges against whole rows: 136 rows of 40
 // blocks 18.8 and 13.4 us, 384 of 40 32.3 and 27.8; at 32 entries more, 384 of 64, 40.4 and 39.4, at 34, 296 of 40, 24.8
-// and 27.7, at 62, 8 of 64, 11.2 and 14.4.)
+// and 27.7, at 62, 8 of 64, 11.2 and 14.4.) The limit is in entries, 8 KB each in these; where an entry is 2 KB (int8, D 64) or
+// 32 KB (fp32, D 256) whole rows may be worth more or less than it says: not measured.
 constexpr int32_t kParts = 8;
 constexpr int32_t kWaste = 32;
 int32_t sparse_range(const pa_config* cfg, int64_t rows, int32_t budget) {
