@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * kScoreWaves, score_waves(D, KV, QT)) void bloc
 // k_scale. The sums go through LDS to a lane per (query, block). Over 108 MB of bounds, three queries a sequence:
 // 114 us with byte dot products in the vector unit, 44 with the columns summed across lanes in fp64, 32 with
 // the sums through LDS, 29 with the codes through LDS as well: whole rows a load instead of half lines, which also lets
-// the loads be non-temporal (67 us without that).
+// the loads be non-temporal (67 us without that); 30 with the digit sums joined in 64 bits.
 constexpr int kDigits = 6;
 constexpr int kInt8Waves = 4;
 constexpr int kInt8Ahead = 2;  // tiles on their way (4: 32.3 us)
