@@ -473,7 +473,7 @@ pa_status pa_sparse_workspace_size(const pa_config* cfg, int32_t num_queries, in
  * a listed token gives zeros. What unused slots of a block hold (NaN, Inf) does not matter. Queries
  * that are not finite, NaN keys, and keys that make a score +Inf give outputs that are not finite, and so do values that are
  * not, in their channel. A score of -Inf counts nothing beside finite ones (fp32 queries of bf16 caches, whose products
- * are formed in parts: it is NaN); a query with no other gives NaN. Sums are in fp32; products are exact, for int8 caches
+ * are formed in parts: it may be NaN); a query with no other gives NaN. Sums are in fp32; products are exact, for int8 caches
  * with queries that were rounded by at most 2^-30 of the largest value of their head (or 2^-126, where that is more) and
  * probabilities whose product with v_scale was rounded to fp32. num_q_heads / num_kv_heads: 1, 2, 4, 8 or
  * 16. q and caches 16-byte aligned. */
