@@ -548,6 +548,91 @@ pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, 
                         float* k_scale, float* v_scale, float* k_absmax, float* v_absmax, void* key_bounds,
                         const int32_t* pairs, int32_t max_pairs, const int32_t* num_pairs);
 
+/* ---- caches of bounded size: a sliding window, first tokens that stay visible, eviction by weight ----
+ * A model with a sliding window sees the last `window` tokens and the first sink_tokens of a sequence; its blocks
+ * between these may go. A model without one can be served from a bounded cache all the same: what weight attention gives each
+ * block is added up, and the blocks that got the least leave their rows. No reference counterpart: the reference attends
+ * to the whole context (DecodeOrchestrator.ComputeDecodeAttention, Phases/DecodeOrchestrator.cs:64-80) and frees a
+ * sequence's blocks only with the sequence (KVCacheBlockManager.cs:70-174).
+ *
+ * Visible tokens: the query at position p sees the tokens t <= p with t > p - window or t < sink_tokens (window 0: every t <= p).
+ * Positions are places in the row's table: when blocks between the sinks and the window have left it, the same
+ * sink_tokens and window still name the same tokens. (Where the model rotates keys by their position, the caller rotates them
+ * before the append, by the position in the text, and they keep it.)
+ * Masses: block_mass [rows][max_blocks_per_seq] fp32, one value for each entry of the block tables, the caller's to set to 0 when a
+ * row begins; a forked row's masses are copied with its table by the caller.
+ * Contexts are read up to max_context_len and max_blocks_per_seq * 16 tokens; blocks whose table entry lies outside
+ * [0, num_blocks) read as zero keys and values. What tokens hold that a query does not see (unused slots of a block, expired
+ * tokens; NaN, Inf) does not matter to it. Queries that are not finite, NaN keys, and keys that make a score +Inf give outputs (and
+ * masses) that are not finite, and so do values that are not, in their channel. A score of -Inf counts nothing beside
+ * finite ones (fp32 queries of bf16 caches and fp32 caches, whose products are formed in parts: it may be NaN); a query with no other
+ * gives NaN. int8 caches: scales must be finite. None of these calls allocates or synchronises; all may be captured
+ * into a graph. Calls that share a workspace or masses must not overlap. */
+
+/* Bytes of workspace of pa_window_decode for up to num_seqs sequences of up to max_context_len tokens (8-byte aligned); with_mass
+ * non-zero: for calls that keep masses. */
+pa_status pa_window_decode_workspace_size(const pa_config* cfg, int32_t num_seqs, int32_t max_context_len,
+                                          int32_t sink_tokens, int32_t window, int32_t with_mass, size_t* bytes);
+/* pa_paged_decode over the visible tokens: one query token per sequence, at position context_lens[s] - 1 (already
+ * appended). Only blocks that hold a visible token are read, their table entries too.
+ *   out: [num_seqs][num_q_heads][head_dim] fp32, q: [num_seqs][num_q_heads][head_dim] of q_dtype
+ * block_mass null, or [num_seqs][max_blocks_per_seq]: every visible block's entry grows by the softmax weights of its
+ * visible tokens, summed over the query heads in a fixed order (num_q_heads in all for each sequence).
+ * A sequence with context_lens[s] <= 0 gives zeros. Any kv_dtype and head_dim; num_q_heads / num_kv_heads: 1, 2, 4, 8 or
+ * 16. Sums are in fp32; products are exact, for int8 caches as pa_sparse_decode forms them. q and caches 16-byte
+ * aligned. (A call of more than 2047 sequences is worked off as several of that many at most, in order.) */
+pa_status pa_window_decode(pa_stream* stream, const pa_config* cfg, float* out, const void* q, const void* k_cache,
+                           const void* v_cache, const float* k_scale, const float* v_scale,
+                           const int32_t* block_tables, const int32_t* context_lens, int32_t num_seqs,
+                           int32_t max_blocks_per_seq, int32_t max_context_len, int32_t sink_tokens, int32_t window,
+                           float* block_mass, void* workspace, size_t workspace_bytes);
+
+/* Bytes of workspace of pa_window_prefill for up to num_seqs chunks of up to max_chunk_len tokens in contexts of up to
+ * max_context_len (16-byte aligned). A call whose keys are not cut needs none. */
+pa_status pa_window_prefill_workspace_size(const pa_config* cfg, int32_t num_seqs, int32_t max_chunk_len,
+                                           int32_t max_context_len, int32_t sink_tokens, int32_t window, size_t* bytes);
+/* pa_chunked_prefill over the visible tokens: chunk s has q_start_loc[s + 1] - q_start_loc[s] query tokens at positions
+ * prefix_lens[s] + i, its keys and values already appended; from single tokens and a few drafted ones to whole prompts.
+ *   out: [total_q][num_q_heads][head_dim] fp32, q: [total_q][num_q_heads][head_dim] of q_dtype
+ *   lse: null, or [total_q][num_q_heads] fp32: ln of the sum of exp(scale q.k) over the visible tokens
+ *   max_chunk_len, max_context_len: host-side upper bounds of the chunks and of prefix + chunk; query tokens beyond
+ *   the former are not computed.
+ * A query that sees no token (its window lies past the table or max_context_len) gives zeros, and -Inf in lse. Any
+ * kv_dtype, head_dim and ratio of heads; num_seqs * num_kv_heads at most 65535. Sums are in fp32. Products are those of fp32:
+ * parts below 2^-24 are left out where an operand is fp32, and bf16 and int8 caches meet probabilities rounded by at most
+ * 2^-18. out, q and caches 16-byte aligned. cfg->flags (masks) are not read. */
+pa_status pa_window_prefill(pa_stream* stream, const pa_config* cfg, float* out, const void* q,
+                            const int32_t* q_start_loc, const int32_t* prefix_lens, const void* k_cache,
+                            const void* v_cache, const float* k_scale, const float* v_scale,
+                            const int32_t* block_tables, int32_t num_seqs, int32_t max_blocks_per_seq,
+                            int32_t max_chunk_len, int32_t max_context_len, int32_t sink_tokens, int32_t window,
+                            float* lse, void* workspace, size_t workspace_bytes);
+
+/* The masses of a prompt, before its first eviction: over the last `last_queries` tokens of every chunk (all of a shorter one)
+ * and their heads,
+ *   block_mass[s][b] += sum of exp(scale q.k - lse) over the visible tokens of block b, in a fixed order.
+ * q, q_start_loc, prefix_lens, sink_tokens and window are those of the pa_window_prefill call that left lse; rows of
+ * q and lse other than the last queries' are not read. Keys alone are read. num_seqs at most 65535; q and k_cache 16-byte
+ * aligned. */
+pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, const void* q, const float* lse,
+                          const int32_t* q_start_loc, const int32_t* prefix_lens, const void* k_cache,
+                          const float* k_scale, const int32_t* block_tables, int32_t num_seqs,
+                          int32_t max_blocks_per_seq, int32_t max_context_len, int32_t last_queries,
+                          int32_t sink_tokens, int32_t window, float* block_mass);
+
+/* Rows over their budget give up blocks. A row of n = ceil(lens[i] / 16) > budget blocks keeps the first sink_blocks, the last
+ * recent_blocks and, of the others, the budget - sink_blocks - recent_blocks of the largest mass (equal masses:
+ * the lowest index; NaN counts as the largest); block_mass null: the last ones. What stays moves down in order, masses along;
+ * entries behind the row's blocks (reserved ahead) move with them, -1 (and mass 0) follows. lens[i] falls by 16 for each
+ * block that left, and its count in refcounts (the page books, see pa_pages_fork) by one
+ * for every row that gave it up; at 0 it is free. Entries outside [0, num_blocks) leave like others, without a count.
+ *   evicted: null, or [num_rows] int32: the blocks that each row gave up (0: the row is as it was)
+ * recent_blocks >= 1 (the newest token's block may be unfinished), sink_blocks + recent_blocks <= budget. The results depend on
+ * the arrays alone. No key or value moves: int8 scales and key bounds stay with their blocks. */
+pa_status pa_evict_blocks(pa_stream* stream, const pa_config* cfg, int32_t* block_tables, int32_t* lens,
+                          float* block_mass, int32_t num_rows, int32_t max_blocks_per_seq, int32_t sink_blocks,
+                          int32_t recent_blocks, int32_t budget, int32_t* refcounts, int32_t* evicted);
+
 /* ---- the projections either side of attention (PagedAttentionLayer.ComputeAttention's
  *      _queryProj/_keyProj/_valueProj.Forward + UpdateKVCache and _outputProj.Forward,
  *      Layers/PagedAttentionLayer.cs:112-142; Linear.Forward y = x W^T without bias,

@@ -1,0 +1,557 @@
+// window_decode.h -- attention of single query tokens over a sliding window and a few first tokens that stay visible.
+//
+// For sequence r of T cached tokens, KV head h and query head g of its group, over the tokens t with t < sink or
+// T - window <= t < T (window 0: all of them):
+//   s_t = scale * q_g . k_t,  out_g = sum_t exp(s_t - max s) v_t / sum_t exp(s_t - max s)
+// and, where masses are kept, mass[r][t / 16] += sum_h sum_g exp(s_t - max s) / sum_t' exp(s_t' - max s).
+//
+// A row is a (sequence, KV head); its list is the blocks that hold a visible token: those of the sinks, then those of
+// the window. The lists are laid end to end and cut into equal ranges, one for each workgroup of a chip full of them, as
+// in sparse_decode.h, whose arithmetic this kernel shares: exact products (an fp32 value as three bf16 parts in
+// the matrix columns that a group of G heads leaves idle), sums in fp32, two register buffers a wave, the waves' states
+// met in LDS at a segment's end. Here the lists follow from the lengths, so nothing but the table is read for them, and the
+// ranges go by what the rows really hold: every workgroup adds up the lengths itself (at most kWindowSeqs a launch).
+#pragma once
+
+#include "sparse_decode.h"
+
+namespace pa {
+
+constexpr int kWindowSeqs = 2047;  // sequences of one launch: their lists' starts stand in LDS
+
+struct WindowArgs {
+    DecodeArgs d;          // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [2 * workgroups][G]
+    int32_t* starts;       // [num_seqs + 1] blocks (of one KV head) before each sequence, then the range
+    float2* parts;         // masses: (maximum, sum) of every list entry's tokens, [Hkv * starts + ..][G]; else null
+    float2* total;         // masses: (maximum, sum) of every row, [num_seqs][Hq]
+    float* mass;           // [num_seqs][max_blocks_per_seq]
+    int32_t num_seqs, sink, window;
+    int32_t least;         // list entries of a range at least
+    int32_t groups;        // workgroups
+};
+
+// The list of a context of T tokens: blocks [0, first), then [low, end).
+struct WindowList {
+    int first, low, end;
+    __device__ __forceinline__ int entries() const { return first + end - low; }
+    __device__ __forceinline__ int block(int e) const { return e < first ? e : e - first + low; }
+};
+__device__ __forceinline__ int window_begin(int T, int window) { return window > 0 ? max(0, T - window) : 0; }
+__device__ __forceinline__ WindowList window_list(int T, int sink, int window) {
+    const int low = window_begin(T, window) / 16;
+    return {min((min(sink, T) + 15) / 16, low), low, (T + 15) / 16};
+}
+
+// The sequences' lists laid end to end: starts[r] in s_starts, and the most that one has. One workgroup, W waves.
+template <int W>
+__device__ __forceinline__ int window_starts(const WindowArgs& a, int32_t* s_starts) {
+    constexpr int PER = (kWindowSeqs + 64 * W) / (64 * W);
+    __shared__ int s_sum[W], s_most[W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int raw[PER], sum = 0, most = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = threadIdx.x * PER + i;
+        raw[i] = r < a.num_seqs ? a.d.context_lens[r] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        raw[i] = window_list(max(0, clamp_len(a.d, raw[i])), a.sink, a.window).entries();
+        sum += raw[i];
+        most = max(most, raw[i]);
+    }
+    const int upto = wave_prefix(sum);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
+    if (lane == 63) s_sum[wave] = upto;
+    if (lane == 0) s_most[wave] = most;
+    __syncthreads();
+    int at = upto - sum;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        at += w < wave ? s_sum[w] : 0;
+        most = max(most, s_most[w]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = threadIdx.x * PER + i;
+        if (r <= a.num_seqs) s_starts[r] = at;
+        at += raw[i];
+    }
+    __syncthreads();
+    return most;
+}
+
+// PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
+template <int D, int KV, bool QF32, int PASSES>
+__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSparseCUs * sparse_waves(D) / 4) void window_decode_kernel(const WindowArgs a) {
+    constexpr bool F32 = KV == PA_DTYPE_FP32;
+    constexpr int NSLAB = D / 32, NT = D / 16;
+    constexpr bool I8 = KV == PA_DTYPE_INT8;
+    constexpr int NI8 = I8 ? D / 64 : 1;           // QK slabs of 64 dims
+    constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
+    constexpr int PP = F32 ? 1 : PASSES;           // passes of P
+    constexpr int W = sparse_waves(D);
+    constexpr int NB = kSparseBuffers;
+    constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
+    __shared__ float s_m[W][16], s_l[W][16];
+    __shared__ float s_o[W][16][CH];
+    __shared__ int32_t s_starts[kWindowSeqs + 1];
+    const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int Hkv = a.d.num_kv_heads, G = a.d.group;
+    const int most = window_starts<W>(a, s_starts);
+    const uint32_t all = static_cast<uint32_t>(s_starts[a.num_seqs]) * Hkv;
+    // Entries a workgroup: equal ranges; whole rows where all are of one length and that gives no workgroup more than
+    // kWindowWaste entries, or a third, over an equal range.
+    uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(a.least));
+    range = (range + W - 1) / W * W;
+    const uint32_t rows = static_cast<uint32_t>(a.num_seqs) * Hkv;
+    if (most > 0 && static_cast<uint32_t>(most) * rows == all) {
+        const uint32_t whole = (rows + a.groups - 1) / a.groups * most;
+        if (whole <= range + 32 || (range > most * 3u / 4 && range <= static_cast<uint32_t>(most))) range = whole;
+    }
+    if (blockIdx.x == 0) {
+        for (int r = threadIdx.x; r <= a.num_seqs; r += 64 * W) a.starts[r] = s_starts[r];
+        if (threadIdx.x == 0) a.starts[a.num_seqs + 1] = static_cast<int32_t>(range);
+    }
+    // sequences without a visible token: zeros
+    for (int r = blockIdx.x; r < a.num_seqs; r += a.groups)
+        if (s_starts[r] == s_starts[r + 1])
+            for (int i = threadIdx.x; i < Hkv * G * D; i += 64 * W) a.d.out[static_cast<int64_t>(r) * Hkv * G * D + i] = 0.0f;
+    uint32_t at_entry = blockIdx.x * range;
+    const uint32_t stop = min(all, at_entry + range);
+    if (blockIdx.x >= (all + range - 1) / range) return;
+    int r = 0;  // the sequence of the first entry: the last one that starts at or before it
+    for (int hi = a.num_seqs; r + 1 < hi;) {
+        const int mid = (r + hi) >> 1;
+        if (static_cast<uint32_t>(s_starts[mid]) * Hkv <= at_entry) r = mid;
+        else hi = mid;
+    }
+    for (; at_entry < stop;) {
+    while (static_cast<uint32_t>(s_starts[r + 1]) * Hkv <= at_entry) r++;
+    const uint32_t base = static_cast<uint32_t>(s_starts[r]) * Hkv;
+    const int held = s_starts[r + 1] - s_starts[r];
+    const int kvh = static_cast<int>((at_entry - base) / held);
+    const int beg = static_cast<int>(at_entry - base) - kvh * held;
+    const int end = static_cast<int>(min(static_cast<uint32_t>(held), beg + (stop - at_entry)));
+    const uint32_t entry0 = base + static_cast<uint32_t>(kvh) * held;  // of the row
+    at_entry += end - beg;
+    const int row = r * Hkv + kvh;
+    const int T = clamp_len(a.d, a.d.context_lens[r]);
+    const int lo = window_begin(T, a.window), sink = min(a.sink, T);
+    const WindowList list = window_list(T, a.sink, a.window);
+    const int32_t* table = a.d.block_tables + static_cast<int64_t>(r) * a.d.max_blocks_per_seq;
+    // Lane l holds the wave's l-th block of a stretch of 64 W entries: its place in the sequence, its physical block. No
+    // load is under a condition, which would make the compiler wait at its end: past the segment the last entry is read again.
+    int lb = list.block(min(beg + wave + W * lane, end - 1));
+    int id = table[lb];
+    bool listed = beg + wave + W * lane < end;
+
+    // Q operand: column n holds head n % G (part n / G of it where Q is split).
+    bf16x8_t qb[F32 || I8 ? 1 : QP][F32 || I8 ? 1 : NSLAB];
+    float qf[F32 ? D / 4 : 1];
+    i32x4_t qd[I8 ? QP : 1][NI8];   // int8: digits of dims (D / 4) q4 + 16 t ..
+    float place[I8 ? QP : 1];       // what a unit of this column's sums is worth
+    const float scale = a.d.scale * kLog2e;
+    {
+        const int64_t q0 = (static_cast<int64_t>(r) * Hkv * G + kvh * G + n % G) * D;
+        if constexpr (F32) {
+#pragma unroll
+            for (int u = 0; u < D / 16; u++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int64_t i = q0 + 16 * u + 4 * q4 + j;
+                    qf[4 * u + j] = QF32 ? static_cast<const float*>(a.d.q)[i]
+                                         : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
+                }
+        } else if constexpr (I8) {
+            float x[D / 4];
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < D / 4; e++) {
+                const int64_t i = q0 + (D / 4) * q4 + e;
+                x[e] = QF32 ? static_cast<const float*>(a.d.q)[i] : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
+                const float f = fabsf(x[e]);
+                top = fmaxf(top, f < INFINITY ? f : INFINITY);  // NaN too
+            }
+            top = rows_max(top);
+            const bool bad = !(top < INFINITY);
+            // |q| < 2^ex; below 2^-96 (nothing that fp32 sums would keep) all of it counts as zero
+            const int ex = max(bad ? 0 : __builtin_amdgcn_frexp_expf(top), -95);
+            int32_t z[D / 4];
+#pragma unroll
+            for (int e = 0; e < D / 4; e++)  // |z| <= 2^30, biased so that its lower three bytes are digits + 128
+                z[e] = (bad ? 0 : static_cast<int32_t>(__builtin_rintf(__builtin_amdgcn_ldexpf(x[e], 30 - ex)))) + 0x808080;
+#pragma unroll
+            for (int p = 0; p < QP; p++) {
+                const int j = QP == 1 ? n / G : p * (16 / G) + n / G;  // this column's digit
+                const int shift = 8 * min(j, 3);
+                const uint32_t flip = j < 3 ? 0x80808080u : 0u, keep = j < 4 ? 0xffffffffu : 0u;
+                place[p] = bad ? __builtin_nanf("") : j < 4 ? __builtin_amdgcn_ldexpf(scale, ex - 30 + 8 * j) : 0.0f;
+#pragma unroll
+                for (int t = 0; t < NI8; t++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        w[k] = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            w[k] |= (static_cast<uint32_t>(z[16 * t + 4 * k + b]) >> shift & 255u) << (8 * b);
+                        w[k] = (w[k] ^ flip) & keep;
+                    }
+                    qd[p][t] = __builtin_bit_cast(i32x4_t, make_uint4(w[0], w[1], w[2], w[3]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < NSLAB; s++) {
+                const int64_t i = q0 + k_dim0<D, KV>(s, q4);
+                if constexpr (!QF32) {
+                    qb[0][s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d.q) + i));
+                } else {
+                    const f32x4_t* src = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.d.q) + i);
+                    const f32x4_t x0 = src[0], x1 = src[1];
+#pragma unroll
+                    for (int p = 0; p < QP; p++) {
+                        const int part_n = PASSES == 1 ? n / G : p * (16 / G) + n / G;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float lo_v = bf16_part(e < 2 ? x0[2 * e] : x1[2 * e - 4], part_n);
+                            const float hi_v = bf16_part(e < 2 ? x0[2 * e + 1] : x1[2 * e - 3], part_n);
+                            w[e] = part_n < 3 ? pack_bf16_trunc(lo_v, hi_v) : 0;
+                        }
+                        qb[p][s] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+                    }
+                }
+            }
+        }
+    }
+    float m_run = -INFINITY, l_run = 0.0f;
+    f32x4_t acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    bool any = false;
+
+    for (int e0 = beg + wave; e0 < end;) {
+        if (!listed || id >= a.d.num_blocks) id = -1;
+        float ks = 0.0f, vs = 0.0f;
+        if constexpr (I8) {
+            if (id >= 0) {
+                ks = a.d.k_scale[static_cast<int64_t>(id) * Hkv + kvh];
+                vs = a.d.v_scale[static_cast<int64_t>(id) * Hkv + kvh];
+            }
+        }
+        const int count = min(64, (end - e0 + W - 1) / W);  // the wave's blocks of this stretch, in lanes 0 ..
+        any = true;
+        int upto = 0;
+        SparseBuf<D, KV> buf[NB];
+        int at[NB];
+        auto load = [&](SparseBuf<D, KV>& b, int& j) {
+            j = upto < count ? upto++ : -1;
+            sparse_load<D, KV>(a.d, b, j >= 0 ? __builtin_amdgcn_readlane(id, j) : -1, kvh);
+        };
+        auto compute = [&](SparseBuf<D, KV>& b, int j) {
+            f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (F32) {
+#pragma unroll
+                for (int u = 0; u < D / 16; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.k[u][i], qf[4 * u + i], s, 0, 0, 0);
+            } else if constexpr (I8) {
+                const float k_scale = readlane_f(ks, j);
+                i32x4_t c[QP];
+#pragma unroll
+                for (int p = 0; p < QP; p++) {
+                    c[p] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+                    for (int t = 0; t < NI8; t++)
+                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                            __builtin_bit_cast(i32x4_t, make_uint4(b.k[2 * t].x, b.k[2 * t].y, b.k[2 * t + 1].x, b.k[2 * t + 1].y)),
+                            qd[p][t], c[p], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+#pragma unroll
+                    for (int p = 0; p < QP; p++) s[i] = __builtin_fmaf(static_cast<float>(c[p][i]), place[p], s[i]);
+                    s[i] *= k_scale;
+                }
+            } else {
+#pragma unroll
+                for (int sl = 0; sl < NSLAB; sl++) {
+                    const bf16x8_t kop = k_operand(b.k[sl]);
+#pragma unroll
+                    for (int p = 0; p < QP; p++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qb[p][sl], s, 0, 0, 0);
+                }
+            }
+            float sc[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = s[i];
+                if constexpr ((QF32 && !F32) || I8) {  // the partial scores of a head's parts
+                    if (G <= 8) x = add_ror<8>(x);
+                    if (G <= 4) x = add_ror<4>(x);
+                    if (G <= 2) x = add_ror<2>(x);
+                    if (G <= 1) x = add_ror<1>(x);
+                }
+                sc[i] = I8 ? x : x * scale;
+            }
+            const int tok = __builtin_amdgcn_readlane(lb, j) * 16;  // the block's first token
+            const int t0 = tok + (KV == PA_DTYPE_BF16 ? 4 * tok_group<KV>(q4) : 4 * q4);
+            if constexpr (I8) {
+#pragma unroll
+                for (int u = 0; u < D / 64; u++) int8_v_transpose(b.v[4 * u], b.v[4 * u + 1], b.v[4 * u + 2], b.v[4 * u + 3]);
+            } else if constexpr (!F32) {
+#pragma unroll
+                for (int u = 0; u < D / 32; u++) bf16_v_exchange(b.v[2 * u], b.v[2 * u + 1]);
+            }
+            if ((tok < lo && tok + 16 > sink) || tok + 16 > T) {  // not every token of the block is seen
+                bool seen[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    seen[i] = t0 + i < T && (t0 + i >= lo || t0 + i < sink);
+                    sc[i] = seen[i] ? sc[i] : -INFINITY;
+                }
+                // their values too: a zero times what an unseen slot may hold (Inf, NaN) is not zero
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) b.v[t][i] = seen[i] ? b.v[t][i] : 0.0f;
+                    } else if constexpr (!I8) {
+                        b.v[t].x &= (seen[0] ? 0xffffu : 0u) | (seen[1] ? 0xffff0000u : 0u);
+                        b.v[t].y &= (seen[2] ? 0xffffu : 0u) | (seen[3] ? 0xffff0000u : 0u);
+                    }
+                }
+            }
+            const float bm = rows_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+            const bool grow = bm > m_run + kSparseRescale || (m_run == -INFINITY && bm > -INFINITY);
+            if (__any(grow)) {
+                const float m_new = grow ? bm : m_run;
+                const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                l_run *= alpha;
+                m_run = m_new;
+                float ar[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * q4 + i, 64);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] *= ar[i];
+            }
+            const float m0 = m_run == -INFINITY ? 0.0f : m_run;  // no score above -inf yet: P is zero
+            float p[4], psum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                p[i] = __builtin_amdgcn_exp2f(sc[i] - m0);
+                psum += p[i];
+            }
+            l_run += psum;
+            if (a.parts) {
+                const float sum = rows_sum(psum);
+                if (lane < G)
+                    a.parts[(static_cast<int64_t>(entry0) + e0 + W * j) * G + lane] = make_float2(m0, sum);
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], b.v[t][i], acc[t], 0, 0, 0);
+            } else {
+                if constexpr (I8) {
+                    const float vf = readlane_f(vs, j);
+                    // (an unseen token's zero stays one whatever the block's scale is)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[i] = p[i] == 0.0f ? 0.0f : p[i] * vf;
+                }
+                s16x4_t pb[PP];
+#pragma unroll
+                for (int q = 0; q < PP; q++) {
+                    const int part_n = PASSES == 1 ? n / G : q * (16 / G) + n / G;
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = part_n < 3 ? bf16_part(p[i], part_n) : 0.0f;
+                    pb[q] = __builtin_bit_cast(s16x4_t, make_uint2(pack_bf16_trunc(x[0], x[1]), pack_bf16_trunc(x[2], x[3])));
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const s16x4_t vop = sparse_v_operand(b.v[t]);
+#pragma unroll
+                    for (int q = 0; q < PP; q++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb[q], vop, acc[t], 0, 0, 0);
+                }
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < NB - 1; i++) load(buf[i], at[i]);
+        bool more = true;
+        while (more) {
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                load(buf[(i + NB - 1) % NB], at[(i + NB - 1) % NB]);
+                if (at[i] < 0) {
+                    more = false;
+                    break;
+                }
+                compute(buf[i], at[i]);
+            }
+        }
+        e0 += 64 * W;
+        if (e0 < end) {
+            lb = list.block(min(e0 + W * lane, end - 1));
+            id = table[lb];
+            listed = e0 + W * lane < end;
+        }
+    }
+
+    // ---- the waves' states meet ----
+    // A wave that saw blocks but no score above -inf is told from one that saw none by the lowest finite maximum:
+    // where no score of the row is, its sum is 0 and the outcome 0 / 0. A NaN score leaves the sum NaN.
+    if (any && m_run == -INFINITY) m_run = -FLT_MAX;
+    const float l_tot = rows_sum(l_run);
+    if (q4 == 0) {
+        s_m[wave][n] = m_run;
+        s_l[wave][n] = l_tot;
+    }
+    constexpr int TT = CH / 16;                                             // tiles per round
+    constexpr int NPART = F32 ? 1 : PASSES == 1 ? 3 : PASSES == 2 ? 2 : 1;  // rows of O that hold a head's parts
+#pragma unroll
+    for (int c = 0; c < D / CH; c++) {
+        if (c > 0) __syncthreads();
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = acc[c * TT + tt][i];
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < G * CH; idx += 64 * W) {
+            const int g = idx / CH, d = idx % CH;
+            // every read of LDS goes out before any is used
+            float m[W], l[W], x[W][NPART];
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                m[w] = s_m[w][g];
+                l[w] = s_l[w][g];
+#pragma unroll
+                for (int k = 0; k < NPART; k++) x[w][k] = s_o[w][g + G * k][d];
+            }
+            float M = m[0];
+#pragma unroll
+            for (int w = 1; w < W; w++) M = fmaxf(M, m[w]);
+            float L = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float f = m[w] == M ? 1.0f : __builtin_amdgcn_exp2f(m[w] - M);
+                float y = x[w][0];
+#pragma unroll
+                for (int k = 1; k < NPART; k++) y += x[w][k];
+                L += l[w] * f;
+                o += y * f;
+            }
+            const int dim = c * CH + d;
+            if (end - beg == held) {
+                a.d.out[(static_cast<int64_t>(row) * G + g) * D + dim] = o / L;
+                if (a.parts && dim == 0) a.total[static_cast<int64_t>(row) * G + g] = make_float2(M, L);
+            } else {
+                const int64_t pi = (2 * static_cast<int64_t>(blockIdx.x) + (beg == 0)) * G + g;
+                a.d.ws_o[pi * D + dim] = o;
+                if (dim == 0) {
+                    a.d.ws_m[pi] = M;
+                    a.d.ws_l[pi] = L;
+                }
+            }
+        }
+    }
+    if (at_entry < stop) __syncthreads();  // the states have been read
+    }
+}
+
+// The parts of a row that was cut: one wave per (row, query head), lanes over dims. The first part lies in slot 1
+// of its range, the others in slot 0 of theirs.
+template <int D>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WindowArgs a) {
+    constexpr int DPL = (D + 63) / 64;
+    const int lane = threadIdx.x & 63, G = a.d.group, Hkv = a.d.num_kv_heads;
+    const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (u >= static_cast<int64_t>(a.num_seqs) * Hkv * G) return;
+    const uint32_t row = static_cast<uint32_t>(u / G), range = a.starts[a.num_seqs + 1];
+    const int g = static_cast<int>(u - static_cast<int64_t>(row) * G);
+    const int r = static_cast<int>(row) / Hkv, kvh = static_cast<int>(row) - r * Hkv;
+    const uint32_t before = a.starts[r], held = a.starts[r + 1] - before;
+    if (held == 0) return;
+    const uint32_t e0 = before * Hkv + kvh * held, first = e0 / range, last = (e0 + held - 1) / range;
+    if (first == last) return;  // written whole
+    const auto part = [&](uint32_t w) { return (2 * static_cast<int64_t>(w) + (w == first)) * G + g; };
+    // Lanes hold the maxima and sums of 64 parts, the outputs are loaded kAhead parts at a time, the first ones
+    // beside the maxima.
+    constexpr int kAhead = 8;
+    float x[kAhead][DPL];
+    auto load = [&](uint32_t w0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t pi = part(min(w0 + j, last));
+#pragma unroll
+            for (int k = 0; k < DPL; k++) x[j][k] = a.d.ws_o[pi * D + min(lane + 64 * k, D - 1)];
+        }
+    };
+    load(first);
+    float M = -INFINITY;
+    for (uint32_t w0 = first; w0 <= last; w0 += 64) M = fmaxf(M, a.d.ws_m[part(min(w0 + lane, last))]);
+    M = wave_max_dpp(M);
+    float L = 0.0f, o[DPL];
+#pragma unroll
+    for (int k = 0; k < DPL; k++) o[k] = 0.0f;
+    for (uint32_t w0 = first; w0 <= last; w0 += 64) {
+        const int64_t pi = part(min(w0 + lane, last));
+        const float m = a.d.ws_m[pi], l = a.d.ws_l[pi];
+        const float f = w0 + lane > last ? 0.0f : m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M);
+        L += w0 + lane > last ? 0.0f : l * f;
+        for (uint32_t w = w0; w <= min(last, w0 + 63); w += kAhead) {
+            if (w > first) load(w);
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                if (w + j > last) break;
+                const float fj = readlane_f(f, static_cast<int>(w + j - w0));
+#pragma unroll
+                for (int k = 0; k < DPL; k++) o[k] += x[j][k] * fj;
+            }
+        }
+    }
+    L = wave_sum(L);
+#pragma unroll
+    for (int k = 0; k < DPL; k++)
+        if (lane + 64 * k < D) a.d.out[u * D + lane + 64 * k] = o[k] / L;
+    if (a.parts && lane == 0) a.total[u] = make_float2(M, L);
+}
+
+template <int D>
+void launch_window_decode(const WindowArgs& a, int kv_dtype, bool q_f32, bool merge, hipStream_t s) {
+    const int G = a.d.group;
+    const auto go = [&](auto kernel) { kernel<<<a.groups, 64 * sparse_waves(D), 0, s>>>(a); };
+    const auto by_q = [&](auto kv, auto passes) {
+        constexpr int KV = decltype(kv)::value, P = decltype(passes)::value;
+        if (q_f32) go(window_decode_kernel<D, KV, true, P>);
+        else go(window_decode_kernel<D, KV, false, P>);
+    };
+    const auto by_group = [&](auto kv) {
+        if (G <= 4) by_q(kv, std::integral_constant<int, 1>());
+        else if (G == 8) by_q(kv, std::integral_constant<int, 2>());
+        else by_q(kv, std::integral_constant<int, 3>());
+    };
+    if (kv_dtype == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>(), std::integral_constant<int, 1>());
+    else if (kv_dtype == PA_DTYPE_BF16) by_group(std::integral_constant<int, PA_DTYPE_BF16>());
+    else if constexpr (D >= 64) by_group(std::integral_constant<int, PA_DTYPE_INT8>());
+    if (merge) {
+        const int64_t waves = static_cast<int64_t>(a.num_seqs) * a.d.num_kv_heads * G;
+        window_merge_kernel<D><<<static_cast<uint32_t>((waves + 3) / 4), 256, 0, s>>>(a);
+    }
+}
+#ifndef PA_WINDOW_INSTANTIATE
+extern template void launch_window_decode<32>(const WindowArgs&, int, bool, bool, hipStream_t);
+extern template void launch_window_decode<64>(const WindowArgs&, int, bool, bool, hipStream_t);
+extern template void launch_window_decode<128>(const WindowArgs&, int, bool, bool, hipStream_t);
+extern template void launch_window_decode<256>(const WindowArgs&, int, bool, bool, hipStream_t);
+#endif
+
+}  // namespace pa

@@ -1,0 +1,5 @@
+// window_decode_d64.hip -- head_dim 64 instantiations of the attention over a window and sinks.
+#define PA_WINDOW_INSTANTIATE
+#include "window_decode.h"
+
+template void pa::launch_window_decode<64>(const pa::WindowArgs&, int, bool, bool, hipStream_t);

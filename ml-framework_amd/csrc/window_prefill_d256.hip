@@ -1,0 +1,7 @@
+// window_prefill_d256.hip -- head_dim 256 instantiations of the chunks' attention over a window and sinks.
+#define PA_WINDOW_INSTANTIATE
+#include <type_traits>
+
+#include "window_prefill.h"
+
+template void pa::launch_window_prefill<256>(const pa::WindowPrefillArgs&, int, bool, int, uint32_t, hipStream_t);

@@ -64,6 +64,8 @@ EXPORTS = (
     "pa_key_bounds_bytes", "pa_key_bounds_update", "pa_select_workspace_size", "pa_select_blocks",
     "pa_sparse_workspace_size", "pa_sparse_decode",
     "pa_pages_fork", "pa_pages_workspace_size", "pa_pages_reserve", "pa_pages_compact", "pa_copy_pages",
+    "pa_window_decode_workspace_size", "pa_window_decode", "pa_window_prefill_workspace_size", "pa_window_prefill",
+    "pa_prefill_mass", "pa_evict_blocks",
 )
 
 
@@ -177,6 +179,12 @@ _SIGNATURES = {
     "pa_pages_reserve": [_P, _CFG, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P, _SZ],
     "pa_pages_compact": [_P, _CFG, _P, _I32, _I32, _P, _I32, _P, _P, _P, _SZ],
     "pa_copy_pages": [_P, _CFG, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P],
+    "pa_window_decode_workspace_size": [_CFG, _I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_SZ)],
+    "pa_window_decode": [_P, _CFG, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _SZ],
+    "pa_window_prefill_workspace_size": [_CFG, _I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_SZ)],
+    "pa_window_prefill": [_P, _CFG, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _SZ],
+    "pa_prefill_mass": [_P, _CFG, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+    "pa_evict_blocks": [_P, _CFG, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P],
 }
 
 _lib = None
@@ -544,6 +552,54 @@ def copy_pages(stream, cfg: PaConfig, k_cache, v_cache, k_scale, v_scale, k_absm
     call("pa_copy_pages", stream.handle if stream else None, ctypes.byref(cfg), _ptr(k_cache), _ptr(v_cache),
          _ptr(k_scale), _ptr(v_scale), _ptr(k_absmax), _ptr(v_absmax), _ptr(key_bounds), _ptr(pairs), max_pairs,
          _ptr(num_pairs))
+
+
+# ---- caches of bounded size: windows, masses, eviction ----------------------------------------
+def window_decode_workspace_size(cfg: PaConfig, num_seqs: int, max_context_len: int, sink_tokens: int, window: int,
+                                 with_mass: bool = False) -> int:
+    n = ctypes.c_size_t()
+    call("pa_window_decode_workspace_size", ctypes.byref(cfg), num_seqs, max_context_len, sink_tokens, window,
+         int(with_mass), ctypes.byref(n))
+    return n.value
+
+
+def window_decode(stream, cfg: PaConfig, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, num_seqs,
+                  max_blocks_per_seq, max_context_len, sink_tokens, window, block_mass=None, workspace=None,
+                  workspace_bytes=0):
+    call("pa_window_decode", stream.handle if stream else None, ctypes.byref(cfg), _ptr(out), _ptr(q), _ptr(k_cache),
+         _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables), _ptr(context_lens), num_seqs,
+         max_blocks_per_seq, max_context_len, sink_tokens, window, _ptr(block_mass), _ptr(workspace), workspace_bytes)
+
+
+def window_prefill_workspace_size(cfg: PaConfig, num_seqs: int, max_chunk_len: int, max_context_len: int, sink_tokens: int,
+                                  window: int) -> int:
+    n = ctypes.c_size_t()
+    call("pa_window_prefill_workspace_size", ctypes.byref(cfg), num_seqs, max_chunk_len, max_context_len, sink_tokens,
+         window, ctypes.byref(n))
+    return n.value
+
+
+def window_prefill(stream, cfg: PaConfig, out, q, q_start_loc, prefix_lens, k_cache, v_cache, k_scale, v_scale,
+                   block_tables, num_seqs, max_blocks_per_seq, max_chunk_len, max_context_len, sink_tokens, window,
+                   lse=None, workspace=None, workspace_bytes=0):
+    call("pa_window_prefill", stream.handle if stream else None, ctypes.byref(cfg), _ptr(out), _ptr(q),
+         _ptr(q_start_loc), _ptr(prefix_lens), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+         _ptr(block_tables), num_seqs, max_blocks_per_seq, max_chunk_len, max_context_len, sink_tokens, window, _ptr(lse),
+         _ptr(workspace), workspace_bytes)
+
+
+def prefill_mass(stream, cfg: PaConfig, q, lse, q_start_loc, prefix_lens, k_cache, k_scale, block_tables, num_seqs,
+                 max_blocks_per_seq, max_context_len, last_queries, sink_tokens, window, block_mass):
+    call("pa_prefill_mass", stream.handle if stream else None, ctypes.byref(cfg), _ptr(q), _ptr(lse), _ptr(q_start_loc),
+         _ptr(prefix_lens), _ptr(k_cache), _ptr(k_scale), _ptr(block_tables), num_seqs, max_blocks_per_seq,
+         max_context_len, last_queries, sink_tokens, window, _ptr(block_mass))
+
+
+def evict_blocks(stream, cfg: PaConfig, block_tables, lens, block_mass, num_rows, max_blocks_per_seq, sink_blocks,
+                 recent_blocks, budget, refcounts, evicted=None):
+    call("pa_evict_blocks", stream.handle if stream else None, ctypes.byref(cfg), _ptr(block_tables), _ptr(lens),
+         _ptr(block_mass), num_rows, max_blocks_per_seq, sink_blocks, recent_blocks, budget, _ptr(refcounts),
+         _ptr(evicted))
 
 
 # ---- projections either side of attention ----------------------------------------------------
