@@ -5,15 +5,18 @@
 //   s_t = scale * q_g . k_t,  out = sum_t exp(s_t - max s) v_t / sum_t exp(s_t - max s),  lse = ln sum_t exp(s_t)
 //
 // The (query, query head) pairs of one (sequence, KV head), query by query, are the columns of the matrix products: a wave
-// takes 32 of them, whatever the ratio of heads is, and a workgroup streams the blocks that any of its columns
-// sees through LDS, two at a time. Per pair of blocks, on v_mfma_f32_32x32x16_bf16:
+// takes 32 of them, whatever the ratio of heads is, and streams the blocks that any of them sees through LDS, two at a time.
+// Per pair of blocks, on v_mfma_f32_32x32x16_bf16:
 //   S^T[32 keys][32 columns] = K . Q^T, whose rows are permuted so that a lane ends up with 8 consecutive tokens of each block for
 //     its column;
 //   O^T[D][32 columns] += V^T . P^T, whose P operand is what the lane then holds and whose accumulators belong to the lane's
 //     own column: maxima, sums and the rescale need one exchange with the other half of the wave.
-// Results are as exact as fp32 sums of exact products: bf16 keys and values and int8 codes are one bf16 operand, fp32 ones the sum of
-// three (8 bits each), and so are fp32 queries; products of parts below 2^-24 are left out. P is two bf16 parts rounded to
-// nearest (off by 2^-18 at most, 0.7e-6 in the mean square), three for fp32 caches.
+// Tiles go from memory straight into LDS (16-byte loads with the LDS bit, in inline asm with explicit waits) in the cache's type. Where
+// columns are many, the four waves of a workgroup take 32 each and share a ring of pairs, two of them in flight; where they are
+// few, the waves share the columns and every one streams pairs of its own through a slot of its own, without a barrier: the next
+// pair's keys go out when this pair's have been read, its values likewise, and the waves' states meet at the end.
+// Results are as exact as fp32 sums of exact products: bf16 keys and values and int8 codes are one bf16 operand, fp32 values
+// (queries, probabilities, caches) the sum of three (8 bits each); products of parts below 2^-24 are left out.
 #pragma once
 
 #include <cfloat>
@@ -90,12 +93,21 @@ __device__ __forceinline__ void load_planes(const void* base, int64_t i, uint4 (
 __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
-// A value made where it stands. hipcc (ROCm 7.2) counts too few waits where a branch, taken, lies between a matrix instruction and the
-// first read of its result: a product's last registers then lacked its last terms now and then (seen at 7 wait states of
-// 11). What reads a product first is therefore kept in the product's own block by this.
+// A matrix product's last register, read where the product stands. hipcc (ROCm 7.2) counts too few waits where a branch, taken, lies
+// between a matrix instruction and the first read of its result: its last registers then lacked its last terms now and then
+// (seen at 7 wait states of 11). A move in the product's own block is waited for as it should be, and what is
+// read after it is safe.
 __device__ __forceinline__ float settled(float x) {
-    asm volatile("" : "+v"(x));
-    return x;
+    float y = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xE4, 0xF, 0xF, true));  // quad_perm 0 1 2 3
+    asm volatile("" : "+v"(y));
+    return y;
+}
+// int8 codes k, k + 1 (k: 0 or 2) of w as two bf16, exactly; w with every byte's top bit flipped (code + 128): the byte is placed in
+// the fraction of 2^23, from which 2^23 + 128 is taken off.
+__device__ __forceinline__ uint32_t i8_pair(uint32_t w, int k) {
+    const float lo = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k)) - 8388736.0f;
+    const float hi = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k + 1)) - 8388736.0f;
+    return pack_bf16_trunc(lo, hi);
 }
 // The other half of the wave's value joined with this lane's.
 __device__ __forceinline__ float halves_max(float x) {
@@ -129,42 +141,114 @@ struct WindowSpan {
     __device__ __forceinline__ bool some_see(int t) const { return t < hi && (t >= lo || t < sink); }
     __device__ __forceinline__ bool all_see(int t) const { return t < hi_all && (t >= lo_all || t < sink); }
     __device__ __forceinline__ bool all_see_block(int t) const { return t + 16 <= hi_all && (t >= lo_all || t + 16 <= sink); }
+    __device__ __forceinline__ bool hides_some(int t) const { return !(t + 16 <= hi && (t >= lo || t + 16 <= sink)); }
     __device__ __forceinline__ bool none_see_block(int t) const { return t >= hi || (t + 16 <= lo && t >= sink); }
 };
 
-// LDS: operands of 8 values (16 bytes). K row r (of 16), operand column c (of D / 8) at kpos; V dim d, tokens 8 h .. at vpos. The
-// 16 lanes that gfx950 serves in one clock (quads {0, 3, 5, 6} and {1, 2, 4, 7} of a half-wave) then read 16 different
-// 16-byte positions of a 256-byte line: their rows are 16 different keys, their dims 8 of either half of 32.
-template <int D>
+// A block's tiles in LDS, in 16-byte pieces: K row r (of 16), piece c (of RC) at kpos; V dim d, piece x (of ELT) at vpos. The 16 lanes
+// that gfx950 serves in one clock (quads {0, 3, 5, 6} and {1, 2, 4, 7} of a half-wave) read one piece column of 16 different keys, or one
+// piece of 16 dims; with these XORs they meet 16 different 16-byte positions of a 256-byte line (int8: 8 bytes of each).
+template <int D, int ELT>
 struct WindowTile {
-    static constexpr int RC = D / 8, CHUNKS = 16 * RC;  // operands per K row, per tile
-    __device__ static constexpr int kpos(int r, int c) {
-        return RC >= 16 ? r * RC + (c ^ r) : r * RC + (c ^ ((r / (16 / RC)) & (RC - 1)));
-    }
-    __device__ static constexpr int vpos(int d, int h) { return 2 * d + (h ^ ((d >> 4) & 1)); }
+    static constexpr int RC = D * ELT / 16, CH = 16 * RC;  // pieces per K row, per tile
+    static constexpr int SEG = CH / 64;                     // loads of a wave per tile
+    __device__ static constexpr int kswz(int r) { return RC >= 16 ? r : (r / (16 / RC)) & (RC - 1); }
+    __device__ static constexpr int vswz(int d) { return ELT == 2 ? (d >> 4) & 1 : ELT == 4 ? (d >> 2) & 3 : 0; }
+    __device__ static constexpr int kpos(int r, int c) { return r * RC + (c ^ kswz(r)); }
+    __device__ static constexpr int vpos(int d, int x) { return d * ELT + (x ^ vswz(d)); }
+    // the memory piece that stands at position p (the XORs are their own inverse)
+    __device__ static constexpr int ksrc(int p) { return p / RC * RC + (p % RC ^ kswz(p / RC)); }
+    __device__ static constexpr int vsrc(int p) { return p / ELT * ELT + (p % ELT ^ vswz(p / ELT)); }
 };
 
-// Waves that share a set of 32 columns where columns are few (each takes its own pair of blocks): as many as LDS has room for.
-__host__ __device__ constexpr int window_key_waves(int d, int kv) { return kv != PA_DTYPE_FP32 || d <= 64 ? 4 : d == 128 ? 2 : 1; }
+// Whether the waves of a workgroup may share 32 columns (the slots of four waves fit LDS).
+__host__ __device__ constexpr bool window_shares(int d, int kv) { return kv != PA_DTYPE_FP32 || d <= 128; }
+// Workgroups a CU holds: by LDS and registers.
+__host__ __device__ constexpr int window_groups(int d, int kv) { return d <= 128 && kv != PA_DTYPE_FP32 ? 2 : 1; }
 
-template <int D, int KV, bool QF32, int KS>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_prefill_kernel(const WindowPrefillArgs a) {
+// What a column is: query token and head, the tokens it sees.
+struct WindowColumn {
+    int64_t row;  // of q, out and lse
+    int hi, lo;
+    __device__ __forceinline__ WindowColumn(const WindowPrefillArgs& a, int64_t c, int q0, int kvh, int P, int T) {
+        const int i = static_cast<int>(c / a.group);
+        row = (static_cast<int64_t>(q0) + i) * a.num_kv_heads * a.group + kvh * a.group + (c - static_cast<int64_t>(i) * a.group);
+        hi = min(T, P + i + 1);
+        lo = a.window > 0 ? max(0, P + i + 1 - a.window) : 0;
+    }
+    __device__ __forceinline__ bool sees(int t, int sink) const { return t < hi && (t >= lo || t < sink); }
+    __device__ __forceinline__ bool any(int sink) const { return hi > lo || min(sink, hi) > 0; }
+};
+
+// Column c over the blocks of list entries [e0, e1), one key at a time: (maximum, sum, O), lanes over dims. For values that are not
+// finite at tokens that some columns of a wave see and others do not.
+template <int D, int KV, bool QF32>
+__device__ void window_column_alone(const WindowPrefillArgs& a, const WindowColumn& c, const WindowSpan& span, const int32_t* table,
+                                    int kvh, int e0, int e1, float& M, float& L, float (&o)[(D + 63) / 64]) {
+    constexpr bool F32 = KV == PA_DTYPE_FP32;
+    constexpr int DPL = (D + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    float q[DPL];
+    M = -INFINITY;
+    L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DPL; k++) {
+        const int64_t at = c.row * D + min(lane + 64 * k, D - 1);
+        q[k] = QF32 ? static_cast<const float*>(a.q)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.q)[at]);
+        o[k] = 0.0f;
+    }
+    for (int e = e0; e < e1; e++) {
+        const int tok = 16 * span.block(e), id = table[tok / 16];
+        const bool real = id >= 0 && id < a.num_blocks;
+        const int64_t tile = (static_cast<int64_t>(real ? id : 0) * a.num_kv_heads + kvh) * 16 * D;
+        for (int j = 0; j < 16; j++) {
+            if (!c.sees(tok + j, span.sink)) continue;
+            float x = 0.0f, v[DPL];
+#pragma unroll
+            for (int k = 0; k < DPL; k++) {
+                v[k] = 0.0f;
+                if (real && lane + 64 * k < D) {
+                    const int64_t ka = tile + j * D + lane + 64 * k, va = tile + (lane + 64 * k) * 16 + j;
+                    const float kx = F32 ? static_cast<const float*>(a.k_cache)[ka] : bf16_to_f32(static_cast<const uint16_t*>(a.k_cache)[ka]);
+                    v[k] = F32 ? static_cast<const float*>(a.v_cache)[va] : bf16_to_f32(static_cast<const uint16_t*>(a.v_cache)[va]);
+                    x = __builtin_fmaf(q[k], kx, x);
+                }
+            }
+            x = wave_sum(x) * (a.scale * 1.4426950408889634f);
+            const float m_new = fmaxf(M, x);
+            const float f = m_new == M ? 1.0f : __builtin_amdgcn_exp2f(M - m_new);
+            const float p = __builtin_amdgcn_exp2f(x - (m_new == -INFINITY ? 0.0f : m_new));
+            L = L * f + p;
+#pragma unroll
+            for (int k = 0; k < DPL; k++) o[k] = o[k] * f + p * v[k];
+            M = m_new;
+        }
+    }
+}
+
+// SHARE: the waves share 32 columns and take pairs of blocks in turn; else each has 32 columns of its own and all take every pair.
+template <int D, int KV, bool QF32, bool SHARE>
+__global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kernel(const WindowPrefillArgs a) {
     constexpr bool F32 = KV == PA_DTYPE_FP32, I8 = KV == PA_DTYPE_INT8;
-    constexpr int NP = F32 ? 3 : 1, NQ = QF32 ? 3 : 1, PP = F32 ? 3 : 2;  // operands of a cache value, a query's, a probability's
-    constexpr int NS = D / 16, ND = D / 32, SETS = 4 / KS, COLS = 32 * SETS;
-    using TL = WindowTile<D>;
-    constexpr int TILE = 16 * D, CH = TL::CHUNKS;
-    __shared__ uint4 s_k[KS][2][NP][CH], s_v[KS][2][NP][CH];
-    __shared__ float s_ks[2 * KS], s_vs[2 * KS];
+    constexpr int NP = F32 ? 3 : 1, NQ = QF32 ? 3 : 1, PP = 3;  // bf16 operands of a cache value, a query's, a probability's
+    constexpr int ELT = F32 ? 4 : I8 ? 1 : 2;
+    constexpr int NS = D / 16, ND = D / 32, COLS = SHARE ? 32 : 128;
+    using TL = WindowTile<D, ELT>;
+    constexpr int TILE = 16 * D, CH = TL::CH, SEG = TL::SEG, SLOT = 4 * CH;  // a slot: K, V of one block, K, V of the other
+    constexpr int RING = F32 && D > 128 ? 2 : 3;                              // slots of the shared ring
+    constexpr int AHEAD = SHARE ? 1 : RING - 1;                               // pairs in flight
+    constexpr int STATE = 32 * D * 4 / 16;                                    // a wave's O in LDS
+    constexpr int PIECES = SHARE ? 4 * (SLOT > STATE ? SLOT : STATE) : RING * SLOT;
+    __shared__ uint4 s_tile[PIECES];
     __shared__ float2 s_ml[4][32];
     __shared__ int s_bad[4];
     const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int set = wave / KS, ks = wave % KS;
+    __builtin_assume(wave >= 0 && wave < 4);
     const int split = blockIdx.y;
     int gi, wk;
     if (!place_workgroup(a.num_groups, a.per, gi, wk)) return;
-    const int Hkv = a.num_kv_heads, G = a.group, Hq = Hkv * G;
+    const int Hkv = a.num_kv_heads, G = a.group;
     const int seq = gi / Hkv, kvh = gi - seq * Hkv;
     const int q0 = a.q_start_loc[seq];
     const int Lc = min(a.q_start_loc[seq + 1] - q0, a.max_chunk_len);
@@ -177,23 +261,23 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_prefill_kernel(co
     const WindowSpan span(P, static_cast<int>(c_wg / G), static_cast<int>((min(columns, c_wg + COLS) - 1) / G), T, a.sink, a.window);
     const int32_t* table = a.block_tables + static_cast<int64_t>(seq) * a.max_blocks_per_seq;
     // this workgroup's part of the list, in pairs of blocks
-    const int pairs = (span.entries() + 1) / 2, share = (pairs + a.splits - 1) / a.splits;
+    const int entries = span.entries();
+    const int pairs = (entries + 1) / 2, share = (pairs + a.splits - 1) / a.splits;
     const int pair0 = min(split * share, pairs), pair1 = min(pair0 + share, pairs);
+    const int count = SHARE ? max(0, (pair1 - pair0 - wave + 3) / 4) : pair1 - pair0;  // this wave's pairs
+    auto pair_of = [&](int j) { return SHARE ? pair0 + wave + 4 * j : pair0 + j; };
 
     // this wave's columns; those past the last are computed as the last and not stored
-    const int64_t c_set = min(c_wg + 32 * set, columns - 1), c_end = min(columns, c_wg + 32 * set + 32);
-    const bool live = c_wg + 32 * set < columns;
-    const WindowSpan mine(P, static_cast<int>(c_set / G), static_cast<int>((max(c_end, c_set + 1) - 1) / G), T, a.sink, a.window);
-    const int64_t col = min(c_wg + 32 * set + n, columns - 1);
-    const int qi = static_cast<int>(col / G), head = kvh * G + static_cast<int>(col - static_cast<int64_t>(qi) * G);
-    const int hi = min(T, P + qi + 1), lo = a.window > 0 ? max(0, P + qi + 1 - a.window) : 0;
-    const int64_t qrow = (static_cast<int64_t>(q0) + qi) * Hq + head;
+    const int64_t c_wave = c_wg + (SHARE ? 0 : 32 * wave);
+    const bool live = c_wave < columns;
+    const WindowSpan mine(P, static_cast<int>(min(c_wave, columns - 1) / G), static_cast<int>((min(columns, c_wave + 32) - 1) / G), T, a.sink, a.window);
+    const WindowColumn col(a, min(c_wave + n, columns - 1), q0, kvh, P, T);
 
     uint4 qv[NQ][NS];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
         uint4 x[NQ];
-        load_planes<QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16, NQ>(a.q, qrow * D + 16 * s + 8 * hf, x);
+        load_planes<QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16, NQ>(a.q, col.row * D + 16 * s + 8 * hf, x);
 #pragma unroll
         for (int p = 0; p < NQ; p++) qv[p][s] = x[p];
     }
@@ -205,81 +289,124 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_prefill_kernel(co
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
 
-    for (int pr = pair0; pr < pair1; pr += KS) {
-        __syncthreads();
-        for (int x = threadIdx.x; x < KS * 2 * 2 * CH; x += 256) {
-            const int b = x / (2 * CH), y = x % (2 * CH), ch = y % CH;
-            const bool is_v = y >= CH;
-            const int e = 2 * pr + b;
-            const int lb = span.block(min(e, max(span.entries() - 1, 0)));
-            int id = e < span.entries() && e < 2 * pair1 ? table[lb] : -1;
-            if (id >= a.num_blocks) id = -1;
-            uint4 plane[NP];
+    // ---- the stream ----
+    // Ids (and int8 scales) of 32 pairs of this wave's at a time: lane l has block l % 2 of pair l / 2. The loads of the tiles are counted
+    // by hand, so nothing else may be under way: the wave waits for a refill at once.
+    int ids = -1;
+    float ks_lane = 0.0f, vs_lane = 0.0f;
+    auto refill = [&](int j) {
+        const int pr = pair_of(j + (lane >> 1)), e = 2 * pr + (lane & 1);
+        ids = -1;
+        if (j + (lane >> 1) < count && e < entries) ids = table[span.block(e)];
+        if (ids >= a.num_blocks) ids = -1;
+        if constexpr (I8) {
+            ks_lane = ids >= 0 ? a.k_scale[static_cast<int64_t>(ids) * Hkv + kvh] : 0.0f;
+            vs_lane = ids >= 0 ? a.v_scale[static_cast<int64_t>(ids) * Hkv + kvh] : 0.0f;
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        asm volatile("" : "+v"(ids), "+v"(ks_lane), "+v"(vs_lane)::"memory");
+    };
+    uint32_t koff[SEG], voff[SEG];  // this lane's place in the tile of each load
 #pragma unroll
-            for (int p = 0; p < NP; p++) plane[p] = make_uint4(0, 0, 0, 0);
-            if (id >= 0)
-                load_planes<KV, NP>(is_v ? a.v_cache : a.k_cache, (static_cast<int64_t>(id) * Hkv + kvh) * TILE + 8 * ch, plane);
-            if (!is_v) {
+    for (int j = 0; j < SEG; j++) {
+        koff[j] = 16 * TL::ksrc(64 * j + lane);
+        voff[j] = 16 * TL::vsrc(64 * j + lane);
+    }
+    const uint32_t base = lds_address(s_tile);
+    const char* const kc = static_cast<const char*>(a.k_cache);
+    const char* const vc = static_cast<const char*>(a.v_cache);
+    // One tile into LDS; no such block reads as zeros through a zero-sized descriptor, so that every pair is as many loads.
+    auto fetch = [&](const char* cache, const uint32_t (&off)[SEG], int id, uint32_t to) {
+        const int64_t at = (static_cast<int64_t>(id >= 0 ? id : 0) * Hkv + kvh) * TILE * ELT;
+        u32x4_t rsrc = buffer_rsrc_words(cache + at, id >= 0 ? TILE * ELT : 0);
 #pragma unroll
-                for (int p = 0; p < NP; p++) s_k[b >> 1][b & 1][p][TL::kpos(ch / TL::RC, ch % TL::RC)] = plane[p];
-            } else {
-                const int t = 16 * lb + 8 * (ch & 1);
-                uint32_t keep[4];  // values that no column sees are zeros: what unused slots hold does not matter
+        for (int i = 0; i < 4; i++) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);  // (uniform, but not seen to be everywhere)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    keep[j] = (span.some_see(t + 2 * j) ? 0xffffu : 0u) | (span.some_see(t + 2 * j + 1) ? 0xffff0000u : 0u);
+        for (int j = 0; j < SEG; j++) lds_load16(rsrc, off[j], to + 1024 * j);
+    };
+    // SHARE: both blocks' K (or V) tiles into this wave's slot.
+    auto fetch_own = [&](bool v, int j) {
 #pragma unroll
-                for (int p = 0; p < NP; p++)
-                    s_v[b >> 1][b & 1][p][TL::vpos(ch >> 1, ch & 1)] =
-                        make_uint4(plane[p].x & keep[0], plane[p].y & keep[1], plane[p].z & keep[2], plane[p].w & keep[3]);
-            }
-            if constexpr (I8) {
-                if (y == 0) {
-                    s_ks[b] = id >= 0 ? a.k_scale[static_cast<int64_t>(id) * Hkv + kvh] : 0.0f;
-                    s_vs[b] = id >= 0 ? a.v_scale[static_cast<int64_t>(id) * Hkv + kvh] : 0.0f;
-                }
+        for (int u = 0; u < 2; u++) {
+            const int id = __builtin_amdgcn_readlane(ids, 2 * (j & 31) + u);
+            fetch(v ? vc : kc, v ? voff : koff, id, base + 16 * (wave * SLOT + (2 * u + v) * CH));
+        }
+    };
+    // Ring: wave w brings tile w % 2 (K, V) of block w / 2 of pair j.
+    auto fetch_shared = [&](int j, int slot) {
+        const int id = __builtin_amdgcn_readlane(ids, 2 * (j & 31) + (wave >> 1));
+        const uint32_t to = base + 16 * (slot * SLOT + wave * CH);
+        if (wave & 1) fetch(vc, voff, id, to);
+        else fetch(kc, koff, id, to);
+    };
+    float sc[AHEAD + 1][4];  // int8: K and V scales of the pairs under way, [0]: of this one
+    auto take_scales = [&](int at, int j) {
+        if constexpr (I8) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                sc[at][u] = readlane_f(ks_lane, 2 * (j & 31) + u);
+                sc[at][2 + u] = readlane_f(vs_lane, 2 * (j & 31) + u);
             }
         }
-        __syncthreads();
-        const int e0 = 2 * (pr + ks);
-        if (!live || pr + ks >= pair1) continue;
-        const int tok0 = 16 * span.block(e0);
-        const int tok1 = e0 + 1 < span.entries() ? 16 * span.block(e0 + 1) : INT32_MAX - 64;  // no such block: past every end
-        if (mine.none_see_block(tok0) && mine.none_see_block(tok1)) continue;
+    };
+    // The bf16 operands of 8 values that stand in `part` (fp32: and the piece behind it), masked by token where `keep` says so.
+    auto operand = [&](const uint4* tile, int p0, int p1, uint4 (&op)[NP]) {
+        if constexpr (I8) {
+            const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(tile + p0) + 8 * hf);
+            const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
+            op[0] = make_uint4(i8_pair(x, 0), i8_pair(x, 2), i8_pair(y, 0), i8_pair(y, 2));
+        } else if constexpr (F32) {
+            const f32x4_t x = __builtin_bit_cast(f32x4_t, tile[p0]), y = __builtin_bit_cast(f32x4_t, tile[p1]);
+            const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            bf16_planes<NP>(v, op);
+        } else {
+            op[0] = tile[p0];
+        }
+    };
+
+    const int krow = key_of_row(n);
+    auto compute = [&](const uint4* slot, int j, auto after_keys, auto before_values) {
+        const int e0 = 2 * pair_of(j);
+        const int tok[2] = {16 * span.block(e0), e0 + 1 < entries ? 16 * span.block(e0 + 1) : INT32_MAX - 64};  // no such block: past every end
         f32x16_t s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
-        const int krow = key_of_row(n);
+        const uint4* const kt = slot + (n >> 4) * 2 * CH;
 #pragma unroll
         for (int sl = 0; sl < NS; sl++) {
             uint4 kop[NP];
-#pragma unroll
-            for (int p = 0; p < NP; p++) kop[p] = s_k[ks][n >> 4][p][TL::kpos(krow, 2 * sl + hf)];
+            if constexpr (I8) operand(kt, TL::kpos(krow, sl), 0, kop);
+            else if constexpr (F32) operand(kt, TL::kpos(krow, 4 * sl + 2 * hf), TL::kpos(krow, 4 * sl + 2 * hf + 1), kop);
+            else operand(kt, TL::kpos(krow, 2 * sl + hf), 0, kop);
 #pragma unroll
             for (int p = 0; p < NP; p++)
 #pragma unroll
                 for (int q = 0; q < NQ; q++)
                     if (p + q <= 2) s = mfma32(kop[p], qv[q][sl], s);
         }
-        // lane: tokens tok_u + 8 hf + j of its column in s[8 u + j]
+        s[15] = settled(s[15]);
+        after_keys();
+        // lane: tokens tok[u] + 8 hf + i of its column in s[8 u + i]
+        float f[2] = {c2, c2};
+        if constexpr (I8) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                f[u] = c2 * sc[0][u];
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[8 * u + i] *= f[u];
+                f[u] = 1.0f;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const float f = I8 ? c2 * s_ks[2 * ks + u] : c2;
+            if (mine.all_see_block(tok[u])) continue;
 #pragma unroll
-            for (int j = 0; j < 8; j++) s[8 * u + j] = settled(s[8 * u + j] * f);
-            const int tok = u ? tok1 : tok0;
-            if (!mine.all_see_block(tok)) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int t = tok + 8 * hf + j;
-                    s[8 * u + j] = t < hi && (t >= lo || t < span.sink) ? s[8 * u + j] : -INFINITY;
-                }
-            }
+            for (int i = 0; i < 8; i++) s[8 * u + i] = col.sees(tok[u] + 8 * hf + i, span.sink) ? s[8 * u + i] : -INFINITY;
         }
         float bm = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) bm = fmaxf(bm, s[i]);
-        bm = halves_max(bm);
+        bm = halves_max(bm) * f[0];
         const bool grow = bm > m_run + 8.0f || (m_run == -INFINITY && bm > -INFINITY);
         if (__any(grow)) {
             const float m_new = grow ? bm : m_run;
@@ -294,55 +421,116 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_prefill_kernel(co
         const float m0 = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - m0);
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f[0], -m0));
             l_run += s[i];
         }
+        before_values();
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             uint4 pop[PP];
             float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[j] = s[8 * u + j];
-                if constexpr (I8) x[j] = x[j] == 0.0f ? 0.0f : x[j] * s_vs[2 * ks + u];  // (whatever the scale of an unseen block is)
+            for (int i = 0; i < 8; i++) {
+                x[i] = s[8 * u + i];
+                if constexpr (I8) x[i] = x[i] == 0.0f ? 0.0f : x[i] * sc[0][2 + u];  // (whatever the scale of an unseen block is)
             }
-            if constexpr (F32) {
-                bf16_planes<PP>(x, pop);
-            } else {
-                uint32_t w[2][4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    w[0][e] = pack_bf16_rne(x[2 * e], x[2 * e + 1]);
-                    w[1][e] = pack_bf16_rne(x[2 * e] - bf16_lo(w[0][e]), x[2 * e + 1] - bf16_hi(w[0][e]));
-                }
-#pragma unroll
-                for (int p = 0; p < 2; p++) pop[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-            }
+            bf16_planes<PP>(x, pop);
+            uint4 vop[ND][NP];
+            const uint4* const vt = slot + (2 * u + 1) * CH;
 #pragma unroll
             for (int t = 0; t < ND; t++) {
-                uint4 vop[NP];
-#pragma unroll
-                for (int p = 0; p < NP; p++) vop[p] = s_v[ks][u][p][TL::vpos(32 * t + n, hf)];
-#pragma unroll
-                for (int p = 0; p < NP; p++)
-#pragma unroll
-                    for (int q = 0; q < PP; q++)
-                        if (p + q <= 2) acc[t] = mfma32(vop[p], pop[q], acc[t]);
+                const int d = 32 * t + n;
+                if constexpr (I8) operand(vt, TL::vpos(d, 0), 0, vop[t]);
+                else if constexpr (F32) operand(vt, TL::vpos(d, 2 * hf), TL::vpos(d, 2 * hf + 1), vop[t]);
+                else operand(vt, TL::vpos(d, hf), 0, vop[t]);
             }
+            if (!I8 && mine.hides_some(tok[u])) {  // values that no column sees are zeros: what unused slots hold does not matter
+                uint32_t keep[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = tok[u] + 8 * hf + 2 * i;
+                    keep[i] = (mine.some_see(t) ? 0xffffu : 0u) | (mine.some_see(t + 1) ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int t = 0; t < ND; t++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+                        vop[t][p] = make_uint4(vop[t][p].x & keep[0], vop[t][p].y & keep[1], vop[t][p].z & keep[2], vop[t][p].w & keep[3]);
+            }
+#pragma unroll
+            for (int q = 0; q < PP; q++)
+#pragma unroll
+                for (int t = 0; t < ND; t++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+                        if (p + q <= 2) acc[t] = mfma32(vop[t][p], pop[q], acc[t]);
+        }
+    };
+    auto none_see = [&](int j) {
+        const int e0 = 2 * pair_of(j);
+        return mine.none_see_block(16 * span.block(e0)) && (e0 + 1 >= entries || mine.none_see_block(16 * span.block(e0 + 1)));
+    };
+
+    if constexpr (SHARE) {
+        if (count > 0) {
+            refill(0);
+            fetch_own(false, 0);
+            fetch_own(true, 0);
+            take_scales(0, 0);
+        }
+        const uint4* const slot = s_tile + wave * SLOT;
+        for (int j = 0; j < count; j++) {
+            // (the next pair's loads go out from the ids of its own stretch; past the last they read nothing)
+            const auto after_keys = [&]() {
+                if (((j + 1) & 31) == 0) refill(j + 1);
+                take_scales(AHEAD, j + 1);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this pair's keys have been read
+                fetch_own(false, j + 1);
+            };
+            const auto before_values = [&]() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * SEG) : "memory"); };
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * SEG) : "memory");  // the keys have come, the values may be under way
+            compute(slot, j, after_keys, before_values);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch_own(true, j + 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) sc[0][i] = sc[AHEAD][i];
+        }
+    } else {
+        refill(0);
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            fetch_shared(j, j);
+            take_scales(j, j);
+        }
+        int at = 0, to = AHEAD;  // slots of this pair and of the one that goes out
+        for (int j = 0; j < count; j++) {
+            // this wave's part of the pair has come, and with the barrier the others'; the slot to be filled has been read
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(SEG * (AHEAD - 1)) : "memory");
+            if (((j + AHEAD) & 31) == 0) refill(j + AHEAD);
+            fetch_shared(j + AHEAD, to);
+            take_scales(AHEAD, j + AHEAD);
+            if (live && !none_see(j)) compute(s_tile + at * SLOT, j, []() {}, []() {});
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[k][i] = sc[k + 1][i];
+            at = at == RING - 1 ? 0 : at + 1;
+            to = to == RING - 1 ? 0 : to + 1;
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no write into LDS may outlive the stream
 
     // ---- the outcome ----
-    const bool stored = live && c_wg + 32 * set + n < columns;
-    const bool sees = hi > lo || min(span.sink, hi) > 0;  // the column has a token at all
-    const int64_t slot = (static_cast<int64_t>(gi) * a.per + wk) * a.splits + split;
-    auto finish = [&](int64_t row, int c, int dim, f32x4_t o, float M, float L, bool any) {
+    const bool stored = live && c_wave + n < columns;
+    const bool sees = col.any(span.sink);
+    const int64_t slot0 = ((static_cast<int64_t>(gi) * a.per + wk) * a.splits + split) * COLS + (SHARE ? 0 : 32 * wave);
+    auto finish = [&](int dim, f32x4_t o, float M, float L) {
         if (a.splits > 1) {
-            *reinterpret_cast<f32x4_t*>(a.ws_o + (slot * COLS + c) * D + dim) = o;
-            if (dim == 0) a.ws_ml[slot * COLS + c] = make_float2(M, L);
+            *reinterpret_cast<f32x4_t*>(a.ws_o + (slot0 + n) * D + dim) = o;
+            if (dim == 0) a.ws_ml[slot0 + n] = make_float2(M, L);
         } else {
-            *reinterpret_cast<f32x4_t*>(a.out + row * D + dim) = any ? o * (1.0f / L) : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            if (a.lse && dim == 0) a.lse[row] = any ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
+            *reinterpret_cast<f32x4_t*>(a.out + col.row * D + dim) = sees ? o * (1.0f / L) : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (a.lse && dim == 0) a.lse[col.row] = sees ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
         }
     };
     // A value that is not finite at a token that some of the wave's columns see and others do not would reach
@@ -356,125 +544,82 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_prefill_kernel(co
 #pragma unroll
             for (int i = 0; i < 16; i++) odd |= !(fabsf(acc[t][i]) < INFINITY);
         bool redo = live && __any(odd);
-        if constexpr (KS > 1) {
+        if constexpr (SHARE) {
             if (lane == 0) s_bad[wave] = redo;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < KS; w++) redo |= s_bad[set * KS + w] != 0;
+            for (int w = 0; w < 4; w++) redo |= s_bad[w] != 0;
         }
         if (redo) {
+            const int e1 = min(2 * pair1, entries);
             bool hit = false;
-            for (int e = 2 * pair0; e < min(2 * pair1, span.entries()); e++) {
-                const int tok = 16 * span.block(e);
-                const int id = table[tok / 16];
+            for (int e = 2 * pair0; e < e1; e++) {
+                const int tok = 16 * span.block(e), id = table[tok / 16];
                 if (id < 0 || id >= a.num_blocks || mine.all_see_block(tok)) continue;
                 for (int i = lane; i < TILE; i += 64) {
-                    const int t = tok + (i & 15);
                     const int64_t at = (static_cast<int64_t>(id) * Hkv + kvh) * TILE + i;
                     const float v = F32 ? static_cast<const float*>(a.v_cache)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.v_cache)[at]);
-                    hit |= span.some_see(t) && !mine.all_see(t) && !(fabsf(v) < INFINITY);
+                    const int t = tok + (i & 15);
+                    hit |= mine.some_see(t) && !mine.all_see(t) && !(fabsf(v) < INFINITY);
                 }
             }
-            if (__any(hit)) {
-                constexpr int DPL = (D + 63) / 64;
-                if (KS == 1 || ks == 0) {
-                    for (int c = 0; c < 32 && c_wg + 32 * set + c < columns; c++) {
-                        const int64_t cc = c_wg + 32 * set + c;
-                        const int i = static_cast<int>(cc / G), h = kvh * G + static_cast<int>(cc - static_cast<int64_t>(i) * G);
-                        const int chi = min(T, P + i + 1), clo = a.window > 0 ? max(0, P + i + 1 - a.window) : 0;
-                        const int64_t row = (static_cast<int64_t>(q0) + i) * Hq + h;
-                        float qx[DPL], o[DPL], M = -INFINITY, L = 0.0f;
+            done = __any(hit);  // (the waves that share columns agree: it follows from the same values)
+            if (done && !(SHARE && wave > 0)) {
+                for (int c = 0; c < 32 && c_wave + c < columns; c++) {
+                    const WindowColumn one(a, c_wave + c, q0, kvh, P, T);
+                    float M, L, o[(D + 63) / 64];
+                    window_column_alone<D, KV, QF32>(a, one, span, table, kvh, 2 * pair0, e1, M, L, o);
+                    const bool any = one.any(span.sink);
 #pragma unroll
-                        for (int k = 0; k < DPL; k++) {
-                            const int64_t at = row * D + min(lane + 64 * k, D - 1);
-                            qx[k] = QF32 ? static_cast<const float*>(a.q)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.q)[at]);
-                            if (lane + 64 * k >= D) qx[k] = 0.0f;
-                            o[k] = 0.0f;
-                        }
-                        for (int e = 2 * pair0; e < min(2 * pair1, span.entries()); e++) {
-                            const int tok = 16 * span.block(e);
-                            int id = table[tok / 16];
-                            if (id >= a.num_blocks) id = -1;
-                            const int64_t tile = (static_cast<int64_t>(max(id, 0)) * Hkv + kvh) * TILE;
-                            for (int j = 0; j < 16; j++) {
-                                if (!(tok + j < chi && (tok + j >= clo || tok + j < span.sink))) continue;
-                                float x = 0.0f, v[DPL];
-#pragma unroll
-                                for (int k = 0; k < DPL; k++) {
-                                    const int d = min(lane + 64 * k, D - 1);
-                                    const int64_t ka = tile + j * D + d, va = tile + d * 16 + j;
-                                    const float kx = F32 ? static_cast<const float*>(a.k_cache)[ka] : bf16_to_f32(static_cast<const uint16_t*>(a.k_cache)[ka]);
-                                    v[k] = F32 ? static_cast<const float*>(a.v_cache)[va] : bf16_to_f32(static_cast<const uint16_t*>(a.v_cache)[va]);
-                                    if (id < 0) v[k] = 0.0f;
-                                    if (lane + 64 * k < D && id >= 0) x = __builtin_fmaf(qx[k], kx, x);
-                                }
-                                x = wave_sum(x) * c2;
-                                const float m_new = fmaxf(M, x);
-                                const float f = m_new == M ? 1.0f : __builtin_amdgcn_exp2f(M - m_new);
-                                const float p = __builtin_amdgcn_exp2f(x - (m_new == -INFINITY ? 0.0f : m_new));
-                                L = L * f + p;
-#pragma unroll
-                                for (int k = 0; k < DPL; k++) o[k] = o[k] * f + p * v[k];
-                                M = m_new;
-                            }
-                        }
-                        const bool any = chi > clo || min(span.sink, chi) > 0;
-#pragma unroll
-                        for (int k = 0; k < DPL; k++) {
-                            if (lane + 64 * k >= D) continue;
-                            if (a.splits > 1) a.ws_o[(slot * COLS + 32 * set + c) * D + lane + 64 * k] = o[k];
-                            else a.out[row * D + lane + 64 * k] = any ? o[k] * (1.0f / L) : 0.0f;
-                        }
-                        if (lane == 0) {
-                            if (a.splits > 1) a.ws_ml[slot * COLS + 32 * set + c] = make_float2(M, L);
-                            else if (a.lse) a.lse[row] = any ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
-                        }
+                    for (int k = 0; k < (D + 63) / 64; k++) {
+                        if (lane + 64 * k >= D) continue;
+                        if (a.splits > 1) a.ws_o[(slot0 + c) * D + lane + 64 * k] = o[k];
+                        else a.out[one.row * D + lane + 64 * k] = any ? o[k] * (1.0f / L) : 0.0f;
+                    }
+                    if (lane == 0) {
+                        if (a.splits > 1) a.ws_ml[slot0 + c] = make_float2(M, L);
+                        else if (a.lse) a.lse[one.row] = any ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
                     }
                 }
-                done = true;  // (the set's waves agree: it follows from the same values)
             }
         }
     }
     const float l_tot = halves_sum(l_run);
-    if constexpr (KS == 1) {
+    if constexpr (!SHARE) {
         if (!stored || done) return;
 #pragma unroll
         for (int t = 0; t < ND; t++)
 #pragma unroll
             for (int b = 0; b < 4; b++)
-                finish(qrow, 32 * set + n, 32 * t + 8 * b + 4 * hf, f32x4_t{acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]},
-                       m_run, l_tot, sees);
+                finish(32 * t + 8 * b + 4 * hf, f32x4_t{acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]}, m_run, l_tot);
     } else {
-        // every wave leaves its state; piece (t, b) of the dims is added up and stored by wave (4 t + b) % KS of the set
-        f32x4_t* const s_o = reinterpret_cast<f32x4_t*>(&s_k[0][0][0][0]);
-        static_assert(sizeof(s_k) >= 2 * 32 * D * sizeof(float), "half of the waves' states fit the keys' tiles");
-        f32x4_t* const s_o2 = reinterpret_cast<f32x4_t*>(&s_v[0][0][0][0]);
+        // every wave leaves its state; piece (t, b) of the dims is added up and stored by wave (4 t + b) % 4
         __syncthreads();
-        const auto place = [&](int w, int i) -> f32x4_t* { return (w < 2 ? s_o : s_o2) + ((w & 1) * 4 * ND + i) * 64 + lane; };
+        const auto place = [&](int w, int i) -> uint4& { return s_tile[w * STATE + i * 64 + lane]; };
         if (hf == 0) s_ml[wave][n] = make_float2(m_run, l_tot);
 #pragma unroll
         for (int t = 0; t < ND; t++)
 #pragma unroll
             for (int b = 0; b < 4; b++)
-                *place(wave, 4 * t + b) = f32x4_t{acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]};
+                place(wave, 4 * t + b) = __builtin_bit_cast(uint4, f32x4_t{acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]});
         __syncthreads();
         if (!stored || done) return;
-        float M = -INFINITY, L = 0.0f, f[KS];
+        float M = -INFINITY, L = 0.0f, f[4];
 #pragma unroll
-        for (int w = 0; w < KS; w++) M = fmaxf(M, s_ml[set * KS + w][n].x);
+        for (int w = 0; w < 4; w++) M = fmaxf(M, s_ml[w][n].x);
 #pragma unroll
-        for (int w = 0; w < KS; w++) {
-            const float2 x = s_ml[set * KS + w][n];
+        for (int w = 0; w < 4; w++) {
+            const float2 x = s_ml[w][n];
             f[w] = x.x == M ? 1.0f : __builtin_amdgcn_exp2f(x.x - M);
             L += x.y * f[w];
         }
 #pragma unroll
         for (int i = 0; i < 4 * ND; i++) {
-            if (i % KS != ks) continue;
+            if (i % 4 != wave) continue;
             f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < KS; w++) o += *place(set * KS + w, i) * f[w];
-            finish(qrow, 32 * set + n, 32 * (i / 4) + 8 * (i % 4) + 4 * hf, o, M, L, sees);
+            for (int w = 0; w < 4; w++) o += __builtin_bit_cast(f32x4_t, place(w, i)) * f[w];
+            finish(32 * (i / 4) + 8 * (i % 4) + 4 * hf, o, M, L);
         }
     }
 }
@@ -517,35 +662,37 @@ __global__ __launch_bounds__(256) void window_prefill_merge_kernel(const WindowP
     if (a.lse && lane == 0) a.lse[row] = sees ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
 }
 
-// ks: waves that share a set of columns, 1 or window_key_waves.
+// share: the waves of a workgroup share 32 columns.
 template <int D>
-void launch_window_prefill(const WindowPrefillArgs& a, int kv_dtype, bool q_f32, int ks, uint32_t nwg, hipStream_t s) {
-    const auto go = [&](auto kv, auto qf, auto k) {
-        constexpr int KV = decltype(kv)::value, KS = decltype(k)::value;
-        window_prefill_kernel<D, KV, decltype(qf)::value, KS><<<dim3(nwg, a.splits), 256, 0, s>>>(a);
-    };
-    const auto by_ks = [&](auto kv, auto qf) {
-        constexpr int KW = window_key_waves(D, decltype(kv)::value);
-        if (KW > 1 && ks > 1) go(kv, qf, std::integral_constant<int, KW>());
-        else go(kv, qf, std::integral_constant<int, 1>());
+void launch_window_prefill(const WindowPrefillArgs& a, int kv_dtype, bool q_f32, bool share, uint32_t nwg, hipStream_t s) {
+    const auto by_share = [&](auto kv, auto qf) {
+        constexpr int KV = decltype(kv)::value;
+        const dim3 grid(nwg, a.splits);
+        if constexpr (window_shares(D, KV)) {
+            if (share) {
+                window_prefill_kernel<D, KV, decltype(qf)::value, true><<<grid, 256, 0, s>>>(a);
+                return;
+            }
+        }
+        window_prefill_kernel<D, KV, decltype(qf)::value, false><<<grid, 256, 0, s>>>(a);
     };
     const auto by_q = [&](auto kv) {
-        if (q_f32) by_ks(kv, std::true_type());
-        else by_ks(kv, std::false_type());
+        if (q_f32) by_share(kv, std::true_type());
+        else by_share(kv, std::false_type());
     };
     if (kv_dtype == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>());
     else if (kv_dtype == PA_DTYPE_BF16) by_q(std::integral_constant<int, PA_DTYPE_BF16>());
     else if constexpr (D >= 64) by_q(std::integral_constant<int, PA_DTYPE_INT8>());
     if (a.splits > 1) {
         const int64_t columns = static_cast<int64_t>(a.max_chunk_len) * a.group;
-        window_prefill_merge_kernel<D><<<dim3(static_cast<uint32_t>((columns + 3) / 4), a.num_groups), 256, 0, s>>>(a, 128 / ks);
+        window_prefill_merge_kernel<D><<<dim3(static_cast<uint32_t>((columns + 3) / 4), a.num_groups), 256, 0, s>>>(a, share ? 32 : 128);
     }
 }
 #ifndef PA_WINDOW_INSTANTIATE
-extern template void launch_window_prefill<32>(const WindowPrefillArgs&, int, bool, int, uint32_t, hipStream_t);
-extern template void launch_window_prefill<64>(const WindowPrefillArgs&, int, bool, int, uint32_t, hipStream_t);
-extern template void launch_window_prefill<128>(const WindowPrefillArgs&, int, bool, int, uint32_t, hipStream_t);
-extern template void launch_window_prefill<256>(const WindowPrefillArgs&, int, bool, int, uint32_t, hipStream_t);
+extern template void launch_window_prefill<32>(const WindowPrefillArgs&, int, bool, bool, uint32_t, hipStream_t);
+extern template void launch_window_prefill<64>(const WindowPrefillArgs&, int, bool, bool, uint32_t, hipStream_t);
+extern template void launch_window_prefill<128>(const WindowPrefillArgs&, int, bool, bool, uint32_t, hipStream_t);
+extern template void launch_window_prefill<256>(const WindowPrefillArgs&, int, bool, bool, uint32_t, hipStream_t);
 #endif
 
 }  // namespace pa

@@ -9,7 +9,8 @@ namespace {
 constexpr int64_t kSplitGroups = 512;  // workgroups of a call whose keys are cut, at most
 
 struct Plan {
-    int32_t ks, cols, per, splits;
+    bool share;
+    int32_t cols, per, splits;
 };
 // Waves share a set of columns, each with its own blocks, where workgroups of 128 columns would leave CUs idle; the keys are
 // cut over workgroups where that still does.
@@ -17,13 +18,12 @@ Plan plan_of(const pa_config* cfg, int32_t num_seqs, int32_t max_chunk_len, int6
     Plan p{};
     const int64_t columns = static_cast<int64_t>(max_chunk_len) * (cfg->num_q_heads / cfg->num_kv_heads);
     const int64_t groups = static_cast<int64_t>(num_seqs) * cfg->num_kv_heads;
-    const int32_t share = pa::window_key_waves(cfg->head_dim, cfg->kv_dtype);
-    p.ks = groups * ((columns + 127) / 128) < 256 ? share : 1;
-    p.cols = 128 / p.ks;
+    p.share = pa::window_shares(cfg->head_dim, cfg->kv_dtype) && groups * ((columns + 127) / 128) < 256;
+    p.cols = p.share ? 32 : 128;
     p.per = static_cast<int32_t>((columns + p.cols - 1) / p.cols);
     const int64_t pairs = (blocks + 1) / 2, wgs = groups * p.per;
     p.splits = 1;
-    if (wgs > 0 && wgs < 256) p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(kSplitGroups / wgs, pairs / (4 * p.ks))));
+    if (wgs > 0 && wgs < 256) p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(kSplitGroups / wgs, pairs / (p.share ? 16 : 4))));
     return p;
 }
 
@@ -61,7 +61,7 @@ pa_status pa_window_prefill_workspace_size(const pa_config* cfg, int32_t num_seq
     if (st != PA_SUCCESS) return st;
     if (!bytes) return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": bytes is null");
     // what no call of at most these sizes exceeds (a smaller one may be cut where a larger one is not)
-    const int64_t cols = 128 / pa::window_key_waves(cfg->head_dim, cfg->kv_dtype);
+    const int64_t cols = pa::window_shares(cfg->head_dim, cfg->kv_dtype) ? 32 : 128;
     *bytes = num_seqs == 0 || max_chunk_len == 0 || max_context_len == 0
                  ? 0
                  : static_cast<size_t>(kSplitGroups * cols) * (cfg->head_dim + 2) * sizeof(float);
@@ -127,10 +127,10 @@ pa_status pa_window_prefill(pa_stream* stream, const pa_config* cfg, float* out,
     const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
     const uint32_t n = static_cast<uint32_t>(nwg);
     switch (cfg->head_dim) {
-        case 32: pa::launch_window_prefill<32>(a, cfg->kv_dtype, q_f32, p.ks, n, s); break;
-        case 64: pa::launch_window_prefill<64>(a, cfg->kv_dtype, q_f32, p.ks, n, s); break;
-        case 128: pa::launch_window_prefill<128>(a, cfg->kv_dtype, q_f32, p.ks, n, s); break;
-        default: pa::launch_window_prefill<256>(a, cfg->kv_dtype, q_f32, p.ks, n, s); break;
+        case 32: pa::launch_window_prefill<32>(a, cfg->kv_dtype, q_f32, p.share, n, s); break;
+        case 64: pa::launch_window_prefill<64>(a, cfg->kv_dtype, q_f32, p.share, n, s); break;
+        case 128: pa::launch_window_prefill<128>(a, cfg->kv_dtype, q_f32, p.share, n, s); break;
+        default: pa::launch_window_prefill<256>(a, cfg->kv_dtype, q_f32, p.share, n, s); break;
     }
     PA_HIP_CHECK(hipGetLastError());
     return pa::clear_error();

@@ -4,4 +4,4 @@
 
 #include "window_prefill.h"
 
-template void pa::launch_window_prefill<32>(const pa::WindowPrefillArgs&, int, bool, int, uint32_t, hipStream_t);
+template void pa::launch_window_prefill<32>(const pa::WindowPrefillArgs&, int, bool, bool, uint32_t, hipStream_t);
