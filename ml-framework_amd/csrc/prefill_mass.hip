@@ -4,8 +4,14 @@
 // window_prefill.h):   mass[s][b] += sum_i sum_h sum_t exp(scale q_ih . k_t - lse_ih)
 // with the softmax's logarithm lse that the attention of the chunk left, so that keys are read once, and values not at all.
 //
-// A wave takes two blocks of a sequence and adds up all their columns (query, head) of all KV heads by itself, 32 columns a product
-// (K . Q^T as in window_prefill.h), so the sum has one order whatever the timing.
+// A wave holds the keys of two blocks of one KV head as matrix operands and meets 32 columns (query, head) after the other
+// (K . Q^T as in window_prefill.h), which four waves with blocks of their own read from LDS: there a column's operands are formed once,
+// the next ones on their way from memory meanwhile. A workgroup has two such sets of waves, for the even and the odd KV heads; a wave
+// adds up a block's weights over its heads and columns in registers, and the two sets' sums are added at the end, so that no timing
+// enters. Keys are read once however many queries there are.
+// What bounds it: each step's operands, products and exponentials in turn behind its barrier (9 prompts of 2-8k tokens, 32 queries,
+// bf16: 44 us, of which 12 go with the operands' exchange, 11 with the keys' loads, 14 with the exponentials). Waves that hold 128 columns in
+// registers instead and load them for themselves, 16 bytes of a row a lane, 65 us; two waves to a set 44 us, and twice the time for fp32 queries.
 #include <algorithm>
 #include <string>
 
@@ -26,12 +32,57 @@ struct MassArgs {
     float scale;
 };
 
+// Eight keys' values as they stand in the cache.
+template <int KV> struct RawKeys { uint4 x; };
+template <> struct RawKeys<PA_DTYPE_FP32> { pa::f32x4_t x, y; };
+template <> struct RawKeys<PA_DTYPE_INT8> { uint2 x; };
+
+template <int KV>
+__device__ __forceinline__ void load_raw(RawKeys<KV>& r, const char* at) {
+    if constexpr (KV == PA_DTYPE_FP32) {
+        r.x = reinterpret_cast<const pa::f32x4_t*>(at)[0];
+        r.y = reinterpret_cast<const pa::f32x4_t*>(at)[1];
+    } else if constexpr (KV == PA_DTYPE_BF16) {
+        r.x = *reinterpret_cast<const uint4*>(at);
+    } else {
+        r.x = *reinterpret_cast<const uint2*>(at);
+    }
+}
+template <int KV, int NP>
+__device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[NP]) {
+    if constexpr (KV == PA_DTYPE_FP32) {
+        const float v[8] = {r.x[0], r.x[1], r.x[2], r.x[3], r.y[0], r.y[1], r.y[2], r.y[3]};
+        pa::bf16_planes<NP>(v, plane);
+    } else if constexpr (KV == PA_DTYPE_BF16) {
+        plane[0] = r.x;
+    } else {
+        const uint32_t x = r.x.x ^ 0x80808080u, y = r.x.y ^ 0x80808080u;
+        plane[0] = make_uint4(pa::i8_pair(x, 0), pa::i8_pair(x, 2), pa::i8_pair(y, 0), pa::i8_pair(y, 2));
+    }
+}
+
+constexpr int kSetWaves = 4;                       // waves that share the columns' operands
+constexpr int kMassThreads = 2 * 64 * kSetWaves;   // two sets
+
+// Whether two workgroups fit a CU: 128 registers a lane.
+__host__ __device__ constexpr bool mass_two(int d, int kv, bool q_f32) { return !q_f32 && kv != PA_DTYPE_FP32 && d <= 128; }
+
 template <int D, int KV, bool QF32>
-__global__ __launch_bounds__(256) void prefill_mass_kernel(const MassArgs a) {
+__global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void prefill_mass_kernel(const MassArgs a) {
     constexpr bool I8 = KV == PA_DTYPE_INT8;
     constexpr int NP = KV == PA_DTYPE_FP32 ? 3 : 1, NQ = QF32 ? 3 : 1, NS = D / 16;
+    constexpr int ELT = KV == PA_DTYPE_FP32 ? 4 : I8 ? 1 : 2, QKV = QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16;
+    constexpr int SET = NS * 64;                                     // 16-byte pieces of 32 columns' operands, of one part
+    constexpr int NB = 4 * NQ * SET * 16 <= (mass_two(D, KV, QF32) ? 64 : 128) * 1024 ? 2 : 1;      // buffers of a set
+    constexpr bool EARLY = !mass_two(D, KV, QF32) && (NP == 1 || D < 256);                       // the next head's keys loaded early: registers for it
+    constexpr int PER = (SET + 64 * kSetWaves - 1) / (64 * kSetWaves);  // pieces a thread brings
+    __shared__ uint4 s_q[2][NB][NQ][SET];
+    __shared__ float s_lse[2][NB][32];
+    __shared__ int s_at[2][NB][32];  // the columns' positions
+    __shared__ float s_sum[2][kSetWaves][2];
     const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int set = wave / kSetWaves, tid = threadIdx.x % (64 * kSetWaves);
     const int seq = blockIdx.y, Hkv = a.num_kv_heads, G = a.group, Hq = Hkv * G;
     const int q0 = a.q_start_loc[seq], Lc = a.q_start_loc[seq + 1] - q0;
     const int m = min(a.last, Lc);
@@ -40,86 +91,169 @@ __global__ __launch_bounds__(256) void prefill_mass_kernel(const MassArgs a) {
     const int T = static_cast<int>(min(min(static_cast<int64_t>(P) + Lc, static_cast<int64_t>(a.max_blocks_per_seq) * 16),
                                        static_cast<int64_t>(a.max_context_len)));
     const pa::WindowSpan span(P, Lc - m, Lc - 1, T, a.sink, a.window);
-    const int e0 = 2 * (static_cast<int>(blockIdx.x) * 4 + wave);
-    if (e0 >= span.entries()) return;
+    const int entries = span.entries();
+    if (2 * kSetWaves * static_cast<int>(blockIdx.x) >= entries) return;
     const int32_t* table = a.block_tables + static_cast<int64_t>(seq) * a.max_blocks_per_seq;
-    const int lb[2] = {span.block(e0), e0 + 1 < span.entries() ? span.block(e0 + 1) : -1};
-    int id[2];
+
+    // this wave's blocks, the same ones in both sets; a wave past the last has none, but brings operands
+    const int e0 = 2 * (kSetWaves * static_cast<int>(blockIdx.x) + wave % kSetWaves);
+    int lb[2], id[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
+        lb[u] = e0 + u < entries ? span.block(e0 + u) : -1;
         id[u] = lb[u] >= 0 ? table[lb[u]] : -1;
         if (id[u] >= a.num_blocks) id[u] = -1;
     }
-    const int tok[2] = {16 * lb[0], lb[1] >= 0 ? 16 * lb[1] : INT32_MAX - 64};
-    const bool all = span.all_see_block(tok[0]) && span.all_see_block(tok[1]);
-    const int64_t columns = static_cast<int64_t>(m) * G;
-    const int mine = n >> 4;  // the block of the lane's row of K
-    const int krow = pa::key_of_row(n);
-    float sum[2] = {0.0f, 0.0f};
-    for (int kvh = 0; kvh < Hkv; kvh++) {
-        uint4 kop[NP][NS];
-        const int64_t tile = (static_cast<int64_t>(max(mine ? id[1] : id[0], 0)) * Hkv + kvh) * 16 * D;
-        const bool real = (mine ? id[1] : id[0]) >= 0;
+    const bool live = lb[0] >= 0;
+    const int tok[2] = {live ? 16 * lb[0] : INT32_MAX - 64, lb[1] >= 0 ? 16 * lb[1] : INT32_MAX - 64};
+    const int krow = pa::key_of_row(n);                                      // the lane's row of K: key krow of
+    const int my_id = __builtin_amdgcn_readfirstlane(id[0]) >= 0 && (n < 16 || id[1] < 0) ? id[0] : id[1];  // its block, or the other where there is none
+    const bool there[2] = {id[0] >= 0, id[1] >= 0};                          // (else the scores are set to 0)
+    const bool plain = there[0] && there[1] && span.all_see_block(tok[0]) && span.all_see_block(tok[1]);
+
+    const int columns = m * G, chunks = (columns + 31) / 32;
+    const int heads = (Hkv - set + 1) / 2, steps = heads * chunks;           // of this set
+    const int most = (Hkv + 1) / 2 * chunks;                                 // of either: the barriers are the workgroup's
+    RawKeys<KV> raw[NS] = {};
+    auto load_keys = [&](int kvh) {
+        if (my_id < 0) return;
+        const char* const at = static_cast<const char*>(a.k_cache) +
+                               ((static_cast<int64_t>(my_id) * Hkv + kvh) * 16 * D + krow * D + 8 * hf) * ELT;
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
-            uint4 x[NP];
+        for (int sl = 0; sl < NS; sl++) load_raw<KV>(raw[sl], at + 16 * sl * ELT);
+    };
+    // Columns 32 chunk .. of KV head kvh: D / 8 threads bring a column, 16 (32) bytes of bf16 (fp32) each, so that a wave reads whole lines.
+    // A lane reads piece 2 slab + half of column n: the pieces of a column lie at column ^ piece, so that the 16 threads that write them
+    // at once meet 16 different 16-byte positions of a 256-byte line.
+    constexpr int PC = D / 8, STEP = 64 * kSetWaves / PC;  // pieces of a column, columns at a time
+    struct Bring {
+        RawKeys<QKV> x[PER];
+        float lse;
+        int at;
+    };
+    const int piece = tid % PC;
+    int load_kvh = set, load_chunk = 0;  // of the columns that are loaded next
+    auto load_columns = [&](Bring& to) {
+        const int kvh = load_kvh, chunk = load_chunk;
+        if (kvh >= Hkv) return;
+        load_chunk = chunk == chunks - 1 ? 0 : chunk + 1;
+        load_kvh = load_chunk == 0 ? kvh + 2 : kvh;
+        const auto row_of = [&](int col, int& i) {
+            const uint32_t c = min(32 * chunk + col, columns - 1);
+            i = static_cast<int>(c / static_cast<uint32_t>(G));
+            return (static_cast<int64_t>(q0) + Lc - m + i) * Hq + kvh * G + (static_cast<int>(c) - i * G);
+        };
+        int i;
 #pragma unroll
-            for (int p = 0; p < NP; p++) x[p] = make_uint4(0, 0, 0, 0);
-            if (real) pa::load_planes<KV, NP>(a.k_cache, tile + krow * D + 16 * s + 8 * hf, x);
-#pragma unroll
-            for (int p = 0; p < NP; p++) kop[p][s] = x[p];
+        for (int j = 0; j < PER; j++) {
+            if (STEP > 32 && tid >= 32 * PC) break;
+            load_raw<QKV>(to.x[j], static_cast<const char*>(a.q) + (row_of(tid / PC + STEP * j, i) * D + 8 * piece) * (QF32 ? 4 : 2));
         }
-        float ks[2] = {1.0f, 1.0f};
-        if constexpr (I8)
+        if (tid < 32) {
+            to.lse = 32 * chunk + tid < columns ? a.lse[row_of(tid, i)] * 1.4426950408889634f : INFINITY;  // no such column: no weight
+            to.at = P + Lc - m + static_cast<int>(min(32 * chunk + tid, columns - 1) / G);
+        }
+    };
+    auto store_columns = [&](const Bring& from, int b) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) ks[u] = id[u] >= 0 ? a.k_scale[static_cast<int64_t>(id[u]) * Hkv + kvh] : 0.0f;
-        for (int64_t c0 = 0; c0 < columns; c0 += 32) {
-            const int64_t c = min(c0 + n, columns - 1);
-            const int i = static_cast<int>(c / G);
-            const int qi = Lc - m + i;
-            const int64_t row = (static_cast<int64_t>(q0) + qi) * Hq + kvh * G + (c - static_cast<int64_t>(i) * G);
-            const float lse = a.lse[row] * 1.4426950408889634f;
-            pa::f32x16_t s;
+        for (int j = 0; j < PER; j++) {
+            if (STEP > 32 && tid >= 32 * PC) break;
+            uint4 op[NQ];
+            raw_planes<QKV, NQ>(from.x[j], op);
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = 0.0f;
+            for (int q = 0; q < NQ; q++) s_q[set][b][q][32 * piece + ((tid / PC + STEP * j) ^ (piece & 15))] = op[q];
+        }
+        if (tid < 32) {
+            s_lse[set][b][tid] = from.lse;
+            s_at[set][b][tid] = from.at;
+        }
+    };
+    const float c2 = a.scale * 1.4426950408889634f;
+    float sum[2] = {0.0f, 0.0f}, f[2] = {c2, c2};
+    uint4 kop[NP][NS];
+    Bring bring;  // the next step's columns, on their way while one is computed
+    if (steps > 0) {
+        if (EARLY) load_keys(set);
+        load_columns(bring);
+        store_columns(bring, 0);
+    }
+    int kvh = set, chunk = 0;  // of step k
+    for (int k = 0; k < most; k++) {
+        const int b = NB == 2 ? k & 1 : 0;
+        __syncthreads();  // step k's operands stand in LDS
+        load_columns(bring);
+        if (k < steps && live) {
+            if (chunk == 0) {
+                if (!EARLY) load_keys(kvh);
 #pragma unroll
-            for (int sl = 0; sl < NS; sl++) {
-                uint4 qx[NQ];
-                pa::load_planes<QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16, NQ>(a.q, row * D + 16 * sl + 8 * hf, qx);
+                for (int sl = 0; sl < NS; sl++) {
+                    uint4 x[NP];
+                    raw_planes<KV, NP>(raw[sl], x);
 #pragma unroll
-                for (int p = 0; p < NP; p++)
-#pragma unroll
-                    for (int q = 0; q < NQ; q++)
-                        if (p + q <= 2) s = pa::mfma32(kop[p][sl], qx[q], s);
-            }
-            const int hi = min(T, P + qi + 1), lo = a.window > 0 ? max(0, P + qi + 1 - a.window) : 0;
-            const bool counts = c0 + n < columns;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const float f = a.scale * 1.4426950408889634f * ks[u];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int t = tok[u] + 8 * hf + j;
-                    const float w = __builtin_amdgcn_exp2f(s[8 * u + j] * f - lse);
-                    const bool seen = counts && (all || (t < hi && (t >= lo || t < span.sink)));
-                    sum[u] += seen ? w : 0.0f;
+                    for (int p = 0; p < NP; p++) kop[p][sl] = x[p];
                 }
+                if constexpr (I8)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) f[u] = there[u] ? c2 * a.k_scale[static_cast<int64_t>(id[u]) * Hkv + kvh] : c2;
+                if (EARLY && kvh + 2 < Hkv) load_keys(kvh + 2);
+            }
+            pa::f32x16_t product;
+#pragma unroll
+            for (int e = 0; e < 16; e++) product[e] = 0.0f;
+#pragma unroll
+            for (int sl = 0; sl < NS; sl++)
+#pragma unroll
+                for (int q = 0; q < NQ; q++) {
+                    const uint4 qop = s_q[set][b][q][32 * (2 * sl + hf) + (n ^ ((2 * sl + hf) & 15))];
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+                        if (p + q <= 2) product = pa::mfma32(kop[p][sl], qop, product);
+                }
+            const float lse = s_lse[set][b][n];
+            const int at = s_at[set][b][n];
+            // (single values from here on: hipcc has mixed up the elements of a product that was changed in place under a branch)
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = e == 15 ? pa::settled(product[e]) : product[e];
+            if (plain) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) sum[u] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + j], f[u], -lse));
+            } else {
+                const int hi = min(T, at + 1), lo = a.window > 0 ? max(0, at + 1 - a.window) : 0;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int t = tok[u] + 8 * hf + j;
+                        const float y = __builtin_fmaf(there[u] ? x[8 * u + j] : 0.0f, f[u], -lse);
+                        // (an unseen token's weight is 0 whatever its score, the block's scale and the logarithm are)
+                        sum[u] += t < hi && (t >= lo || t < span.sink) ? __builtin_amdgcn_exp2f(y) : 0.0f;
+                    }
             }
         }
+        if (NB == 1) __syncthreads();
+        if (k + 1 < steps) store_columns(bring, NB == 2 ? b ^ 1 : 0);
+        chunk = chunk == chunks - 1 ? 0 : chunk + 1;
+        kvh = chunk == 0 ? kvh + 2 : kvh;
     }
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const float w = pa::wave_sum(sum[u]);
-        if (lane == 0 && lb[u] >= 0) a.mass[static_cast<int64_t>(seq) * a.max_blocks_per_seq + lb[u]] += w;
+        if (lane == 0) s_sum[set][wave % kSetWaves][u] = w;
     }
+    __syncthreads();
+    if (set == 0 && lane < 2 && (lane ? lb[1] : lb[0]) >= 0)
+        a.mass[static_cast<int64_t>(seq) * a.max_blocks_per_seq + (lane ? lb[1] : lb[0])] += s_sum[0][wave][lane] + s_sum[1][wave][lane];
 }
 
 template <int D>
 void launch(const MassArgs& a, int kv, bool q_f32, dim3 grid, hipStream_t s) {
     const auto by_q = [&](auto k) {
         constexpr int KV = decltype(k)::value;
-        if (q_f32) prefill_mass_kernel<D, KV, true><<<grid, 256, 0, s>>>(a);
-        else prefill_mass_kernel<D, KV, false><<<grid, 256, 0, s>>>(a);
+        if (q_f32) prefill_mass_kernel<D, KV, true><<<grid, kMassThreads, 0, s>>>(a);
+        else prefill_mass_kernel<D, KV, false><<<grid, kMassThreads, 0, s>>>(a);
     };
     if (kv == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>());
     else if (kv == PA_DTYPE_BF16) by_q(std::integral_constant<int, PA_DTYPE_BF16>());
@@ -143,6 +277,8 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     if (max_blocks_per_seq > INT32_MAX / pa::kBlockSize)
         return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": max_blocks_per_seq * 16 must fit 32 bits");
     if (num_seqs > 65535) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": num_seqs must be <= 65535");
+    if (static_cast<int64_t>(last_queries) * cfg->num_q_heads > INT32_MAX / 2)
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": last_queries * num_q_heads must fit 30 bits");
     if (num_seqs == 0 || last_queries == 0 || max_context_len == 0 || max_blocks_per_seq == 0) return pa::clear_error();
     if (!q || !lse || !q_start_loc || !prefix_lens || !k_cache || !block_tables || !block_mass)
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
@@ -159,7 +295,7 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
                      cfg->num_blocks, max_context_len, last_queries, sink_tokens, window, pa::resolve_scale(cfg)};
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
-    const dim3 grid(static_cast<uint32_t>((blocks + 7) / 8), num_seqs);
+    const dim3 grid(static_cast<uint32_t>((blocks + 2 * kSetWaves - 1) / (2 * kSetWaves)), num_seqs);
     const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
     switch (cfg->head_dim) {
         case 32: launch<32>(a, cfg->kv_dtype, q_f32, grid, s); break;

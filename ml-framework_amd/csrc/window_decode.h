@@ -42,9 +42,16 @@ __device__ __forceinline__ WindowList window_list(int T, int sink, int window) {
     return {min((min(sink, T) + 15) / 16, low), low, (T + 15) / 16};
 }
 
-// The sequences' lists laid end to end: starts[r] in s_starts, and the most that one has. One workgroup, W waves.
+// Waves of a workgroup, workgroups of a full chip.
+__host__ __device__ constexpr int window_waves(int) { return 4; }
+__host__ __device__ constexpr int window_decode_groups(int head_dim, int kv) {
+    return sparse_groups(head_dim, kv) * sparse_waves(head_dim) / window_waves(head_dim);
+}
+
+// The sequences' lists laid end to end: starts[r] in s_starts, their lengths in s_lens, and the most that one list has. One
+// workgroup, W waves.
 template <int W>
-__device__ __forceinline__ int window_starts(const WindowArgs& a, int32_t* s_starts) {
+__device__ __forceinline__ int window_starts(const WindowArgs& a, int32_t* s_starts, int32_t* s_lens) {
     constexpr int PER = (kWindowSeqs + 64 * W) / (64 * W);
     __shared__ int s_sum[W], s_most[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -56,7 +63,9 @@ __device__ __forceinline__ int window_starts(const WindowArgs& a, int32_t* s_sta
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        raw[i] = window_list(max(0, clamp_len(a.d, raw[i])), a.sink, a.window).entries();
+        const int len = max(0, clamp_len(a.d, raw[i]));
+        s_lens[threadIdx.x * PER + i] = len;
+        raw[i] = window_list(len, a.sink, a.window).entries();
         sum += raw[i];
         most = max(most, raw[i]);
     }
@@ -84,32 +93,32 @@ __device__ __forceinline__ int window_starts(const WindowArgs& a, int32_t* s_sta
 
 // PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
 template <int D, int KV, bool QF32, int PASSES>
-__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSparseCUs * sparse_waves(D) / 4) void window_decode_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) / kSparseCUs * window_waves(D) / 4) void window_decode_kernel(const WindowArgs a) {
     constexpr bool F32 = KV == PA_DTYPE_FP32;
     constexpr int NSLAB = D / 32, NT = D / 16;
     constexpr bool I8 = KV == PA_DTYPE_INT8;
     constexpr int NI8 = I8 ? D / 64 : 1;           // QK slabs of 64 dims
     constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
     constexpr int PP = F32 ? 1 : PASSES;           // passes of P
-    constexpr int W = sparse_waves(D);
+    constexpr int W = window_waves(D);
     constexpr int NB = kSparseBuffers;
     constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
     __shared__ float s_m[W][16], s_l[W][16];
     __shared__ float s_o[W][16][CH];
-    __shared__ int32_t s_starts[kWindowSeqs + 1];
+    __shared__ int32_t s_starts[kWindowSeqs + 1], s_lens[kWindowSeqs + 64 * W];
     const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.d.num_kv_heads, G = a.d.group;
-    const int most = window_starts<W>(a, s_starts);
+    const int most = window_starts<W>(a, s_starts, s_lens);
     const uint32_t all = static_cast<uint32_t>(s_starts[a.num_seqs]) * Hkv;
-    // Entries a workgroup: equal ranges; whole rows where all are of one length and that gives no workgroup more than
-    // kWindowWaste entries, or a third, over an equal range.
+    // Entries a workgroup: equal ranges; whole rows where all are of one length and that gives no CU more than 32 entries, or a
+    // third, over an equal share: a cut row costs another start, another exchange of states and the merge.
     uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(a.least));
     range = (range + W - 1) / W * W;
     const uint32_t rows = static_cast<uint32_t>(a.num_seqs) * Hkv;
     if (most > 0 && static_cast<uint32_t>(most) * rows == all) {
-        const uint32_t whole = (rows + a.groups - 1) / a.groups * most;
-        if (whole <= range + 32 || (range > most * 3u / 4 && range <= static_cast<uint32_t>(most))) range = whole;
+        const uint32_t even = (all + kSparseCUs - 1) / kSparseCUs, whole = (rows + kSparseCUs - 1) / kSparseCUs * most;  // a CU's
+        if (whole <= even + 32 || 3 * whole < 4 * even) range = (rows + a.groups - 1) / a.groups * most;
     }
     if (blockIdx.x == 0) {
         for (int r = threadIdx.x; r <= a.num_seqs; r += 64 * W) a.starts[r] = s_starts[r];
@@ -138,7 +147,7 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
     const uint32_t entry0 = base + static_cast<uint32_t>(kvh) * held;  // of the row
     at_entry += end - beg;
     const int row = r * Hkv + kvh;
-    const int T = clamp_len(a.d, a.d.context_lens[r]);
+    const int T = s_lens[r];
     const int lo = window_begin(T, a.window), sink = min(a.sink, T);
     const WindowList list = window_list(T, a.sink, a.window);
     const int32_t* table = a.d.block_tables + static_cast<int64_t>(r) * a.d.max_blocks_per_seq;
@@ -528,7 +537,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowArgs a) {
 template <int D>
 void launch_window_decode(const WindowArgs& a, int kv_dtype, bool q_f32, bool merge, hipStream_t s) {
     const int G = a.d.group;
-    const auto go = [&](auto kernel) { kernel<<<a.groups, 64 * sparse_waves(D), 0, s>>>(a); };
+    const auto go = [&](auto kernel) { kernel<<<a.groups, 64 * window_waves(D), 0, s>>>(a); };
     const auto by_q = [&](auto kv, auto passes) {
         constexpr int KV = decltype(kv)::value, P = decltype(passes)::value;
         if (q_f32) go(window_decode_kernel<D, KV, true, P>);

@@ -56,12 +56,12 @@ struct Plan {
 
 // List entries of a range at least: two a wave, or one where that cuts no row into more than eight parts.
 Plan plan_of(const pa_config* cfg, int32_t num_seqs, int64_t blocks) {
-    const int32_t waves = pa::sparse_waves(cfg->head_dim), G = cfg->num_q_heads / cfg->num_kv_heads;
+    const int32_t waves = pa::window_waves(cfg->head_dim), G = cfg->num_q_heads / cfg->num_kv_heads;
     Plan p{};
     p.seqs = std::min(num_seqs, pa::kWindowSeqs);
     p.entries = static_cast<int64_t>(p.seqs) * cfg->num_kv_heads * blocks;
     p.least = blocks <= 8 * waves ? waves : 2 * waves;
-    const int64_t full = pa::sparse_groups(cfg->head_dim, cfg->kv_dtype);
+    const int64_t full = pa::window_decode_groups(cfg->head_dim, cfg->kv_dtype);
     p.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min(full, (p.entries + p.least - 1) / p.least)));
     p.merge = p.groups > 1;
     // (of the smallest range, so that a workspace of the largest call serves every smaller one)

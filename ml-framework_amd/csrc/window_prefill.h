@@ -368,9 +368,9 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
     auto compute = [&](const uint4* slot, int j, auto after_keys, auto before_values) {
         const int e0 = 2 * pair_of(j);
         const int tok[2] = {16 * span.block(e0), e0 + 1 < entries ? 16 * span.block(e0 + 1) : INT32_MAX - 64};  // no such block: past every end
-        f32x16_t s;
+        f32x16_t product;
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+        for (int i = 0; i < 16; i++) product[i] = 0.0f;
         const uint4* const kt = slot + (n >> 4) * 2 * CH;
 #pragma unroll
         for (int sl = 0; sl < NS; sl++) {
@@ -382,9 +382,12 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
             for (int p = 0; p < NP; p++)
 #pragma unroll
                 for (int q = 0; q < NQ; q++)
-                    if (p + q <= 2) s = mfma32(kop[p], qv[q][sl], s);
+                    if (p + q <= 2) product = mfma32(kop[p], qv[q][sl], product);
         }
-        s[15] = settled(s[15]);
+        // (single values from here on: hipcc has mixed up the elements of a product that was changed in place under a branch)
+        float s[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = i == 15 ? settled(product[i]) : product[i];
         after_keys();
         // lane: tokens tok[u] + 8 hf + i of its column in s[8 u + i]
         float f[2] = {c2, c2};
@@ -414,9 +417,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
             l_run *= alpha;
             m_run = m_new;
 #pragma unroll
-            for (int t = 0; t < ND; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) acc[t][i] *= alpha;
+            for (int t = 0; t < ND; t++) acc[t] *= alpha;
         }
         const float m0 = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll

@@ -18,7 +18,7 @@ Plan plan_of(const pa_config* cfg, int32_t num_seqs, int32_t max_chunk_len, int6
     Plan p{};
     const int64_t columns = static_cast<int64_t>(max_chunk_len) * (cfg->num_q_heads / cfg->num_kv_heads);
     const int64_t groups = static_cast<int64_t>(num_seqs) * cfg->num_kv_heads;
-    p.share = pa::window_shares(cfg->head_dim, cfg->kv_dtype) && groups * ((columns + 127) / 128) < 256;
+    p.share = pa::window_shares(cfg->head_dim, cfg->kv_dtype) && (columns <= 64 || groups * ((columns + 127) / 128) < 256);
     p.cols = p.share ? 32 : 128;
     p.per = static_cast<int32_t>((columns + p.cols - 1) / p.cols);
     const int64_t pairs = (blocks + 1) / 2, wgs = groups * p.per;
