@@ -5,8 +5,9 @@
 // the reference counts of the others fall by one. No key or value moves.
 //
 // One workgroup a row. The border between what stays and what goes is the k-th largest mass, found digit by digit
-// (8 bits a pass, from the top) over the masses as ordered 32-bit integers; blocks at the border itself are dealt out by index.
-// Traffic is 16 bytes a block; a row's chain of passes and barriers is what it costs.
+// (11 bits a pass, from the top) over the masses as ordered 32-bit integers; blocks at the border itself are dealt out by index.
+// Traffic is 16 bytes a block; a row's chain of loads, passes and barriers is what it costs, so rows of up to 16384 blocks
+// are read once into registers, a thread every 1024th block, and what stays is numbered by the waves' ballots of all of them at once.
 #include <algorithm>
 #include <string>
 
@@ -41,6 +42,137 @@ __device__ __forceinline__ int place(bool flag, int* s_count, int& base) {
     return at;
 }
 
+// Rows of at most 1024 K blocks.
+template <int K>
+__global__ __launch_bounds__(kThreads) void evict_short_kernel(int32_t* __restrict__ tables, int32_t* __restrict__ lens,
+                                                               float* __restrict__ mass, int32_t width, int32_t sink,
+                                                               int32_t recent, int32_t budget, int32_t num_blocks,
+                                                               int32_t* __restrict__ refcounts, int32_t* __restrict__ evicted) {
+    __shared__ int s_hist[2048], s_count[K * kWaves], s_sum[kWaves];
+    __shared__ int s_digit, s_rest;
+    const int r = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int len = lens[r];
+    const int n = static_cast<int>(min((static_cast<int64_t>(len) + 15) / 16, static_cast<int64_t>(width)));
+    if (len <= 0 || n <= budget) {
+        if (evicted && threadIdx.x == 0) evicted[r] = 0;
+        return;
+    }
+    int32_t* const row = tables + static_cast<int64_t>(r) * width;
+    float* const weight = mass ? mass + static_cast<int64_t>(r) * width : nullptr;
+    const int lo = sink, hi = n - recent;  // what may go
+    int rest = budget - sink - recent;     // of these, how many stay
+    int id[K];
+    float w[K];
+    bool may[K];
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        const int b = i * kThreads + static_cast<int>(threadIdx.x);
+        may[i] = b >= lo && b < hi;
+        id[i] = b < width ? row[b] : -1;
+        w[i] = weight && b < width ? weight[b] : 0.0f;
+    }
+    // Numbers the set flags in the order of the blocks: at[i] for block i * kThreads + thread. (Its barriers also stand between the reads
+    // above and the writes below.)
+    const auto number = [&](const bool (&flag)[K], int (&at)[K]) {
+        uint64_t votes[K];
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            votes[i] = __ballot(flag[i]);
+            if (lane == 0) s_count[i * kWaves + wave] = __popcll(votes[i]);
+        }
+        __syncthreads();
+        if (wave == 0) {  // lane l: K / 4 of the counts in turn
+            constexpr int PER = (K * kWaves + 63) / 64;
+            int c[PER], sum = 0;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                c[j] = PER * lane + j < K * kWaves ? s_count[PER * lane + j] : 0;
+                sum += c[j];
+            }
+            int before = pa::wave_prefix(sum) - sum;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                if (PER * lane + j < K * kWaves) s_count[PER * lane + j] = before;
+                before += c[j];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < K; i++) at[i] = s_count[i * kWaves + wave] + __popcll(votes[i] & ((1ull << lane) - 1));
+        __syncthreads();  // s_count is free again
+    };
+    bool stays[K];
+    int to[K];
+    if (weight && rest > 0) {
+        uint32_t border = 0;  // above it stays, at it the first `rest` do
+#pragma unroll
+        for (int pass = 0; pass < 3; pass++) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+            for (int i = threadIdx.x; i < 2048; i += kThreads) s_hist[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                const uint32_t k = ordered(w[i]);
+                if (may[i] && (pass == 0 || (k ^ border) >> (shift + bits) == 0)) atomicAdd(&s_hist[k >> shift & ((1u << bits) - 1)], 1);
+            }
+            __syncthreads();
+            // thread t: digits 2 t, 2 t + 1; what lies above each
+            const int c0 = s_hist[2 * threadIdx.x], c1 = s_hist[2 * threadIdx.x + 1];
+            const int upto = pa::wave_prefix(c0 + c1);
+            if (lane == 63) s_sum[wave] = upto;
+            __syncthreads();
+            int above = -upto;
+#pragma unroll
+            for (int v = 0; v < kWaves; v++) above += v >= wave ? s_sum[v] : 0;
+            if (above < rest && above + c1 >= rest) {
+                s_digit = 2 * threadIdx.x + 1;
+                s_rest = rest - above;
+            }
+            above += c1;
+            if (above < rest && above + c0 >= rest) {
+                s_digit = 2 * threadIdx.x;
+                s_rest = rest - above;
+            }
+            __syncthreads();
+            border |= static_cast<uint32_t>(s_digit) << shift;
+            rest = s_rest;
+        }
+        bool tie[K];
+#pragma unroll
+        for (int i = 0; i < K; i++) tie[i] = may[i] && ordered(w[i]) == border;
+        number(tie, to);
+#pragma unroll
+        for (int i = 0; i < K; i++) stays[i] = !may[i] || ordered(w[i]) > border || (tie[i] && to[i] < rest);
+    } else {
+#pragma unroll
+        for (int i = 0; i < K; i++) stays[i] = !may[i] || i * kThreads + static_cast<int>(threadIdx.x) >= hi - (weight ? 0 : rest);
+    }
+#pragma unroll
+    for (int i = 0; i < K; i++) stays[i] &= i * kThreads + static_cast<int>(threadIdx.x) < width;
+    number(stays, to);
+    const int gone = n - budget;
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        const int b = i * kThreads + static_cast<int>(threadIdx.x);
+        if (stays[i]) {
+            row[to[i]] = id[i];
+            if (weight) weight[to[i]] = w[i];
+        } else if (b < width && id[i] >= 0 && id[i] < num_blocks) {
+            atomicSub(&refcounts[id[i]], 1);
+        }
+        if (b < width && b >= width - gone) {  // behind the last that stays
+            row[b] = -1;
+            if (weight) weight[b] = 0.0f;
+        }
+    }
+    if (threadIdx.x == 0) {
+        lens[r] = len - 16 * gone;
+        if (evicted) evicted[r] = gone;
+    }
+}
+
+// Rows of any width, in chunks of 1024 blocks.
 __global__ __launch_bounds__(kThreads) void evict_kernel(int32_t* __restrict__ tables, int32_t* __restrict__ lens,
                                                          float* __restrict__ mass, int32_t width, int32_t sink,
                                                          int32_t recent, int32_t budget, int32_t num_blocks,
@@ -146,8 +278,14 @@ extern "C" pa_status pa_evict_blocks(pa_stream* stream, const pa_config* cfg, in
         return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": max_blocks_per_seq * 16 must fit 32 bits");
     if (!pa::fits_grid(num_rows, kThreads)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many rows for one call");
     pa::StreamDevice dev(stream);
-    evict_kernel<<<num_rows, kThreads, 0, pa::native(stream)>>>(block_tables, lens, block_mass, max_blocks_per_seq, sink_blocks,
-                                                               recent_blocks, budget, cfg->num_blocks, refcounts, evicted);
+    const auto go = [&](auto kernel) {
+        kernel<<<num_rows, kThreads, 0, pa::native(stream)>>>(block_tables, lens, block_mass, max_blocks_per_seq, sink_blocks,
+                                                              recent_blocks, budget, cfg->num_blocks, refcounts, evicted);
+    };
+    if (max_blocks_per_seq <= kThreads) go(evict_short_kernel<1>);
+    else if (max_blocks_per_seq <= 4 * kThreads) go(evict_short_kernel<4>);
+    else if (max_blocks_per_seq <= 16 * kThreads) go(evict_short_kernel<16>);
+    else go(evict_kernel);
     PA_HIP_CHECK(hipGetLastError());
     return pa::clear_error();
 }

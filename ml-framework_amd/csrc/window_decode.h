@@ -23,11 +23,13 @@ struct WindowArgs {
     DecodeArgs d;          // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [2 * workgroups][G]
     int32_t* starts;       // [num_seqs + 1] blocks (of one KV head) before each sequence, then the range
     float2* parts;         // masses: (maximum, sum) of every list entry's tokens, [Hkv * starts + ..][G]; else null
-    float2* total;         // masses: (maximum, sum) of every row, [num_seqs][Hq]
+    float2* total;         // masses: (maximum, sum) of every row that was not cut, [num_seqs][Hq]
     float* mass;           // [num_seqs][max_blocks_per_seq]
     int32_t num_seqs, sink, window;
     int32_t least;         // list entries of a range at least
     int32_t groups;        // workgroups
+    int32_t merge_groups;  // of the launch behind: workgroups that join cut rows, and (masses) per sequence
+    int32_t mass_chunks;
 };
 
 // The list of a context of T tokens: blocks [0, first), then [low, end).
@@ -109,8 +111,8 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.d.num_kv_heads, G = a.d.group;
-    const int most = window_starts<W>(a, s_starts, s_lens);
-    const uint32_t all = static_cast<uint32_t>(s_starts[a.num_seqs]) * Hkv;
+    const int most = __builtin_amdgcn_readfirstlane(window_starts<W>(a, s_starts, s_lens));
+    const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(s_starts[a.num_seqs])) * Hkv;
     // Entries a workgroup: equal ranges; whole rows where all are of one length and that gives no CU more than 32 entries, or a
     // third, over an equal share: a cut row costs another start, another exchange of states and the merge.
     uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(a.least));
@@ -132,22 +134,24 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     const uint32_t stop = min(all, at_entry + range);
     if (blockIdx.x >= (all + range - 1) / range) return;
     int r = 0;  // the sequence of the first entry: the last one that starts at or before it
+    // (what LDS gives is the same in every lane, and has to be seen to be: descriptors and branches follow from it)
+    const auto start_of = [&](int i) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(s_starts[i])); };
     for (int hi = a.num_seqs; r + 1 < hi;) {
         const int mid = (r + hi) >> 1;
-        if (static_cast<uint32_t>(s_starts[mid]) * Hkv <= at_entry) r = mid;
+        if (start_of(mid) * Hkv <= at_entry) r = mid;
         else hi = mid;
     }
     for (; at_entry < stop;) {
-    while (static_cast<uint32_t>(s_starts[r + 1]) * Hkv <= at_entry) r++;
-    const uint32_t base = static_cast<uint32_t>(s_starts[r]) * Hkv;
-    const int held = s_starts[r + 1] - s_starts[r];
+    while (start_of(r + 1) * Hkv <= at_entry) r++;
+    const uint32_t base = start_of(r) * Hkv;
+    const int held = static_cast<int>(start_of(r + 1) - start_of(r));
     const int kvh = static_cast<int>((at_entry - base) / held);
     const int beg = static_cast<int>(at_entry - base) - kvh * held;
     const int end = static_cast<int>(min(static_cast<uint32_t>(held), beg + (stop - at_entry)));
     const uint32_t entry0 = base + static_cast<uint32_t>(kvh) * held;  // of the row
     at_entry += end - beg;
     const int row = r * Hkv + kvh;
-    const int T = s_lens[r];
+    const int T = __builtin_amdgcn_readfirstlane(s_lens[r]);
     const int lo = window_begin(T, a.window), sink = min(a.sink, T);
     const WindowList list = window_list(T, a.sink, a.window);
     const int32_t* table = a.d.block_tables + static_cast<int64_t>(r) * a.d.max_blocks_per_seq;
@@ -476,10 +480,69 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     }
 }
 
-// The parts of a row that was cut: one wave per (row, query head), lanes over dims. The first part lies in slot 1
-// of its range, the others in slot 0 of theirs.
+// What a row's parts are: list entries [e0, e0 + held), parts in the ranges first .. last. The first part lies in slot 1 of its range, the
+// others in slot 0 of theirs.
+__device__ __forceinline__ int64_t window_part(uint32_t w, uint32_t first, int G, int g) {
+    return (2 * static_cast<int64_t>(w) + (w == first)) * G + g;
+}
+
+// The masses of sequence r's list entries from 256 chunk: entry e gets the weights of its block, the sum over query heads h of
+// parts.sum * exp2(parts.max - M_h) / L_h in the order of the heads, so that no timing enters. A thread an entry; the heads' M and
+// 1 / L stand in LDS. 8 bytes a query head and block are read, against 32 D of the keys and values that the decode reads for it.
+__device__ __forceinline__ void window_masses(const WindowArgs& a, int r, int chunk) {
+    constexpr int kHeads = 128;  // in LDS at a time
+    __shared__ float2 s_total[kHeads];
+    const int G = a.d.group, Hkv = a.d.num_kv_heads, Hq = Hkv * G;
+    const uint32_t before = a.starts[r], held = a.starts[r + 1] - before, range = a.starts[a.num_seqs + 1];
+    const uint32_t e = 256u * chunk + threadIdx.x;
+    if (256u * chunk >= held) return;
+    float sum = 0.0f;
+    for (int h0 = 0; h0 < Hq; h0 += kHeads) {
+        if (h0 > 0) __syncthreads();
+        const int own = h0 + static_cast<int>(threadIdx.x);
+        if (threadIdx.x < kHeads && own < Hq) {
+            const int kvh = own / G, g = own - kvh * G;
+            const uint32_t e0 = before * Hkv + kvh * held, first = e0 / range, last = (e0 + held - 1) / range;
+            float M, L;
+            if (first == last) {
+                const float2 t = a.total[static_cast<int64_t>(r) * Hq + own];
+                M = t.x;
+                L = t.y;
+            } else {
+                M = -INFINITY;
+                L = 0.0f;
+                for (uint32_t w = first; w <= last; w++) M = fmaxf(M, a.d.ws_m[window_part(w, first, G, g)]);
+                for (uint32_t w = first; w <= last; w++) {
+                    const int64_t pi = window_part(w, first, G, g);
+                    const float m = a.d.ws_m[pi];
+                    L += a.d.ws_l[pi] * (m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M));
+                }
+            }
+            s_total[threadIdx.x] = make_float2(M, 1.0f / L);
+        }
+        __syncthreads();
+        if (e >= held) continue;
+        for (int h = h0; h < min(Hq, h0 + kHeads); h++) {
+            const int kvh = h / G;
+            const float2 p = a.parts[(static_cast<int64_t>(before) * Hkv + static_cast<int64_t>(kvh) * held + e) * G + (h - kvh * G)];
+            const float2 t = s_total[h - h0];
+            sum += p.y * __builtin_amdgcn_exp2f(p.x - t.x) * t.y;
+        }
+    }
+    if (e >= held) return;
+    const int T = clamp_len(a.d, a.d.context_lens[r]);
+    a.mass[static_cast<int64_t>(r) * a.d.max_blocks_per_seq + window_list(T, a.sink, a.window).block(e)] += sum;
+}
+
+// What follows the decode, in one launch: the parts of rows that were cut, a wave per (row, query head), lanes over dims, in the first
+// a.merge_groups workgroups; then the masses.
 template <int D>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(256) void window_finish_kernel(const WindowArgs a) {
+    if (static_cast<int>(blockIdx.x) >= a.merge_groups) {
+        const int i = static_cast<int>(blockIdx.x) - a.merge_groups;
+        window_masses(a, i / a.mass_chunks, i % a.mass_chunks);
+        return;
+    }
     constexpr int DPL = (D + 63) / 64;
     const int lane = threadIdx.x & 63, G = a.d.group, Hkv = a.d.num_kv_heads;
     const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -491,7 +554,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowArgs a) {
     if (held == 0) return;
     const uint32_t e0 = before * Hkv + kvh * held, first = e0 / range, last = (e0 + held - 1) / range;
     if (first == last) return;  // written whole
-    const auto part = [&](uint32_t w) { return (2 * static_cast<int64_t>(w) + (w == first)) * G + g; };
+    const auto part = [&](uint32_t w) { return window_part(w, first, G, g); };
     // Lanes hold the maxima and sums of 64 parts, the outputs are loaded kAhead parts at a time, the first ones
     // beside the maxima.
     constexpr int kAhead = 8;
@@ -531,11 +594,10 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WindowArgs a) {
 #pragma unroll
     for (int k = 0; k < DPL; k++)
         if (lane + 64 * k < D) a.d.out[u * D + lane + 64 * k] = o[k] / L;
-    if (a.parts && lane == 0) a.total[u] = make_float2(M, L);
 }
 
 template <int D>
-void launch_window_decode(const WindowArgs& a, int kv_dtype, bool q_f32, bool merge, hipStream_t s) {
+void launch_window_decode(const WindowArgs& a, int kv_dtype, bool q_f32, hipStream_t s) {
     const int G = a.d.group;
     const auto go = [&](auto kernel) { kernel<<<a.groups, 64 * window_waves(D), 0, s>>>(a); };
     const auto by_q = [&](auto kv, auto passes) {
@@ -551,16 +613,14 @@ void launch_window_decode(const WindowArgs& a, int kv_dtype, bool q_f32, bool me
     if (kv_dtype == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>(), std::integral_constant<int, 1>());
     else if (kv_dtype == PA_DTYPE_BF16) by_group(std::integral_constant<int, PA_DTYPE_BF16>());
     else if constexpr (D >= 64) by_group(std::integral_constant<int, PA_DTYPE_INT8>());
-    if (merge) {
-        const int64_t waves = static_cast<int64_t>(a.num_seqs) * a.d.num_kv_heads * G;
-        window_merge_kernel<D><<<static_cast<uint32_t>((waves + 3) / 4), 256, 0, s>>>(a);
-    }
+    const uint32_t behind = a.merge_groups + static_cast<uint32_t>(a.num_seqs) * a.mass_chunks;
+    if (behind > 0) window_finish_kernel<D><<<behind, 256, 0, s>>>(a);
 }
 #ifndef PA_WINDOW_INSTANTIATE
-extern template void launch_window_decode<32>(const WindowArgs&, int, bool, bool, hipStream_t);
-extern template void launch_window_decode<64>(const WindowArgs&, int, bool, bool, hipStream_t);
-extern template void launch_window_decode<128>(const WindowArgs&, int, bool, bool, hipStream_t);
-extern template void launch_window_decode<256>(const WindowArgs&, int, bool, bool, hipStream_t);
+extern template void launch_window_decode<32>(const WindowArgs&, int, bool, hipStream_t);
+extern template void launch_window_decode<64>(const WindowArgs&, int, bool, hipStream_t);
+extern template void launch_window_decode<128>(const WindowArgs&, int, bool, hipStream_t);
+extern template void launch_window_decode<256>(const WindowArgs&, int, bool, hipStream_t);
 #endif
 
 }  // namespace pa

@@ -1,44 +1,10 @@
-// window_decode.hip -- entry points of the attention over a window and sinks for single tokens (window_decode.h), and the
-// masses of its blocks.
+// window_decode.hip -- entry points of the attention over a window and sinks for single tokens (window_decode.h).
 #include <algorithm>
 #include <string>
 
 #include "window_decode.h"
 
 namespace {
-
-// The masses of one launch's sequences: entry e of sequence r's list gets the weights of its block, the sum over
-// query heads h of parts.sum * exp2(parts.max - M_h) / L_h in the order of the heads, so that no timing enters. A thread an entry;
-// the heads' M and 1 / L stand in LDS. 8 bytes a query head and block are read, against 32 D of the keys and values that the
-// decode reads for it.
-constexpr int kMassThreads = 256;
-constexpr int kMassHeads = 128;  // heads in LDS at a time
-__global__ __launch_bounds__(kMassThreads) void window_mass_kernel(const pa::WindowArgs a) {
-    __shared__ float2 s_total[kMassHeads];
-    const int r = blockIdx.y, G = a.d.group, Hkv = a.d.num_kv_heads, Hq = Hkv * G;
-    const int before = a.starts[r], held = a.starts[r + 1] - before;
-    const int e = blockIdx.x * kMassThreads + threadIdx.x;
-    if (static_cast<int>(blockIdx.x) * kMassThreads >= held) return;
-    float sum = 0.0f;
-    for (int h0 = 0; h0 < Hq; h0 += kMassHeads) {
-        __syncthreads();
-        if (threadIdx.x < kMassHeads && h0 + static_cast<int>(threadIdx.x) < Hq) {
-            const float2 t = a.total[static_cast<int64_t>(r) * Hq + h0 + threadIdx.x];
-            s_total[threadIdx.x] = make_float2(t.x, 1.0f / t.y);
-        }
-        __syncthreads();
-        if (e >= held) continue;
-        for (int h = h0; h < min(Hq, h0 + kMassHeads); h++) {
-            const int kvh = h / G;
-            const float2 p = a.parts[(static_cast<int64_t>(before) * Hkv + static_cast<int64_t>(kvh) * held + e) * G + (h - kvh * G)];
-            const float2 t = s_total[h - h0];
-            sum += p.y * __builtin_amdgcn_exp2f(p.x - t.x) * t.y;
-        }
-    }
-    if (e >= held) return;
-    const int T = pa::clamp_len(a.d, a.d.context_lens[r]);
-    a.mass[static_cast<int64_t>(r) * a.d.max_blocks_per_seq + pa::window_list(T, a.sink, a.window).block(e)] += sum;
-}
 
 // The most blocks that a context of up to max_len tokens shows of itself.
 int64_t most_blocks(int32_t max_len, int32_t sink, int32_t window) {
@@ -139,8 +105,8 @@ pa_status pa_window_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     if (reinterpret_cast<uintptr_t>(workspace) & 7)
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": workspace must be 8-byte aligned");
     const int32_t G = cfg->num_q_heads / cfg->num_kv_heads;
-    // the parts of cut rows are joined by a wave per (row, query head), four to a workgroup
-    if (!pa::fits_grid((static_cast<int64_t>(p.seqs) * cfg->num_q_heads + 3) / 4, 256))
+    // the parts of cut rows are joined by a wave per (row, query head), four to a workgroup, masses added by a thread a block
+    if (!pa::fits_grid((static_cast<int64_t>(p.seqs) * cfg->num_q_heads + 3) / 4 + p.seqs * ((blocks + 255) / 256), 256))
         return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many heads for one call");
     char* const ws = static_cast<char*>(workspace);
     pa::WindowArgs a{};
@@ -163,6 +129,7 @@ pa_status pa_window_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     a.sink = sink_tokens;
     a.window = window;
     a.least = p.least;
+    a.mass_chunks = block_mass ? static_cast<int32_t>((blocks + 255) / 256) : 0;
     a.groups = p.groups;
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
@@ -175,18 +142,14 @@ pa_status pa_window_decode(pa_stream* stream, const pa_config* cfg, float* out, 
         a.d.block_tables = block_tables + static_cast<int64_t>(s0) * max_blocks_per_seq;
         a.d.context_lens = context_lens + s0;
         a.mass = block_mass ? block_mass + static_cast<int64_t>(s0) * max_blocks_per_seq : nullptr;
+        a.merge_groups = p.merge ? static_cast<int32_t>((static_cast<int64_t>(a.num_seqs) * cfg->num_q_heads + 3) / 4) : 0;
         switch (cfg->head_dim) {
-            case 32: pa::launch_window_decode<32>(a, cfg->kv_dtype, q_f32, p.merge, s); break;
-            case 64: pa::launch_window_decode<64>(a, cfg->kv_dtype, q_f32, p.merge, s); break;
-            case 128: pa::launch_window_decode<128>(a, cfg->kv_dtype, q_f32, p.merge, s); break;
-            default: pa::launch_window_decode<256>(a, cfg->kv_dtype, q_f32, p.merge, s); break;
+            case 32: pa::launch_window_decode<32>(a, cfg->kv_dtype, q_f32, s); break;
+            case 64: pa::launch_window_decode<64>(a, cfg->kv_dtype, q_f32, s); break;
+            case 128: pa::launch_window_decode<128>(a, cfg->kv_dtype, q_f32, s); break;
+            default: pa::launch_window_decode<256>(a, cfg->kv_dtype, q_f32, s); break;
         }
         PA_HIP_CHECK(hipGetLastError());
-        if (a.mass && blocks > 0) {
-            const dim3 grid(static_cast<uint32_t>((blocks + kMassThreads - 1) / kMassThreads), a.num_seqs);
-            window_mass_kernel<<<grid, kMassThreads, 0, s>>>(a);
-            PA_HIP_CHECK(hipGetLastError());
-        }
     }
     return pa::clear_error();
 }

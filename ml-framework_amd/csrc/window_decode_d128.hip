@@ -2,4 +2,4 @@
 #define PA_WINDOW_INSTANTIATE
 #include "window_decode.h"
 
-template void pa::launch_window_decode<128>(const pa::WindowArgs&, int, bool, bool, hipStream_t);
+template void pa::launch_window_decode<128>(const pa::WindowArgs&, int, bool, hipStream_t);
