@@ -290,12 +290,14 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     if (window > 0)
         blocks = std::min(blocks, (static_cast<int64_t>(std::min(sink_tokens, max_context_len)) + 15) / 16 +
                                       (static_cast<int64_t>(window) + last_queries + 14) / 16 + 1);
+    const int64_t groups = (blocks + 2 * kSetWaves - 1) / (2 * kSetWaves);
+    if (!pa::fits_grid(groups, kMassThreads)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
     const MassArgs a{q,          lse,       q_start_loc,       prefix_lens,          k_cache,         k_scale,
                      block_tables, block_mass, cfg->num_kv_heads, cfg->num_q_heads / cfg->num_kv_heads, max_blocks_per_seq,
                      cfg->num_blocks, max_context_len, last_queries, sink_tokens, window, pa::resolve_scale(cfg)};
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
-    const dim3 grid(static_cast<uint32_t>((blocks + 2 * kSetWaves - 1) / (2 * kSetWaves)), num_seqs);
+    const dim3 grid(static_cast<uint32_t>(groups), num_seqs);
     const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
     switch (cfg->head_dim) {
         case 32: launch<32>(a, cfg->kv_dtype, q_f32, grid, s); break;

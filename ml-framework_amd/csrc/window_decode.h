@@ -364,8 +364,8 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
             l_run += psum;
             if (a.parts) {
                 const float sum = rows_sum(psum);
-                if (lane < G)
-                    a.parts[(static_cast<int64_t>(entry0) + e0 + W * j) * G + lane] = make_float2(m0, sum);
+                if (lane < G)  // (no score above -inf: a maximum that makes nothing of the sum, which is 0 or NaN)
+                    a.parts[(static_cast<int64_t>(entry0) + e0 + W * j) * G + lane] = make_float2(m_run == -INFINITY ? -FLT_MAX : m_run, sum);
             }
             if constexpr (F32) {
 #pragma unroll

@@ -5,8 +5,7 @@ Tolerances, from fp32 sums of products. A score is a sum of D products whose mag
 addition rounds by at most 2^-24 of a partial sum no larger than S, the roundings have no common sign, so their sum is taken
 as 4 sqrt(D) 2^-24 S. Where an operand is fp32, products are formed of bf16 parts and those of parts below 2^-24 are left out,
 at most four of them a product: 2^-22 S. exp of the score adds 2^-22 (its argument's rounding near the maximum, and its own).
-That is `e`. A probability is off by twice that with its normalisation, and by 2^-18 where a chunk's probabilities are two
-rounded bf16 parts; the T additions of P V and of the sum add 4 sqrt(T) 2^-24, each relative to the largest |v|."""
+That is `e`. A probability is off by twice that with its normalisation; the T additions of P V and of the sum add 4 sqrt(T) 2^-24, each relative to the largest |v|."""
 import numpy as np
 
 from longctx_ref import BLOCK, f64
@@ -34,7 +33,7 @@ def context(p, s, length, max_len=None):
     return k[:, :t], v[:, :t]
 
 
-def attend(p, q, rows, positions, sink, window, lens, max_len=None, two_parts=False):
+def attend(p, q, rows, positions, sink, window, lens, max_len=None):
     """Query r of row rows[r] at position positions[r], in a context of lens[r] tokens. (out, tolerance, lse, its
     tolerance, weights per row and block [len(tables), width], their tolerance)"""
     n, g = len(rows), p.hq // p.hkv
@@ -61,7 +60,7 @@ def attend(p, q, rows, positions, sink, window, lens, max_len=None, two_parts=Fa
             S = (np.abs(kk) @ np.abs(qv[r, h])).max() * scale
             e = (4 * np.sqrt(p.d) * EPS + (4 * EPS if p.kv == 0 or p.q == 0 else 0)) * S + 4 * EPS
             t = 2 * e + 4 * np.sqrt(len(vis)) * EPS
-            tol[r, h] = (t + (2.0 ** -18 if two_parts else 0)) * np.abs(vv).max()
+            tol[r, h] = t * np.abs(vv).max()
             # in log2 units and back: three roundings of a value of that size
             lse_tol[r, h] = e + 4 * np.sqrt(len(vis)) * EPS + 4 * EPS * (1 + abs(lse[r, h]) + np.abs(x).max())
             b = np.bincount(vis // BLOCK, w / total, minlength=p.width)

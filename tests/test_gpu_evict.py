@@ -152,7 +152,7 @@ def test_serving_from_a_bounded_cache(kv, q, window, sink, budget, graph):
     rows, at = bref.chunk_rows(S.lens0, S.lens0)
     qs = p.queries(len(rows))
     out, lse = run_prefill(p, g, qs, S.lens0, S.lens0, sink, window)
-    want = bref.attend(p, qs, rows, at, sink, window, [S.lens0[s] for s in rows], two_parts=kv != 0)
+    want = bref.attend(p, qs, rows, at, sink, window, [S.lens0[s] for s in rows])
     close(out, want[0], want[1])
     close(lse, want[2], want[3])
     mass = S.mass
@@ -257,3 +257,14 @@ def test_serving_from_a_bounded_cache(kv, q, window, sink, budget, graph):
         gr.destroy()
     ts.destroy()
     dev.close()
+
+
+def test_evict_the_same_block_twice():
+    """A block that stands twice in a row, and in another row: a count for every entry that leaves."""
+    tables = np.array([[3, 3, 4, 3, 5, -1], [3, 6, 6, 7, -1, -1]], I32)
+    lens, mass = np.array([70, 64], I32), np.array([[1, 2, 0, 3, 4, 9], [0, 0, 5, 1, 9, 9]], np.float32)
+    refs = np.bincount(tables[tables >= 0], minlength=9).astype(I32)
+    for m in (mass, None):
+        got = run_evict(9, tables, lens, m, 0, 1, 2, refs)
+        same(got, bref.evict(tables, lens, m, 0, 1, 2, refs))
+        np.testing.assert_array_equal(got[3], np.bincount(got[0][got[0] >= 0], minlength=9))
