@@ -10,7 +10,8 @@
 // in sparse_decode.h, whose arithmetic this kernel shares: exact products (an fp32 value as three bf16 parts in
 // the matrix columns that a group of G heads leaves idle), sums in fp32, two register buffers a wave, the waves' states
 // met in LDS at a segment's end. Here the lists follow from the lengths, so nothing but the table is read for them, and the
-// ranges go by what the rows really hold: every workgroup adds up the lengths itself (at most kWindowSeqs a launch).
+// ranges go by what the rows really hold: every workgroup adds up the lengths itself (at most kWindowSeqs a launch). Where the chip
+// is not full, every row is filled up to whole ranges in what is laid end to end.
 #pragma once
 
 #include "sparse_decode.h"
@@ -21,12 +22,12 @@ constexpr int kWindowSeqs = 2047;  // sequences of one launch: their lists' star
 
 struct WindowArgs {
     DecodeArgs d;          // caches, q, out, tables, lengths, shape; ws_o / ws_m / ws_l: [2 * workgroups][G]
-    int32_t* starts;       // [num_seqs + 1] blocks (of one KV head) before each sequence, then the range
+    int32_t* starts;       // [num_seqs + 1] entries (of one KV head) before each sequence, then the range
     float2* parts;         // masses: (maximum, sum) of every list entry's tokens, [Hkv * starts + ..][G]; else null
     float2* total;         // masses: (maximum, sum) of every row that was not cut, [num_seqs][Hq]
     float* mass;           // [num_seqs][max_blocks_per_seq]
     int32_t num_seqs, sink, window;
-    int32_t least;         // list entries of a range at least
+    int32_t least_log;     // list entries of a range at least: 2^least_log, a multiple of the waves
     int32_t groups;        // workgroups
     int32_t merge_groups;  // of the launch behind: workgroups that join cut rows, and (masses) per sequence
     int32_t mass_chunks;
@@ -50,47 +51,82 @@ __host__ __device__ constexpr int window_decode_groups(int head_dim, int kv) {
     return sparse_groups(head_dim, kv) * sparse_waves(head_dim) / window_waves(head_dim);
 }
 
-// The sequences' lists laid end to end: starts[r] in s_starts, their lengths in s_lens, and the most that one list has. One
-// workgroup, W waves.
+// How the lists are dealt out: sequence r's entries (of one KV head) from s_starts[r], its length in s_lens[r]; what a workgroup
+// takes. One workgroup, W waves. The rule, for lists of `all` entries in all:
+//   whole rows where all are of one length and that gives no CU more than 32 entries, or a third, over an equal share: a cut row costs
+//   another start, another exchange of states and the merge;
+//   the least range where there are workgroups for every row's last range to be a part of one (the chip is not full): no workgroup
+//   starts twice (one sequence of 1028 tokens, 8 KV heads: 11.7 us, with ranges across rows 13.5);
+//   equal ranges.
 template <int W>
-__device__ __forceinline__ int window_starts(const WindowArgs& a, int32_t* s_starts, int32_t* s_lens) {
+__device__ __forceinline__ uint32_t window_starts(const WindowArgs& a, int32_t* s_starts, int32_t* s_lens) {
     constexpr int PER = (kWindowSeqs + 64 * W) / (64 * W);
-    __shared__ int s_sum[W], s_most[W];
+    __shared__ int s_sum[W], s_ranges[W], s_most[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int raw[PER], sum = 0, most = 0;
+    const int least = 1 << a.least_log, per = (a.num_seqs + 64 * W) / (64 * W);  // sequences a thread: 1 .. PER
+    const auto ranges_of = [&](int entries) { return (entries + least - 1) >> a.least_log; };
+    int raw[PER], sum = 0, most = 0, ranges = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        const int r = threadIdx.x * PER + i;
+        if (i >= per) break;
+        const int r = threadIdx.x * per + i;
         raw[i] = r < a.num_seqs ? a.d.context_lens[r] : 0;
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
+        if (i >= per) break;
         const int len = max(0, clamp_len(a.d, raw[i]));
-        s_lens[threadIdx.x * PER + i] = len;
+        s_lens[threadIdx.x * per + i] = len;
         raw[i] = window_list(len, a.sink, a.window).entries();
         sum += raw[i];
         most = max(most, raw[i]);
+        ranges += ranges_of(raw[i]);
     }
-    const int upto = wave_prefix(sum);
+    const int upto = wave_prefix(sum), ranges_upto = wave_prefix(ranges);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
-    if (lane == 63) s_sum[wave] = upto;
-    if (lane == 0) s_most[wave] = most;
+    if (lane == 63) {
+        s_sum[wave] = upto;
+        s_ranges[wave] = ranges_upto;
+        s_most[wave] = most;
+    }
     __syncthreads();
-    int at = upto - sum;
+    int at = upto - sum, ranges_at = ranges_upto - ranges, total = 0, ranges_total = 0;
 #pragma unroll
     for (int w = 0; w < W; w++) {
         at += w < wave ? s_sum[w] : 0;
+        ranges_at += w < wave ? s_ranges[w] : 0;
+        total += s_sum[w];
+        ranges_total += s_ranges[w];
         most = max(most, s_most[w]);
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    ranges_total = __builtin_amdgcn_readfirstlane(ranges_total);
+    most = __builtin_amdgcn_readfirstlane(most);
+    const uint32_t Hkv = a.d.num_kv_heads, rows = a.num_seqs * Hkv, all = total * Hkv;
+    uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(least));
+    range = (range + W - 1) / W * W;
+    bool fill = ranges_total * Hkv <= static_cast<uint32_t>(a.groups);
+    if (most > 0 && most * rows == all) {
+        const uint32_t even = (all + kSparseCUs - 1) / kSparseCUs, whole = (rows + kSparseCUs - 1) / kSparseCUs * most;  // a CU's
+        if (whole <= even + 32 || 3 * whole < 4 * even) {
+            range = (rows + a.groups - 1) / a.groups * most;
+            fill = false;
+        }
+    }
+    if (fill) {
+        range = least;
+        at = ranges_at << a.least_log;
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        const int r = threadIdx.x * PER + i;
+        if (i >= per) break;
+        const int r = threadIdx.x * per + i;
         if (r <= a.num_seqs) s_starts[r] = at;
-        at += raw[i];
+        at += fill ? ranges_of(raw[i]) << a.least_log : raw[i];
     }
     __syncthreads();
-    return most;
+    return range;
 }
 
 // PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
@@ -111,17 +147,8 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.d.num_kv_heads, G = a.d.group;
-    const int most = __builtin_amdgcn_readfirstlane(window_starts<W>(a, s_starts, s_lens));
+    const uint32_t range = window_starts<W>(a, s_starts, s_lens);
     const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(s_starts[a.num_seqs])) * Hkv;
-    // Entries a workgroup: equal ranges; whole rows where all are of one length and that gives no CU more than 32 entries, or a
-    // third, over an equal share: a cut row costs another start, another exchange of states and the merge.
-    uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(a.least));
-    range = (range + W - 1) / W * W;
-    const uint32_t rows = static_cast<uint32_t>(a.num_seqs) * Hkv;
-    if (most > 0 && static_cast<uint32_t>(most) * rows == all) {
-        const uint32_t even = (all + kSparseCUs - 1) / kSparseCUs, whole = (rows + kSparseCUs - 1) / kSparseCUs * most;  // a CU's
-        if (whole <= even + 32 || 3 * whole < 4 * even) range = (rows + a.groups - 1) / a.groups * most;
-    }
     if (blockIdx.x == 0) {
         for (int r = threadIdx.x; r <= a.num_seqs; r += 64 * W) a.starts[r] = s_starts[r];
         if (threadIdx.x == 0) a.starts[a.num_seqs + 1] = static_cast<int32_t>(range);
@@ -144,16 +171,16 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     for (; at_entry < stop;) {
     while (start_of(r + 1) * Hkv <= at_entry) r++;
     const uint32_t base = start_of(r) * Hkv;
-    const int held = static_cast<int>(start_of(r + 1) - start_of(r));
-    const int kvh = static_cast<int>((at_entry - base) / held);
-    const int beg = static_cast<int>(at_entry - base) - kvh * held;
-    const int end = static_cast<int>(min(static_cast<uint32_t>(held), beg + (stop - at_entry)));
-    const uint32_t entry0 = base + static_cast<uint32_t>(kvh) * held;  // of the row
-    at_entry += end - beg;
+    const uint32_t pitch = start_of(r + 1) - start_of(r);  // of a row: its entries, filled up where ranges do not cross rows
+    const int kvh = static_cast<int>((at_entry - base) / pitch);
+    const uint32_t entry0 = base + kvh * pitch;  // of the row
+    const int beg = static_cast<int>(at_entry - entry0);
+    at_entry += min(pitch - beg, stop - at_entry);
     const int row = r * Hkv + kvh;
     const int T = __builtin_amdgcn_readfirstlane(s_lens[r]);
     const int lo = window_begin(T, a.window), sink = min(a.sink, T);
     const WindowList list = window_list(T, a.sink, a.window);
+    const int held = list.entries(), end = min(held, static_cast<int>(at_entry - entry0));
     const int32_t* table = a.d.block_tables + static_cast<int64_t>(r) * a.d.max_blocks_per_seq;
     // Lane l holds the wave's l-th block of a stretch of 64 W entries: its place in the sequence, its physical block. No
     // load is under a condition, which would make the compiler wait at its end: past the segment the last entry is read again.
@@ -491,10 +518,12 @@ __device__ __forceinline__ int64_t window_part(uint32_t w, uint32_t first, int G
 // 1 / L stand in LDS. 8 bytes a query head and block are read, against 32 D of the keys and values that the decode reads for it.
 __device__ __forceinline__ void window_masses(const WindowArgs& a, int r, int chunk) {
     constexpr int kHeads = 128;  // in LDS at a time
+    constexpr int kAhead = 8;    // loads that go out together
     __shared__ float2 s_total[kHeads];
     const int G = a.d.group, Hkv = a.d.num_kv_heads, Hq = Hkv * G;
-    const uint32_t before = a.starts[r], held = a.starts[r + 1] - before, range = a.starts[a.num_seqs + 1];
-    const uint32_t e = 256u * chunk + threadIdx.x;
+    const uint32_t before = a.starts[r], pitch = a.starts[r + 1] - before, range = a.starts[a.num_seqs + 1];
+    const WindowList list = window_list(max(0, clamp_len(a.d, a.d.context_lens[r])), a.sink, a.window);
+    const uint32_t held = list.entries(), e = 256u * chunk + threadIdx.x;
     if (256u * chunk >= held) return;
     float sum = 0.0f;
     for (int h0 = 0; h0 < Hq; h0 += kHeads) {
@@ -502,7 +531,7 @@ __device__ __forceinline__ void window_masses(const WindowArgs& a, int r, int ch
         const int own = h0 + static_cast<int>(threadIdx.x);
         if (threadIdx.x < kHeads && own < Hq) {
             const int kvh = own / G, g = own - kvh * G;
-            const uint32_t e0 = before * Hkv + kvh * held, first = e0 / range, last = (e0 + held - 1) / range;
+            const uint32_t e0 = before * Hkv + kvh * pitch, first = e0 / range, last = (e0 + held - 1) / range;
             float M, L;
             if (first == last) {
                 const float2 t = a.total[static_cast<int64_t>(r) * Hq + own];
@@ -511,27 +540,44 @@ __device__ __forceinline__ void window_masses(const WindowArgs& a, int r, int ch
             } else {
                 M = -INFINITY;
                 L = 0.0f;
-                for (uint32_t w = first; w <= last; w++) M = fmaxf(M, a.d.ws_m[window_part(w, first, G, g)]);
-                for (uint32_t w = first; w <= last; w++) {
-                    const int64_t pi = window_part(w, first, G, g);
-                    const float m = a.d.ws_m[pi];
-                    L += a.d.ws_l[pi] * (m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M));
+                for (uint32_t w0 = first; w0 <= last; w0 += kAhead) {
+                    float m[kAhead], l[kAhead];
+#pragma unroll
+                    for (int j = 0; j < kAhead; j++) {
+                        const int64_t pi = window_part(min(w0 + j, last), first, G, g);
+                        m[j] = a.d.ws_m[pi];
+                        l[j] = w0 + j <= last ? a.d.ws_l[pi] : 0.0f;
+                    }
+                    float top = M;
+#pragma unroll
+                    for (int j = 0; j < kAhead; j++) top = fmaxf(top, m[j]);
+                    L *= M == top ? 1.0f : __builtin_amdgcn_exp2f(M - top);
+#pragma unroll
+                    for (int j = 0; j < kAhead; j++) L += l[j] * (m[j] == top ? 1.0f : __builtin_amdgcn_exp2f(m[j] - top));
+                    M = top;
                 }
             }
             s_total[threadIdx.x] = make_float2(M, 1.0f / L);
         }
         __syncthreads();
         if (e >= held) continue;
-        for (int h = h0; h < min(Hq, h0 + kHeads); h++) {
-            const int kvh = h / G;
-            const float2 p = a.parts[(static_cast<int64_t>(before) * Hkv + static_cast<int64_t>(kvh) * held + e) * G + (h - kvh * G)];
-            const float2 t = s_total[h - h0];
-            sum += p.y * __builtin_amdgcn_exp2f(p.x - t.x) * t.y;
+        const int end = min(Hq, h0 + kHeads);
+        for (int h = h0; h < end; h += kAhead) {
+            float2 p[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const int own = min(h + j, end - 1), kvh = own / G;
+                p[j] = a.parts[(static_cast<int64_t>(before) * Hkv + static_cast<int64_t>(kvh) * pitch + e) * G + (own - kvh * G)];
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const float2 t = s_total[min(h + j, end - 1) - h0];
+                if (h + j < end) sum += p[j].y * __builtin_amdgcn_exp2f(p[j].x - t.x) * t.y;
+            }
         }
     }
     if (e >= held) return;
-    const int T = clamp_len(a.d, a.d.context_lens[r]);
-    a.mass[static_cast<int64_t>(r) * a.d.max_blocks_per_seq + window_list(T, a.sink, a.window).block(e)] += sum;
+    a.mass[static_cast<int64_t>(r) * a.d.max_blocks_per_seq + list.block(e)] += sum;
 }
 
 // What follows the decode, in one launch: the parts of rows that were cut, a wave per (row, query head), lanes over dims, in the first
@@ -550,9 +596,9 @@ __global__ __launch_bounds__(256) void window_finish_kernel(const WindowArgs a) 
     const uint32_t row = static_cast<uint32_t>(u / G), range = a.starts[a.num_seqs + 1];
     const int g = static_cast<int>(u - static_cast<int64_t>(row) * G);
     const int r = static_cast<int>(row) / Hkv, kvh = static_cast<int>(row) - r * Hkv;
-    const uint32_t before = a.starts[r], held = a.starts[r + 1] - before;
-    if (held == 0) return;
-    const uint32_t e0 = before * Hkv + kvh * held, first = e0 / range, last = (e0 + held - 1) / range;
+    const uint32_t before = a.starts[r], pitch = a.starts[r + 1] - before;
+    if (pitch == 0) return;
+    const uint32_t e0 = before * Hkv + kvh * pitch, first = e0 / range, last = (e0 + pitch - 1) / range;
     if (first == last) return;  // written whole
     const auto part = [&](uint32_t w) { return window_part(w, first, G, g); };
     // Lanes hold the maxima and sums of 64 parts, the outputs are loaded kAhead parts at a time, the first ones
