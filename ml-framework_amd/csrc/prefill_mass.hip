@@ -6,12 +6,15 @@
 //
 // A wave holds the keys of two blocks of one KV head as matrix operands and meets 32 columns (query, head) after the other
 // (K . Q^T as in window_prefill.h), which four waves with blocks of their own read from LDS: there a column's operands are formed once,
-// the next ones on their way from memory meanwhile. A workgroup has two such sets of waves, for the even and the odd KV heads; a wave
-// adds up a block's weights over its heads and columns in registers, and the two sets' sums are added at the end, so that no timing
-// enters. Keys are read once however many queries there are.
-// What bounds it: each step's operands, products and exponentials in turn behind its barrier (9 prompts of 2-8k tokens, 32 queries,
-// bf16: 44 us, of which 12 go with the operands' exchange, 11 with the keys' loads, 14 with the exponentials). Waves that hold 128 columns in
-// registers instead and load them for themselves, 16 bytes of a row a lane, 65 us; two waves to a set 44 us, and twice the time for fp32 queries.
+// the next ones on their way from memory meanwhile. A workgroup has two (four) such sets of waves, which share out its (KV head, 32 columns)
+// in order; a wave adds up a block's weights over its heads and columns in registers, and the sets' sums are added at the end, so that
+// no timing enters. Keys are read once however many queries there are.
+// What bounds it: 9 prompts of 2-8k tokens, 32 queries, bf16: 42 us, 17 of them the keys' bytes; 31 us for a workgroup alone on its
+// CU, 40 for two, and no more than that are there: each step is operands, eight products that wait for one another, exponentials and a
+// barrier in turn (1.4 us). Waves that hold 128 columns in registers instead and load them for themselves, 16 bytes of a row a lane,
+// 65 us; two waves to a set 44 us, and twice the time for fp32 queries; columns loaded two steps ahead 46 us (registers).
+// fp32 queries (three products): one of 30000 tokens, 64 queries, int8: 68 us, 37 of them at the rate of a large matrix product; LDS
+// gives their operands no faster than the products take them. Two sets instead of four 78 us.
 #include <algorithm>
 #include <string>
 
@@ -61,25 +64,31 @@ __device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[
     }
 }
 
-constexpr int kSetWaves = 4;                       // waves that share the columns' operands
-constexpr int kMassThreads = 2 * 64 * kSetWaves;   // two sets
+constexpr int kSetWaves = 4;  // waves that share the columns' operands
 
 // Whether two workgroups fit a CU: 128 registers a lane.
 __host__ __device__ constexpr bool mass_two(int d, int kv, bool q_f32) { return !q_f32 && kv != PA_DTYPE_FP32 && d <= 128; }
+// Sets of a workgroup: four where registers allow four waves a SIMD, but LDS (three parts of each column) only one workgroup a CU.
+__host__ __device__ constexpr int mass_sets(int d, int kv, bool q_f32) { return q_f32 && kv != PA_DTYPE_FP32 && d <= 128 ? 4 : 2; }
+__host__ __device__ constexpr int mass_threads(int d, int kv, bool q_f32) { return 64 * kSetWaves * mass_sets(d, kv, q_f32); }
+
+// A barrier for what stands in LDS: loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int D, int KV, bool QF32>
-__global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void prefill_mass_kernel(const MassArgs a) {
+__global__ __launch_bounds__(mass_threads(D, KV, QF32), mass_two(D, KV, QF32) || mass_sets(D, KV, QF32) == 4 ? 4 : 2) void prefill_mass_kernel(const MassArgs a) {
     constexpr bool I8 = KV == PA_DTYPE_INT8;
     constexpr int NP = KV == PA_DTYPE_FP32 ? 3 : 1, NQ = QF32 ? 3 : 1, NS = D / 16;
     constexpr int ELT = KV == PA_DTYPE_FP32 ? 4 : I8 ? 1 : 2, QKV = QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16;
+    constexpr int SETS = mass_sets(D, KV, QF32);
     constexpr int SET = NS * 64;                                     // 16-byte pieces of 32 columns' operands, of one part
-    constexpr int NB = 4 * NQ * SET * 16 <= (mass_two(D, KV, QF32) ? 64 : 128) * 1024 ? 2 : 1;      // buffers of a set
-    constexpr bool EARLY = !mass_two(D, KV, QF32) && (NP == 1 || D < 256);                       // the next head's keys loaded early: registers for it
+    constexpr int NB = 2 * SETS * NQ * SET * 16 <= (mass_two(D, KV, QF32) ? 64 : 128) * 1024 ? 2 : 1;  // buffers of a set
+    constexpr bool EARLY = !mass_two(D, KV, QF32) && SETS == 2 && (NP == 1 || D < 256);                       // the next head's keys loaded early: registers for it
     constexpr int PER = (SET + 64 * kSetWaves - 1) / (64 * kSetWaves);  // pieces a thread brings
-    __shared__ uint4 s_q[2][NB][NQ][SET];
-    __shared__ float s_lse[2][NB][32];
-    __shared__ int s_at[2][NB][32];  // the columns' positions
-    __shared__ float s_sum[2][kSetWaves][2];
+    __shared__ uint4 s_q[SETS][NB][NQ][SET];
+    __shared__ float s_lse[SETS][NB][32];
+    __shared__ int s_at[SETS][NB][32];  // the columns' positions
+    __shared__ float s_sum[SETS][kSetWaves][2];
     const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int set = wave / kSetWaves, tid = threadIdx.x % (64 * kSetWaves);
@@ -95,7 +104,7 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
     if (2 * kSetWaves * static_cast<int>(blockIdx.x) >= entries) return;
     const int32_t* table = a.block_tables + static_cast<int64_t>(seq) * a.max_blocks_per_seq;
 
-    // this wave's blocks, the same ones in both sets; a wave past the last has none, but brings operands
+    // this wave's blocks, the same ones in all sets; a wave past the last has none, but brings operands
     const int e0 = 2 * (kSetWaves * static_cast<int>(blockIdx.x) + wave % kSetWaves);
     int lb[2], id[2];
 #pragma unroll
@@ -112,15 +121,21 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
     const bool plain = there[0] && there[1] && span.all_see_block(tok[0]) && span.all_see_block(tok[1]);
 
     const int columns = m * G, chunks = (columns + 31) / 32;
-    const int heads = (Hkv - set + 1) / 2, steps = heads * chunks;           // of this set
-    const int most = (Hkv + 1) / 2 * chunks;                                 // of either: the barriers are the workgroup's
-    RawKeys<KV> raw[NS] = {};
+    // (KV head, chunk) by (KV head, chunk) in a row, cut evenly over the sets
+    const int all = Hkv * chunks, first = set * all / SETS, steps = (set + 1) * all / SETS - first;
+    const int most = (all + SETS - 1) / SETS;  // of any set: the barriers are the workgroup's
+    // bf16 keys are their own operands: the next head's are loaded straight into the registers that the last chunk's products have left
+    constexpr bool DIRECT = KV == PA_DTYPE_BF16;
+    RawKeys<KV> raw[DIRECT ? 1 : NS] = {};
+    uint4 kop[NP][NS] = {};
     auto load_keys = [&](int kvh) {
         if (my_id < 0) return;
         const char* const at = static_cast<const char*>(a.k_cache) +
                                ((static_cast<int64_t>(my_id) * Hkv + kvh) * 16 * D + krow * D + 8 * hf) * ELT;
 #pragma unroll
-        for (int sl = 0; sl < NS; sl++) load_raw<KV>(raw[sl], at + 16 * sl * ELT);
+        for (int sl = 0; sl < NS; sl++)
+            if constexpr (DIRECT) kop[0][sl] = *reinterpret_cast<const uint4*>(at + 16 * sl * ELT);
+            else load_raw<KV>(raw[sl], at + 16 * sl * ELT);
     };
     // Columns 32 chunk .. of KV head kvh: D / 8 threads bring a column, 16 (32) bytes of bf16 (fp32) each, so that a wave reads whole lines.
     // A lane reads piece 2 slab + half of column n: the pieces of a column lie at column ^ piece, so that the 16 threads that write them
@@ -132,16 +147,23 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
         int at;
     };
     const int piece = tid % PC;
-    int load_kvh = set, load_chunk = 0;  // of the columns that are loaded next
+    // of the columns that are loaded next: how many steps', which; query and head of the chunk's first column
+    int left = steps, load_kvh = first / chunks, load_chunk = first % chunks, load_i = 32 * load_chunk / G, load_g = 32 * load_chunk % G;
+    const int add_i = 32 / G, add_g = 32 % G;
+    const float per_g = 1.0f / static_cast<float>(G);
     auto load_columns = [&](Bring& to) {
-        const int kvh = load_kvh, chunk = load_chunk;
-        if (kvh >= Hkv) return;
-        load_chunk = chunk == chunks - 1 ? 0 : chunk + 1;
-        load_kvh = load_chunk == 0 ? kvh + 2 : kvh;
+        if (left-- <= 0) return;
+        const int kvh = load_kvh, chunk = load_chunk, i0 = load_i, g0 = load_g;
+        const bool wrap = chunk == chunks - 1;
+        load_chunk = wrap ? 0 : chunk + 1;
+        load_kvh = wrap ? kvh + 1 : kvh;
+        load_g = wrap ? 0 : g0 + add_g >= G ? g0 + add_g - G : g0 + add_g;
+        load_i = wrap ? 0 : i0 + add_i + (g0 + add_g >= G);
+        // (the quotient of a number below G + 32 by G, exact: its half above a whole number outweighs what the product is off by)
         const auto row_of = [&](int col, int& i) {
-            const uint32_t c = min(32 * chunk + col, columns - 1);
-            i = static_cast<int>(c / static_cast<uint32_t>(G));
-            return (static_cast<int64_t>(q0) + Lc - m + i) * Hq + kvh * G + (static_cast<int>(c) - i * G);
+            const int x = g0 + min(col, columns - 1 - 32 * chunk), by = static_cast<int>((static_cast<float>(x) + 0.5f) * per_g);
+            i = i0 + by;
+            return (static_cast<int64_t>(q0) + Lc - m + i) * Hq + kvh * G + (x - by * G);
         };
         int i;
 #pragma unroll
@@ -150,8 +172,9 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
             load_raw<QKV>(to.x[j], static_cast<const char*>(a.q) + (row_of(tid / PC + STEP * j, i) * D + 8 * piece) * (QF32 ? 4 : 2));
         }
         if (tid < 32) {
-            to.lse = 32 * chunk + tid < columns ? a.lse[row_of(tid, i)] * 1.4426950408889634f : INFINITY;  // no such column: no weight
-            to.at = P + Lc - m + static_cast<int>(min(32 * chunk + tid, columns - 1) / G);
+            const int64_t row = row_of(tid, i);
+            to.lse = 32 * chunk + tid < columns ? a.lse[row] * 1.4426950408889634f : INFINITY;  // no such column: no weight
+            to.at = P + Lc - m + i;
         }
     };
     auto store_columns = [&](const Bring& from, int b) {
@@ -170,32 +193,33 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
     };
     const float c2 = a.scale * 1.4426950408889634f;
     float sum[2] = {0.0f, 0.0f}, f[2] = {c2, c2};
-    uint4 kop[NP][NS];
     Bring bring;  // the next step's columns, on their way while one is computed
+    int kvh = load_kvh, chunk = load_chunk;  // of step k
     if (steps > 0) {
-        if (EARLY) load_keys(set);
+        if (EARLY || DIRECT) load_keys(kvh);
         load_columns(bring);
         store_columns(bring, 0);
     }
-    int kvh = set, chunk = 0;  // of step k
     for (int k = 0; k < most; k++) {
         const int b = NB == 2 ? k & 1 : 0;
-        __syncthreads();  // step k's operands stand in LDS
+        lds_barrier();  // step k's operands stand in LDS
         load_columns(bring);
         if (k < steps && live) {
-            if (chunk == 0) {
-                if (!EARLY) load_keys(kvh);
+            if (k == 0 || chunk == 0) {
+                if constexpr (!DIRECT) {
+                    if (!EARLY) load_keys(kvh);
 #pragma unroll
-                for (int sl = 0; sl < NS; sl++) {
-                    uint4 x[NP];
-                    raw_planes<KV, NP>(raw[sl], x);
+                    for (int sl = 0; sl < NS; sl++) {
+                        uint4 x[NP];
+                        raw_planes<KV, NP>(raw[sl], x);
 #pragma unroll
-                    for (int p = 0; p < NP; p++) kop[p][sl] = x[p];
+                        for (int p = 0; p < NP; p++) kop[p][sl] = x[p];
+                    }
                 }
                 if constexpr (I8)
 #pragma unroll
                     for (int u = 0; u < 2; u++) f[u] = there[u] ? c2 * a.k_scale[static_cast<int64_t>(id[u]) * Hkv + kvh] : c2;
-                if (EARLY && kvh + 2 < Hkv) load_keys(kvh + 2);
+                if (!DIRECT && EARLY && (kvh + 1) * chunks < first + steps) load_keys(kvh + 1);
             }
             pa::f32x16_t product;
 #pragma unroll
@@ -215,6 +239,7 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
             float x[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) x[e] = e == 15 ? pa::settled(product[e]) : product[e];
+            if (DIRECT && chunk == chunks - 1 && k + 1 < steps) load_keys(kvh + 1);
             if (plain) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
@@ -233,10 +258,10 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
                     }
             }
         }
-        if (NB == 1) __syncthreads();
+        if (NB == 1) lds_barrier();
         if (k + 1 < steps) store_columns(bring, NB == 2 ? b ^ 1 : 0);
         chunk = chunk == chunks - 1 ? 0 : chunk + 1;
-        kvh = chunk == 0 ? kvh + 2 : kvh;
+        kvh = chunk == 0 ? kvh + 1 : kvh;
     }
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -244,16 +269,20 @@ __global__ __launch_bounds__(kMassThreads, mass_two(D, KV, QF32) ? 4 : 2) void p
         if (lane == 0) s_sum[set][wave % kSetWaves][u] = w;
     }
     __syncthreads();
-    if (set == 0 && lane < 2 && (lane ? lb[1] : lb[0]) >= 0)
-        a.mass[static_cast<int64_t>(seq) * a.max_blocks_per_seq + (lane ? lb[1] : lb[0])] += s_sum[0][wave][lane] + s_sum[1][wave][lane];
+    if (set == 0 && lane < 2 && (lane ? lb[1] : lb[0]) >= 0) {
+        float w = s_sum[0][wave][lane];
+#pragma unroll
+        for (int i = 1; i < SETS; i++) w += s_sum[i][wave][lane];
+        a.mass[static_cast<int64_t>(seq) * a.max_blocks_per_seq + (lane ? lb[1] : lb[0])] += w;
+    }
 }
 
 template <int D>
 void launch(const MassArgs& a, int kv, bool q_f32, dim3 grid, hipStream_t s) {
     const auto by_q = [&](auto k) {
         constexpr int KV = decltype(k)::value;
-        if (q_f32) prefill_mass_kernel<D, KV, true><<<grid, kMassThreads, 0, s>>>(a);
-        else prefill_mass_kernel<D, KV, false><<<grid, kMassThreads, 0, s>>>(a);
+        if (q_f32) prefill_mass_kernel<D, KV, true><<<grid, mass_threads(D, KV, true), 0, s>>>(a);
+        else prefill_mass_kernel<D, KV, false><<<grid, mass_threads(D, KV, false), 0, s>>>(a);
     };
     if (kv == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>());
     else if (kv == PA_DTYPE_BF16) by_q(std::integral_constant<int, PA_DTYPE_BF16>());
@@ -279,6 +308,8 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     if (num_seqs > 65535) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": num_seqs must be <= 65535");
     if (static_cast<int64_t>(last_queries) * cfg->num_q_heads > INT32_MAX / 2)
         return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": last_queries * num_q_heads must fit 30 bits");
+    if (cfg->num_q_heads / cfg->num_kv_heads > 1 << 20)
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": num_q_heads / num_kv_heads must be <= 2^20");
     if (num_seqs == 0 || last_queries == 0 || max_context_len == 0 || max_blocks_per_seq == 0) return pa::clear_error();
     if (!q || !lse || !q_start_loc || !prefix_lens || !k_cache || !block_tables || !block_mass)
         return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
@@ -291,7 +322,7 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
         blocks = std::min(blocks, (static_cast<int64_t>(std::min(sink_tokens, max_context_len)) + 15) / 16 +
                                       (static_cast<int64_t>(window) + last_queries + 14) / 16 + 1);
     const int64_t groups = (blocks + 2 * kSetWaves - 1) / (2 * kSetWaves);
-    if (!pa::fits_grid(groups, kMassThreads)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
+    if (!pa::fits_grid(groups, 1024)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
     const MassArgs a{q,          lse,       q_start_loc,       prefix_lens,          k_cache,         k_scale,
                      block_tables, block_mass, cfg->num_kv_heads, cfg->num_q_heads / cfg->num_kv_heads, max_blocks_per_seq,
                      cfg->num_blocks, max_context_len, last_queries, sink_tokens, window, pa::resolve_scale(cfg)};

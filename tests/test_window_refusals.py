@@ -73,7 +73,8 @@ def mass(c=None, q=FAKE, lse=FAKE, start=FAKE, prefix=FAKE, k=FAKE, ks=None, tab
     (INVALID, "must not be negative", dict(sink=-1)), (INVALID, "must not be negative", dict(window=-1)),
     (INVALID, "k_scale", dict(c=cfg(kv_dtype=2))), (INVALID, "aligned", dict(q=FAKE + 8)), (INVALID, "aligned", dict(k=FAKE + 8)),
     (UNSUPPORTED, "65535", dict(n=65536)), (UNSUPPORTED, "32 bits", dict(width=1 << 27)),
-    (UNSUPPORTED, "30 bits", dict(last=2 ** 27)), (UNSUPPORTED, "too many blocks", dict(most=2 ** 31 - 1, width=2 ** 27 - 1))])
+    (UNSUPPORTED, "30 bits", dict(last=2 ** 27)),
+    (UNSUPPORTED, "2^20", dict(c=cfg(num_q_heads=2 ** 22, num_kv_heads=2))), (UNSUPPORTED, "too many blocks", dict(most=2 ** 31 - 1, width=2 ** 27 - 1))])
 def test_prefill_mass(status, text, kw):
     refused(pa.prefill_mass, status, text, *mass(**kw))
 
