@@ -7,7 +7,9 @@
 // One workgroup a row. The border between what stays and what goes is the k-th largest mass, found digit by digit
 // (11 bits a pass, from the top) over the masses as ordered 32-bit integers; blocks at the border itself are dealt out by index.
 // Traffic is 16 bytes a block; a row's chain of loads, passes and barriers is what it costs, so rows of up to 16384 blocks
-// are read once into registers, a thread every 1024th block, and what stays is numbered by the waves' ballots of all of them at once.
+// are read once into registers, a thread every 1024th block, and what stays is numbered by the waves' ballots of all of them at once
+// (64 rows of 262 blocks 5.7 us; counting every block's rank among the others instead, from LDS, 8.8). Longer rows are bound by one CU's
+// scattered writes and atomics (32 rows of 2-8k blocks 25 us, 12 of them with the reference counts; with registers for 16k blocks 29.5).
 #include <algorithm>
 #include <string>
 
@@ -52,25 +54,29 @@ __global__ __launch_bounds__(kThreads) void evict_short_kernel(int32_t* __restri
     __shared__ int s_digit, s_rest;
     const int r = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t* const row = tables + static_cast<int64_t>(r) * width;
+    float* const weight = mass ? mass + static_cast<int64_t>(r) * width : nullptr;
+    int id[K];
+    float w[K];
+#pragma unroll
+    for (int i = 0; i < K; i++) {  // beside the length's load, whether the row is cut or not
+        const int b = i * kThreads + static_cast<int>(threadIdx.x);
+        id[i] = b < width ? row[b] : -1;
+        w[i] = weight && b < width ? weight[b] : 0.0f;
+    }
     const int len = lens[r];
     const int n = static_cast<int>(min((static_cast<int64_t>(len) + 15) / 16, static_cast<int64_t>(width)));
     if (len <= 0 || n <= budget) {
         if (evicted && threadIdx.x == 0) evicted[r] = 0;
         return;
     }
-    int32_t* const row = tables + static_cast<int64_t>(r) * width;
-    float* const weight = mass ? mass + static_cast<int64_t>(r) * width : nullptr;
     const int lo = sink, hi = n - recent;  // what may go
     int rest = budget - sink - recent;     // of these, how many stay
-    int id[K];
-    float w[K];
     bool may[K];
 #pragma unroll
     for (int i = 0; i < K; i++) {
         const int b = i * kThreads + static_cast<int>(threadIdx.x);
         may[i] = b >= lo && b < hi;
-        id[i] = b < width ? row[b] : -1;
-        w[i] = weight && b < width ? weight[b] : 0.0f;
     }
     // Numbers the set flags in the order of the blocks: at[i] for block i * kThreads + thread. (Its barriers also stand between the reads
     // above and the writes below.)
@@ -284,6 +290,7 @@ extern "C" pa_status pa_evict_blocks(pa_stream* stream, const pa_config* cfg, in
     };
     if (max_blocks_per_seq <= kThreads) go(evict_short_kernel<1>);
     else if (max_blocks_per_seq <= 4 * kThreads) go(evict_short_kernel<4>);
+    else if (max_blocks_per_seq <= 8 * kThreads) go(evict_short_kernel<8>);
     else if (max_blocks_per_seq <= 16 * kThreads) go(evict_short_kernel<16>);
     else go(evict_kernel);
     PA_HIP_CHECK(hipGetLastError());
