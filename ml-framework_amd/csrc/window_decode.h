@@ -12,6 +12,10 @@
 // met in LDS at a segment's end. Here the lists follow from the lengths, so nothing but the table is read for them, and the
 // ranges go by what the rows really hold: every workgroup adds up the lengths itself (at most kWindowSeqs a launch). Where the chip
 // is not full, every row is filled up to whole ranges in what is laid end to end.
+// What bounds it: memory where rows are many (64 sequences, window 1024 and 4 sinks, (32, 8, 128) bf16: 50 us, the decode itself 43 at 4.5 TB/s; 48
+// over 4096 tokens, int8: 91 us, 4.5 TB/s in runs of 2 KiB; 32 of 2-8k tokens with masses: 113 us, of which the decode 92 at 6.3 TB/s and what
+// follows 9), else round trips: 7 us and the launch behind (one sequence 10.8 us). Eight waves a workgroup with whole-list ranges, values from
+// LDS that the compiler did not see to be uniform, and a launch each for cut rows and masses took 10 to 15 % more.
 #pragma once
 
 #include "sparse_decode.h"
@@ -27,7 +31,6 @@ struct WindowArgs {
     float2* total;         // masses: (maximum, sum) of every row that was not cut, [num_seqs][Hq]
     float* mass;           // [num_seqs][max_blocks_per_seq]
     int32_t num_seqs, sink, window;
-    int32_t least_log;     // list entries of a range at least: 2^least_log, a multiple of the waves
     int32_t groups;        // workgroups
     int32_t merge_groups;  // of the launch behind: workgroups that join cut rows, and (masses) per sequence
     int32_t mass_chunks;
@@ -45,16 +48,18 @@ __device__ __forceinline__ WindowList window_list(int T, int sink, int window) {
     return {min((min(sink, T) + 15) / 16, low), low, (T + 15) / 16};
 }
 
-// Waves of a workgroup, workgroups of a full chip.
+// Waves of a workgroup, list entries of a range at least, workgroups of a full chip.
 __host__ __device__ constexpr int window_waves(int) { return 4; }
+constexpr int kWindowLeast = 8;  // (one sequence, 8 KV heads, (32, 8, 128) bf16: 4 / 8 / 16 entries 11.4 / 11.3 / 12.1 us at 1040 tokens, 17.2 / 14.0 / 13.2 at 4096)
 __host__ __device__ constexpr int window_decode_groups(int head_dim, int kv) {
     return sparse_groups(head_dim, kv) * sparse_waves(head_dim) / window_waves(head_dim);
 }
 
 // How the lists are dealt out: sequence r's entries (of one KV head) from s_starts[r], its length in s_lens[r]; what a workgroup
 // takes. One workgroup, W waves. The rule, for lists of `all` entries in all:
-//   whole rows where all are of one length and that gives no CU more than 32 entries, or a third, over an equal share: a cut row costs
-//   another start, another exchange of states and the merge;
+//   whole rows where all are of one length and that gives no CU more than 24 entries, or a third, over an equal share: a cut row costs
+//   another start, another exchange of states and the merge ((32, 8, 128) bf16, whole / cut: one sequence of 16 blocks 9.6 / 10.2 us, of 32
+//   12.1 / 10.4, of 40 13.7 / 10.8; 16 of 32 blocks 13.9 / 14.8; 60 of 64 blocks 45.1 / 49.7; 40 of 64, a CU's share 128 for 80, 39.1 / 36.8);
 //   the least range where there are workgroups for every row's last range to be a part of one (the chip is not full): no workgroup
 //   starts twice (one sequence of 1028 tokens, 8 KV heads: 11.7 us, with ranges across rows 13.5);
 //   equal ranges.
@@ -63,8 +68,8 @@ __device__ __forceinline__ uint32_t window_starts(const WindowArgs& a, int32_t* 
     constexpr int PER = (kWindowSeqs + 64 * W) / (64 * W);
     __shared__ int s_sum[W], s_ranges[W], s_most[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int least = 1 << a.least_log, per = (a.num_seqs + 64 * W) / (64 * W);  // sequences a thread: 1 .. PER
-    const auto ranges_of = [&](int entries) { return (entries + least - 1) >> a.least_log; };
+    const int per = (a.num_seqs + 64 * W) / (64 * W);  // sequences a thread: 1 .. PER
+    const auto ranges_of = [&](int entries) { return (entries + kWindowLeast - 1) / kWindowLeast; };
     int raw[PER], sum = 0, most = 0, ranges = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
@@ -104,26 +109,26 @@ __device__ __forceinline__ uint32_t window_starts(const WindowArgs& a, int32_t* 
     ranges_total = __builtin_amdgcn_readfirstlane(ranges_total);
     most = __builtin_amdgcn_readfirstlane(most);
     const uint32_t Hkv = a.d.num_kv_heads, rows = a.num_seqs * Hkv, all = total * Hkv;
-    uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(least));
+    uint32_t range = max((all + a.groups - 1) / a.groups, static_cast<uint32_t>(kWindowLeast));
     range = (range + W - 1) / W * W;
     bool fill = ranges_total * Hkv <= static_cast<uint32_t>(a.groups);
     if (most > 0 && most * rows == all) {
         const uint32_t even = (all + kSparseCUs - 1) / kSparseCUs, whole = (rows + kSparseCUs - 1) / kSparseCUs * most;  // a CU's
-        if (whole <= even + 32 || 3 * whole < 4 * even) {
+        if (whole <= even + 24 || 3 * whole < 4 * even) {
             range = (rows + a.groups - 1) / a.groups * most;
             fill = false;
         }
     }
     if (fill) {
-        range = least;
-        at = ranges_at << a.least_log;
+        range = kWindowLeast;
+        at = ranges_at * kWindowLeast;
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         if (i >= per) break;
         const int r = threadIdx.x * per + i;
         if (r <= a.num_seqs) s_starts[r] = at;
-        at += fill ? ranges_of(raw[i]) << a.least_log : raw[i];
+        at += fill ? ranges_of(raw[i]) * kWindowLeast : raw[i];
     }
     __syncthreads();
     return range;

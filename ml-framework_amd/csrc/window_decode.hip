@@ -15,25 +15,21 @@ int64_t most_blocks(int32_t max_len, int32_t sink, int32_t window) {
 
 // A call's launches take at most kWindowSeqs sequences each, one after another over the same workspace.
 struct Plan {
-    int32_t seqs, groups, least_log;
+    int32_t seqs, groups;
     int64_t slots, entries;  // entries: with every row filled up to whole ranges
     bool merge;
 };
 
-// List entries of a range at least: two a wave, or one where that cuts no row into more than eight parts.
 Plan plan_of(const pa_config* cfg, int32_t num_seqs, int64_t blocks) {
-    const int32_t waves = pa::window_waves(cfg->head_dim), G = cfg->num_q_heads / cfg->num_kv_heads;
+    const int32_t G = cfg->num_q_heads / cfg->num_kv_heads;
     Plan p{};
     p.seqs = std::min(num_seqs, pa::kWindowSeqs);
-    static_assert(pa::window_waves(0) == 4, "a power of two");
-    p.least_log = blocks <= 8 * waves ? 2 : 3;
-    const int64_t least = int64_t{1} << p.least_log;
     const int64_t full = pa::window_decode_groups(cfg->head_dim, cfg->kv_dtype), rows = static_cast<int64_t>(p.seqs) * cfg->num_kv_heads;
-    p.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min(full, rows * ((blocks + least - 1) / least))));
+    const int64_t ranges = rows * ((blocks + pa::kWindowLeast - 1) / pa::kWindowLeast);
+    p.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min(full, ranges)));
     p.merge = p.groups > 1;
-    // (so that a workspace of the largest call serves every smaller one: slots of the smallest range, entries filled up to the largest)
-    p.slots = 2 * std::min(full, rows * ((blocks + waves - 1) / waves)) * G;
-    p.entries = rows * ((blocks + 2 * waves - 1) / (2 * waves) * (2 * waves));
+    p.slots = 2 * std::min(full, ranges) * G;
+    p.entries = ranges * pa::kWindowLeast;
     return p;
 }
 
@@ -130,7 +126,6 @@ pa_status pa_window_decode(pa_stream* stream, const pa_config* cfg, float* out, 
     a.total = reinterpret_cast<float2*>(ws + w.total);
     a.sink = sink_tokens;
     a.window = window;
-    a.least_log = p.least_log;
     a.mass_chunks = block_mass ? static_cast<int32_t>((blocks + 255) / 256) : 0;
     a.groups = p.groups;
     pa::StreamDevice dev(stream);

@@ -12,18 +12,23 @@ struct Plan {
     bool share;
     int32_t cols, per, splits;
 };
-// Waves share a set of columns, each with its own blocks, where workgroups of 128 columns would leave CUs idle; the keys are
-// cut over workgroups where that still does.
+// Waves share a set of columns, each with its own blocks, where a (sequence, KV head) has few or workgroups of 128 columns would leave CUs
+// half empty. Measured at (32, 8, 128) bf16, window 1024, shared / own: 32 sequences of 16 tokens 35 / 52 us, 20: 52 / 57, 32: 60 / 61, 64:
+// 113 / 84; 512 tokens of one sequence 29 / 45 (128 workgroups of own columns), of two 55 / 59, of four 105 / 83.
+// The keys are cut over workgroups up to one a CU, of 16 pairs of blocks at least, and up to two where that leaves 32: 4 sequences of 4 tokens
+// on 8192: 36 us in 8 parts of 32 pairs, 41 in 4 and in 16; on 2048: 18 us in 4 parts of 16, 21 in 2, 19 in 8; one chunk of 256 on 8192, 256
+// workgroups: 87 us in 2 parts, 105 whole.
 Plan plan_of(const pa_config* cfg, int32_t num_seqs, int32_t max_chunk_len, int64_t blocks) {
     Plan p{};
     const int64_t columns = static_cast<int64_t>(max_chunk_len) * (cfg->num_q_heads / cfg->num_kv_heads);
     const int64_t groups = static_cast<int64_t>(num_seqs) * cfg->num_kv_heads;
-    p.share = pa::window_shares(cfg->head_dim, cfg->kv_dtype) && (columns <= 64 || groups * ((columns + 127) / 128) < 256);
+    p.share = pa::window_shares(cfg->head_dim, cfg->kv_dtype) && (columns <= 96 || groups * ((columns + 127) / 128) <= 256);
     p.cols = p.share ? 32 : 128;
     p.per = static_cast<int32_t>((columns + p.cols - 1) / p.cols);
     const int64_t pairs = (blocks + 1) / 2, wgs = groups * p.per;
     p.splits = 1;
-    if (wgs > 0 && wgs < 256) p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(kSplitGroups / wgs, pairs / (p.share ? 16 : 4))));
+    const int64_t least = p.share ? 16 : 4;  // (four waves of a set of columns take the pairs in turn)
+    if (wgs > 0) p.splits = static_cast<int32_t>(std::max({int64_t{1}, std::min(256 / wgs, pairs / least), std::min(kSplitGroups / wgs, pairs / (2 * least))}));
     return p;
 }
 
