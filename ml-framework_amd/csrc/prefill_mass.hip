@@ -8,7 +8,7 @@
 // (K . Q^T as in window_prefill.h), which four waves with blocks of their own read from LDS: there a column's operands are formed once,
 // the next ones on their way from memory meanwhile. A workgroup has two (four) such sets of waves, which share out its (KV head, 32 columns)
 // in order; a wave adds up a block's weights over its heads and columns in registers, and the sets' sums are added at the end, so that
-// no timing enters. Keys are read once however many queries there are.
+// no timing enters. Few blocks: sets of one wave, six to eight of them, which share out the same two blocks' (KV head, 32 columns). Keys are read once however many queries there are.
 // What bounds it: 9 prompts of 2-8k tokens, 32 queries, bf16: 42 us, 17 of them the keys' bytes; 31 us for a workgroup alone on its
 // CU, 40 for two, and no more than that are there: each step is operands, eight products that wait for one another, exponentials and a
 // barrier in turn (1.4 us). Waves that hold 128 columns in registers instead and load them for themselves, 16 bytes of a row a lane,
@@ -64,34 +64,41 @@ __device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[
     }
 }
 
-constexpr int kSetWaves = 4;  // waves that share the columns' operands
+// Waves of a set, which share the columns' operands. few: one.
+__host__ __device__ constexpr int mass_waves(bool few) { return few ? 1 : 4; }
 
 // Whether two workgroups fit a CU: 128 registers a lane.
 __host__ __device__ constexpr bool mass_two(int d, int kv, bool q_f32) { return !q_f32 && kv != PA_DTYPE_FP32 && d <= 128; }
 // Sets of a workgroup: four where registers allow four waves a SIMD, but LDS (three parts of each column) only one workgroup a CU.
-__host__ __device__ constexpr int mass_sets(int d, int kv, bool q_f32) { return q_f32 && kv != PA_DTYPE_FP32 && d <= 128 ? 4 : 2; }
-__host__ __device__ constexpr int mass_threads(int d, int kv, bool q_f32) { return 64 * kSetWaves * mass_sets(d, kv, q_f32); }
+// few: what LDS holds, at most eight.
+__host__ __device__ constexpr int mass_sets(int d, int kv, bool q_f32, bool few) {
+    const int fit = 150 * 1024 / ((q_f32 ? 3 : 1) * d * 64);
+    return few ? fit < 8 ? fit : 8 : q_f32 && kv != PA_DTYPE_FP32 && d <= 128 ? 4 : 2;
+}
+__host__ __device__ constexpr int mass_threads(int d, int kv, bool q_f32, bool few) { return 64 * mass_waves(few) * mass_sets(d, kv, q_f32, few); }
+// Whether there is such a form: where LDS holds more sets than workgroups of many blocks have, and registers the keys' three parts.
+__host__ __device__ constexpr bool mass_has_few(int d, int kv, bool q_f32) { return d <= 128 || (kv != PA_DTYPE_FP32 && !q_f32); }
 
 // A barrier for what stands in LDS: loads from memory stay under way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int D, int KV, bool QF32>
-__global__ __launch_bounds__(mass_threads(D, KV, QF32), mass_two(D, KV, QF32) || mass_sets(D, KV, QF32) == 4 ? 4 : 2) void prefill_mass_kernel(const MassArgs a) {
+template <int D, int KV, bool QF32, bool FEW>
+__global__ __launch_bounds__(mass_threads(D, KV, QF32, FEW), !FEW && (mass_two(D, KV, QF32) || mass_sets(D, KV, QF32, FEW) == 4) ? 4 : 2) void prefill_mass_kernel(const MassArgs a) {
     constexpr bool I8 = KV == PA_DTYPE_INT8;
     constexpr int NP = KV == PA_DTYPE_FP32 ? 3 : 1, NQ = QF32 ? 3 : 1, NS = D / 16;
     constexpr int ELT = KV == PA_DTYPE_FP32 ? 4 : I8 ? 1 : 2, QKV = QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16;
-    constexpr int SETS = mass_sets(D, KV, QF32);
+    constexpr int SW = mass_waves(FEW), SETS = mass_sets(D, KV, QF32, FEW);
     constexpr int SET = NS * 64;                                     // 16-byte pieces of 32 columns' operands, of one part
-    constexpr int NB = 2 * SETS * NQ * SET * 16 <= (mass_two(D, KV, QF32) ? 64 : 128) * 1024 ? 2 : 1;  // buffers of a set
-    constexpr bool EARLY = !mass_two(D, KV, QF32) && SETS == 2 && (NP == 1 || D < 256);                       // the next head's keys loaded early: registers for it
-    constexpr int PER = (SET + 64 * kSetWaves - 1) / (64 * kSetWaves);  // pieces a thread brings
+    constexpr int NB = 2 * SETS * NQ * SET * 16 <= (!FEW && mass_two(D, KV, QF32) ? 64 : 128) * 1024 ? 2 : 1;  // buffers of a set
+    constexpr bool EARLY = !FEW && !mass_two(D, KV, QF32) && SETS == 2 && (NP == 1 || D < 256);                       // the next head's keys loaded early: registers for it
+    constexpr int PER = (SET + 64 * SW - 1) / (64 * SW);  // pieces a thread brings
     __shared__ uint4 s_q[SETS][NB][NQ][SET];
     __shared__ float s_lse[SETS][NB][32];
     __shared__ int s_at[SETS][NB][32];  // the columns' positions
-    __shared__ float s_sum[SETS][kSetWaves][2];
+    __shared__ float s_sum[SETS][SW][2];
     const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int set = wave / kSetWaves, tid = threadIdx.x % (64 * kSetWaves);
+    const int set = wave / SW, tid = threadIdx.x % (64 * SW);
     const int seq = blockIdx.y, Hkv = a.num_kv_heads, G = a.group, Hq = Hkv * G;
     const int q0 = a.q_start_loc[seq], Lc = a.q_start_loc[seq + 1] - q0;
     const int m = min(a.last, Lc);
@@ -101,11 +108,11 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32), mass_two(D, KV, QF32) ||
                                        static_cast<int64_t>(a.max_context_len)));
     const pa::WindowSpan span(P, Lc - m, Lc - 1, T, a.sink, a.window);
     const int entries = span.entries();
-    if (2 * kSetWaves * static_cast<int>(blockIdx.x) >= entries) return;
+    if (2 * SW * static_cast<int>(blockIdx.x) >= entries) return;
     const int32_t* table = a.block_tables + static_cast<int64_t>(seq) * a.max_blocks_per_seq;
 
     // this wave's blocks, the same ones in all sets; a wave past the last has none, but brings operands
-    const int e0 = 2 * (kSetWaves * static_cast<int>(blockIdx.x) + wave % kSetWaves);
+    const int e0 = 2 * (SW * static_cast<int>(blockIdx.x) + wave % SW);
     int lb[2], id[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -140,7 +147,7 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32), mass_two(D, KV, QF32) ||
     // Columns 32 chunk .. of KV head kvh: D / 8 threads bring a column, 16 (32) bytes of bf16 (fp32) each, so that a wave reads whole lines.
     // A lane reads piece 2 slab + half of column n: the pieces of a column lie at column ^ piece, so that the 16 threads that write them
     // at once meet 16 different 16-byte positions of a 256-byte line.
-    constexpr int PC = D / 8, STEP = 64 * kSetWaves / PC;  // pieces of a column, columns at a time
+    constexpr int PC = D / 8, STEP = 64 * SW / PC;  // pieces of a column, columns at a time
     struct Bring {
         RawKeys<QKV> x[PER];
         float lse;
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32), mass_two(D, KV, QF32) ||
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const float w = pa::wave_sum(sum[u]);
-        if (lane == 0) s_sum[set][wave % kSetWaves][u] = w;
+        if (lane == 0) s_sum[set][wave % SW][u] = w;
     }
     __syncthreads();
     if (set == 0 && lane < 2 && (lane ? lb[1] : lb[0]) >= 0) {
@@ -278,16 +285,32 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32), mass_two(D, KV, QF32) ||
 }
 
 template <int D>
-void launch(const MassArgs& a, int kv, bool q_f32, dim3 grid, hipStream_t s) {
-    const auto by_q = [&](auto k) {
+void launch(const MassArgs& a, int kv, bool q_f32, bool few, dim3 grid, hipStream_t s) {
+    const auto by_few = [&](auto k, auto q) {
         constexpr int KV = decltype(k)::value;
-        if (q_f32) prefill_mass_kernel<D, KV, true><<<grid, mass_threads(D, KV, true), 0, s>>>(a);
-        else prefill_mass_kernel<D, KV, false><<<grid, mass_threads(D, KV, false), 0, s>>>(a);
+        constexpr bool Q = decltype(q)::value;
+        if constexpr (mass_has_few(D, KV, Q)) {
+            if (few) {
+                prefill_mass_kernel<D, KV, Q, true><<<grid, mass_threads(D, KV, Q, true), 0, s>>>(a);
+                return;
+            }
+        }
+        prefill_mass_kernel<D, KV, Q, false><<<grid, mass_threads(D, KV, Q, false), 0, s>>>(a);
+    };
+    const auto by_q = [&](auto k) {
+        if (q_f32) by_few(k, std::true_type());
+        else by_few(k, std::false_type());
     };
     if (kv == PA_DTYPE_FP32) by_q(std::integral_constant<int, PA_DTYPE_FP32>());
     else if (kv == PA_DTYPE_BF16) by_q(std::integral_constant<int, PA_DTYPE_BF16>());
     else if constexpr (D >= 64) by_q(std::integral_constant<int, PA_DTYPE_INT8>());
 }
+
+// Workgroups of eight blocks up to which workgroups of two (so at most one a CU) share the work: every step's operands are then formed four times
+// as often, but a set has an eighth of the steps instead of half (fp32 queries: a sixth, a quarter). Measured at (32, 8, 128) bf16, eight / two: one
+// prompt of 500 tokens, 46 queries 35 / 16 us, of 8000 (63 workgroups of eight) 36 / 17, of 16000 38 / 33, of 30000 42 / 64; 16 of 500, 16 queries
+// 19 / 10; fp32 queries 46 / 32, 47 / 36, 51 / 70, 55 / 133; 23 / 18.
+constexpr int64_t kFewGroups = 64;
 
 }  // namespace
 
@@ -321,7 +344,9 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     if (window > 0)
         blocks = std::min(blocks, (static_cast<int64_t>(std::min(sink_tokens, max_context_len)) + 15) / 16 +
                                       (static_cast<int64_t>(window) + last_queries + 14) / 16 + 1);
-    const int64_t groups = (blocks + 2 * kSetWaves - 1) / (2 * kSetWaves);
+    const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
+    const bool few = mass_has_few(cfg->head_dim, cfg->kv_dtype, q_f32) && num_seqs * ((blocks + 7) / 8) <= kFewGroups;
+    const int64_t a_group = 2 * mass_waves(few), groups = (blocks + a_group - 1) / a_group;
     if (!pa::fits_grid(groups, 1024)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
     const MassArgs a{q,          lse,       q_start_loc,       prefix_lens,          k_cache,         k_scale,
                      block_tables, block_mass, cfg->num_kv_heads, cfg->num_q_heads / cfg->num_kv_heads, max_blocks_per_seq,
@@ -329,12 +354,11 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     pa::StreamDevice dev(stream);
     hipStream_t s = pa::native(stream);
     const dim3 grid(static_cast<uint32_t>(groups), num_seqs);
-    const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
     switch (cfg->head_dim) {
-        case 32: launch<32>(a, cfg->kv_dtype, q_f32, grid, s); break;
-        case 64: launch<64>(a, cfg->kv_dtype, q_f32, grid, s); break;
-        case 128: launch<128>(a, cfg->kv_dtype, q_f32, grid, s); break;
-        default: launch<256>(a, cfg->kv_dtype, q_f32, grid, s); break;
+        case 32: launch<32>(a, cfg->kv_dtype, q_f32, few, grid, s); break;
+        case 64: launch<64>(a, cfg->kv_dtype, q_f32, few, grid, s); break;
+        case 128: launch<128>(a, cfg->kv_dtype, q_f32, few, grid, s); break;
+        default: launch<256>(a, cfg->kv_dtype, q_f32, few, grid, s); break;
     }
     PA_HIP_CHECK(hipGetLastError());
     return pa::clear_error();

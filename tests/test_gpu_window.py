@@ -320,6 +320,28 @@ def test_short_chunks_on_long_contexts(kv, q, chunk, sink, window):
     close_mass(run_mass(p, g, qs, glse, lens, chunks, 40, sink, window, before), before, added, mass_tol)
 
 
+@pytest.mark.parametrize("kv,q", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 32), (8, 2, 64), (8, 1, 64), (32, 8, 128), (3, 1, 256), (20, 4, 128)])
+def test_masses_of_many_prompts(kv, q, hq, hkv, d):
+    """Calls that fill the chip, of long and short contexts, with block counts that no workgroup divides."""
+    if kv == INT8 and d == 32:
+        pytest.skip("int8 caches take head_dim 64 and more")
+    lens = [310, 17, 130, 0, 270] + [i % 23 + 1 for i in range(65)]
+    chunks = [min(t, (7 * i) % 37) for i, t in enumerate(lens)]
+    p = ref.Pool(395 + kv + 3 * q, lens, hq, hkv, d, kv, q)
+    g = gpu_pool(p)
+    rows, at = bref.chunk_rows(lens, chunks)
+    for sink, window, last in ((0, 0, 13), (4, 90, 2000)):
+        qs = p.queries(len(rows))
+        want, tol, lse, lse_tol, _, _ = bref.attend(p, qs, rows, at, sink, window, [lens[s] for s in rows])
+        got, glse = run_prefill(p, g, qs, lens, chunks, sink, window)
+        close(got, want, tol)
+        close(glse, lse, lse_tol)
+        before = masses(p)
+        close_mass(run_mass(p, g, qs, glse, lens, chunks, last, sink, window, before), before,
+                   *bref.prompt_mass(p, qs, glse, lens, chunks, last, sink, window))
+
+
 def test_max_chunk_len_bounds_what_is_computed():
     lens, chunks = [100, 50], [40, 6]
     p = ref.Pool(410, lens, 4, 2, 64)
