@@ -86,7 +86,7 @@ def test_evict_masses_of_every_kind():
         same(run_evict(nb, tables, lens, m, 2, 3, budget, refs), bref.evict(tables, lens, m, 2, 3, budget, refs))
 
 
-@pytest.mark.parametrize("blocks", [1024, 1025, 8192, 40000, 140000])
+@pytest.mark.parametrize("blocks", [1024, 1025, 8192, 16384, 40000, 140000])
 @pytest.mark.parametrize("with_mass", [True, False])
 def test_evict_long_rows(blocks, with_mass):
     rng = np.random.default_rng(520)
