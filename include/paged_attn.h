@@ -599,7 +599,8 @@ pa_status pa_window_prefill_workspace_size(const pa_config* cfg, int32_t num_seq
  *   the former are not computed.
  * A query that sees no token (its window lies past the table or max_context_len) gives zeros, and -Inf in lse. Any
  * kv_dtype, head_dim and ratio of heads; num_seqs * num_kv_heads at most 65535. Sums are in fp32. Products are exact,
- * but for parts below 2^-24 that are left out where both operands are fp32 (queries, probabilities, caches). out, q and caches 16-byte aligned. cfg->flags (masks) are not read. */
+ * but for at most 2^-22 of each, of either sign, where both operands are fp32 (queries, probabilities, caches). out, q
+ * and caches 16-byte aligned. cfg->flags (masks) are not read. */
 pa_status pa_window_prefill(pa_stream* stream, const pa_config* cfg, float* out, const void* q,
                             const int32_t* q_start_loc, const int32_t* prefix_lens, const void* k_cache,
                             const void* v_cache, const float* k_scale, const float* v_scale,
@@ -611,7 +612,7 @@ pa_status pa_window_prefill(pa_stream* stream, const pa_config* cfg, float* out,
  * and their heads,
  *   block_mass[s][b] += sum of exp(scale q.k - lse) over the visible tokens of block b, in a fixed order.
  * q, q_start_loc, prefix_lens, sink_tokens and window are those of the pa_window_prefill call that left lse; rows of
- * q and lse other than the last queries' are not read. Keys alone are read. num_seqs at most 65535,
+ * q and lse other than the last queries' are not read. Keys alone are read, products are that call's. num_seqs at most 65535,
  * num_q_heads / num_kv_heads at most 2^20, last_queries * num_q_heads below 2^30, max_context_len at most 10^9 where there is no
  * window; q and k_cache 16-byte aligned. */
 pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, const void* q, const float* lse,

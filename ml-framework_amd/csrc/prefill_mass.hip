@@ -51,11 +51,11 @@ __device__ __forceinline__ void load_raw(RawKeys<KV>& r, const char* at) {
         r.x = *reinterpret_cast<const uint2*>(at);
     }
 }
-template <int KV, int NP>
+template <int KV, int NP, bool NEAR>
 __device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[NP]) {
     if constexpr (KV == PA_DTYPE_FP32) {
         const float v[8] = {r.x[0], r.x[1], r.x[2], r.x[3], r.y[0], r.y[1], r.y[2], r.y[3]};
-        pa::bf16_planes<NP>(v, plane);
+        pa::bf16_planes<NP, NEAR>(v, plane);
     } else if constexpr (KV == PA_DTYPE_BF16) {
         plane[0] = r.x;
     } else {
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32, FEW), !FEW && (mass_two(D
         for (int j = 0; j < PER; j++) {
             if (STEP > 32 && tid >= 32 * PC) break;
             uint4 op[NQ];
-            raw_planes<QKV, NQ>(from.x[j], op);
+            raw_planes<QKV, NQ, NP == 3>(from.x[j], op);
 #pragma unroll
             for (int q = 0; q < NQ; q++) s_q[set][b][q][32 * piece + ((tid / PC + STEP * j) ^ (piece & 15))] = op[q];
         }
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32, FEW), !FEW && (mass_two(D
 #pragma unroll
                     for (int sl = 0; sl < NS; sl++) {
                         uint4 x[NP];
-                        raw_planes<KV, NP>(raw[sl], x);
+                        raw_planes<KV, NP, NQ == 3>(raw[sl], x);
 #pragma unroll
                         for (int p = 0; p < NP; p++) kop[p][sl] = x[p];
                     }

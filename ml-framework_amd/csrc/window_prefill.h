@@ -16,8 +16,8 @@
 // few, the waves share the columns and every one streams pairs of its own through a slot of its own, without a barrier: the next
 // pair's keys go out when this pair's have been read, its values likewise, and the waves' states meet at the end.
 // Results are as exact as fp32 sums of exact products: bf16 keys and values and int8 codes are one bf16 operand, fp32 values
-// (queries, probabilities, caches) the sum of three (8 bits each); products of parts below 2^-24 are left out. (With probabilities of two
-// rounded parts results are 2.5e-6 from 64 bits, so 0.4e-6.)
+// (queries, probabilities, caches) the sum of three (8 bits each); where both operands are such, at most 2^-22 of a product is left out
+// (bf16_planes). (With probabilities of two rounded parts results are 2.5e-6 from 64 bits, so 0.4e-6.)
 // What bounds it: few columns, memory (32 sequences, 3-5 tokens each over a window of 1024, (32, 8, 128) bf16: 32 us, 27 traced, 5.2 TB/s); many, the
 // matrix products and what is issued beside them in two waves a SIMD (8 x 512 tokens over that window 136 us, 2 x 4096 267 us: 0.9 and 1.0 PFLOP/s
 // counting the four products of exact probabilities, where a large matrix product reaches 1.26). Probabilities in two fp16 parts, values
@@ -60,8 +60,13 @@ __device__ __forceinline__ void bf16_split3(float x, float (&part)[3]) {
     part[1] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
     part[2] = r - part[1];
 }
-// Eight values as NP bf16 operands: one (values that are exact in bf16) or three.
-template <int NP>
+// Eight values as NP bf16 operands: one (values that are exact in bf16) or three, which sum to the value. Where both factors of a
+// product are in parts, those of parts 1 x 2, 2 x 1 and 2 x 2 are left out. For such (NEAR) the second part is rounded to the
+// nearest instead of cut off: the third is then at most 2^-16 of the value and of either sign, and what is left out at most 2^-22 of
+// the product (2 * 2^-7 * 2^-16), of either sign too. (Of parts cut off it was up to 2^-21 and always missing.)
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+template <int NP, bool NEAR>
 __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[NP]) {
     uint32_t w[NP][4];
 #pragma unroll
@@ -74,13 +79,18 @@ __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[
             bf16_split3(x[2 * e + 1], b);
 #pragma unroll
             for (int p = 0; p < NP; p++) w[p][e] = pack_bf16_trunc(a[p], b[p]);
+            if constexpr (NEAR) {
+                const float ra = x[2 * e] - a[0], rb = x[2 * e + 1] - b[0];
+                w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{ra, rb}), bf16x2_t));
+                w[2][e] = pack_bf16_trunc(ra - bf16_lo(w[1][e]), rb - bf16_hi(w[1][e]));
+            }
         }
     }
 #pragma unroll
     for (int p = 0; p < NP; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 // Elements i .. i + 7 of a cache or of the queries as NP bf16 operands (i a multiple of 8, the array 16-byte aligned).
-template <int KV, int NP>
+template <int KV, int NP, bool NEAR>
 __device__ __forceinline__ void load_planes(const void* base, int64_t i, uint4 (&plane)[NP]) {
     if constexpr (KV == PA_DTYPE_BF16) {
         static_assert(NP == 1, "bf16 is its own operand");
@@ -89,7 +99,7 @@ __device__ __forceinline__ void load_planes(const void* base, int64_t i, uint4 (
         const f32x4_t a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(base) + i);
         const f32x4_t b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(base) + i + 4);
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        bf16_planes<NP>(x, plane);
+        bf16_planes<NP, NEAR>(x, plane);
     } else {
         const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(base) + i);
         plane[0] = make_uint4(pack_i8pair(w.x, 0), pack_i8pair(w.x, 2), pack_i8pair(w.y, 0), pack_i8pair(w.y, 2));
@@ -282,7 +292,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
 #pragma unroll
     for (int s = 0; s < NS; s++) {
         uint4 x[NQ];
-        load_planes<QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16, NQ>(a.q, col.row * D + 16 * s + 8 * hf, x);
+        load_planes<QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16, NQ, F32>(a.q, col.row * D + 16 * s + 8 * hf, x);
 #pragma unroll
         for (int p = 0; p < NQ; p++) qv[p][s] = x[p];
     }
@@ -363,7 +373,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
         } else if constexpr (F32) {
             const f32x4_t x = __builtin_bit_cast(f32x4_t, tile[p0]), y = __builtin_bit_cast(f32x4_t, tile[p1]);
             const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            bf16_planes<NP>(v, op);
+            bf16_planes<NP, true>(v, op);
         } else {
             op[0] = tile[p0];
         }
@@ -440,7 +450,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
                 x[i] = s[8 * u + i];
                 if constexpr (I8) x[i] = x[i] == 0.0f ? 0.0f : x[i] * sc[0][2 + u];  // (whatever the scale of an unseen block is)
             }
-            bf16_planes<PP>(x, pop);
+            bf16_planes<PP, F32>(x, pop);
             uint4 vop[ND][NP];
             const uint4* const vt = slot + (2 * u + 1) * CH;
 #pragma unroll
