@@ -613,8 +613,8 @@ pa_status pa_window_prefill(pa_stream* stream, const pa_config* cfg, float* out,
  *   block_mass[s][b] += sum of exp(scale q.k - lse) over the visible tokens of block b, in a fixed order.
  * q, q_start_loc, prefix_lens, sink_tokens and window are those of the pa_window_prefill call that left lse; rows of
  * q and lse other than the last queries' are not read. Keys alone are read, products are that call's. num_seqs at most 65535,
- * num_q_heads / num_kv_heads at most 2^20, last_queries * num_q_heads below 2^30, max_context_len at most 10^9 where there is no
- * window; q and k_cache 16-byte aligned. */
+ * num_q_heads / num_kv_heads at most 2^20, last_queries * num_q_heads below 2^30, and where there is no window max_context_len
+ * up to 5 * 10^8 (some types take more); q and k_cache 16-byte aligned. */
 pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, const void* q, const float* lse,
                           const int32_t* q_start_loc, const int32_t* prefix_lens, const void* k_cache,
                           const float* k_scale, const int32_t* block_tables, int32_t num_seqs,

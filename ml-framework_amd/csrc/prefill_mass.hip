@@ -334,12 +334,6 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     if (cfg->num_q_heads / cfg->num_kv_heads > 1 << 20)
         return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": num_q_heads / num_kv_heads must be <= 2^20");
     if (num_seqs == 0 || last_queries == 0 || max_context_len == 0 || max_blocks_per_seq == 0) return pa::clear_error();
-    if (!q || !lse || !q_start_loc || !prefix_lens || !k_cache || !block_tables || !block_mass)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
-    if (cfg->kv_dtype == PA_DTYPE_INT8 && !k_scale)
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": int8 cache needs k_scale");
-    if (!pa::aligned16(k_cache) || !pa::aligned16(q))
-        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": q and k_cache must be 16-byte aligned");
     int64_t blocks = std::min<int64_t>((static_cast<int64_t>(max_context_len) + 15) / 16, max_blocks_per_seq);
     if (window > 0)
         blocks = std::min(blocks, (static_cast<int64_t>(std::min(sink_tokens, max_context_len)) + 15) / 16 +
@@ -347,7 +341,14 @@ extern "C" pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, co
     const bool q_f32 = cfg->q_dtype == PA_DTYPE_FP32;
     const bool few = mass_has_few(cfg->head_dim, cfg->kv_dtype, q_f32) && num_seqs * ((blocks + 7) / 8) <= kFewGroups;
     const int64_t a_group = 2 * mass_waves(few), groups = (blocks + a_group - 1) / a_group;
-    if (!pa::fits_grid(groups, 1024)) return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
+    if (!pa::fits_grid(groups, mass_threads(cfg->head_dim, cfg->kv_dtype, q_f32, few)))
+        return pa::set_error(PA_ERROR_UNSUPPORTED, std::string(f) + ": too many blocks for one call");
+    if (!q || !lse || !q_start_loc || !prefix_lens || !k_cache || !block_tables || !block_mass)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": null pointer");
+    if (cfg->kv_dtype == PA_DTYPE_INT8 && !k_scale)
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": int8 cache needs k_scale");
+    if (!pa::aligned16(k_cache) || !pa::aligned16(q))
+        return pa::set_error(PA_ERROR_INVALID_ARGUMENT, std::string(f) + ": q and k_cache must be 16-byte aligned");
     const MassArgs a{q,          lse,       q_start_loc,       prefix_lens,          k_cache,         k_scale,
                      block_tables, block_mass, cfg->num_kv_heads, cfg->num_q_heads / cfg->num_kv_heads, max_blocks_per_seq,
                      cfg->num_blocks, max_context_len, last_queries, sink_tokens, window, pa::resolve_scale(cfg)};
