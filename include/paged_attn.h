@@ -573,8 +573,10 @@ pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, 
  * non-zero: for calls that keep masses. */
 pa_status pa_window_decode_workspace_size(const pa_config* cfg, int32_t num_seqs, int32_t max_context_len,
                                           int32_t sink_tokens, int32_t window, int32_t with_mass, size_t* bytes);
-/* pa_paged_decode over the visible tokens: one query token per sequence, at position context_lens[s] - 1 (already
- * appended). Only blocks that hold a visible token are read, their table entries too.
+/* pa_paged_decode over the visible tokens: one query token per sequence, at the last position of its context (already
+ * appended). A context longer than max_context_len or max_blocks_per_seq * 16 counts as one of that length, its window too, as in
+ * pa_paged_decode (a chunk's queries keep their positions, see pa_window_prefill). Only blocks that hold a visible token
+ * are read, their table entries too.
  *   out: [num_seqs][num_q_heads][head_dim] fp32, q: [num_seqs][num_q_heads][head_dim] of q_dtype
  * block_mass null, or [num_seqs][max_blocks_per_seq]: every visible block's entry grows by the softmax weights of its
  * visible tokens, summed over the query heads in a fixed order (num_q_heads in all for each sequence).

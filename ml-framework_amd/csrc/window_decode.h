@@ -3,7 +3,8 @@
 // For sequence r of T cached tokens, KV head h and query head g of its group, over the tokens t with t < sink or
 // T - window <= t < T (window 0: all of them):
 //   s_t = scale * q_g . k_t,  out_g = sum_t exp(s_t - max s) v_t / sum_t exp(s_t - max s)
-// and, where masses are kept, mass[r][t / 16] += sum_h sum_g exp(s_t - max s) / sum_t' exp(s_t' - max s).
+// and, where masses are kept, mass[r][t / 16] += sum_h sum_g exp(s_t - max s) / sum_t' exp(s_t' - max s). T is cut at the table's width and
+// max_context_len first: the query stands at the end of what is read.
 //
 // A row is a (sequence, KV head); its list is the blocks that hold a visible token: those of the sinks, then those of
 // the window. The lists are laid end to end and cut into equal ranges, one for each workgroup of a chip full of them, as

@@ -158,3 +158,20 @@ def test_prompt_masses_of_contexts_past_the_bounds(kv, q, sink, window):
         for last in (2, 17, 64):
             added, mass_tol = bref.prompt_mass(p, qs, glse, long, chunks, last, sink, window, most)
             close_mass(run_mass(p, g, qs, glse, long, chunks, last, sink, window, before, most), before, added, mass_tol)
+
+
+@pytest.mark.parametrize("kv,q", [(BF16, BF16), (FP32, FP32)])
+def test_single_tokens_and_chunks_past_the_bounds(kv, q):
+    """A context that is longer than the host's bounds: for a single token it ends there, window and masses too; a chunk's token keeps its
+    position, and where its window lies past the bounds it sees nothing."""
+    lens, sink, window, most = [200, 45, 200], 0, 20, 50
+    p = ref.Pool(670, lens, 8, 2, 64, kv, q)
+    g, qs, before = gpu_pool(p), p.queries(3), masses(p)
+    out, tol, _, _, added, mass_tol = bref.attend(p, qs, range(3), [49, 44, 49], sink, window, [50, 45, 50])
+    for long in ([200, 45, 5000], [50, 45, 50]):
+        got, mass = run_decode(p, g, qs, long, sink, window, before, max_len=most)
+        close(got, out, tol)
+        close_mass(mass, before, added, mass_tol)
+    got, lse = run_prefill(p, g, qs, [200, 45, 5000], [1, 1, 1], sink, window, max_len=most)
+    close(got[1:2], out[1:2], tol[1:2])
+    assert (got[[0, 2]] == 0).all() and (lse[[0, 2]] == -np.inf).all()
