@@ -613,10 +613,12 @@ pa_status pa_window_prefill(pa_stream* stream, const pa_config* cfg, float* out,
 /* The masses of a prompt, before its first eviction: over the last `last_queries` tokens of every chunk (all of a shorter one)
  * and their heads,
  *   block_mass[s][b] += sum of exp(scale q.k - lse) over the visible tokens of block b, in a fixed order.
- * q, q_start_loc, prefix_lens, sink_tokens and window are those of the pa_window_prefill call that left lse; rows of
- * q and lse other than the last queries' are not read. Keys alone are read, products are that call's. num_seqs at most 65535,
- * num_q_heads / num_kv_heads at most 2^20, last_queries * num_q_heads below 2^30, and where there is no window max_context_len
- * up to 5 * 10^8 (some types take more); q and k_cache 16-byte aligned. */
+ * q, q_start_loc, prefix_lens, max_context_len, sink_tokens and window are those of the pa_window_prefill call that left lse,
+ * and no chunk may be longer than that call's max_chunk_len (the lse of tokens beyond it was never written, and weights by
+ * it would stay in the masses). Rows of q and lse other than the last queries' are not read. Keys alone are read,
+ * products are that call's. num_seqs at most 65535, num_q_heads / num_kv_heads at most 2^20, last_queries * num_q_heads
+ * below 2^30, and where there is no window max_context_len up to 5 * 10^8 (some types take more); q and k_cache 16-byte
+ * aligned. */
 pa_status pa_prefill_mass(pa_stream* stream, const pa_config* cfg, const void* q, const float* lse,
                           const int32_t* q_start_loc, const int32_t* prefix_lens, const void* k_cache,
                           const float* k_scale, const int32_t* block_tables, int32_t num_seqs,
