@@ -210,14 +210,23 @@ __device__ __forceinline__ uint32_t pack_bf16_trunc(float lo, float hi) {
 
 // fp32 -> bf16 bits rounded to nearest even, two at a time (gfx950's v_cvt_pk_bf16_f32).
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16_rne(float lo, float hi) {
-    const bf16x2_t v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
-    return __builtin_bit_cast(uint32_t, v);
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), bf16x2_t));
 }
 
 __device__ __forceinline__ uint32_t pack_i8pair(uint32_t w, int k) {
     // Codes k and k+1 of w as two bf16 (exact: |code| <= 128 needs 8 significant bits).
     return pack_bf16_trunc(pa::i8_at(w, k), pa::i8_at(w, k + 1));
+}
+
+// int8 codes k, k + 1 of w (k: 0 or 2) as two bf16, exactly; w with every byte's top bit flipped (code + 128): the byte is placed in
+// the fraction of 2^23, from which 2^23 + 128 is taken off.
+__device__ __forceinline__ uint32_t bf16_pair_of(uint32_t w, int k) {
+    const float base = 8388736.0f;  // 2^23 + 128
+    const float lo = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k)) - base;
+    const float hi = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k + 1)) - base;
+    return pack_bf16_trunc(lo, hi);
 }
 
 // Reductions across the 4 rows of 16 lanes with gfx950's v_permlane16/32_swap (VALU, no LDS):

@@ -60,7 +60,7 @@ __device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[
         plane[0] = r.x;
     } else {
         const uint32_t x = r.x.x ^ 0x80808080u, y = r.x.y ^ 0x80808080u;
-        plane[0] = make_uint4(pa::i8_pair(x, 0), pa::i8_pair(x, 2), pa::i8_pair(y, 0), pa::i8_pair(y, 2));
+        plane[0] = make_uint4(pa::bf16_pair_of(x, 0), pa::bf16_pair_of(x, 2), pa::bf16_pair_of(y, 0), pa::bf16_pair_of(y, 2));
     }
 }
 

@@ -106,13 +106,6 @@ __device__ __forceinline__ void sparse_load(const DecodeArgs& a, SparseBuf<D, KV
     }
 }
 
-// int8 codes k, k + 1 of w (of k: 0 or 2) as two bf16, exactly; w with every byte's top bit flipped (code + 128).
-__device__ __forceinline__ uint32_t bf16_pair_of(uint32_t w, int k) {
-    const float base = 8388736.0f;  // 2^23 + 128
-    const float lo = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k)) - base;
-    const float hi = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k + 1)) - base;
-    return pack_bf16_trunc(lo, hi);
-}
 // The PV operand of four tokens of one dim.
 __device__ __forceinline__ s16x4_t sparse_v_operand(const uint2& r) { return v_operand(r); }
 __device__ __forceinline__ s16x4_t sparse_v_operand(uint32_t r) {

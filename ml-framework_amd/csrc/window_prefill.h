@@ -64,8 +64,6 @@ __device__ __forceinline__ void bf16_split3(float x, float (&part)[3]) {
 // product are in parts, those of parts 1 x 2, 2 x 1 and 2 x 2 are left out. For such (NEAR) the second part is rounded to the
 // nearest instead of cut off: the third is then at most 2^-16 of the value and of either sign, and what is left out at most 2^-22 of
 // the product (2 * 2^-7 * 2^-16), of either sign too. (Of parts cut off it was up to 2^-21 and always missing.)
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 template <int NP, bool NEAR>
 __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[NP]) {
     uint32_t w[NP][4];
@@ -81,7 +79,7 @@ __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[
             for (int p = 0; p < NP; p++) w[p][e] = pack_bf16_trunc(a[p], b[p]);
             if constexpr (NEAR) {
                 const float ra = x[2 * e] - a[0], rb = x[2 * e + 1] - b[0];
-                w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{ra, rb}), bf16x2_t));
+                w[1][e] = pack_bf16_rne(ra, rb);
                 w[2][e] = pack_bf16_trunc(ra - bf16_lo(w[1][e]), rb - bf16_hi(w[1][e]));
             }
         }
@@ -89,20 +87,16 @@ __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[
 #pragma unroll
     for (int p = 0; p < NP; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
-// Elements i .. i + 7 of a cache or of the queries as NP bf16 operands (i a multiple of 8, the array 16-byte aligned).
-template <int KV, int NP, bool NEAR>
-__device__ __forceinline__ void load_planes(const void* base, int64_t i, uint4 (&plane)[NP]) {
-    if constexpr (KV == PA_DTYPE_BF16) {
-        static_assert(NP == 1, "bf16 is its own operand");
-        plane[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
-    } else if constexpr (KV == PA_DTYPE_FP32) {
-        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(base) + i);
-        const f32x4_t b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(base) + i + 4);
+// Elements i .. i + 7 of the queries as NP bf16 operands (i a multiple of 8, the array 16-byte aligned).
+template <int NP, bool NEAR>
+__device__ __forceinline__ void load_planes(const void* q, int64_t i, uint4 (&plane)[NP]) {
+    if constexpr (NP == 1) {
+        plane[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + i);
+    } else {
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(q) + i);
+        const f32x4_t b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(q) + i + 4);
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         bf16_planes<NP, NEAR>(x, plane);
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(base) + i);
-        plane[0] = make_uint4(pack_i8pair(w.x, 0), pack_i8pair(w.x, 2), pack_i8pair(w.y, 0), pack_i8pair(w.y, 2));
     }
 }
 __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, const f32x16_t& c) {
@@ -116,13 +110,6 @@ __device__ __forceinline__ float settled(float x) {
     float y = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xE4, 0xF, 0xF, true));  // quad_perm 0 1 2 3
     asm volatile("" : "+v"(y));
     return y;
-}
-// int8 codes k, k + 1 (k: 0 or 2) of w as two bf16, exactly; w with every byte's top bit flipped (code + 128): the byte is placed in
-// the fraction of 2^23, from which 2^23 + 128 is taken off.
-__device__ __forceinline__ uint32_t i8_pair(uint32_t w, int k) {
-    const float lo = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k)) - 8388736.0f;
-    const float hi = __uint_as_float(__builtin_amdgcn_perm(0x4b000000u, w, 0x07060500u + k + 1)) - 8388736.0f;
-    return pack_bf16_trunc(lo, hi);
 }
 // The other half of the wave's value joined with this lane's.
 __device__ __forceinline__ float halves_max(float x) {
@@ -292,7 +279,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
 #pragma unroll
     for (int s = 0; s < NS; s++) {
         uint4 x[NQ];
-        load_planes<QF32 ? PA_DTYPE_FP32 : PA_DTYPE_BF16, NQ, F32>(a.q, col.row * D + 16 * s + 8 * hf, x);
+        load_planes<NQ, F32>(a.q, col.row * D + 16 * s + 8 * hf, x);
 #pragma unroll
         for (int p = 0; p < NQ; p++) qv[p][s] = x[p];
     }
@@ -369,7 +356,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
         if constexpr (I8) {
             const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(tile + p0) + 8 * hf);
             const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
-            op[0] = make_uint4(i8_pair(x, 0), i8_pair(x, 2), i8_pair(y, 0), i8_pair(y, 2));
+            op[0] = make_uint4(bf16_pair_of(x, 0), bf16_pair_of(x, 2), bf16_pair_of(y, 0), bf16_pair_of(y, 2));
         } else if constexpr (F32) {
             const f32x4_t x = __builtin_bit_cast(f32x4_t, tile[p0]), y = __builtin_bit_cast(f32x4_t, tile[p1]);
             const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
