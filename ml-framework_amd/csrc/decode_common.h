@@ -229,6 +229,22 @@ __device__ __forceinline__ uint32_t bf16_pair_of(uint32_t w, int k) {
     return pack_bf16_trunc(lo, hi);
 }
 
+// hipcc (ROCm 7.2) counts too few waits where branches lie between a matrix instruction and the first read of its result and the
+// reading block can be reached on several ways: a product's last registers then lacked its last terms now and then (seen at 7 wait states of
+// 12). Two ways round it, both in the product's own block; tests/test_matrix_waits.py looks for places that need one.
+// The product's last register is moved: the move is waited for as it should be, and what is read after it is safe.
+__device__ __forceinline__ float settled(float x) {
+    float y = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xE4, 0xF, 0xF, true));  // quad_perm 0 1 2 3
+    asm volatile("" : "+v"(y));
+    return y;
+}
+// Behind many products, of which the compiler may choose any to be the last: N wait states pass that it does not count.
+template <int N>
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop %0" ::"n"(N - 1));
+}
+
 // Reductions across the 4 rows of 16 lanes with gfx950's v_permlane16/32_swap (VALU, no LDS):
 // each swap returns the pair {x[l], x[l ^ 16]} (resp. x[l ^ 32]) in some order.
 __device__ __forceinline__ float rows_max(float x) {

@@ -579,6 +579,7 @@ __device__ __forceinline__ void mfma_piece(const DecodeArgs& a, const Piece& g, 
 #pragma unroll
             for (int t = 0; t < NT; t++)
                 acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb, v_operand(vr[t]), acc[t], 0, 0, 0);
+            if constexpr (D == 256 && QF32 && SHARED) settle<2>();  // (read 7 wait states of 8 later otherwise)
         } else {
 #pragma unroll
             for (int u = 0; u < D / 32; u++) bf16_v_exchange(vr[2 * u], vr[2 * u + 1]);

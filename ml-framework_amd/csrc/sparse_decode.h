@@ -370,6 +370,7 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], b.v[t][i], acc[t], 0, 0, 0);
+                if constexpr (D == 256) settle<2>();  // (read 9 wait states of 10 later otherwise)
             } else {
                 if constexpr (KV == PA_DTYPE_INT8) {
                     const float vf = readlane_f(vs, j);

@@ -102,15 +102,6 @@ __device__ __forceinline__ void load_planes(const void* q, int64_t i, uint4 (&pl
 __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
-// A matrix product's last register, read where the product stands. hipcc (ROCm 7.2) counts too few waits where a branch, taken, lies
-// between a matrix instruction and the first read of its result: its last registers then lacked its last terms now and then
-// (seen at 7 wait states of 11). A move in the product's own block is waited for as it should be, and what is
-// read after it is safe.
-__device__ __forceinline__ float settled(float x) {
-    float y = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xE4, 0xF, 0xF, true));  // quad_perm 0 1 2 3
-    asm volatile("" : "+v"(y));
-    return y;
-}
 // The other half of the wave's value joined with this lane's.
 __device__ __forceinline__ float halves_max(float x) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
