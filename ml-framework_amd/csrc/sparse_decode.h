@@ -117,67 +117,28 @@ __device__ __forceinline__ s16x4_t sparse_v_operand(uint32_t r) {
 // less: bf16 47.7 us of two, 47.9 of three; int8 86.6, 88.5, 91.7 of four, 96.6 of six; one: 107.)
 constexpr int kSparseBuffers = 2;
 
-// PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
+// The Q operand of a row, whose head 0 starts at q0: column n holds head n % G (part n / G of it where Q is split).
 template <int D, int KV, bool QF32, int PASSES>
-__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSparseCUs * sparse_waves(D) / 4) void sparse_decode_kernel(const SparseArgs a) {
-    constexpr bool F32 = KV == PA_DTYPE_FP32;
-    constexpr int NSLAB = D / 32, NT = D / 16;
-    constexpr bool I8 = KV == PA_DTYPE_INT8;
-    constexpr int NI8 = I8 ? D / 64 : 1;           // QK slabs of 64 dims
-    constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
-    constexpr int PP = F32 ? 1 : PASSES;           // passes of P
-    constexpr int W = sparse_waves(D);
-    constexpr int NB = kSparseBuffers;
-    constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
-    __shared__ float s_m[W][16], s_l[W][16];
-    __shared__ float s_o[W][16][CH];
-    const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int Hkv = a.d.num_kv_heads, G = a.d.group;
-    const uint32_t budget = a.budget, all = static_cast<uint32_t>(a.rows) * budget;
-    uint32_t at_entry = blockIdx.x * static_cast<uint32_t>(a.range);
-    const uint32_t stop = min(all, at_entry + a.range);
-    for (; at_entry < stop;) {
-    const int row = static_cast<int>(at_entry / budget);
-    const int beg = static_cast<int>(at_entry - row * budget);
-    const int end = static_cast<int>(min(budget, beg + (stop - at_entry)));
-    at_entry += end - beg;
-    const int r = row / Hkv, kvh = row - r * Hkv;
-    // Lane l holds the wave's l-th block of a stretch of 64 W entries: its place in the sequence, its physical block. The
-    // first stretch's places come together with the sequence's number and length, its blocks while Q is split. No load is
-    // under a condition, which would make the compiler wait at its end: past the segment the last entry is read again,
-    // and where there is no table or place in it, the list.
-    const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
-    int lb = list[min(beg + wave + W * lane, end - 1)];
-    const int raw_len = a.d.context_lens[r], named = (a.query_seqs ? a.query_seqs : a.d.context_lens)[r];
-    const int seq = a.query_seqs ? named : r;
-    const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, raw_len) : 0;
-    const int nblk = T <= 0 ? 0 : (T + 15) / 16;
-    const int32_t* table = T > 0 ? a.d.block_tables + static_cast<int64_t>(seq) * a.d.max_blocks_per_seq : list;
-    int id;
-    bool listed;
-    auto find = [&](int e0) {
-        listed = (e0 + W * lane < end) & (lb >= 0) & (lb < nblk);
-        id = table[listed ? lb : 0];
-    };
-    find(beg + wave);
-
-    // Q operand: column n holds head n % G (part n / G of it where Q is split).
+struct SparseQuery {
+    static constexpr bool F32 = KV == PA_DTYPE_FP32, I8 = KV == PA_DTYPE_INT8;
+    static constexpr int NSLAB = D / 32;
+    static constexpr int NI8 = I8 ? D / 64 : 1;  // QK slabs of 64 dims
+    static constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
     bf16x8_t qb[F32 || I8 ? 1 : QP][F32 || I8 ? 1 : NSLAB];
     float qf[F32 ? D / 4 : 1];
     i32x4_t qd[I8 ? QP : 1][NI8];   // int8: digits of dims (D / 4) q4 + 16 t ..
     float place[I8 ? QP : 1];       // what a unit of this column's sums is worth
-    const float scale = a.d.scale * kLog2e;
-    {
-        const int64_t q0 = (static_cast<int64_t>(r) * Hkv * G + kvh * G + n % G) * D;
+    __device__ __forceinline__ SparseQuery(const DecodeArgs& a, int64_t q0, float scale, int q4, int n) {
+        const int G = a.group;
+        q0 = (q0 + n % G) * D;
         if constexpr (F32) {
 #pragma unroll
             for (int u = 0; u < D / 16; u++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int64_t i = q0 + 16 * u + 4 * q4 + j;
-                    qf[4 * u + j] = QF32 ? static_cast<const float*>(a.d.q)[i]
-                                         : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
+                    qf[4 * u + j] = QF32 ? static_cast<const float*>(a.q)[i]
+                                         : bf16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
                 }
         } else if constexpr (I8) {
             float x[D / 4];
@@ -185,7 +146,7 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
 #pragma unroll
             for (int e = 0; e < D / 4; e++) {
                 const int64_t i = q0 + (D / 4) * q4 + e;
-                x[e] = QF32 ? static_cast<const float*>(a.d.q)[i] : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
+                x[e] = QF32 ? static_cast<const float*>(a.q)[i] : bf16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
                 const float f = fabsf(x[e]);
                 top = fmaxf(top, f < INFINITY ? f : INFINITY);  // NaN too
             }
@@ -222,9 +183,9 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
             for (int s = 0; s < NSLAB; s++) {
                 const int64_t i = q0 + k_dim0<D, KV>(s, q4);
                 if constexpr (!QF32) {
-                    qb[0][s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d.q) + i));
+                    qb[0][s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + i));
                 } else {
-                    const f32x4_t* src = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.d.q) + i);
+                    const f32x4_t* src = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.q) + i);
                     const f32x4_t x0 = src[0], x1 = src[1];
 #pragma unroll
                     for (int p = 0; p < QP; p++) {
@@ -242,10 +203,172 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
             }
         }
     }
+    // The scores of a block's tokens (this lane: its four, for its column's head) in log2 units.
+    __device__ __forceinline__ void scores(const SparseBuf<D, KV>& b, float ks, int j, int G, float scale, float (&sc)[4]) const {
+        f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (F32) {
+#pragma unroll
+            for (int u = 0; u < D / 16; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.k[u][i], qf[4 * u + i], s, 0, 0, 0);
+        } else if constexpr (I8) {
+            const float k_scale = readlane_f(ks, j);
+            i32x4_t c[QP];
+#pragma unroll
+            for (int p = 0; p < QP; p++) {
+                c[p] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < NI8; t++)
+                    c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                        __builtin_bit_cast(i32x4_t, make_uint4(b.k[2 * t].x, b.k[2 * t].y, b.k[2 * t + 1].x, b.k[2 * t + 1].y)),
+                        qd[p][t], c[p], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int p = 0; p < QP; p++) s[i] = __builtin_fmaf(static_cast<float>(c[p][i]), place[p], s[i]);
+                s[i] *= k_scale;
+            }
+        } else {
+#pragma unroll
+            for (int sl = 0; sl < NSLAB; sl++) {
+                const bf16x8_t kop = k_operand(b.k[sl]);
+#pragma unroll
+                for (int p = 0; p < QP; p++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qb[p][sl], s, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float x = s[i];
+            if constexpr ((QF32 && !F32) || I8) {  // the partial scores of a head's parts
+                if (G <= 8) x = add_ror<8>(x);
+                if (G <= 4) x = add_ror<4>(x);
+                if (G <= 2) x = add_ror<2>(x);
+                if (G <= 1) x = add_ror<1>(x);
+            }
+            sc[i] = I8 ? x : x * scale;
+        }
+    }
+};
+
+// Values as P V takes them.
+template <int D, int KV>
+__device__ __forceinline__ void sparse_v_arrange(SparseBuf<D, KV>& b) {
+    if constexpr (KV == PA_DTYPE_INT8) {
+#pragma unroll
+        for (int u = 0; u < D / 64; u++) int8_v_transpose(b.v[4 * u], b.v[4 * u + 1], b.v[4 * u + 2], b.v[4 * u + 3]);
+    } else if constexpr (KV == PA_DTYPE_BF16) {
+#pragma unroll
+        for (int u = 0; u < D / 32; u++) bf16_v_exchange(b.v[2 * u], b.v[2 * u + 1]);
+    }
+}
+
+// A wave's running maxima, sums and outputs. (The waves' exchange at a segment's end stands in each kernel: shared as well, the int8
+// decodes took 1 to 2 % more.)
+template <int D, int KV, int PASSES>
+struct SparseState {
+    static constexpr bool F32 = KV == PA_DTYPE_FP32;
+    static constexpr int NT = D / 16;
+    static constexpr int PP = F32 ? 1 : PASSES;  // passes of P
     float m_run = -INFINITY, l_run = 0.0f;
     f32x4_t acc[NT];
+    __device__ __forceinline__ SparseState() {
 #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // The maximum follows a block's scores; what is subtracted from them.
+    __device__ __forceinline__ float follow(const float (&sc)[4], int q4) {
+        const float bm = rows_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+        const bool grow = bm > m_run + kSparseRescale || (m_run == -INFINITY && bm > -INFINITY);
+        if (__any(grow)) {
+            const float m_new = grow ? bm : m_run;
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+            l_run *= alpha;
+            m_run = m_new;
+            float ar[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * q4 + i, 64);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[t][i] *= ar[i];
+        }
+        return m_run == -INFINITY ? 0.0f : m_run;  // no score above -inf yet: P is zero
+    }
+    // O += P V
+    __device__ __forceinline__ void add(const float (&p)[4], const SparseBuf<D, KV>& b, int G, int n) {
+        if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], b.v[t][i], acc[t], 0, 0, 0);
+            if constexpr (D == 256) settle<2>();  // (read 9 wait states of 10 later otherwise)
+        } else {
+            s16x4_t pb[PP];
+#pragma unroll
+            for (int q = 0; q < PP; q++) {
+                const int part_n = PASSES == 1 ? n / G : q * (16 / G) + n / G;
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = part_n < 3 ? bf16_part(p[i], part_n) : 0.0f;
+                pb[q] = __builtin_bit_cast(s16x4_t, make_uint2(pack_bf16_trunc(x[0], x[1]), pack_bf16_trunc(x[2], x[3])));
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const s16x4_t vop = sparse_v_operand(b.v[t]);
+#pragma unroll
+                for (int q = 0; q < PP; q++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb[q], vop, acc[t], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
+template <int D, int KV, bool QF32, int PASSES>
+__global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSparseCUs * sparse_waves(D) / 4) void sparse_decode_kernel(const SparseArgs a) {
+    constexpr bool F32 = KV == PA_DTYPE_FP32;
+    constexpr int NT = D / 16;
+    constexpr int W = sparse_waves(D);
+    constexpr int NB = kSparseBuffers;
+    constexpr int CH = D < 64 ? D : 64;  // dims per exchange round
+    __shared__ float s_m[W][16], s_l[W][16];
+    __shared__ float s_o[W][16][CH];
+    const int lane = threadIdx.x & 63, q4 = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int Hkv = a.d.num_kv_heads, G = a.d.group;
+    const uint32_t budget = a.budget, all = static_cast<uint32_t>(a.rows) * budget;
+    uint32_t at_entry = blockIdx.x * static_cast<uint32_t>(a.range);
+    const uint32_t stop = min(all, at_entry + a.range);
+    for (; at_entry < stop;) {
+    const int row = static_cast<int>(at_entry / budget);
+    const int beg = static_cast<int>(at_entry - row * budget);
+    const int end = static_cast<int>(min(budget, beg + (stop - at_entry)));
+    at_entry += end - beg;
+    const int r = row / Hkv, kvh = row - r * Hkv;
+    // Lane l holds the wave's l-th block of a stretch of 64 W entries: its place in the sequence, its physical block. The
+    // first stretch's places come together with the sequence's number and length, its blocks while Q is split. No load is
+    // under a condition, which would make the compiler wait at its end: past the segment the last entry is read again,
+    // and where there is no table or place in it, the list.
+    const int32_t* list = a.selected + static_cast<int64_t>(row) * a.budget;
+    int lb = list[min(beg + wave + W * lane, end - 1)];
+    const int raw_len = a.d.context_lens[r], named = (a.query_seqs ? a.query_seqs : a.d.context_lens)[r];
+    const int seq = a.query_seqs ? named : r;
+    const int T = seq >= 0 && seq < a.num_seqs ? clamp_len(a.d, raw_len) : 0;
+    const int nblk = T <= 0 ? 0 : (T + 15) / 16;
+    const int32_t* table = T > 0 ? a.d.block_tables + static_cast<int64_t>(seq) * a.d.max_blocks_per_seq : list;
+    int id;
+    bool listed;
+    auto find = [&](int e0) {
+        listed = (e0 + W * lane < end) & (lb >= 0) & (lb < nblk);
+        id = table[listed ? lb : 0];
+    };
+    find(beg + wave);
+
+    const float scale = a.d.scale * kLog2e;
+    const SparseQuery<D, KV, QF32, PASSES> query(a.d, static_cast<int64_t>(r) * Hkv * G + kvh * G, scale, q4, n);
+    SparseState<D, KV, PASSES> state;
     bool any = false;
 
     for (int e0 = beg + wave; e0 < end;) {
@@ -272,60 +395,11 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
             sparse_load<D, KV>(a.d, b, j >= 0 ? __builtin_amdgcn_readlane(id, j) : -1, kvh);
         };
         auto compute = [&](SparseBuf<D, KV>& b, int j) {
-            f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (F32) {
-#pragma unroll
-                for (int u = 0; u < D / 16; u++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.k[u][i], qf[4 * u + i], s, 0, 0, 0);
-            } else if constexpr (I8) {
-                const float k_scale = readlane_f(ks, j);
-                i32x4_t c[QP];
-#pragma unroll
-                for (int p = 0; p < QP; p++) {
-                    c[p] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-                    for (int t = 0; t < NI8; t++)
-                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                            __builtin_bit_cast(i32x4_t, make_uint4(b.k[2 * t].x, b.k[2 * t].y, b.k[2 * t + 1].x, b.k[2 * t + 1].y)),
-                            qd[p][t], c[p], 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-#pragma unroll
-                    for (int p = 0; p < QP; p++) s[i] = __builtin_fmaf(static_cast<float>(c[p][i]), place[p], s[i]);
-                    s[i] *= k_scale;
-                }
-            } else {
-#pragma unroll
-                for (int sl = 0; sl < NSLAB; sl++) {
-                    const bf16x8_t kop = k_operand(b.k[sl]);
-#pragma unroll
-                    for (int p = 0; p < QP; p++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qb[p][sl], s, 0, 0, 0);
-                }
-            }
             float sc[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float x = s[i];
-                if constexpr ((QF32 && !F32) || I8) {  // the partial scores of a head's parts
-                    if (G <= 8) x = add_ror<8>(x);
-                    if (G <= 4) x = add_ror<4>(x);
-                    if (G <= 2) x = add_ror<2>(x);
-                    if (G <= 1) x = add_ror<1>(x);
-                }
-                sc[i] = I8 ? x : x * scale;
-            }
+            query.scores(b, ks, j, G, scale, sc);
             const int lbj = __builtin_amdgcn_readlane(lb, j);
             const int t0 = KV == PA_DTYPE_BF16 ? 4 * tok_group<KV>(q4) : 4 * q4;
-            if constexpr (KV == PA_DTYPE_INT8) {
-#pragma unroll
-                for (int u = 0; u < D / 64; u++) int8_v_transpose(b.v[4 * u], b.v[4 * u + 1], b.v[4 * u + 2], b.v[4 * u + 3]);
-            } else if constexpr (KV == PA_DTYPE_BF16) {
-#pragma unroll
-                for (int u = 0; u < D / 32; u++) bf16_v_exchange(b.v[2 * u], b.v[2 * u + 1]);
-            }
+            sparse_v_arrange<D, KV>(b);
             if (static_cast<int64_t>(lbj) * 16 + 16 > T) {  // the context ends inside the block
                 const int lim = T - lbj * 16 - t0;          // of this lane's four tokens
 #pragma unroll
@@ -342,57 +416,19 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
                     }
                 }
             }
-            const float bm = rows_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
-            const bool grow = bm > m_run + kSparseRescale || (m_run == -INFINITY && bm > -INFINITY);
-            if (__any(grow)) {
-                const float m_new = grow ? bm : m_run;
-                const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-                l_run *= alpha;
-                m_run = m_new;
-                float ar[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * q4 + i, 64);
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] *= ar[i];
-            }
-            const float m0 = m_run == -INFINITY ? 0.0f : m_run;  // no score above -inf yet: P is zero
+            const float m0 = state.follow(sc, q4);
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 p[i] = __builtin_amdgcn_exp2f(sc[i] - m0);
-                l_run += p[i];
+                state.l_run += p[i];
             }
-            if constexpr (F32) {
+            if constexpr (KV == PA_DTYPE_INT8) {
+                const float vf = readlane_f(vs, j);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], b.v[t][i], acc[t], 0, 0, 0);
-                if constexpr (D == 256) settle<2>();  // (read 9 wait states of 10 later otherwise)
-            } else {
-                if constexpr (KV == PA_DTYPE_INT8) {
-                    const float vf = readlane_f(vs, j);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) p[i] *= vf;
-                }
-                s16x4_t pb[PP];
-#pragma unroll
-                for (int q = 0; q < PP; q++) {
-                    const int part_n = PASSES == 1 ? n / G : q * (16 / G) + n / G;
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[i] = part_n < 3 ? bf16_part(p[i], part_n) : 0.0f;
-                    pb[q] = __builtin_bit_cast(s16x4_t, make_uint2(pack_bf16_trunc(x[0], x[1]), pack_bf16_trunc(x[2], x[3])));
-                }
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const s16x4_t vop = sparse_v_operand(b.v[t]);
-#pragma unroll
-                    for (int q = 0; q < PP; q++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb[q], vop, acc[t], 0, 0, 0);
-                }
+                for (int i = 0; i < 4; i++) p[i] *= vf;
             }
+            state.add(p, b, G, n);
         };
 #pragma unroll
         for (int i = 0; i < NB - 1; i++) load(buf[i], at[i]);
@@ -420,10 +456,10 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
     // where no score of the row is, its sum is 0 and the outcome 0 / 0. A NaN score leaves the sum NaN. (The exchange
     // with a branch per wave and its reads one by one took 8000 of 17000 cycles at 8 rows of 64 blocks: 12.1 us for
     // 10.8 with the merge.)
-    if (any && m_run == -INFINITY) m_run = -FLT_MAX;
-    const float l_tot = rows_sum(l_run);
+    if (any && state.m_run == -INFINITY) state.m_run = -FLT_MAX;
+    const float l_tot = rows_sum(state.l_run);
     if (q4 == 0) {
-        s_m[wave][n] = m_run;
+        s_m[wave][n] = state.m_run;
         s_l[wave][n] = l_tot;
     }
     constexpr int TT = CH / 16;                                             // tiles per round
@@ -434,7 +470,7 @@ __global__ __launch_bounds__(64 * sparse_waves(D), sparse_groups(D, KV) / kSpars
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = acc[c * TT + tt][i];
+            for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = state.acc[c * TT + tt][i];
         __syncthreads();
         for (int idx = threadIdx.x; idx < G * CH; idx += 64 * W) {
             const int g = idx / CH, d = idx % CH;

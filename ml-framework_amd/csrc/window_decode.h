@@ -138,15 +138,11 @@ __device__ __forceinline__ uint32_t window_starts(const WindowArgs& a, int32_t* 
 // PASSES: matrix passes of a split operand, 16 / G parts a pass (G <= 4: 1, 8: 2, 16: 3).
 template <int D, int KV, bool QF32, int PASSES>
 __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) / kSparseCUs * window_waves(D) / 4) void window_decode_kernel(const WindowArgs a) {
-    constexpr bool F32 = KV == PA_DTYPE_FP32;
-    constexpr int NSLAB = D / 32, NT = D / 16;
-    constexpr bool I8 = KV == PA_DTYPE_INT8;
-    constexpr int NI8 = I8 ? D / 64 : 1;           // QK slabs of 64 dims
-    constexpr int QP = I8 ? (PASSES == 3 ? 4 : PASSES) : QF32 && !F32 ? PASSES : 1;  // passes of Q
-    constexpr int PP = F32 ? 1 : PASSES;           // passes of P
+    constexpr bool F32 = KV == PA_DTYPE_FP32, I8 = KV == PA_DTYPE_INT8;
+    constexpr int NT = D / 16;
     constexpr int W = window_waves(D);
     constexpr int NB = kSparseBuffers;
-    constexpr int CH = D < 64 ? D : 64;            // dims per exchange round
+    constexpr int CH = D < 64 ? D : 64;  // dims per exchange round
     __shared__ float s_m[W][16], s_l[W][16];
     __shared__ float s_o[W][16][CH];
     __shared__ int32_t s_starts[kWindowSeqs + 1], s_lens[kWindowSeqs + 64 * W];
@@ -194,90 +190,9 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     int id = table[lb];
     bool listed = beg + wave + W * lane < end;
 
-    // Q operand: column n holds head n % G (part n / G of it where Q is split).
-    bf16x8_t qb[F32 || I8 ? 1 : QP][F32 || I8 ? 1 : NSLAB];
-    float qf[F32 ? D / 4 : 1];
-    i32x4_t qd[I8 ? QP : 1][NI8];   // int8: digits of dims (D / 4) q4 + 16 t ..
-    float place[I8 ? QP : 1];       // what a unit of this column's sums is worth
     const float scale = a.d.scale * kLog2e;
-    {
-        const int64_t q0 = (static_cast<int64_t>(r) * Hkv * G + kvh * G + n % G) * D;
-        if constexpr (F32) {
-#pragma unroll
-            for (int u = 0; u < D / 16; u++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int64_t i = q0 + 16 * u + 4 * q4 + j;
-                    qf[4 * u + j] = QF32 ? static_cast<const float*>(a.d.q)[i]
-                                         : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
-                }
-        } else if constexpr (I8) {
-            float x[D / 4];
-            float top = 0.0f;
-#pragma unroll
-            for (int e = 0; e < D / 4; e++) {
-                const int64_t i = q0 + (D / 4) * q4 + e;
-                x[e] = QF32 ? static_cast<const float*>(a.d.q)[i] : bf16_to_f32(static_cast<const uint16_t*>(a.d.q)[i]);
-                const float f = fabsf(x[e]);
-                top = fmaxf(top, f < INFINITY ? f : INFINITY);  // NaN too
-            }
-            top = rows_max(top);
-            const bool bad = !(top < INFINITY);
-            // |q| < 2^ex; below 2^-96 (nothing that fp32 sums would keep) all of it counts as zero
-            const int ex = max(bad ? 0 : __builtin_amdgcn_frexp_expf(top), -95);
-            int32_t z[D / 4];
-#pragma unroll
-            for (int e = 0; e < D / 4; e++)  // |z| <= 2^30, biased so that its lower three bytes are digits + 128
-                z[e] = (bad ? 0 : static_cast<int32_t>(__builtin_rintf(__builtin_amdgcn_ldexpf(x[e], 30 - ex)))) + 0x808080;
-#pragma unroll
-            for (int p = 0; p < QP; p++) {
-                const int j = QP == 1 ? n / G : p * (16 / G) + n / G;  // this column's digit
-                const int shift = 8 * min(j, 3);
-                const uint32_t flip = j < 3 ? 0x80808080u : 0u, keep = j < 4 ? 0xffffffffu : 0u;
-                place[p] = bad ? __builtin_nanf("") : j < 4 ? __builtin_amdgcn_ldexpf(scale, ex - 30 + 8 * j) : 0.0f;
-#pragma unroll
-                for (int t = 0; t < NI8; t++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        w[k] = 0;
-#pragma unroll
-                        for (int b = 0; b < 4; b++)
-                            w[k] |= (static_cast<uint32_t>(z[16 * t + 4 * k + b]) >> shift & 255u) << (8 * b);
-                        w[k] = (w[k] ^ flip) & keep;
-                    }
-                    qd[p][t] = __builtin_bit_cast(i32x4_t, make_uint4(w[0], w[1], w[2], w[3]));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < NSLAB; s++) {
-                const int64_t i = q0 + k_dim0<D, KV>(s, q4);
-                if constexpr (!QF32) {
-                    qb[0][s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d.q) + i));
-                } else {
-                    const f32x4_t* src = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.d.q) + i);
-                    const f32x4_t x0 = src[0], x1 = src[1];
-#pragma unroll
-                    for (int p = 0; p < QP; p++) {
-                        const int part_n = PASSES == 1 ? n / G : p * (16 / G) + n / G;
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float lo_v = bf16_part(e < 2 ? x0[2 * e] : x1[2 * e - 4], part_n);
-                            const float hi_v = bf16_part(e < 2 ? x0[2 * e + 1] : x1[2 * e - 3], part_n);
-                            w[e] = part_n < 3 ? pack_bf16_trunc(lo_v, hi_v) : 0;
-                        }
-                        qb[p][s] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-                    }
-                }
-            }
-        }
-    }
-    float m_run = -INFINITY, l_run = 0.0f;
-    f32x4_t acc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const SparseQuery<D, KV, QF32, PASSES> query(a.d, static_cast<int64_t>(r) * Hkv * G + kvh * G, scale, q4, n);
+    SparseState<D, KV, PASSES> state;
     bool any = false;
 
     for (int e0 = beg + wave; e0 < end;) {
@@ -299,60 +214,11 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
             sparse_load<D, KV>(a.d, b, j >= 0 ? __builtin_amdgcn_readlane(id, j) : -1, kvh);
         };
         auto compute = [&](SparseBuf<D, KV>& b, int j) {
-            f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (F32) {
-#pragma unroll
-                for (int u = 0; u < D / 16; u++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.k[u][i], qf[4 * u + i], s, 0, 0, 0);
-            } else if constexpr (I8) {
-                const float k_scale = readlane_f(ks, j);
-                i32x4_t c[QP];
-#pragma unroll
-                for (int p = 0; p < QP; p++) {
-                    c[p] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-                    for (int t = 0; t < NI8; t++)
-                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                            __builtin_bit_cast(i32x4_t, make_uint4(b.k[2 * t].x, b.k[2 * t].y, b.k[2 * t + 1].x, b.k[2 * t + 1].y)),
-                            qd[p][t], c[p], 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-#pragma unroll
-                    for (int p = 0; p < QP; p++) s[i] = __builtin_fmaf(static_cast<float>(c[p][i]), place[p], s[i]);
-                    s[i] *= k_scale;
-                }
-            } else {
-#pragma unroll
-                for (int sl = 0; sl < NSLAB; sl++) {
-                    const bf16x8_t kop = k_operand(b.k[sl]);
-#pragma unroll
-                    for (int p = 0; p < QP; p++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qb[p][sl], s, 0, 0, 0);
-                }
-            }
             float sc[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float x = s[i];
-                if constexpr ((QF32 && !F32) || I8) {  // the partial scores of a head's parts
-                    if (G <= 8) x = add_ror<8>(x);
-                    if (G <= 4) x = add_ror<4>(x);
-                    if (G <= 2) x = add_ror<2>(x);
-                    if (G <= 1) x = add_ror<1>(x);
-                }
-                sc[i] = I8 ? x : x * scale;
-            }
+            query.scores(b, ks, j, G, scale, sc);
             const int tok = __builtin_amdgcn_readlane(lb, j) * 16;  // the block's first token
             const int t0 = tok + (KV == PA_DTYPE_BF16 ? 4 * tok_group<KV>(q4) : 4 * q4);
-            if constexpr (I8) {
-#pragma unroll
-                for (int u = 0; u < D / 64; u++) int8_v_transpose(b.v[4 * u], b.v[4 * u + 1], b.v[4 * u + 2], b.v[4 * u + 3]);
-            } else if constexpr (!F32) {
-#pragma unroll
-                for (int u = 0; u < D / 32; u++) bf16_v_exchange(b.v[2 * u], b.v[2 * u + 1]);
-            }
+            sparse_v_arrange<D, KV>(b);
             if ((tok < lo && tok + 16 > sink) || tok + 16 > T) {  // not every token of the block is seen
                 bool seen[4];
 #pragma unroll
@@ -372,63 +238,26 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
                     }
                 }
             }
-            const float bm = rows_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
-            const bool grow = bm > m_run + kSparseRescale || (m_run == -INFINITY && bm > -INFINITY);
-            if (__any(grow)) {
-                const float m_new = grow ? bm : m_run;
-                const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-                l_run *= alpha;
-                m_run = m_new;
-                float ar[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * q4 + i, 64);
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] *= ar[i];
-            }
-            const float m0 = m_run == -INFINITY ? 0.0f : m_run;  // no score above -inf yet: P is zero
+            const float m0 = state.follow(sc, q4);
             float p[4], psum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 p[i] = __builtin_amdgcn_exp2f(sc[i] - m0);
                 psum += p[i];
             }
-            l_run += psum;
+            state.l_run += psum;
             if (a.parts) {
                 const float sum = rows_sum(psum);
                 if (lane < G)  // (no score above -inf: a maximum that makes nothing of the sum, which is 0 or NaN)
-                    a.parts[(static_cast<int64_t>(entry0) + e0 + W * j) * G + lane] = make_float2(m_run == -INFINITY ? -FLT_MAX : m_run, sum);
+                    a.parts[(static_cast<int64_t>(entry0) + e0 + W * j) * G + lane] = make_float2(state.m_run == -INFINITY ? -FLT_MAX : state.m_run, sum);
             }
-            if constexpr (F32) {
+            if constexpr (I8) {
+                const float vf = readlane_f(vs, j);
+                // (an unseen token's zero stays one whatever the block's scale is)
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[i], b.v[t][i], acc[t], 0, 0, 0);
-            } else {
-                if constexpr (I8) {
-                    const float vf = readlane_f(vs, j);
-                    // (an unseen token's zero stays one whatever the block's scale is)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) p[i] = p[i] == 0.0f ? 0.0f : p[i] * vf;
-                }
-                s16x4_t pb[PP];
-#pragma unroll
-                for (int q = 0; q < PP; q++) {
-                    const int part_n = PASSES == 1 ? n / G : q * (16 / G) + n / G;
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[i] = part_n < 3 ? bf16_part(p[i], part_n) : 0.0f;
-                    pb[q] = __builtin_bit_cast(s16x4_t, make_uint2(pack_bf16_trunc(x[0], x[1]), pack_bf16_trunc(x[2], x[3])));
-                }
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const s16x4_t vop = sparse_v_operand(b.v[t]);
-#pragma unroll
-                    for (int q = 0; q < PP; q++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pb[q], vop, acc[t], 0, 0, 0);
-                }
+                for (int i = 0; i < 4; i++) p[i] = p[i] == 0.0f ? 0.0f : p[i] * vf;
             }
+            state.add(p, b, G, n);
         };
 #pragma unroll
         for (int i = 0; i < NB - 1; i++) load(buf[i], at[i]);
@@ -455,10 +284,10 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
     // ---- the waves' states meet ----
     // A wave that saw blocks but no score above -inf is told from one that saw none by the lowest finite maximum:
     // where no score of the row is, its sum is 0 and the outcome 0 / 0. A NaN score leaves the sum NaN.
-    if (any && m_run == -INFINITY) m_run = -FLT_MAX;
-    const float l_tot = rows_sum(l_run);
+    if (any && state.m_run == -INFINITY) state.m_run = -FLT_MAX;
+    const float l_tot = rows_sum(state.l_run);
     if (q4 == 0) {
-        s_m[wave][n] = m_run;
+        s_m[wave][n] = state.m_run;
         s_l[wave][n] = l_tot;
     }
     constexpr int TT = CH / 16;                                             // tiles per round
@@ -469,7 +298,7 @@ __global__ __launch_bounds__(64 * window_waves(D), window_decode_groups(D, KV) /
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = acc[c * TT + tt][i];
+            for (int i = 0; i < 4; i++) s_o[wave][4 * q4 + i][16 * tt + n] = state.acc[c * TT + tt][i];
         __syncthreads();
         for (int idx = threadIdx.x; idx < G * CH; idx += 64 * W) {
             const int g = idx / CH, d = idx % CH;
