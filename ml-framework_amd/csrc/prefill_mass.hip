@@ -55,7 +55,8 @@ template <int KV, int NP, bool NEAR>
 __device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[NP]) {
     if constexpr (KV == PA_DTYPE_FP32) {
         const float v[8] = {r.x[0], r.x[1], r.x[2], r.x[3], r.y[0], r.y[1], r.y[2], r.y[3]};
-        pa::bf16_planes<NP, NEAR>(v, plane);
+        if constexpr (NEAR) pa::bf16_planes_near<true>(v, plane);  // (fp32 keys under fp32 queries)
+        else pa::bf16_planes<NP>(v, plane);
     } else if constexpr (KV == PA_DTYPE_BF16) {
         plane[0] = r.x;
     } else {
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(mass_threads(D, KV, QF32, FEW), !FEW && (mass_two(D
         for (int j = 0; j < PER; j++) {
             if (STEP > 32 && tid >= 32 * PC) break;
             uint4 op[NQ];
-            raw_planes<QKV, NQ, NP == 3>(from.x[j], op);
+            raw_planes<QKV, NQ, false>(from.x[j], op);
 #pragma unroll
             for (int q = 0; q < NQ; q++) s_q[set][b][q][32 * piece + ((tid / PC + STEP * j) ^ (piece & 15))] = op[q];
         }

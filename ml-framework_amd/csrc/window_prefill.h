@@ -17,7 +17,7 @@
 // pair's keys go out when this pair's have been read, its values likewise, and the waves' states meet at the end.
 // Results are as exact as fp32 sums of exact products: bf16 keys and values and int8 codes are one bf16 operand, fp32 values
 // (queries, probabilities, caches) the sum of three (8 bits each); where both operands are such, at most 2^-22 of a product is left out
-// (bf16_planes). (With probabilities of two rounded parts results are 2.5e-6 from 64 bits, so 0.4e-6.)
+// (bf16_planes_near). (With probabilities of two rounded parts results are 2.5e-6 from 64 bits, so 0.4e-6.)
 // What bounds it: few columns, memory (32 sequences, 3-5 tokens each over a window of 1024, (32, 8, 128) bf16: 32 us, 27 traced, 5.2 TB/s); many, the
 // matrix products and what is issued beside them in two waves a SIMD (8 x 512 tokens over that window 136 us, 2 x 4096 267 us: 0.9 and 1.0 PFLOP/s
 // counting the four products of exact probabilities, where a large matrix product reaches 1.26). Probabilities in two fp16 parts, values
@@ -60,11 +60,8 @@ __device__ __forceinline__ void bf16_split3(float x, float (&part)[3]) {
     part[1] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
     part[2] = r - part[1];
 }
-// Eight values as NP bf16 operands: one (values that are exact in bf16) or three, which sum to the value. Where both factors of a
-// product are in parts, those of parts 1 x 2, 2 x 1 and 2 x 2 are left out. For such (NEAR) the second part is rounded to the
-// nearest instead of cut off: the third is then at most 2^-16 of the value and of either sign, and what is left out at most 2^-22 of
-// the product (2 * 2^-7 * 2^-16), of either sign too. (Of parts cut off it was up to 2^-21 and always missing.)
-template <int NP, bool NEAR>
+// Eight values as NP bf16 operands: one (values that are exact in bf16) or three, which sum to the value.
+template <int NP>
 __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[NP]) {
     uint32_t w[NP][4];
 #pragma unroll
@@ -77,17 +74,38 @@ __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[
             bf16_split3(x[2 * e + 1], b);
 #pragma unroll
             for (int p = 0; p < NP; p++) w[p][e] = pack_bf16_trunc(a[p], b[p]);
-            if constexpr (NEAR) {
-                const float ra = x[2 * e] - a[0], rb = x[2 * e + 1] - b[0];
-                asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w[1][e]) : "v"(ra), "v"(rb));  // (as a conversion in C++ prompts' masses took 1 to 10 % more)
-                w[2][e] = pack_bf16_trunc(ra - bf16_lo(w[1][e]), rb - bf16_hi(w[1][e]));
-            }
         }
     }
 #pragma unroll
     for (int p = 0; p < NP; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
-// Elements i .. i + 7 of the queries as NP bf16 operands (i a multiple of 8, the array 16-byte aligned).
+// v_cvt_pk_bf16_f32, two values rounded to the nearest. (As conversions in C++ prompts' masses took 1 to 10 % more.)
+__device__ __forceinline__ uint32_t pack_bf16_near(float lo, float hi) {
+    uint32_t w;
+    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w) : "v"(lo), "v"(hi));
+    return w;
+}
+// Three operands whose first and second are rounded to the nearest instead of cut off, for one factor of products that have both
+// in parts, where those of parts 1 x 2, 2 x 1 and 2 x 2 are left out. Of parts that are all cut off this is up to 2^-21 of a product (2 * 2^-7 *
+// 2^-15), and always missing. Rounded parts are at most 2^-8 (the second) and 2^-17 (the third) of the value and of either sign, so it is
+// less than 2^-22 (2^-8 * 2^-15 + 2^-17 * 2^-7), of either sign. The other factor stays cut off: the one that is split more often.
+// LARGE: values that rounding would make infinite too.
+template <bool LARGE>
+__device__ __forceinline__ void bf16_planes_near(const float (&x)[8], uint4 (&plane)[3]) {
+    const float most = __uint_as_float(0x7f7f0000u);  // the largest of bf16
+    uint32_t w[3][4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float a = x[2 * e], b = x[2 * e + 1];
+        w[0][e] = LARGE ? pack_bf16_near(fminf(fmaxf(a, -most), most), fminf(fmaxf(b, -most), most)) : pack_bf16_near(a, b);
+        const float ra = a - bf16_lo(w[0][e]), rb = b - bf16_hi(w[0][e]);
+        w[1][e] = pack_bf16_near(ra, rb);
+        w[2][e] = pack_bf16_trunc(ra - bf16_lo(w[1][e]), rb - bf16_hi(w[1][e]));
+    }
+#pragma unroll
+    for (int p = 0; p < 3; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+// Elements i .. i + 7 of the queries as NP bf16 operands (i a multiple of 8, the array 16-byte aligned). NEAR: of products with fp32 keys.
 template <int NP, bool NEAR>
 __device__ __forceinline__ void load_planes(const void* q, int64_t i, uint4 (&plane)[NP]) {
     if constexpr (NP == 1) {
@@ -96,7 +114,8 @@ __device__ __forceinline__ void load_planes(const void* q, int64_t i, uint4 (&pl
         const f32x4_t a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(q) + i);
         const f32x4_t b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(q) + i + 4);
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        bf16_planes<NP, NEAR>(x, plane);
+        if constexpr (NEAR) bf16_planes_near<true>(x, plane);
+        else bf16_planes<NP>(x, plane);
     }
 }
 __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, const f32x16_t& c) {
@@ -351,7 +370,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
         } else if constexpr (F32) {
             const f32x4_t x = __builtin_bit_cast(f32x4_t, tile[p0]), y = __builtin_bit_cast(f32x4_t, tile[p1]);
             const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            bf16_planes<NP, true>(v, op);
+            bf16_planes<NP>(v, op);
         } else {
             op[0] = tile[p0];
         }
@@ -428,7 +447,8 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
                 x[i] = s[8 * u + i];
                 if constexpr (I8) x[i] = x[i] == 0.0f ? 0.0f : x[i] * sc[0][2 + u];  // (whatever the scale of an unseen block is)
             }
-            bf16_planes<PP, F32>(x, pop);
+            if constexpr (F32) bf16_planes_near<false>(x, pop);
+            else bf16_planes<PP>(x, pop);
             uint4 vop[ND][NP];
             const uint4* const vt = slot + (2 * u + 1) * CH;
 #pragma unroll

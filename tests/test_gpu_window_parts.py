@@ -1,5 +1,5 @@
 """What fp32 operands in bf16 parts leave out of a product, in the attention of chunks and the masses of prompts over fp32 caches with fp32
-queries: at most 2^-22 of it, and nothing that these operands would show."""
+queries: less than 2^-22 of it."""
 import numpy as np
 import pytest
 
@@ -10,7 +10,8 @@ from test_gpu_window import gpu_pool, run_mass, run_prefill
 pytestmark = pytest.mark.gpu
 
 # Just below a multiple of 2^-7 (2^-8, 2^-9) above 1: parts that are cut off leave two full lower ones, of whose products 2^-21 (2^-23,
-# 2^-25) would be missing; rounded to the nearest the second is a power of two and the third -2^-23.
+# 2^-25) would be missing. With one factor's parts rounded (1 + 2^-7, -2^-23, 0 for the first, 1, 2^-8, -2^-23 for the second, and so on)
+# what is left out is at most 2^-8 (2^-15 - 2^-23) + 2^-23 2^-7, less than 2^-23 + 2^-29 of the product.
 LOW = [1 + 2.0 ** -7 - 2.0 ** -23, 1 + 2.0 ** -8 - 2.0 ** -23, 1 + 2.0 ** -9 - 2.0 ** -23, 1.5 + 2.0 ** -7 - 2.0 ** -23]
 PAIRS = [(sx * x, y) for x in LOW for y in LOW for sx in (1, -1)]
 
@@ -31,20 +32,21 @@ def pool(d, at, grow):
 @pytest.mark.parametrize("d,at", [(32, 0), (64, 21), (128, 127), (256, 200)])
 @pytest.mark.parametrize("bound", [1, 20000])
 def test_scores_of_chunks(d, at, bound):
-    """One token's lse is its score. Its products' sum is exact here but for what is left out, 2^-28 at most; in log2 units (the scale times log2 e
-    is 1, off by 2^-24 at most) and back it is rounded three times. (bound: waves that share columns, that own them.)"""
+    """One token's lse is its score. Off it is by what is left out of its product (2 2^-24, see LOW), by the additions of the parts' products,
+    of which the last three have bits below 2^-23 (the second parts', the third ones' of either factor), and by the way back from log2 units
+    (the scale times log2 e is 1): 6 2^-24. (bound: waves that share columns, that own them.)"""
     p, qs = pool(d, at, 1)
     n = len(PAIRS)
     _, lse = run_prefill(p, gpu_pool(p), qs, [1] * n, [1] * n, 0, 0, max_chunk=bound)
     want = np.array([p.cfg.scale * x * y for x, y in PAIRS])
     off = np.abs(lse[:, 0] - want) / np.abs(want)
-    assert off.max() <= (4 + 2.0 ** -4) * bref.EPS, f"off by {off.max() / bref.EPS:.2f} 2^-24"
+    assert off.max() <= (6 + 2.0 ** -4) * bref.EPS, f"off by {off.max() / bref.EPS:.2f} 2^-24"
 
 
 @pytest.mark.parametrize("d,at", [(32, 0), (64, 21), (128, 127), (256, 200)])
 def test_masses_of_prompts(d, at):
-    """Scores of 2^5 times the products: exp makes what they are off by relative. The given logarithm is multiplied by a rounded log2 e and
-    rounded again (1.5 2^-24 of its size in log2 units); the difference, exp2 and the sum add 4 2^-24."""
+    """Scores of 2^5 times the products, which are off by 5 2^-24 of their size (as above); exp makes that relative. The given logarithm is
+    multiplied by a rounded log2 e and rounded again (1.5 2^-24 of its size in log2 units); the difference, exp2 and the sum add 4 2^-24."""
     p, qs = pool(d, at, 32)
     n = len(PAIRS)
     score = np.array([p.cfg.scale * 32 * x * y for x, y in PAIRS])
@@ -53,5 +55,5 @@ def test_masses_of_prompts(d, at):
     got = run_mass(p, gpu_pool(p), qs, lse, [1] * n, [1] * n, 1, 0, 0, zero)[:, 0]
     want = np.exp(score - lse[:, 0].astype(np.float64))
     rel = np.abs(got - want) / want
-    tol = (np.abs(score) * 1.5 + 4) * bref.EPS
+    tol = (np.abs(score) * (1.5 + 5) + 4) * bref.EPS
     assert (rel <= tol).all(), f"off by {(rel / bref.EPS).max():.1f} 2^-24"
