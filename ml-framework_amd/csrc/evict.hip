@@ -9,7 +9,8 @@
 // Traffic is 16 bytes a block; a row's chain of loads, passes and barriers is what it costs, so rows of up to 16384 blocks
 // are read once into registers, a thread every 1024th block, and what stays is numbered by the waves' ballots of all of them at once
 // (64 rows of 262 blocks 5.7 us; counting every block's rank among the others instead, from LDS, 8.8). Longer rows are bound by one CU's
-// scattered writes and atomics (32 rows of 2-8k blocks 25 us, 12 of them with the reference counts; with registers for 16k blocks 29.5).
+// scattered writes and atomics (32 rows of 2-8k blocks 25 us, 12 of them with the reference counts; with registers for 16k blocks 29.5), and
+// rows whose masses are all equal by the one counter that they meet in (16 us more there).
 #include <algorithm>
 #include <string>
 

@@ -9,6 +9,7 @@ import pytest
 
 import bounded_ref as bref
 import longctx_ref as ref
+import paged_attention as pa
 from test_gpu_window import BF16, FP32, I32, INT8, TYPES, close, close_mass, gpu_pool, masses, run_decode, run_mass, run_prefill
 
 pytestmark = pytest.mark.gpu
@@ -175,3 +176,35 @@ def test_single_tokens_and_chunks_past_the_bounds(kv, q):
     got, lse = run_prefill(p, g, qs, [200, 45, 5000], [1, 1, 1], sink, window, max_len=most)
     close(got[1:2], out[1:2], tol[1:2])
     assert (got[[0, 2]] == 0).all() and (lse[[0, 2]] == -np.inf).all()
+
+
+@pytest.mark.parametrize("kv,q", [(BF16, BF16), (INT8, FP32)])
+def test_masses_by_the_last_tokens_of_prompts_alone(kv, q):
+    """Prompts attended to by the chunks' other kernel, their last tokens once more for the logarithms that their masses need."""
+    import torch
+    from helpers import check_close, empty_gpu, to_gpu, to_np, tol_for
+    lens, last = [700, 90, 20], 32
+    p = ref.Pool(680, lens, 8, 2, 64, kv, q)
+    g = gpu_pool(p)
+    whole = p.queries(sum(lens))
+    start = np.concatenate([[0], np.cumsum(lens)]).astype(I32)
+    out = empty_gpu(whole.shape, np.float32)
+    pa.chunked_prefill(None, p.cfg, out, to_gpu(whole), to_gpu(start), to_gpu(np.zeros(3, I32)), g["k"], g["v"], g["stats"][0], g["stats"][1],
+                       g["tables"], 3, p.width, max(lens))
+    torch.cuda.synchronize()
+    chunks = [min(last, t) for t in lens]
+    tail = np.concatenate([np.arange(start[s + 1] - n, start[s + 1]) for s, n in enumerate(chunks)])
+    rows, at = bref.chunk_rows(lens, chunks)
+    want, tol, lse, lse_tol, _, _ = bref.attend(p, whole[tail], rows, at, 0, 0, [lens[s] for s in rows])
+    check_close(to_np(out)[tail], want, **tol_for(kv), what="chunked prefill")
+    again, glse = run_prefill(p, g, whole[tail], lens, chunks, 0, 0)
+    close(again, want, tol)
+    close(glse, lse, lse_tol)
+    before = masses(p)
+    added, mass_tol = bref.prompt_mass(p, whole[tail], glse, lens, chunks, last, 0, 0)
+    got = run_mass(p, g, whole[tail], glse, lens, chunks, last, 0, 0, before)
+    close_mass(got, before, added, mass_tol)
+    # a row's weights are the heads of its last tokens, by their own logarithms
+    total = (got.astype(np.float64) - before).sum(1)
+    slack = 2 * bref.EPS * got.sum(1) + mass_tol.sum(1) + added.sum(1) * lse_tol.max()
+    assert (np.abs(total - 8 * np.array(chunks)) <= slack).all()
