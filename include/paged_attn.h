@@ -566,7 +566,8 @@ pa_status pa_copy_pages(pa_stream* stream, const pa_config* cfg, void* k_cache, 
  * tokens; NaN, Inf) does not matter to it. Queries that are not finite, NaN keys, and keys that make a score +Inf give outputs (and
  * masses) that are not finite, and so do values that are not, in their channel. A score of -Inf counts nothing beside
  * finite ones (fp32 queries of bf16 caches and fp32 caches, whose products are formed in parts: it may be NaN); a query with no other
- * gives NaN. int8 caches: scales must be finite. None of these calls allocates or synchronises; all may be captured
+ * gives NaN. int8 caches: scales must be finite. Values are added up before the sum is divided by the softmax's, so beyond 2^116 /
+ * (tokens seen) they may overflow. None of these calls allocates or synchronises; all may be captured
  * into a graph. Calls that share a workspace or masses must not overlap. */
 
 /* Bytes of workspace of pa_window_decode for up to num_seqs sequences of up to max_context_len tokens (8-byte aligned); with_mass
