@@ -80,10 +80,12 @@ __device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[
 #pragma unroll
     for (int p = 0; p < NP; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
-// v_cvt_pk_bf16_f32, two values rounded to the nearest. (As conversions in C++ prompts' masses took 1 to 10 % more.)
+// Two values rounded to the nearest in one conversion. (The empty asm keeps the conversions where they are written: prompts' masses of
+// (32, 8, 128) 122 us for 166. The instruction itself in inline asm would read what v_exp_f32 has only just formed: hipcc sees to no wait there.)
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16_near(float lo, float hi) {
-    uint32_t w;
-    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w) : "v"(lo), "v"(hi));
+    uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), bf16x2_t));
+    asm("" : "+v"(w));
     return w;
 }
 // Three operands whose first and second are rounded to the nearest instead of cut off, for one factor of products that have both

@@ -57,3 +57,19 @@ def test_masses_of_prompts(d, at):
     rel = np.abs(got - want) / want
     tol = (np.abs(score) * (1.5 + 5) + 4) * bref.EPS
     assert (rel <= tol).all(), f"off by {(rel / bref.EPS).max():.1f} 2^-24"
+
+
+@pytest.mark.parametrize("q", [0, 1])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("bound", [40, 9000])
+def test_queries_that_see_one_token_give_its_value(q, d, bound):
+    """A window of one token: its weight p is 1 but for the rounding of its score, and out = p v / p: the six products of their parts are
+    added up, divided and multiplied, 2^-24 each. (A part that is lost would show as 2^-8 or 2^-16.)"""
+    lens, chunks = [200, 70, 33, 7], [40, 40, 33, 7]
+    p = ref.Pool(810 + d, lens, 4, 2, d, 0, q)
+    rows, at = bref.chunk_rows(lens, chunks)
+    got, _ = run_prefill(p, gpu_pool(p), p.queries(len(rows)), lens, chunks, 0, 1, max_chunk=bound)
+    want = np.stack([p.v[p.tables[s, t // 16], :, :, t % 16] for s, t in zip(rows, at)])
+    want = np.repeat(want[:, :, None], 2, 2).astype(np.float64)
+    off = np.abs(got.reshape(len(rows), 2, 2, d) - want) / np.abs(want)
+    assert off.max() <= 8 * bref.EPS, f"off by {off.max() / bref.EPS:.1f} 2^-24"

@@ -1,4 +1,6 @@
-"""Reads of a matrix instruction's result, in the assembly that hipcc writes for every kernel: along every way through the branches, as many
+"""Waits that hipcc puts into the assembly of the kernels, and what it cannot see to.
+
+Reads of a matrix instruction's result, in the assembly that hipcc writes for every kernel: along every way through the branches, as many
 wait states as the instruction needs lie between it and the first vector instruction that reads or overwrites its result (the
 hardware does not wait by itself; hipcc counts too few where a block can be reached on several ways). No GPU needed."""
 import concurrent.futures
@@ -99,17 +101,35 @@ def test_the_search_itself():
     assert len(too_early(instructions(text.format(0).replace("v_accvgpr_read_b32 v9, a3", "ds_write_b32 v1, a2 offset:8")))) > 0
 
 
-@pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
-def test_results_are_waited_for():
+@pytest.fixture(scope="module")
+def assembly():
+    """[(source, kernel, its assembly)] of every kernel."""
+    if not os.path.exists(HIPCC):
+        pytest.skip("needs hipcc")
     sources = sorted(os.path.basename(f) for f in glob.glob(os.path.join(PKG, "csrc", "*.hip")))
     flags = {"chunked_prefill.hip": ["-fno-honor-nans"]}  # as in the Makefile
     with concurrent.futures.ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
         built = list(pool.map(lambda s: kernels(s, *flags.get(s, [])), sources))
+    return [(source, name, text) for source, texts in zip(sources, built) for name, text in texts.items()]
+
+
+def test_results_are_waited_for(assembly):
     products, found = 0, []
-    for source, texts in zip(sources, built):
-        for name, text in texts.items():
-            code = instructions(text)
-            products += sum(n.startswith("v_mfma") for n, _ in code)
-            found += [(source, name, *x) for x in too_early(code)]
+    for source, name, text in assembly:
+        code = instructions(text)
+        products += sum(n.startswith("v_mfma") for n, _ in code)
+        found += [(source, name, *x) for x in too_early(code)]
     assert products > 1000
     assert not found, "\n".join(str(x) for x in found)
+
+
+def test_inline_asm_forms_no_values(assembly):
+    """hipcc knows no instruction of inline asm by what it reads and writes, so it leaves out the waits between one and the vector instructions
+    around it: inline asm holds waits, barriers and loads alone."""
+    blocks = 0
+    for source, name, text in assembly:
+        for block in re.findall(r";;#ASMSTART(.*?);;#ASMEND", text, flags=re.S):
+            names = [line.split(";")[0].split()[0] for line in block.splitlines() if line.split(";")[0].strip()]
+            assert not [x for x in names if x.startswith("v_")], (source, name, block)
+            blocks += len(names) > 0
+    assert blocks > 100
