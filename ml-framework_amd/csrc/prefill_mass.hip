@@ -56,7 +56,7 @@ __device__ __forceinline__ void raw_planes(const RawKeys<KV>& r, uint4 (&plane)[
     if constexpr (KV == PA_DTYPE_FP32) {
         const float v[8] = {r.x[0], r.x[1], r.x[2], r.x[3], r.y[0], r.y[1], r.y[2], r.y[3]};
         if constexpr (NEAR) pa::bf16_planes_near<true>(v, plane);  // (fp32 keys under fp32 queries)
-        else pa::bf16_planes<NP>(v, plane);
+        else pa::bf16_planes(v, plane);
     } else if constexpr (KV == PA_DTYPE_BF16) {
         plane[0] = r.x;
     } else {

@@ -61,24 +61,19 @@ __device__ __forceinline__ void bf16_split3(float x, float (&part)[3]) {
     part[1] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
     part[2] = r - part[1];
 }
-// Eight values as NP bf16 operands: one (values that are exact in bf16) or three, which sum to the value.
-template <int NP>
-__device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[NP]) {
-    uint32_t w[NP][4];
+// Eight values as three bf16 operands that sum to them.
+__device__ __forceinline__ void bf16_planes(const float (&x)[8], uint4 (&plane)[3]) {
+    uint32_t w[3][4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        if constexpr (NP == 1) {
-            w[0][e] = pack_bf16_trunc(x[2 * e], x[2 * e + 1]);
-        } else {
-            float a[3], b[3];
-            bf16_split3(x[2 * e], a);
-            bf16_split3(x[2 * e + 1], b);
+        float a[3], b[3];
+        bf16_split3(x[2 * e], a);
+        bf16_split3(x[2 * e + 1], b);
 #pragma unroll
-            for (int p = 0; p < NP; p++) w[p][e] = pack_bf16_trunc(a[p], b[p]);
-        }
+        for (int p = 0; p < 3; p++) w[p][e] = pack_bf16_trunc(a[p], b[p]);
     }
 #pragma unroll
-    for (int p = 0; p < NP; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    for (int p = 0; p < 3; p++) plane[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 // Two values rounded to the nearest in one conversion. (The empty asm keeps the conversions where they are written: prompts' masses of
 // (32, 8, 128) 122 us for 166. The instruction itself in inline asm would read what v_exp_f32 has only just formed: hipcc sees to no wait there.)
@@ -88,7 +83,7 @@ __device__ __forceinline__ uint32_t pack_bf16_near(float lo, float hi) {
     asm("" : "+v"(w));
     return w;
 }
-// Three operands whose first and second are rounded to the nearest instead of cut off, for one factor of products that have both
+// As bf16_planes, the first and second operand rounded to the nearest instead of cut off, for one factor of products that have both
 // in parts, where those of parts 1 x 2, 2 x 1 and 2 x 2 are left out. Of parts that are all cut off this is up to 2^-21 of a product (2 * 2^-7 *
 // 2^-15), and always missing. Rounded parts are at most 2^-8 (the second) and 2^-17 (the third) of the value and of either sign, so it is
 // less than 2^-22 (2^-8 * 2^-15 + 2^-17 * 2^-7), of either sign. The other factor stays cut off: the one that is split more often.
@@ -118,7 +113,7 @@ __device__ __forceinline__ void load_planes(const void* q, int64_t i, uint4 (&pl
         const f32x4_t b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(q) + i + 4);
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         if constexpr (NEAR) bf16_planes_near<true>(x, plane);
-        else bf16_planes<NP>(x, plane);
+        else bf16_planes(x, plane);
     }
 }
 __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, const f32x16_t& c) {
@@ -373,7 +368,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
         } else if constexpr (F32) {
             const f32x4_t x = __builtin_bit_cast(f32x4_t, tile[p0]), y = __builtin_bit_cast(f32x4_t, tile[p1]);
             const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            bf16_planes<NP>(v, op);
+            bf16_planes(v, op);
         } else {
             op[0] = tile[p0];
         }
@@ -451,7 +446,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
                 if constexpr (I8) x[i] = x[i] == 0.0f ? 0.0f : x[i] * sc[0][2 + u];  // (whatever the scale of an unseen block is)
             }
             if constexpr (F32) bf16_planes_near<false>(x, pop);
-            else bf16_planes<PP>(x, pop);
+            else bf16_planes(x, pop);
             uint4 vop[ND][NP];
             const uint4* const vt = slot + (2 * u + 1) * CH;
 #pragma unroll
