@@ -116,6 +116,10 @@ __device__ __forceinline__ void load_planes(const void* q, int64_t i, uint4 (&pl
         else bf16_planes(x, plane);
     }
 }
+// Which of two bf16 are not finite: bit 15, bit 31.
+__device__ __forceinline__ uint32_t bf16_odd(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+// A mask of those that are.
+__device__ __forceinline__ uint32_t bf16_finite(uint32_t w) { return ~((bf16_odd(w) >> 15) * 0xffffu); }
 __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
@@ -149,7 +153,6 @@ struct WindowSpan {
     __device__ __forceinline__ int entries() const { return first + end - low; }
     __device__ __forceinline__ int block(int e) const { return e < first ? e : e - first + low; }
     __device__ __forceinline__ bool some_see(int t) const { return t < hi && (t >= lo || t < sink); }
-    __device__ __forceinline__ bool all_see(int t) const { return t < hi_all && (t >= lo_all || t < sink); }
     __device__ __forceinline__ bool all_see_block(int t) const { return t + 16 <= hi_all && (t >= lo_all || t + 16 <= sink); }
     __device__ __forceinline__ bool hides_some(int t) const { return !(t + 16 <= hi && (t >= lo || t + 16 <= sink)); }
     __device__ __forceinline__ bool none_see_block(int t) const { return t >= hi || (t + 16 <= lo && t >= sink); }
@@ -190,52 +193,6 @@ struct WindowColumn {
     __device__ __forceinline__ bool any(int sink) const { return hi > lo || min(sink, hi) > 0; }
 };
 
-// Column c over the blocks of list entries [e0, e1), one key at a time: (maximum, sum, O), lanes over dims. For values that are not
-// finite at tokens that some columns of a wave see and others do not.
-template <int D, int KV, bool QF32>
-__device__ void window_column_alone(const WindowPrefillArgs& a, const WindowColumn& c, const WindowSpan& span, const int32_t* table,
-                                    int kvh, int e0, int e1, float& M, float& L, float (&o)[(D + 63) / 64]) {
-    constexpr bool F32 = KV == PA_DTYPE_FP32;
-    constexpr int DPL = (D + 63) / 64;
-    const int lane = threadIdx.x & 63;
-    float q[DPL];
-    M = -INFINITY;
-    L = 0.0f;
-#pragma unroll
-    for (int k = 0; k < DPL; k++) {
-        const int64_t at = c.row * D + min(lane + 64 * k, D - 1);
-        q[k] = QF32 ? static_cast<const float*>(a.q)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.q)[at]);
-        o[k] = 0.0f;
-    }
-    for (int e = e0; e < e1; e++) {
-        const int tok = 16 * span.block(e), id = table[tok / 16];
-        const bool real = id >= 0 && id < a.num_blocks;
-        const int64_t tile = (static_cast<int64_t>(real ? id : 0) * a.num_kv_heads + kvh) * 16 * D;
-        for (int j = 0; j < 16; j++) {
-            if (!c.sees(tok + j, span.sink)) continue;
-            float x = 0.0f, v[DPL];
-#pragma unroll
-            for (int k = 0; k < DPL; k++) {
-                v[k] = 0.0f;
-                if (real && lane + 64 * k < D) {
-                    const int64_t ka = tile + j * D + lane + 64 * k, va = tile + (lane + 64 * k) * 16 + j;
-                    const float kx = F32 ? static_cast<const float*>(a.k_cache)[ka] : bf16_to_f32(static_cast<const uint16_t*>(a.k_cache)[ka]);
-                    v[k] = F32 ? static_cast<const float*>(a.v_cache)[va] : bf16_to_f32(static_cast<const uint16_t*>(a.v_cache)[va]);
-                    x = __builtin_fmaf(q[k], kx, x);
-                }
-            }
-            x = wave_sum(x) * (a.scale * 1.4426950408889634f);
-            const float m_new = fmaxf(M, x);
-            const float f = m_new == M ? 1.0f : __builtin_amdgcn_exp2f(M - m_new);
-            const float p = __builtin_amdgcn_exp2f(x - (m_new == -INFINITY ? 0.0f : m_new));
-            L = L * f + p;
-#pragma unroll
-            for (int k = 0; k < DPL; k++) o[k] = o[k] * f + p * v[k];
-            M = m_new;
-        }
-    }
-}
-
 // SHARE: the waves share 32 columns and take pairs of blocks in turn; else each has 32 columns of its own and all take every pair.
 template <int D, int KV, bool QF32, bool SHARE>
 __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kernel(const WindowPrefillArgs a) {
@@ -251,7 +208,6 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
     constexpr int PIECES = SHARE ? 4 * (SLOT > STATE ? SLOT : STATE) : RING * SLOT;
     __shared__ uint4 s_tile[PIECES];
     __shared__ float2 s_ml[4][32];
-    __shared__ int s_bad[4];
     const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __builtin_assume(wave >= 0 && wave < 4);
@@ -374,6 +330,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
         }
     };
 
+    bool any_odd = false;  // values that are not finite have been met at tokens that some of the wave's columns see and others may not
     const int krow = key_of_row(n);
     auto compute = [&](const uint4* slot, int j, auto after_keys, auto before_values) {
         const int e0 = 2 * pair_of(j);
@@ -456,18 +413,37 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
                 else if constexpr (F32) operand(vt, TL::vpos(d, 2 * hf), TL::vpos(d, 2 * hf + 1), vop[t]);
                 else operand(vt, TL::vpos(d, hf), 0, vop[t]);
             }
-            if (!I8 && mine.hides_some(tok[u])) {  // values that no column sees are zeros: what unused slots hold does not matter
-                uint32_t keep[4];
+            if (!I8 && !mine.all_see_block(tok[u])) {
+                if (mine.hides_some(tok[u])) {  // values that no column sees are zeros: what unused slots hold does not matter
+                    uint32_t keep[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int t = tok[u] + 8 * hf + 2 * i;
-                    keep[i] = (mine.some_see(t) ? 0xffffu : 0u) | (mine.some_see(t + 1) ? 0xffff0000u : 0u);
+                    for (int i = 0; i < 4; i++) {
+                        const int t = tok[u] + 8 * hf + 2 * i;
+                        keep[i] = (mine.some_see(t) ? 0xffffu : 0u) | (mine.some_see(t + 1) ? 0xffff0000u : 0u);
+                    }
+#pragma unroll
+                    for (int t = 0; t < ND; t++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++)
+                            vop[t][p] = make_uint4(vop[t][p].x & keep[0], vop[t][p].y & keep[1], vop[t][p].z & keep[2], vop[t][p].w & keep[3]);
                 }
+                uint32_t odd = 0;
 #pragma unroll
-                for (int t = 0; t < ND; t++)
+                for (int t = 0; t < ND; t++) odd |= bf16_odd(vop[t][0].x) | bf16_odd(vop[t][0].y) | bf16_odd(vop[t][0].z) | bf16_odd(vop[t][0].w);
+                if (__any(odd != 0)) {  // they would reach columns that do not see them as 0 times them: zeros for now
+                    any_odd = true;
 #pragma unroll
-                    for (int p = 0; p < NP; p++)
-                        vop[t][p] = make_uint4(vop[t][p].x & keep[0], vop[t][p].y & keep[1], vop[t][p].z & keep[2], vop[t][p].w & keep[3]);
+                    for (int t = 0; t < ND; t++) {
+                        const uint4 x = vop[t][0];
+#pragma unroll
+                        for (int p = 0; p < NP; p++) {
+                            vop[t][p].x &= bf16_finite(x.x);
+                            vop[t][p].y &= bf16_finite(x.y);
+                            vop[t][p].z &= bf16_finite(x.z);
+                            vop[t][p].w &= bf16_finite(x.w);
+                        }
+                    }
+                }
             }
 #pragma unroll
             for (int q = 0; q < PP; q++)
@@ -545,60 +521,47 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
             if (a.lse && dim == 0) a.lse[col.row] = sees ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
         }
     };
-    // A value that is not finite at a token that some of the wave's columns see and others do not would reach
-    // the others as 0 times it. Where the outcome is not finite the values of such tokens are looked at, and if that is the cause
-    // the columns are computed again one by one (each over its own tokens only).
-    bool done = false;
+    // The zeros that stood in for such values become NaN in the columns that see their tokens: how many of them a column sees in a channel is a
+    // matrix product too, of the values' operand with 1 for each of them and the probabilities' with 1 for each token that is seen. (2 prompts
+    // of 4096 whose values are all NaN: 1.1 times the time of finite ones; their columns one by one, a key at a time, 280 times. Looking at the
+    // values of such blocks takes 5 % where they are most of what is read, windows of 64 at head size 64, else nothing that shows.)
     if constexpr (!I8) {
-        bool odd = !(fabsf(l_run) < INFINITY);
-#pragma unroll
-        for (int t = 0; t < ND; t++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) odd |= !(fabsf(acc[t][i]) < INFINITY);
-        bool redo = live && __any(odd);
-        if constexpr (SHARE) {
-            if (lane == 0) s_bad[wave] = redo;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 4; w++) redo |= s_bad[w] != 0;
-        }
-        if (redo) {
-            const int e1 = min(2 * pair1, entries);
-            bool hit = false;
-            for (int e = 2 * pair0; e < e1; e++) {
+        if (any_odd) {
+            for (int j = 0; j < 2 * count; j++) {
+                const int e = 2 * pair_of(j >> 1) + (j & 1);
+                if (e >= entries) continue;
                 const int tok = 16 * span.block(e), id = table[tok / 16];
                 if (id < 0 || id >= a.num_blocks || mine.all_see_block(tok)) continue;
-                for (int i = lane; i < TILE; i += 64) {
-                    const int64_t at = (static_cast<int64_t>(id) * Hkv + kvh) * TILE + i;
-                    const float v = F32 ? static_cast<const float*>(a.v_cache)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.v_cache)[at]);
-                    const int t = tok + (i & 15);
-                    hit |= mine.some_see(t) && !mine.all_see(t) && !(fabsf(v) < INFINITY);
-                }
-            }
-            done = __any(hit);  // (the waves that share columns agree: it follows from the same values)
-            if (done && !(SHARE && wave > 0)) {
-                for (int c = 0; c < 32 && c_wave + c < columns; c++) {
-                    const WindowColumn one(a, c_wave + c, q0, kvh, P, T);
-                    float M, L, o[(D + 63) / 64];
-                    window_column_alone<D, KV, QF32>(a, one, span, table, kvh, 2 * pair0, e1, M, L, o);
-                    const bool any = one.any(span.sink);
+                uint32_t sees[4];
 #pragma unroll
-                    for (int k = 0; k < (D + 63) / 64; k++) {
-                        if (lane + 64 * k >= D) continue;
-                        if (a.splits > 1) a.ws_o[(slot0 + c) * D + lane + 64 * k] = o[k];
-                        else a.out[one.row * D + lane + 64 * k] = any ? o[k] * (1.0f / L) : 0.0f;
+                for (int i = 0; i < 4; i++) {
+                    const int t = tok + 8 * hf + 2 * i;
+                    sees[i] = (col.sees(t, span.sink) ? 0x3f80u : 0u) | (col.sees(t + 1, span.sink) ? 0x3f800000u : 0u);
+                }
+                const char* const tile = vc + (static_cast<int64_t>(id) * Hkv + kvh) * TILE * ELT;
+#pragma unroll
+                for (int t = 0; t < ND; t++) {
+                    uint32_t odd[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const char* const at = tile + ((32 * t + n) * 16 + 8 * hf + 2 * i) * ELT;
+                        odd[i] = F32 ? bf16_odd(pack_bf16_trunc(reinterpret_cast<const float*>(at)[0], reinterpret_cast<const float*>(at)[1]))
+                                     : bf16_odd(*reinterpret_cast<const uint32_t*>(at));
+                        odd[i] = (odd[i] >> 15) * 0x3f80u;
                     }
-                    if (lane == 0) {
-                        if (a.splits > 1) a.ws_ml[slot0 + c] = make_float2(M, L);
-                        else if (a.lse) a.lse[one.row] = any ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : -INFINITY;
-                    }
+                    f32x16_t sum;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[i] = 0.0f;
+                    sum = mfma32(make_uint4(odd[0], odd[1], odd[2], odd[3]), make_uint4(sees[0], sees[1], sees[2], sees[3]), sum);
+                    sum = sum * 3e38f * 3e38f;  // 0 or infinite
+                    acc[t] += sum - sum;
                 }
             }
         }
     }
     const float l_tot = halves_sum(l_run);
     if constexpr (!SHARE) {
-        if (!stored || done) return;
+        if (!stored) return;
 #pragma unroll
         for (int t = 0; t < ND; t++)
 #pragma unroll
@@ -615,7 +578,7 @@ __global__ __launch_bounds__(256, window_groups(D, KV)) void window_prefill_kern
             for (int b = 0; b < 4; b++)
                 place(wave, 4 * t + b) = __builtin_bit_cast(uint4, f32x4_t{acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]});
         __syncthreads();
-        if (!stored || done) return;
+        if (!stored) return;
         float M = -INFINITY, L = 0.0f, f[4];
 #pragma unroll
         for (int w = 0; w < 4; w++) M = fmaxf(M, s_ml[w][n].x);

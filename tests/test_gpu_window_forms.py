@@ -10,6 +10,7 @@ import pytest
 import bounded_ref as bref
 import longctx_ref as ref
 import paged_attention as pa
+from helpers import check_close, empty_gpu, to_gpu, to_np, tol_for
 from test_gpu_window import BF16, FP32, I32, INT8, TYPES, close, close_mass, gpu_pool, masses, run_decode, run_mass, run_prefill
 
 pytestmark = pytest.mark.gpu
@@ -182,7 +183,6 @@ def test_single_tokens_and_chunks_past_the_bounds(kv, q):
 def test_masses_by_the_last_tokens_of_prompts_alone(kv, q):
     """Prompts attended to by the chunks' other kernel, their last tokens once more for the logarithms that their masses need."""
     import torch
-    from helpers import check_close, empty_gpu, to_gpu, to_np, tol_for
     lens, last = [700, 90, 20], 32
     p = ref.Pool(680, lens, 8, 2, 64, kv, q)
     g = gpu_pool(p)
@@ -208,3 +208,35 @@ def test_masses_by_the_last_tokens_of_prompts_alone(kv, q):
     total = (got.astype(np.float64) - before).sum(1)
     slack = 2 * bref.EPS * got.sum(1) + mass_tol.sum(1) + added.sum(1) * lse_tol.max()
     assert (np.abs(total - 8 * np.array(chunks)) <= slack).all()
+
+
+@pytest.mark.parametrize("kv", [BF16, FP32])
+@pytest.mark.parametrize("window", [0, 700])
+def test_values_that_are_not_finite_cost_little_time(kv, window):
+    """Prompts whose values are NaN throughout, or at one token of many, take a small multiple of the time of finite ones."""
+    import torch
+    lens = [2048, 2048]
+    p = ref.Pool(690, lens, 8, 2, 64, kv, kv)
+    g, n = gpu_pool(p), sum(lens)
+    q, out = to_gpu(p.queries(n)), empty_gpu((n, 8, 64), np.float32)
+    start, prefix = to_gpu(np.array([0, 2048, 4096], I32)), to_gpu(np.zeros(2, I32))
+    size = pa.window_prefill_workspace_size(p.cfg, 2, 2048, 2048, 0, window)
+    ws = empty_gpu((max(size, 16),), np.uint8)
+
+    def took(v):
+        values, times = to_gpu(v), []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            pa.window_prefill(None, p.cfg, out, q, start, prefix, g["k"], values, None, None, g["tables"], 2, p.width, 2048, 2048, 0, window,
+                              None, ws, size)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    bad = ref.of_type(np.full(1, np.nan, np.float32), kv)[0]
+    one, whole = p.v.copy(), np.full_like(p.v, bad)
+    one[p.tables[0, 64], :, 5, 3] = bad
+    finite = took(p.v)
+    assert took(one) < 10 * finite and took(whole) < 10 * finite
