@@ -22,7 +22,7 @@
 // matrix products and what is issued beside them in two waves a SIMD (8 x 512 tokens over that window 136 to 144 us, 2 x 4096 267 to 290 from card to
 // card: 0.85 to 0.9 and 0.9 to 1.0 PFLOP/s counting the four products of exact probabilities, where a large matrix product reaches 1.26). On one card:
 // probabilities in two fp16 parts, values converted in LDS by the waves, 163 and 317 us against 143 and 282 (registers); the next pair's scores
-// beside this pair's probabilities 147 and 290. fp32 caches: 275 us for 16 x 42 tokens on 4982, (16, 4, 128).
+// beside this pair's probabilities 147 and 290. fp32 caches: 270 us for 16 x 42 tokens on 4982, (16, 4, 128).
 #pragma once
 
 #include <cfloat>

@@ -93,3 +93,46 @@ def test_eviction(first):
             m = rng.choice(np.array([np.inf, -np.inf, np.nan, -1, 0, -0.0, 1e-42, 3e38, 1], np.float32), tables.shape)
         lens = np.array(lens, I32)
         same(run_evict(nb, tables, lens, m, sink, recent, budget, refs), bref.evict(tables, lens, m, sink, recent, budget, refs))
+
+
+@pytest.mark.parametrize("first", range(0, 300, 100))
+def test_values_that_are_not_finite(first):
+    """They reach the queries that see their tokens, in their channels, and nothing else."""
+    for seed in range(first, first + 100):
+        rnd = random.Random(10 ** 6 + seed)
+        p, lens = a_pool(rnd, seed)
+        if p.kv == INT8 or sum(lens) == 0:
+            continue
+        p.tables[:] = -1
+        at = 0
+        for s, t in enumerate(lens):  # every block in one place (the pool may have renamed some)
+            p.tables[s, :(t + 15) // 16] = np.arange(at, at + (t + 15) // 16)
+            at += (t + 15) // 16
+        p.k[:], p.v[:] = (ref.of_type(p.rng.standard_normal(x.shape, np.float32), p.kv) for x in (p.k, p.v))
+        window, sink = rnd.choice([0, 0, rnd.randint(1, 60), rnd.randint(1, 1000)]), rnd.choice([0, 1, rnd.randint(1, 100)])
+        chunks = [min(t, rnd.choice([0, 1, 5, rnd.randint(0, 150)])) for t in lens]
+        if sum(chunks) == 0 or sum(chunks) * p.hq > 6000:
+            continue
+        rows, at = bref.chunk_rows(lens, chunks)
+        qs, one = p.queries(len(rows)), p.queries(len(lens))
+        want, tol, lse, lse_tol, _, _ = bref.attend(p, qs, rows, at, sink, window, [lens[s] for s in rows])
+        dwant, dtol, _, _, _, _ = bref.decode(p, one, lens, sink, window)
+        touched, dtouched = np.zeros(want.shape, bool), np.zeros(dwant.shape, bool)
+        for _ in range(rnd.choice([1, 3, 30])):
+            s = rnd.choice([s for s, t in enumerate(lens) if t])
+            t, h, c = rnd.randrange(max(0, lens[s] - 2 * chunks[s] - 40), lens[s]), rnd.randrange(p.hkv), rnd.randrange(p.d)
+            p.v[p.tables[s, t // 16], h, c, t % 16] = ref.of_type(np.full(1, rnd.choice([np.nan, np.inf, -np.inf]), np.float32), p.kv)[0]
+            heads = slice(h * (p.hq // p.hkv), (h + 1) * (p.hq // p.hkv))
+            for r, (x, pos) in enumerate(zip(rows, at)):
+                if x == s and bref.seen(pos, t, sink, window):
+                    touched[r, heads, c] = True
+            if bref.seen(lens[s] - 1, t, sink, window):
+                dtouched[s, heads, c] = True
+        g = gpu_pool(p)
+        got, glse = run_prefill(p, g, qs, lens, chunks, sink, window, max_chunk=rnd.choice([max(chunks), 5000]))
+        what = f"seed {seed}: types {p.kv} {p.q}, heads {p.hq} {p.hkv} {p.d}, {lens[:5]}, {chunks[:5]}, window {window}, sink {sink}"
+        seen = np.isfinite(lse)
+        close(glse[seen], lse[seen], lse_tol[seen], what)
+        for x, w, t, hit in ((got, want, tol, touched), (run_decode(p, g, one, lens, sink, window)[0], dwant, dtol, dtouched)):
+            assert not np.isfinite(x[hit]).any(), what
+            close(x[~hit], w[~hit], np.broadcast_to(t, w.shape)[~hit], what)
